@@ -212,6 +212,10 @@ class _Signatures:
     jllm_delta_recurrent = [P, I, I, I, I, I, P, P, I, F, P, I, P, P, P, P, P, I, P, I, F, P, I, I, I, I, I, P]
     jllm_delta_chunked = [P, I, I, I, I, I, P, P, I, F, P, I, P, P, P, P, P, P, P, P, I, P, I, F, P, I, I, I, I, I, I, P]
     jllm_sample = [P, I, I, I, P, P, P, P, P, P, P]
+    jllm_quantize_int8 = [P, I, I, P, I, P, I, I, P]
+    jllm_add_rmsnorm_int8 = [P, I, P, I, I, P, I, P, I, F, P, I, P, I, I, P]
+    jllm_int8_values = [P, I, P, P, I, I, I, I, P]
+    jllm_gemm_int8 = [P, I, P, P, P, I, P, I, P, I, I, I, I, I, I, I, P]
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -1543,3 +1547,167 @@ def decode_splits(rows, kv_heads, kv_bucket, heads, head_dim, scratch, places: i
     while splits > 1 and attention_decode_scratch_floats(rows, heads, head_dim, splits) > scratch.numel():
         splits -= 1
     return splits
+
+
+# ---- linears in 8-bit integers ---------------------------------------------------------------------------
+
+INT8_MAX_K = 131071      # a product's sum of k products of two 8-bit integers stays exact in 32 bits up to here
+
+
+def _refuse(name, why):
+    raise KernelError(f"{name}: {why}")
+
+
+class Int8Rows:
+    """Rows of activations in 8-bit integers: row r stands for data[r] * scale[r]. data int8 [rows, cols], its rows beginning at
+    multiples of 16 bytes (`int8_rows` makes such); scale float32 [rows]. A slice of rows is `rows8[lo:hi]`."""
+    __slots__ = ("data", "scale", "rows", "cols", "stride", "address", "scale_address", "on_gpu")
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor):
+        if data.dtype != torch.int8 or scale.dtype != torch.float32 or data.dim() != 2 or scale.shape != data.shape[:1]:
+            _refuse("Int8Rows", f"int8 data [rows, cols] and a float32 scale for each row, got {data.dtype} {tuple(data.shape)} and {scale.dtype} {tuple(scale.shape)}")
+        self.data, self.scale = data, scale
+        self.rows, self.cols = data.shape
+        self.stride, self.address, self.scale_address = data.stride(0), data.data_ptr(), scale.data_ptr()
+        self.on_gpu = data.is_cuda and scale.is_cuda
+        if self.rows == 1:                       # (a single row's stride says nothing)
+            self.stride = max(self.stride, -(-self.cols // 16) * 16)
+        if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or self.stride < self.cols or self.stride % 16 or self.address % 16
+                or (self.rows > 1 and scale.stride(0) != 1)):
+            _refuse("Int8Rows", f"rows of neighbouring values that begin at multiples of 16 bytes, got strides {data.stride()}, {scale.stride()} at {self.address:#x}")
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    def __getitem__(self, rows: slice) -> "Int8Rows":
+        if not isinstance(rows, slice):
+            _refuse("Int8Rows", "a slice of rows is what can be taken")
+        return Int8Rows(self.data[rows], self.scale[rows])
+
+
+def int8_rows(rows: int, cols: int, device) -> Int8Rows:
+    """Room for `rows` rows of `cols` values in 8 bits (what `quantize_int8` and `add_rmsnorm_int8` write)."""
+    data = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)
+    return Int8Rows(data[:, :cols], torch.empty((rows,), dtype=torch.float32, device=device))
+
+
+def _row_stride(name, what, t, shape):
+    """The row stride of a [rows, cols] matrix with neighbouring values on the GPU."""
+    if t.shape != shape or not t.is_cuda or (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
+        _refuse(name, f"{what} is a {tuple(shape)} matrix of neighbouring values on the GPU, got {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def quantize_int8(x: torch.Tensor, out: Int8Rows) -> None:
+    """out = the rows of x in 8 bits: q = round(x * (127 / m)), half to even, scale = m / 127 with m a row's largest magnitude. x
+    float32 or bfloat16 [rows, cols], any row stride. A row whose largest magnitude is below 2^-100 becomes zeros with scale 0, one that
+    holds an infinity or a NaN zeros with scale NaN (what is computed from it is then NaN)."""
+    if x.dtype not in _DT or not out.on_gpu:
+        _refuse("quantize_int8", f"float32 or bfloat16 rows and room on the GPU, got {x.dtype} and {out.data.device}")
+    ld = _row_stride("quantize_int8", "x", x, out.shape)
+    _call("jllm_quantize_int8", x.data_ptr(), _DT[x.dtype], ld, out.address, out.stride, out.scale_address, out.rows, out.cols, _stream())
+
+
+def add_rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, out: Int8Rows, y: torch.Tensor | None = None,
+                     total: torch.Tensor | None = None) -> None:
+    """out = rmsnorm(x + y) * gain in 8 bits (as `quantize_int8` has them), total = x + y: the residual's addition, the norm behind it
+    and the rounding in one pass. x float32 [rows, dim]; y float32 or bfloat16 of x's shape, or None (nothing is added, and there is no
+    total); total float32 of x's shape, x itself by default; gain float32 or bfloat16 [dim]."""
+    name = "add_rmsnorm_int8"
+    if x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != (out.cols,) or gain.stride(0) != 1 or not gain.is_cuda or not out.on_gpu:
+        _refuse(name, f"on the GPU, float32 rows and a float32 or bfloat16 gain of {out.cols} values, got {x.dtype} and {gain.dtype} {tuple(gain.shape)}")
+    ldx = _row_stride(name, "x", x, out.shape)
+    ldy = ldt = 0
+    if y is None:
+        if total is not None:
+            _refuse(name, "a total goes with a y to add")
+    else:
+        total = x if total is None else total
+        if y.dtype not in _DT or total.dtype != torch.float32:
+            _refuse(name, f"y is float32 or bfloat16 and the total float32, got {y.dtype} and {total.dtype}")
+        ldy, ldt = _row_stride(name, "y", y, out.shape), _row_stride(name, "the total", total, out.shape)
+    _call("jllm_add_rmsnorm_int8", x.data_ptr(), ldx, _p(y), _DT[y.dtype] if y is not None else BF16, ldy, _p(total), ldt, gain.data_ptr(),
+          _DT[gain.dtype], float(eps), out.address, out.stride, out.scale_address, out.rows, out.cols, _stream())
+
+
+def int8_values(rows8: Int8Rows, out: torch.Tensor) -> torch.Tensor:
+    """out = the values that the rows stand for, data * scale, float32 or bfloat16; returns out."""
+    if out.dtype not in _DT or not rows8.on_gpu:
+        _refuse("int8_values", f"float32 or bfloat16 values and rows on the GPU, got {out.dtype} and {rows8.data.device}")
+    ld = _row_stride("int8_values", "out", out, rows8.shape)
+    _call("jllm_int8_values", rows8.address, rows8.stride, rows8.scale_address, out.data_ptr(), _DT[out.dtype], ld, rows8.rows, rows8.cols,
+          _stream())
+    return out
+
+
+class PackedInt8:
+    """A [rows, cols] weight in 8-bit integers with a float32 scale a row, in the layout the tensor cores stream: tiles of 128 rows x
+    128 k, each the 16 KB image of its 128-byte-swizzled shared-memory form (as `PackedWeight`, whose tiles hold 64 k of 16 bits), rows and
+    k filled up with zeros. `glu`: the rows are blocks of 8 gate rows and their 8 up rows."""
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int, glu: bool = False):
+        self.data, self.scale, self.rows, self.cols, self.glu = data, scale, rows, cols, glu
+        self.tiles, self.k_blocks = data.shape[0], data.shape[1]
+        self.address, self.scale_address, self.on_gpu = data.data_ptr(), scale.data_ptr(), data.is_cuda and scale.is_cuda
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    def unpack(self) -> torch.Tensor:
+        """The [rows, cols] integers again, in the order they were packed in."""
+        T, KB = self.tiles, self.k_blocks
+        idx = _swizzle_index(self.data.device).expand(T, KB, 128, 8, 16)
+        plain = self.data.view(T, KB, 128, 8, 16).gather(3, idx).permute(0, 2, 1, 3, 4).reshape(T * 128, KB * 128)
+        return plain[:self.rows, :self.cols].contiguous()
+
+
+def _glu_order(t: torch.Tensor) -> torch.Tensor:
+    """All gate rows, then all up rows -> blocks of 8 gate rows and their 8 up rows."""
+    half = t.shape[0] // 2
+    return torch.stack([t[:half].reshape(half // 8, 8, -1), t[half:].reshape(half // 8, 8, -1)], dim=1).reshape(t.shape)
+
+
+def pack_int8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> PackedInt8:
+    """Packs an int8 weight [rows, cols] with a float32 scale a row for `gemm_int8` (done once, at load). `glu`: the rows are all gate
+    rows, then all up rows (a multiple of 8 each), and are laid out for a product with `swiglu`."""
+    if data.dim() != 2 or data.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != data.shape[:1] or not data.numel():
+        _refuse("pack_int8", f"an int8 matrix and a float32 scale a row, got {data.dtype} {tuple(data.shape)} and {scale.dtype} {tuple(scale.shape)}")
+    N, K = data.shape
+    if K > INT8_MAX_K or (glu and N % 16):
+        _refuse("pack_int8", f"at most {INT8_MAX_K} columns, and gate and up rows in eights, got {N} x {K}")
+    if glu:
+        data, scale = _glu_order(data), _glu_order(scale)
+    T, KB = -(-N // 128), -(-K // 128)
+    padded = torch.zeros((T * 128, KB * 128), dtype=torch.int8, device=data.device)
+    padded[:N, :K] = data
+    tiles = padded.view(T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)                  # [T, KB, 128 rows, 8 chunks, 16]
+    packed = tiles.gather(3, _swizzle_index(data.device).expand(T, KB, 128, 8, 16)).contiguous().view(T, KB, 128, 128)
+    return PackedInt8(packed, scale.contiguous(), N, K, glu)
+
+
+def quantize_weight_int8(w: torch.Tensor, glu: bool = False) -> PackedInt8:
+    """A float32 or bfloat16 weight [rows, cols] rounded to 8 bits, one scale a row (`quantize_int8`), and packed."""
+    rows8 = int8_rows(w.shape[0], w.shape[1], w.device)
+    quantize_int8(w, rows8)
+    return pack_int8(rows8.data, rows8.scale, glu)
+
+
+def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate=False, swiglu=False) -> None:
+    """out (+)= a @ w^T (+ bias): the integers' sums are exact, the result is sum * scale of the token * scale of the weight row in
+    float32, so a row's result is the same bits in any batch. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or
+    bfloat16; `accumulate` as the other products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`;
+    no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]."""
+    name = "gemm_int8"
+    word = glu_kind(swiglu)
+    if isinstance(swiglu, GluUnits) or bool(word) != w.glu:
+        _refuse(name, "a gated unit without weights of its own goes with a weight packed for it, and only with one")
+    if a.cols != w.cols or out.dtype not in _DT or not (a.on_gpu and w.on_gpu):
+        _refuse(name, f"rows of {w.cols} values and a float32 or bfloat16 result on the GPU, got {a.cols} and {out.dtype}")
+    ldo = _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows))
+    if bias is not None and (bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_cuda or bias.stride(0) != 1):
+        _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
+    _call("jllm_gemm_int8", a.address, a.stride, a.scale_address, w.address, w.scale_address, w.k_blocks, _p(bias),
+          _DT[bias.dtype] if bias is not None else F32, out.data_ptr(), _DT[out.dtype], ldo, int(accumulate), a.rows, w.rows, w.cols, word,
+          _stream())
