@@ -215,7 +215,7 @@ class _Signatures:
     jllm_quantize_int8 = [P, I, I, P, I, P, I, I, P]
     jllm_add_rmsnorm_int8 = [P, I, P, I, I, P, I, P, I, F, P, I, P, I, I, P]
     jllm_int8_values = [P, I, P, P, I, I, I, I, P]
-    jllm_gemm_int8 = [P, I, P, P, P, I, P, I, P, I, I, I, I, I, I, I, P]
+    jllm_gemm_int8 = [P, I, P, P, P, I, P, I, P, I, I, I, I, I, I, I, I, P]
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -1194,7 +1194,8 @@ def bounds_errors() -> dict:
 
 
 # Which kernel a code in an error word is from: the products share one word, the attention kernels another.
-WAIT_KERNELS = {"products": ((1, 3, "gemm_tcgen05"), (11, 13, "gemm_stream"), (14, 16, "gemm_stream (clusters)"), (21, 23, "gemm_pair")),
+WAIT_KERNELS = {"products": ((1, 3, "gemm_tcgen05"), (11, 13, "gemm_stream"), (14, 16, "gemm_stream (clusters)"), (21, 23, "gemm_pair"),
+                             (31, 33, "gemm_int8 (few tokens)"), (34, 36, "gemm_int8 (pairs)")),
                 "attention": ((21, 23, "attention_prefill_tc"), (31, 33, "attention_prefill_pair"), (41, 43, "attention_prefill_latent"),
                               (51, 52, "attention_decode_ring"))}
 
@@ -1644,12 +1645,16 @@ def int8_values(rows8: Int8Rows, out: torch.Tensor) -> torch.Tensor:
 class PackedInt8:
     """A [rows, cols] weight in 8-bit integers with a float32 scale a row, in the layout the tensor cores stream: tiles of 128 rows x
     128 k, each the 16 KB image of its 128-byte-swizzled shared-memory form (as `PackedWeight`, whose tiles hold 64 k of 16 bits), rows and
-    k filled up with zeros. `glu`: the rows are blocks of 8 gate rows and their 8 up rows."""
+    k filled up with zeros (the scales too, to whole tiles). `glu`: the rows are blocks of 8 gate rows and their 8 up rows."""
 
-    def __init__(self, data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int, glu: bool = False):
-        self.data, self.scale, self.rows, self.cols, self.glu = data, scale, rows, cols, glu
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, glu: bool = False):
+        self.data, self.scales, self.rows, self.cols, self.glu = data, scales, rows, cols, glu
         self.tiles, self.k_blocks = data.shape[0], data.shape[1]
-        self.address, self.scale_address, self.on_gpu = data.data_ptr(), scale.data_ptr(), data.is_cuda and scale.is_cuda
+        self.address, self.scale_address, self.on_gpu = data.data_ptr(), scales.data_ptr(), data.is_cuda and scales.is_cuda
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self.scales[:self.rows]
 
     @property
     def shape(self):
@@ -1684,7 +1689,9 @@ def pack_int8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> Pac
     padded[:N, :K] = data
     tiles = padded.view(T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)                  # [T, KB, 128 rows, 8 chunks, 16]
     packed = tiles.gather(3, _swizzle_index(data.device).expand(T, KB, 128, 8, 16)).contiguous().view(T, KB, 128, 128)
-    return PackedInt8(packed, scale.contiguous(), N, K, glu)
+    scales = torch.zeros((T * 128,), dtype=torch.float32, device=data.device)
+    scales[:N] = scale
+    return PackedInt8(packed, scales, N, K, glu)
 
 
 def quantize_weight_int8(w: torch.Tensor, glu: bool = False) -> PackedInt8:
@@ -1694,11 +1701,13 @@ def quantize_weight_int8(w: torch.Tensor, glu: bool = False) -> PackedInt8:
     return pack_int8(rows8.data, rows8.scale, glu)
 
 
-def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate=False, swiglu=False) -> None:
+def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate=False, swiglu=False,
+              cut: int = 0) -> None:
     """out (+)= a @ w^T (+ bias): the integers' sums are exact, the result is sum * scale of the token * scale of the weight row in
     float32, so a row's result is the same bits in any batch. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or
     bfloat16; `accumulate` as the other products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`;
-    no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]."""
+    no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. `cut` (tests): the blocks of a cluster that share 128
+    weight rows, or minus the weight rows of a tile of 256 tokens; 0: as the sizes have it."""
     name = "gemm_int8"
     word = glu_kind(swiglu)
     if isinstance(swiglu, GluUnits) or bool(word) != w.glu:
@@ -1710,4 +1719,4 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
         _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
     _call("jllm_gemm_int8", a.address, a.stride, a.scale_address, w.address, w.scale_address, w.k_blocks, _p(bias),
           _DT[bias.dtype] if bias is not None else F32, out.data_ptr(), _DT[out.dtype], ldo, int(accumulate), a.rows, w.rows, w.cols, word,
-          _stream())
+          int(cut), _stream())

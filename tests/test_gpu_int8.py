@@ -298,6 +298,26 @@ def test_product_gated(ops, rows, hidden, kind):
     ops.check_kernel_errors()
 
 
+@pytest.mark.parametrize("cut,rows,width,dim", [(1, 1, 128, 128), (1, 256, 300, 1300), (2, 3, 200, 300), (3, 17, 129, 1000), (4, 40, 1003, 2049), (5, 200, 70, 900),
+                                                (6, 256, 260, 4096), (7, 100, 256, 1025), (8, 256, 400, 3000), (8, 8, 384, 8192), (8, 1, 100, 1024), (7, 24, 64, 12000),
+                                                (-64, 1, 10, 20), (-64, 130, 250, 700), (-64, 700, 400, 333), (-64, 2048, 3000, 256),
+                                                (-128, 257, 129, 500), (-128, 256, 1000, 640), (-128, 1200, 4224, 300),
+                                                (-256, 300, 128, 200), (-256, 513, 700, 1111), (-256, 2100, 5000, 300), (-256, 5, 257, 150)])
+def test_product_cut_up(ops, cut, rows, width, dim):
+    """Every way of cutting the work gives the same bits."""
+    (a, sa), (w, sw) = integers(rows, dim, 11), integers(width, dim, 12)
+    bias, old = rnd(width), rnd(rows, width, seed=5)
+    a8, packed = on_gpu(ops, a, sa), ops.pack_int8(w.to(DEV), sw.to(DEV))
+    for _ in range(3):
+        out = old.to(DEV)
+        ops.gemm_int8(a8, packed, out, bias.to(DEV), accumulate=True, cut=cut)
+        out16 = torch.empty(rows, width, dtype=torch.bfloat16, device=DEV)
+        ops.gemm_int8(a8, packed, out16, cut=cut)
+        ops.check_kernel_errors()
+        assert torch.equal(out.cpu(), plain_product(a, sa, w, sw, bias, old))
+        assert torch.equal(out16.cpu(), plain_product(a, sa, w, sw).to(torch.bfloat16))
+
+
 def test_a_rows_bits_do_not_depend_on_its_batch(ops):
     """Every kernel and every way of cutting the work: a row alone, in small and in large batches."""
     dim, width = 1111, 2050
@@ -408,6 +428,9 @@ def test_refusals(ops):
             lambda: ops.gemm_int8(a8, glu, half, accumulate=True, swiglu="silu"),
             lambda: ops.gemm_int8(a8, packed, out, torch.zeros(31, device=DEV)),
             lambda: ops.gemm_int8(a8, packed, out, accumulate=7),
+            lambda: ops.gemm_int8(a8, packed, out, cut=2),                # one k block
+            lambda: ops.gemm_int8(a8, packed, out, cut=9),
+            lambda: ops.gemm_int8(a8, packed, out, cut=-32),
             lambda: ops.gemm_int8(ops.int8_rows(4, 48, DEV), packed, out),
             lambda: ops.gemm_int8(ops.Int8Rows(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4)), packed, out)):
         with pytest.raises(E):
