@@ -1,29 +1,111 @@
 // Rows in 8-bit integers: q[r, j] = rint(v[r, j] * (127 / m_r)), scale[r] = m_r / 127 with m_r = max_j |v[r, j]|, so that v is about
 // q * scale. Where the values come from: a part's result as it is (quantize_int8), or the residual's addition and the RMS norm in
-// front of a product (add_rmsnorm_int8: t = x + y, v = t / sqrt(mean(t^2) + eps) * gain). Sums, maxima and values are float32; the one
-// rounding to fewer bits is the one to 8, half to even.
+// front of a product (add_rmsnorm_int8: t = x + y, v = t root gain, root = 1 / sqrt(mean(t^2) + eps)). Sums, maxima and values are
+// float32; the one rounding to fewer bits is the one to 8, half to even.
+//
+// The norm's q does not need the root: with w = t gain it is rint(w * (127 / max |w|)), and scale = root * max |w| / 127. So the sum of
+// squares and the maximum are ONE reduction, a row is read once, kept in registers and rounded behind one meeting of its threads.
 //
 // What a row cannot say in 8 bits: a row whose largest magnitude is below 2^-100 is zeros with scale 0 (127 / m would leave
-// float32), a row that holds an infinity or a NaN has the scale NaN and zeros, so that what is made of it is NaN and not a wrong number.
+// float32; of the norm's results such a row may keep its numbers), a row that holds an infinity or a NaN has the scale NaN and zeros, so that what is made of it is NaN and not a wrong number.
+//
+// A thread takes V chunks of 8 neighbouring values, chunk i of a row being thread i % T's. V and T follow from the row's width alone, so
+// a row's sum has one order whatever else is in the batch. Rows of up to 512 values are a warp's each, wider ones a block's, beyond 32,768
+// values (`wide`) a thread's chunks are fetched again behind the reduction.
 #include "head_rotate.cuh"
 
 namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;      // 2^-100
+constexpr int MOST_CHUNKS = 4, MOST_THREADS = 1024;   // what a row's threads hold: 32,768 values
 
 // The larger of two magnitudes; a NaN stays (fmaxf would drop it).
 __device__ __forceinline__ float mag_max(float a, float b) { return a >= b || a != a ? a : b; }
-__device__ __forceinline__ float block_mag_max(float v, float* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+
+// Sum and largest magnitude over the threads of a row: a warp, or (BLOCK) the block's warps. `scratch` holds 64 floats.
+template <bool BLOCK>
+__device__ __forceinline__ void row_reduce(float& sum, float& m, float* scratch) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = mag_max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (lane == 0) scratch[warp] = v;
-    __syncthreads();
-    v = lane < warps ? scratch[lane] : 0.f;
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        m = mag_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    if constexpr (BLOCK) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        __syncthreads();               // (what a reduction in front of this one left has been read)
+        if (lane == 0) scratch[warp] = sum, scratch[32 + warp] = m;
+        __syncthreads();
+        sum = lane < warps ? scratch[lane] : 0.f;
+        m = lane < warps ? scratch[32 + lane] : 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = mag_max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            m = mag_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+    }
+}
+
+// Eight values from element i of a row on (`left` of them exist); `vec`: 16-byte accesses are allowed.
+__device__ __forceinline__ void load8(float (&v)[8], const float* p, int left, bool vec) {
+    if (vec && left >= 8) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+    }
+}
+__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* p, int left, bool vec) {
+    if (vec && left >= 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? to_float(p[j]) : 0.f;
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8], int left, bool vec) {
+    if (vec && left >= 8) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = v[j];
+    }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8], int left, bool vec) {
+    if (vec && left >= 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = __float2bfloat16_rn(v[j]);
+    }
+}
+// ... rounded to 8 bits (q's rows begin at multiples of 16 bytes)
+__device__ __forceinline__ void store8(int8_t* p, const float (&v)[8], float inverse, int left) {
+    int q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = inverse == 0.f ? 0 : max(-127, min(127, __float2int_rn(__fmul_rn(v[j], inverse))));
+    if (left >= 8) {
+        uint2 w;
+        w.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
+        w.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
+        *reinterpret_cast<uint2*>(p) = w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = (int8_t)q[j];
+    }
 }
 
 struct RowScale {
@@ -34,83 +116,254 @@ __device__ __forceinline__ RowScale row_scale(float m) {
     if (m < kTiny) return {0.f, 0.f};
     return {__fdiv_rn(m, 127.f), __fdiv_rn(127.f, m)};
 }
-__device__ __forceinline__ int to_int8(float v, float inverse) {
-    return inverse == 0.f ? 0 : max(-127, min(127, __float2int_rn(__fmul_rn(v, inverse))));
-}
 
-// 1 / sqrt(mean of t^2 + eps) from the sum of squares; where that left float32 (or nearly vanished in it) `again(f)` sums (t f)^2.
-template <typename Again>
-__device__ __forceinline__ float row_root(float ss, int dim, float eps, Again again) {
-    if (ss > 1e-24f && ss < 1e30f) return rms_scale(ss, dim, eps);
-    const float f = ss > 1.f ? 8.271806125530277e-25f : 1.2089258196146292e+24f;           // 2^-80, 2^80
-    return (float)(1.0 / sqrt((double)again(f) / ((double)f * (double)f) / dim + (double)eps));
-}
+// The row of this thread and its place among the row's threads: (BLOCK) a block's threads have one row, else each warp its own.
+template <bool BLOCK> __device__ __forceinline__ int my_row() { return BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); }
+template <bool BLOCK> __device__ __forceinline__ int my_place() { return BLOCK ? threadIdx.x : threadIdx.x & 31; }
 
-template <typename T>
-__global__ void quantize_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int dim) {
-    __shared__ float scratch[33];
+template <typename T, int V, bool BLOCK>
+__global__ void quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
+                                int dim) {
+    __shared__ float scratch[64];
     pdl_wait();
     pdl_trigger();
-    const T* src = x + (size_t)blockIdx.x * ldx;
-    float m = 0.f;
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) m = mag_max(m, fabsf(to_float(src[i])));
-    const RowScale s = row_scale(block_mag_max(m, scratch));
-    int8_t* dst = q + (size_t)blockIdx.x * ldq;
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) dst[i] = (int8_t)to_int8(to_float(src[i]), s.inverse);
-    if (threadIdx.x == 0) scale[blockIdx.x] = s.scale;
-}
-
-template <typename Ty>
-__global__ void add_rmsnorm_kernel(const float* x, int ldx, const Ty* __restrict__ y, int ldy, float* total /* may be x */,
-                                   int ldt, VecRef gain, float eps, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int dim) {
-    __shared__ float scratch[33];
-    pdl_wait();
-    pdl_trigger();
-    const size_t r = blockIdx.x;
-    auto sum_of = [&](int i) { return y != nullptr ? __fadd_rn(x[r * ldx + i], to_float(y[r * ldy + i])) : x[r * ldx + i]; };
-    float ss = 0.f, m = 0.f;
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) {
-        const float t = sum_of(i);
-        ss = fmaf(t, t, ss);
-    }
-    const float root = row_root(block_sum(ss, scratch), dim, eps, [&](float f) {
-        float again = 0.f;
-        for (int i = threadIdx.x; i < dim; i += blockDim.x) {
-            const float t = __fmul_rn(sum_of(i), f);
-            again = fmaf(t, t, again);
+    const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8;
+    if (r >= rows) return;
+    const T* src = x + (size_t)r * ldx;
+    int8_t* dst = q + (size_t)r * ldq;
+    float v[V][8], m = 0.f, unused = 0.f;
+    if constexpr (V <= MOST_CHUNKS) {
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) load8(v[c], src + at + c * step, dim - at - c * step, vec);
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(v[c][j]));
+            }
+        row_reduce<BLOCK>(unused, m, scratch);
+        const RowScale s = row_scale(m);
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) store8(dst + at + c * step, v[c], s.inverse, dim - at - c * step);
+        if (at == 0) scale[r] = s.scale;
+    } else {
+        for (int i = at; i < dim; i += step) {
+            load8(v[0], src + i, dim - i, vec);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(v[0][j]));
         }
-        return block_sum(again, scratch);
-    });
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) m = mag_max(m, fabsf(__fmul_rn(__fmul_rn(sum_of(i), root), gain[i])));
-    const RowScale s = row_scale(block_mag_max(m, scratch));
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) {
-        const float t = sum_of(i);
-        q[r * ldq + i] = (int8_t)to_int8(__fmul_rn(__fmul_rn(t, root), gain[i]), s.inverse);
-        if (y != nullptr) total[r * ldt + i] = t;
+        row_reduce<BLOCK>(unused, m, scratch);
+        const RowScale s = row_scale(m);
+        for (int i = at; i < dim; i += step) {
+            load8(v[0], src + i, dim - i, vec);
+            store8(dst + i, v[0], s.inverse, dim - i);
+        }
+        if (at == 0) scale[r] = s.scale;
     }
-    if (threadIdx.x == 0) scale[r] = s.scale;
+}
+
+struct NormArgs {
+    const float* x;
+    const void* y;
+    float* total;           // may be x
+    VecRef gain;
+    int8_t* q;
+    float* scale;
+    int ldx, ldy, ldt, ldq, rows, dim;
+    float eps;
+    bool x_vec, y_vec, t_vec, g_vec;
+};
+
+// w = t gain from t's eight values
+__device__ __forceinline__ void times_gain(float (&w)[8], const NormArgs& a, int i) {
+    float g[8];
+    if (a.gain.dtype == JLLM_F32) load8(g, static_cast<const float*>(a.gain.p) + i, a.dim - i, a.g_vec);
+    else load8(g, static_cast<const __nv_bfloat16*>(a.gain.p) + i, a.dim - i, a.g_vec);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __fmul_rn(w[j], g[j]);
+}
+
+template <typename Ty, int V, bool BLOCK>
+__global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
+    __shared__ float scratch[64];
+    pdl_wait();
+    pdl_trigger();
+    const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8, dim = a.dim;
+    if (r >= a.rows) return;
+    const float* x = a.x + (size_t)r * a.ldx;
+    const Ty* y = a.y ? static_cast<const Ty*>(a.y) + (size_t)r * a.ldy : nullptr;
+    float* total = a.y ? a.total + (size_t)r * a.ldt : nullptr;
+    int8_t* dst = a.q + (size_t)r * a.ldq;
+    // t = x + y of the chunk at i, left in `total`
+    auto fetch = [&](float (&t)[8], int i) {
+        load8(t, x + i, dim - i, a.x_vec);
+        if (y) {
+            float b[8];
+            load8(b, y + i, dim - i, a.y_vec);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], b[j]);
+        }
+    };
+    float ss = 0.f, m = 0.f;
+    auto take = [&](float (&t)[8], int i) {      // t becomes w
+        if (y) store8(total + i, t, dim - i, a.t_vec);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(t[j], t[j], ss);
+        times_gain(t, a, i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(t[j]));
+    };
+    constexpr bool HELD = V <= MOST_CHUNKS;
+    float w[HELD ? V : 1][8];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) fetch(w[c], at + c * step);
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) take(w[c], at + c * step);
+    } else {
+        for (int i = at; i < dim; i += step) {
+            fetch(w[0], i);
+            take(w[0], i);
+        }
+    }
+    row_reduce<BLOCK>(ss, m, scratch);
+    const float* t_row = y ? total : x;          // (from here on t is read back: the thread's own writes)
+    const bool t_vec = y ? a.t_vec : a.x_vec;
+    if (ss > 1e-24f && ss < 1e30f && m >= kTiny && m < 1e30f) {
+        const float inverse = __fdiv_rn(127.f, m);
+        if constexpr (HELD) {
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+                if (at + c * step < dim) store8(dst + at + c * step, w[c], inverse, dim - at - c * step);
+        } else {
+            for (int i = at; i < dim; i += step) {
+                load8(w[0], t_row + i, dim - i, t_vec);
+                times_gain(w[0], a, i);
+                store8(dst + i, w[0], inverse, dim - i);
+            }
+        }
+        if (at == 0) a.scale[r] = __fmul_rn(rms_scale(ss, dim, a.eps), __fdiv_rn(m, 127.f));
+        return;
+    }
+    // Squares or products left float32, or vanished in it, or the row is zeros or not numbers: once more with t scaled by powers of two.
+    const float fs = ss < 1e30f ? (ss > 1e-24f ? 1.f : 1.2089258196146292e+24f) : 8.271806125530277e-25f;               // 2^80, 2^-80
+    const float fm = m < 1e30f ? (m >= kTiny ? 1.f : 1.2676506002282294e+30f) : 7.52316384526264e-37f;                 // 2^100, 2^-120
+    ss = m = 0.f;
+    for (int i = at; i < dim; i += step) {
+        float t[8], u[8];
+        load8(t, t_row + i, dim - i, t_vec);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            u[j] = __fmul_rn(t[j], fs);
+            ss = fmaf(u[j], u[j], ss);
+            t[j] = __fmul_rn(t[j], fm);
+        }
+        times_gain(t, a, i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(t[j]));
+    }
+    row_reduce<BLOCK>(ss, m, scratch);
+    const double root = 1.0 / sqrt((double)ss / ((double)fs * (double)fs) / dim + (double)a.eps);
+    const double most = root * ((double)m / (double)fm);             // (NaN where the row has one, or is 0 / 0)
+    const bool whole = ss < INFINITY && most < (double)INFINITY;
+    const float inverse = whole && most >= (double)kTiny ? __fdiv_rn(127.f, m) : 0.f;
+    for (int i = at; i < dim; i += step) {
+        float t[8];
+        load8(t, t_row + i, dim - i, t_vec);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], fm);
+        times_gain(t, a, i);
+        store8(dst + i, t, inverse, dim - i);
+    }
+    if (at == 0) a.scale[r] = !whole ? __int_as_float(0x7fffffff) : (inverse == 0.f ? 0.f : (float)(most / 127.0));
 }
 
 template <typename T>
-__global__ void values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ scale, T* __restrict__ out, int ldo, int dim) {
+__global__ void __launch_bounds__(256)
+values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ scale, T* __restrict__ out, int ldo, bool vec, int rows, int dim) {
     pdl_wait();
     pdl_trigger();
-    const size_t r = blockIdx.x;
-    const float s = scale[r];
-    for (int i = threadIdx.x; i < dim; i += blockDim.x) out[r * ldo + i] = from_float<T>(__fmul_rn((float)q[r * ldq + i], s));
+    const int chunks = (dim + 7) / 8;
+    const long long total = (long long)rows * chunks;
+    for (long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x; item < total; item += (long long)gridDim.x * blockDim.x) {
+        int r, c;
+        split_item(item, chunks, r, c);
+        const int left = dim - c * 8;
+        const int8_t* src = q + (size_t)r * ldq + c * 8;
+        const float s = scale[r];
+        float v[8];
+        if (left >= 8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = __fmul_rn((float)(int8_t)(w.x >> (8 * j)), s);
+                v[4 + j] = __fmul_rn((float)(int8_t)(w.y >> (8 * j)), s);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < left ? __fmul_rn((float)src[j], s) : 0.f;
+        }
+        store8(out + (size_t)r * ldo + c * 8, v, left, vec);
+    }
+}
+
+// The threads that share a row of `dim` values and the chunks each holds: two where 256 threads are enough, else four.
+struct RowCut {
+    int threads, chunks;
+};
+RowCut row_cut(int dim) {
+    const int all = (dim + 7) / 8;
+    if (all <= 32) return {32, 1};
+    if (all <= 64) return {32, 2};
+    const int chunks = all <= 512 ? 2 : MOST_CHUNKS;
+    const int threads = ((all + chunks - 1) / chunks + 31) / 32 * 32;
+    return threads <= MOST_THREADS ? RowCut{threads, chunks} : RowCut{MOST_THREADS, MOST_CHUNKS + 1};
+}
+constexpr int WARPS = 4;       // rows of a block whose warps have one each
+
+bool vec16(const void* p, int ld, int size) { return (uintptr_t)p % 16 == 0 && (long long)ld * size % 16 == 0; }
+
+// GO(V, BLOCK): the launch for a row's cut
+#define JLLM_ROW_CUT(cut)                                                                    \
+    if ((cut).threads == 32 && (cut).chunks == 1) JLLM_GO(1, false);                         \
+    else if ((cut).threads == 32) JLLM_GO(2, false);                                         \
+    else if ((cut).chunks == 2) JLLM_GO(2, true);                                            \
+    else if ((cut).chunks == MOST_CHUNKS) JLLM_GO(MOST_CHUNKS, true);                        \
+    else JLLM_GO(MOST_CHUNKS + 1, true)
+
+template <typename T>
+void launch_quantize(const void* x, int ldx, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
+    const RowCut cut = row_cut(dim);
+    const bool vec = vec16(x, ldx, sizeof(T));
+#define JLLM_GO(V, BLOCK)                                                                                                             \
+    jllm_launch(quantize_kernel<T, V, BLOCK>, dim3(BLOCK ? rows : (rows + WARPS - 1) / WARPS), dim3(BLOCK ? cut.threads : 32 * WARPS), 0, \
+                stream, LAUNCH_DEPENDENT, static_cast<const T*>(x), ldx, vec, q, ldq, scale, rows, dim)
+    JLLM_ROW_CUT(cut);
+#undef JLLM_GO
+}
+template <typename Ty>
+void launch_norm(const NormArgs& a, cudaStream_t stream) {
+    const RowCut cut = row_cut(a.dim);
+#define JLLM_GO(V, BLOCK)                                                                                                                  \
+    jllm_launch(add_rmsnorm_kernel<Ty, V, BLOCK>, dim3(BLOCK ? a.rows : (a.rows + WARPS - 1) / WARPS), dim3(BLOCK ? cut.threads : 32 * WARPS), 0, \
+                stream, LAUNCH_DEPENDENT, a)
+    JLLM_ROW_CUT(cut);
+#undef JLLM_GO
 }
 
 }  // namespace
 
-// x [rows, dim] float32 or bfloat16 (row stride ldx) -> q int8 (row stride ldq), scale [rows].
+// x [rows, dim] float32 or bfloat16 (row stride ldx) -> q int8 (row stride ldq, rows at multiples of 16 bytes), scale [rows].
 JLLM_EXPORT int jllm_quantize_int8(const void* x, int x_dtype, int ldx, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
     JLLM_REQUIRE(rows >= 0 && dim > 0 && ldx >= dim && ldq >= dim, "quantize_int8: rows=%d dim=%d ldx=%d ldq=%d", rows, dim, ldx, ldq);
+    JLLM_REQUIRE(vec16(q, ldq, 1), "quantize_int8: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
     if (rows == 0) return JLLM_OK;
-    if (x_dtype == JLLM_F32)
-        jllm_launch(quantize_kernel<float>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, (const float*)x, ldx, q, ldq, scale, dim);
-    else
-        jllm_launch(quantize_kernel<__nv_bfloat16>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, (const __nv_bfloat16*)x, ldx, q, ldq,
-                    scale, dim);
+    if (x_dtype == JLLM_F32) launch_quantize<float>(x, ldx, q, ldq, scale, rows, dim, stream);
+    else launch_quantize<__nv_bfloat16>(x, ldx, q, ldq, scale, rows, dim, stream);
     return jllm_check_launch("quantize_int8");
 }
 
@@ -120,14 +373,12 @@ JLLM_EXPORT int jllm_add_rmsnorm_int8(const float* x, int ldx, const void* y, in
                                       int gain_dtype, float eps, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
     JLLM_REQUIRE(rows >= 0 && dim > 0 && ldx >= dim && ldq >= dim && (!y || (ldy >= dim && ldt >= dim && total)),
                  "add_rmsnorm_int8: rows=%d dim=%d ldx=%d ldy=%d ldt=%d ldq=%d", rows, dim, ldx, ldy, ldt, ldq);
+    JLLM_REQUIRE(vec16(q, ldq, 1), "add_rmsnorm_int8: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
     if (rows == 0) return JLLM_OK;
-    const VecRef g{gain, gain_dtype};
-    if (y_dtype == JLLM_F32)
-        jllm_launch(add_rmsnorm_kernel<float>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, x, ldx, (const float*)y, ldy, total, ldt, g, eps,
-                    q, ldq, scale, dim);
-    else
-        jllm_launch(add_rmsnorm_kernel<__nv_bfloat16>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, x, ldx, (const __nv_bfloat16*)y, ldy,
-                    total, ldt, g, eps, q, ldq, scale, dim);
+    const NormArgs a{x, y, total, VecRef{gain, gain_dtype}, q, scale, ldx, ldy, ldt, ldq, rows, dim, eps, vec16(x, ldx, 4),
+                     vec16(y, ldy, y_dtype == JLLM_F32 ? 4 : 2), vec16(total, ldt, 4), (uintptr_t)gain % 16 == 0};
+    if (y_dtype == JLLM_F32) launch_norm<float>(a, stream);
+    else launch_norm<__nv_bfloat16>(a, stream);
     return jllm_check_launch("add_rmsnorm_int8");
 }
 
@@ -135,10 +386,15 @@ JLLM_EXPORT int jllm_add_rmsnorm_int8(const float* x, int ldx, const void* y, in
 JLLM_EXPORT int jllm_int8_values(const int8_t* q, int ldq, const float* scale, void* out, int out_dtype, int ldo, int rows, int dim,
                                  cudaStream_t stream) {
     JLLM_REQUIRE(rows >= 0 && dim > 0 && ldq >= dim && ldo >= dim, "int8_values: rows=%d dim=%d ldq=%d ldo=%d", rows, dim, ldq, ldo);
+    JLLM_REQUIRE(vec16(q, ldq, 1), "int8_values: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
     if (rows == 0) return JLLM_OK;
+    const long long items = (long long)rows * ((dim + 7) / 8), most = (long long)(jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 1) * 16;
+    const int blocks = (int)((items + 255) / 256 > most ? most : (items + 255) / 256);
     if (out_dtype == JLLM_F32)
-        jllm_launch(values_kernel<float>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (float*)out, ldo, dim);
+        jllm_launch(values_kernel<float>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (float*)out, ldo, vec16(out, ldo, 4),
+                    rows, dim);
     else
-        jllm_launch(values_kernel<__nv_bfloat16>, dim3(rows), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (__nv_bfloat16*)out, ldo, dim);
+        jllm_launch(values_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (__nv_bfloat16*)out, ldo,
+                    vec16(out, ldo, 2), rows, dim);
     return jllm_check_launch("int8_values");
 }
