@@ -12,6 +12,7 @@
 // k blocks of 128 weight rows. Many tokens (`pair`): two SMs to a tile of 256 tokens x 64, 128 or 256 weight rows. Every wait is bounded
 // and raises the products' error word (codes 31-33 swap, 34-36 pair).
 #include "gemm_epilogue.cuh"
+#include "int8_view.h"
 
 namespace {
 
@@ -668,14 +669,17 @@ int choose(int M, int N, int k_blocks, int sms) {
 
 }  // namespace
 
-// a [M, K] int8 (row stride lda, a multiple of 16), w_packed: ops.pack_int8 of the [N, K] weight, scale_w filled up to a multiple of 128
-// and 16-byte aligned, out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a cluster (swap), minus the
-// weight rows of a tile (pair), 0 as the sizes have it.
-JLLM_EXPORT int jllm_gemm_int8(const int8_t* a, int lda, const float* scale_a, const int8_t* w_packed, const float* scale_w, int k_blocks,
-                               const void* bias, int bias_dtype, void* out, int out_dtype, int ldo, int accumulate, int M, int N, int K,
-                               int swiglu_word, int cut, cudaStream_t stream) {
+// `rows`: the int8 activations [M, K], their rows at multiples of 16 bytes; `weight`: ops.pack_int8 of the [N, K] weight, its scales filled
+// up to a multiple of 128 and 16-byte aligned; out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a
+// cluster (swap), minus the weight rows of a tile (pair), 0 as the sizes have it.
+JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo,
+                               int accumulate, int swiglu_word, int cut, cudaStream_t stream) {
+    const int8_t *a = rows->data, *w_packed = weight->data;
+    const float *scale_a = rows->scale, *scale_w = weight->scale;
+    const int M = rows->rows, K = rows->cols, lda = rows->stride, N = weight->rows, k_blocks = weight->stride;
     const GluArgs glu = glu_args(swiglu_word, nullptr);
-    JLLM_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= MAX_K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d)", M, N, K, MAX_K);
+    JLLM_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= MAX_K && weight->cols == K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d) against a weight of %d",
+                 M, N, K, MAX_K, weight->cols);
     JLLM_REQUIRE(lda >= K && lda % 16 == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)w_packed % 16) == 0 && ((uintptr_t)scale_w % 16) == 0,
                  "gemm_int8: rows and weights begin at multiples of 16 bytes (lda=%d, K=%d)", lda, K);
     JLLM_REQUIRE(k_blocks == (K + BK - 1) / BK, "gemm_int8: the packed weight has %d k blocks, K=%d needs %d", k_blocks, K, (K + BK - 1) / BK);

@@ -13,6 +13,7 @@
 // a row's sum has one order whatever else is in the batch. Rows of up to 512 values are a warp's each, wider ones a block's, beyond 32,768
 // values (`wide`) a thread's chunks are fetched again behind the reduction.
 #include "head_rotate.cuh"
+#include "int8_view.h"
 
 namespace {
 
@@ -357,44 +358,54 @@ void launch_norm(const NormArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-// x [rows, dim] float32 or bfloat16 (row stride ldx) -> q int8 (row stride ldq, rows at multiples of 16 bytes), scale [rows].
-JLLM_EXPORT int jllm_quantize_int8(const void* x, int x_dtype, int ldx, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
-    JLLM_REQUIRE(rows >= 0 && dim > 0 && ldx >= dim && ldq >= dim, "quantize_int8: rows=%d dim=%d ldx=%d ldq=%d", rows, dim, ldx, ldq);
-    JLLM_REQUIRE(vec16(q, ldq, 1), "quantize_int8: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
-    if (rows == 0) return JLLM_OK;
-    if (x_dtype == JLLM_F32) launch_quantize<float>(x, ldx, q, ldq, scale, rows, dim, stream);
-    else launch_quantize<__nv_bfloat16>(x, ldx, q, ldq, scale, rows, dim, stream);
+// What all three ask of the int8 rows
+#define JLLM_REQUIRE_ROWS(name, v)                                                                                                 \
+    JLLM_REQUIRE((v).rows >= 0 && (v).cols > 0 && (v).stride >= (v).cols && vec16((v).data, (v).stride, 1),                         \
+                 name ": %d int8 rows of %d values begin at multiples of 16 bytes (stride %d)", (v).rows, (v).cols, (v).stride)
+
+// x [rows, cols] float32 or bfloat16 (row stride ldx) -> the int8 rows of `view`.
+JLLM_EXPORT int jllm_quantize_int8(const void* x, int x_dtype, int ldx, const Int8View* view, cudaStream_t stream) {
+    const Int8View v = *view;
+    JLLM_REQUIRE_ROWS("quantize_int8", v);
+    JLLM_REQUIRE(ldx >= v.cols, "quantize_int8: ldx=%d for %d values", ldx, v.cols);
+    if (v.rows == 0) return JLLM_OK;
+    int8_t* q = const_cast<int8_t*>(v.data);
+    float* scale = const_cast<float*>(v.scale);
+    if (x_dtype == JLLM_F32) launch_quantize<float>(x, ldx, q, v.stride, scale, v.rows, v.cols, stream);
+    else launch_quantize<__nv_bfloat16>(x, ldx, q, v.stride, scale, v.rows, v.cols, stream);
     return jllm_check_launch("quantize_int8");
 }
 
-// t = x + y (y null: t = x, and `total` is not written), v = t / sqrt(mean(t^2) + eps) * gain as int8 rows; x, total float32, y float32
-// or bfloat16; total may be x.
+// t = x + y (y null: t = x, and `total` is not written), v = t / sqrt(mean(t^2) + eps) * gain as the int8 rows of `view`; x, total
+// float32, y float32 or bfloat16; total may be x.
 JLLM_EXPORT int jllm_add_rmsnorm_int8(const float* x, int ldx, const void* y, int y_dtype, int ldy, float* total, int ldt, const void* gain,
-                                      int gain_dtype, float eps, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
-    JLLM_REQUIRE(rows >= 0 && dim > 0 && ldx >= dim && ldq >= dim && (!y || (ldy >= dim && ldt >= dim && total)),
-                 "add_rmsnorm_int8: rows=%d dim=%d ldx=%d ldy=%d ldt=%d ldq=%d", rows, dim, ldx, ldy, ldt, ldq);
-    JLLM_REQUIRE(vec16(q, ldq, 1), "add_rmsnorm_int8: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
-    if (rows == 0) return JLLM_OK;
-    const NormArgs a{x, y, total, VecRef{gain, gain_dtype}, q, scale, ldx, ldy, ldt, ldq, rows, dim, eps, vec16(x, ldx, 4),
-                     vec16(y, ldy, y_dtype == JLLM_F32 ? 4 : 2), vec16(total, ldt, 4), (uintptr_t)gain % 16 == 0};
+                                      int gain_dtype, float eps, const Int8View* view, cudaStream_t stream) {
+    const Int8View v = *view;
+    JLLM_REQUIRE_ROWS("add_rmsnorm_int8", v);
+    JLLM_REQUIRE(ldx >= v.cols && (!y || (ldy >= v.cols && ldt >= v.cols && total)), "add_rmsnorm_int8: ldx=%d ldy=%d ldt=%d for %d values", ldx,
+                 ldy, ldt, v.cols);
+    if (v.rows == 0) return JLLM_OK;
+    const NormArgs a{x, y, total, VecRef{gain, gain_dtype}, const_cast<int8_t*>(v.data), const_cast<float*>(v.scale), ldx, ldy, ldt, v.stride,
+                     v.rows, v.cols, eps, vec16(x, ldx, 4), vec16(y, ldy, y_dtype == JLLM_F32 ? 4 : 2), vec16(total, ldt, 4),
+                     (uintptr_t)gain % 16 == 0};
     if (y_dtype == JLLM_F32) launch_norm<float>(a, stream);
     else launch_norm<__nv_bfloat16>(a, stream);
     return jllm_check_launch("add_rmsnorm_int8");
 }
 
 // out[r, j] = q[r, j] * scale[r], float32 or bfloat16.
-JLLM_EXPORT int jllm_int8_values(const int8_t* q, int ldq, const float* scale, void* out, int out_dtype, int ldo, int rows, int dim,
-                                 cudaStream_t stream) {
-    JLLM_REQUIRE(rows >= 0 && dim > 0 && ldq >= dim && ldo >= dim, "int8_values: rows=%d dim=%d ldq=%d ldo=%d", rows, dim, ldq, ldo);
-    JLLM_REQUIRE(vec16(q, ldq, 1), "int8_values: int8 rows begin at multiples of 16 bytes (ldq=%d)", ldq);
-    if (rows == 0) return JLLM_OK;
-    const long long items = (long long)rows * ((dim + 7) / 8), most = (long long)(jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 1) * 16;
+JLLM_EXPORT int jllm_int8_values(const Int8View* view, void* out, int out_dtype, int ldo, cudaStream_t stream) {
+    const Int8View v = *view;
+    JLLM_REQUIRE_ROWS("int8_values", v);
+    JLLM_REQUIRE(ldo >= v.cols, "int8_values: ldo=%d for %d values", ldo, v.cols);
+    if (v.rows == 0) return JLLM_OK;
+    const long long items = (long long)v.rows * ((v.cols + 7) / 8), most = (long long)(jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 1) * 16;
     const int blocks = (int)((items + 255) / 256 > most ? most : (items + 255) / 256);
     if (out_dtype == JLLM_F32)
-        jllm_launch(values_kernel<float>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (float*)out, ldo, vec16(out, ldo, 4),
-                    rows, dim);
+        jllm_launch(values_kernel<float>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale, (float*)out, ldo,
+                    vec16(out, ldo, 4), v.rows, v.cols);
     else
-        jllm_launch(values_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, q, ldq, scale, (__nv_bfloat16*)out, ldo,
-                    vec16(out, ldo, 2), rows, dim);
+        jllm_launch(values_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale,
+                    (__nv_bfloat16*)out, ldo, vec16(out, ldo, 2), v.rows, v.cols);
     return jllm_check_launch("int8_values");
 }

@@ -212,10 +212,10 @@ class _Signatures:
     jllm_delta_recurrent = [P, I, I, I, I, I, P, P, I, F, P, I, P, P, P, P, P, I, P, I, F, P, I, I, I, I, I, P]
     jllm_delta_chunked = [P, I, I, I, I, I, P, P, I, F, P, I, P, P, P, P, P, P, P, P, I, P, I, F, P, I, I, I, I, I, I, P]
     jllm_sample = [P, I, I, I, P, P, P, P, P, P, P]
-    jllm_quantize_int8 = [P, I, I, P, I, P, I, I, P]
-    jllm_add_rmsnorm_int8 = [P, I, P, I, I, P, I, P, I, F, P, I, P, I, I, P]
-    jllm_int8_values = [P, I, P, P, I, I, I, I, P]
-    jllm_gemm_int8 = [P, I, P, P, P, I, P, I, P, I, I, I, I, I, I, I, I, P]
+    jllm_quantize_int8 = [P, I, I, P, P]
+    jllm_add_rmsnorm_int8 = [P, I, P, I, I, P, I, P, I, F, P, P]
+    jllm_int8_values = [P, P, I, I, P]
+    jllm_gemm_int8 = [P, P, P, I, P, I, I, I, I, I, P]
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -1559,27 +1559,28 @@ def _refuse(name, why):
     raise KernelError(f"{name}: {why}")
 
 
+class _Int8View(ctypes.Structure):          # (Int8View in int8_view.h)
+    _fields_ = [("data", c_void_p), ("scale", c_void_p), ("rows", c_int), ("cols", c_int), ("stride", c_int)]
+
+
 class Int8Rows:
     """Rows of activations in 8-bit integers: row r stands for data[r] * scale[r]. data int8 [rows, cols], its rows beginning at
     multiples of 16 bytes (`int8_rows` makes such); scale float32 [rows]. A slice of rows is `rows8[lo:hi]`."""
-    __slots__ = ("data", "scale", "rows", "cols", "stride", "address", "scale_address", "on_gpu")
+    __slots__ = ("data", "scale", "rows", "cols", "shape", "stride", "on_gpu", "_view", "view")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor):
         if data.dtype != torch.int8 or scale.dtype != torch.float32 or data.dim() != 2 or scale.shape != data.shape[:1]:
             _refuse("Int8Rows", f"int8 data [rows, cols] and a float32 scale for each row, got {data.dtype} {tuple(data.shape)} and {scale.dtype} {tuple(scale.shape)}")
         self.data, self.scale = data, scale
-        self.rows, self.cols = data.shape
-        self.stride, self.address, self.scale_address = data.stride(0), data.data_ptr(), scale.data_ptr()
-        self.on_gpu = data.is_cuda and scale.is_cuda
-        if self.rows == 1:                       # (a single row's stride says nothing)
-            self.stride = max(self.stride, -(-self.cols // 16) * 16)
-        if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or self.stride < self.cols or self.stride % 16 or self.address % 16
-                or (self.rows > 1 and scale.stride(0) != 1)):
-            _refuse("Int8Rows", f"rows of neighbouring values that begin at multiples of 16 bytes, got strides {data.stride()}, {scale.stride()} at {self.address:#x}")
-
-    @property
-    def shape(self):
-        return (self.rows, self.cols)
+        self.rows, self.cols = self.shape = tuple(data.shape)
+        self.on_gpu = data.is_cuda and scale.is_cuda and data.device == scale.device
+        self.stride = data.stride(0) if self.rows > 1 else -(-self.cols // 16) * 16          # (a single row's stride says nothing)
+        if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or self.stride < self.cols or self.stride % 16 or data.data_ptr() % 16
+                or (self.rows > 1 and scale.stride(0) != 1) or max(self.stride, self.rows) > 0x7fffffff):
+            _refuse("Int8Rows", f"rows of neighbouring values that begin at multiples of 16 bytes, got strides {data.stride()}, {scale.stride()} at {data.data_ptr():#x}")
+        # what the launchers are told of the rows, laid out once
+        self._view = _Int8View(data.data_ptr(), scale.data_ptr(), self.rows, self.cols, self.stride)
+        self.view = ctypes.addressof(self._view)
 
     def __getitem__(self, rows: slice) -> "Int8Rows":
         if not isinstance(rows, slice):
@@ -1595,9 +1596,13 @@ def int8_rows(rows: int, cols: int, device) -> Int8Rows:
 
 def _row_stride(name, what, t, shape):
     """The row stride of a [rows, cols] matrix with neighbouring values on the GPU."""
-    if t.shape != shape or not t.is_cuda or (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
-        _refuse(name, f"{what} is a {tuple(shape)} matrix of neighbouring values on the GPU, got {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    return t.stride(0) if shape[0] > 1 else shape[1]
+    if t.shape == shape and t.is_cuda:
+        down, along = t.stride()
+        if shape[0] <= 1:
+            down = shape[1]
+        if (along == 1 or shape[1] == 1) and shape[1] <= down <= 0x7fffffff:
+            return down
+    _refuse(name, f"{what} is a {shape} matrix of neighbouring values on the GPU, got {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 def quantize_int8(x: torch.Tensor, out: Int8Rows) -> None:
@@ -1606,39 +1611,40 @@ def quantize_int8(x: torch.Tensor, out: Int8Rows) -> None:
     holds an infinity or a NaN zeros with scale NaN (what is computed from it is then NaN)."""
     if x.dtype not in _DT or not out.on_gpu:
         _refuse("quantize_int8", f"float32 or bfloat16 rows and room on the GPU, got {x.dtype} and {out.data.device}")
-    ld = _row_stride("quantize_int8", "x", x, out.shape)
-    _call("jllm_quantize_int8", x.data_ptr(), _DT[x.dtype], ld, out.address, out.stride, out.scale_address, out.rows, out.cols, _stream())
+    _call("jllm_quantize_int8", x.data_ptr(), _DT[x.dtype], _row_stride("quantize_int8", "x", x, out.shape), out.view, _stream())
 
 
 def add_rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, out: Int8Rows, y: torch.Tensor | None = None,
                      total: torch.Tensor | None = None) -> None:
-    """out = rmsnorm(x + y) * gain in 8 bits (as `quantize_int8` has them), total = x + y: the residual's addition, the norm behind it
-    and the rounding in one pass. x float32 [rows, dim]; y float32 or bfloat16 of x's shape, or None (nothing is added, and there is no
-    total); total float32 of x's shape, x itself by default; gain float32 or bfloat16 [dim]."""
+    """out = rmsnorm(x + y) * gain in 8 bits (as `quantize_int8` has them; a row of results below 2^-100 may keep its numbers), total =
+    x + y: the residual's addition, the norm behind it and the rounding in one pass. x float32 [rows, dim]; y float32 or bfloat16 of x's
+    shape, or None (nothing is added, and there is no total); total float32 of x's shape, x itself by default (no other overlap of what
+    is read and written); gain float32 or bfloat16 [dim]."""
     name = "add_rmsnorm_int8"
-    if x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != (out.cols,) or gain.stride(0) != 1 or not gain.is_cuda or not out.on_gpu:
+    if (x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != out.shape[1:] or (gain.stride(0) != 1 and out.cols > 1)
+            or not gain.is_cuda or not out.on_gpu):
         _refuse(name, f"on the GPU, float32 rows and a float32 or bfloat16 gain of {out.cols} values, got {x.dtype} and {gain.dtype} {tuple(gain.shape)}")
     ldx = _row_stride(name, "x", x, out.shape)
-    ldy = ldt = 0
     if y is None:
         if total is not None:
             _refuse(name, "a total goes with a y to add")
+        _call("jllm_add_rmsnorm_int8", x.data_ptr(), ldx, 0, BF16, 0, 0, 0, gain.data_ptr(), _DT[gain.dtype], eps, out.view, _stream())
+        return
+    if total is None:
+        total, ldt = x, ldx
     else:
-        total = x if total is None else total
-        if y.dtype not in _DT or total.dtype != torch.float32:
-            _refuse(name, f"y is float32 or bfloat16 and the total float32, got {y.dtype} and {total.dtype}")
-        ldy, ldt = _row_stride(name, "y", y, out.shape), _row_stride(name, "the total", total, out.shape)
-    _call("jllm_add_rmsnorm_int8", x.data_ptr(), ldx, _p(y), _DT[y.dtype] if y is not None else BF16, ldy, _p(total), ldt, gain.data_ptr(),
-          _DT[gain.dtype], float(eps), out.address, out.stride, out.scale_address, out.rows, out.cols, _stream())
+        ldt = _row_stride(name, "the total", total, out.shape)
+    if y.dtype not in _DT or total.dtype != torch.float32:
+        _refuse(name, f"y is float32 or bfloat16 and the total float32, got {y.dtype} and {total.dtype}")
+    _call("jllm_add_rmsnorm_int8", x.data_ptr(), ldx, y.data_ptr(), _DT[y.dtype], _row_stride(name, "y", y, out.shape), total.data_ptr(), ldt,
+          gain.data_ptr(), _DT[gain.dtype], eps, out.view, _stream())
 
 
 def int8_values(rows8: Int8Rows, out: torch.Tensor) -> torch.Tensor:
     """out = the values that the rows stand for, data * scale, float32 or bfloat16; returns out."""
     if out.dtype not in _DT or not rows8.on_gpu:
         _refuse("int8_values", f"float32 or bfloat16 values and rows on the GPU, got {out.dtype} and {rows8.data.device}")
-    ld = _row_stride("int8_values", "out", out, rows8.shape)
-    _call("jllm_int8_values", rows8.address, rows8.stride, rows8.scale_address, out.data_ptr(), _DT[out.dtype], ld, rows8.rows, rows8.cols,
-          _stream())
+    _call("jllm_int8_values", rows8.view, out.data_ptr(), _DT[out.dtype], _row_stride("int8_values", "out", out, rows8.shape), _stream())
     return out
 
 
@@ -1649,16 +1655,14 @@ class PackedInt8:
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, glu: bool = False):
         self.data, self.scales, self.rows, self.cols, self.glu = data, scales, rows, cols, glu
-        self.tiles, self.k_blocks = data.shape[0], data.shape[1]
-        self.address, self.scale_address, self.on_gpu = data.data_ptr(), scales.data_ptr(), data.is_cuda and scales.is_cuda
+        self.shape, self.tiles, self.k_blocks = (rows, cols), data.shape[0], data.shape[1]
+        self.on_gpu = data.is_cuda and scales.is_cuda and data.device == scales.device
+        self._view = _Int8View(data.data_ptr(), scales.data_ptr(), rows, cols, self.k_blocks)
+        self.view = ctypes.addressof(self._view)
 
     @property
     def scale(self) -> torch.Tensor:
         return self.scales[:self.rows]
-
-    @property
-    def shape(self):
-        return (self.rows, self.cols)
 
     def unpack(self) -> torch.Tensor:
         """The [rows, cols] integers again, in the order they were packed in."""
@@ -1709,14 +1713,16 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
     no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. `cut` (tests): the blocks of a cluster that share 128
     weight rows, or minus the weight rows of a tile of 256 tokens; 0: as the sizes have it."""
     name = "gemm_int8"
-    word = glu_kind(swiglu)
-    if isinstance(swiglu, GluUnits) or bool(word) != w.glu:
+    word = glu_kind(swiglu) if swiglu else 0
+    if bool(word) != w.glu or isinstance(swiglu, GluUnits):
         _refuse(name, "a gated unit without weights of its own goes with a weight packed for it, and only with one")
     if a.cols != w.cols or out.dtype not in _DT or not (a.on_gpu and w.on_gpu):
         _refuse(name, f"rows of {w.cols} values and a float32 or bfloat16 result on the GPU, got {a.cols} and {out.dtype}")
-    ldo = _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows))
-    if bias is not None and (bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_cuda or bias.stride(0) != 1):
-        _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
-    _call("jllm_gemm_int8", a.address, a.stride, a.scale_address, w.address, w.scale_address, w.k_blocks, _p(bias),
-          _DT[bias.dtype] if bias is not None else F32, out.data_ptr(), _DT[out.dtype], ldo, int(accumulate), a.rows, w.rows, w.cols, word,
-          int(cut), _stream())
+    if bias is None:
+        b, b_dtype = 0, F32
+    else:
+        if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_cuda or (bias.stride(0) != 1 and w.rows > 1):
+            _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
+        b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
+    _call("jllm_gemm_int8", a.view, w.view, b, b_dtype, out.data_ptr(), _DT[out.dtype],
+          _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows)), int(accumulate), word, cut, _stream())
