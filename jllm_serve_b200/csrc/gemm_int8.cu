@@ -43,11 +43,19 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, ui
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr)
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -96,6 +104,7 @@ template <typename Tout>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ SwapArgs g, Tout* __restrict__ out) {
     extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(16) float token_scales[256];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
     const int stages = g.stages, blocks = g.blocks, share = g.share;
@@ -201,6 +210,9 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const float b = g.has_bias && n < g.N ? g.bias[n] : 0.f;
         pdl_wait();          // the token scales, and what is added into, were written by the kernels before
         pdl_trigger();
+        // (into shared memory while the weights come: asked for in front of every store they were 1 us for 8 tokens)
+        for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < g.M ? g.scale_a[i] : 0.f;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
         ok = mbar_wait(acc_bar, 0, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
@@ -211,60 +223,105 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 // of block p's blocks - 1 parts this block's is number `rank`, or rank - 1 if p is below it
                 const uint32_t dst = in_block(base + parts_at + (uint32_t)(rank - (rank > p ? 1 : 0)) * part_bytes + (uint32_t)row * 16, p);
                 const uint32_t bar = in_block(parts_bar, p);
-                for (int t = t0; t < t1; t += 8) {
-                    uint32_t v[8];
-                    tmem_ld_x8(taddr + t, v);
+                auto send = [&](auto& v, int t) {
+                    tmem_ld(taddr + t, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
+                    for (int q = 0; q < (int)(sizeof(v) / 16); ++q)
                         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
                                      ::"r"(dst + (uint32_t)((t - t0) / 4 + q) * 2048u), "r"(v[4 * q]), "r"(v[4 * q + 1]), "r"(v[4 * q + 2]),
                                      "r"(v[4 * q + 3]), "r"(bar)
                                      : "memory");
-                }
+                };
+                int t = t0;
+                uint32_t v16[16], v8[8];
+                for (; t + 16 <= t1; t += 16) send(v16, t);
+                if (t < t1) send(v8, t);
             }
         if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag));
         if (ok) {
             const uint8_t* parts = aligned + parts_at + (size_t)row * 16;
-            for (int t = mine; t < mine_end; t += 8) {
-                uint32_t sum[8];
-                tmem_ld_x8(taddr + t, sum);
-                float sa[8], old[8], v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sa[j] = t + j < g.M ? g.scale_a[t + j] : 0.f;
-                    old[j] = g.accumulate == EPI_ADD && n < g.N && t + j < g.M ? to_float(out[(size_t)(t + j) * g.ldo + n]) : 0.f;
-                }
+            // Results leave 16 bytes a lane: a warp parks its 32 weight rows x J tokens in the ring (idle by now: every MMA is done) and takes
+            // them back token by token. A lane that stores its own values stores 2 bytes of every token's row, with all that a store costs.
+            Tout* park = reinterpret_cast<Tout*>(aligned + (size_t)quad * 4096);
+            const int width = g.glu ? 16 : 32, column = g.glu ? (tile * 128 + quad * 32) >> 1 : tile * 128 + quad * 32;
+            const bool vec = tile * 128 + quad * 32 + 32 <= g.N && ((uintptr_t)out & 15u) == 0 && (((size_t)g.ldo * sizeof(Tout)) & 15u) == 0;
+            auto finish = [&](auto& sum, int t) {
+                constexpr int J = sizeof(sum) / 4, PER = 16 / sizeof(Tout);       // tokens; values of a 16-byte piece
+                tmem_ld(taddr + t, sum);
+                float v[J];
                 tmem_ld_wait();
                 for (int p = 0; p < blocks - 1; ++p) {
                     const uint8_t* src = parts + (size_t)p * part_bytes + (size_t)((t - mine) / 4) * 2048;
-                    const uint4 x = *reinterpret_cast<const uint4*>(src), y = *reinterpret_cast<const uint4*>(src + 2048);
-                    sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w, sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
-                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = scaled(sum[j], sa[j], sw);
-                if (g.glu) {
-                    // rows come in blocks of 16: 8 gate rows, then the 8 up rows of the same hidden units
-                    const int unit = (n >> 4) * 8 + (n & 7);
-                    float other[8], units[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(0xffffffffu, v[j], 8);
-                    if ((lane & 8) == 0 && n + 8 < g.N) {
-                        glu_units<8>(g.glu.word, [&](int j) { return v[j]; }, [&](int j) { return other[j]; }, 1.f, units);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (t + j < g.M) out[(size_t)(t + j) * g.ldo + unit] = from_float<Tout>(units[j]);
+                    for (int q = 0; q < J / 4; ++q) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(src + q * 2048);
+                        sum[4 * q] += x.x, sum[4 * q + 1] += x.y, sum[4 * q + 2] += x.z, sum[4 * q + 3] += x.w;
                     }
-                } else if (n < g.N) {
-                    Tout* dst = out + (size_t)t * g.ldo + n;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (t + j < g.M) {
-                            const float r = epilogue_act(g.has_bias ? __fadd_rn(v[j], b) : v[j], g.accumulate);
-                            dst[(size_t)j * g.ldo] = from_float<Tout>(g.accumulate == EPI_ADD ? __fadd_rn(r, old[j]) : r);
-                        }
                 }
-            }
+#pragma unroll
+                for (int j = 0; j < J; j += 4) {
+                    const float4 sa = *reinterpret_cast<const float4*>(token_scales + t + j);
+                    v[j] = scaled(sum[j], sa.x, sw);
+                    v[j + 1] = scaled(sum[j + 1], sa.y, sw);
+                    v[j + 2] = scaled(sum[j + 2], sa.z, sw);
+                    v[j + 3] = scaled(sum[j + 3], sa.w, sw);
+                }
+                if (g.glu) {
+                    // rows come in blocks of 16, 8 gate rows and the 8 up rows of the same hidden units: the gates' lanes take the first half of
+                    // the tokens, the others the second
+                    const bool up_lane = lane & 8;
+                    float gate[J / 2], up[J / 2], units[J / 2];
+#pragma unroll
+                    for (int j = 0; j < J / 2; ++j) {
+                        const float other = __shfl_xor_sync(0xffffffffu, up_lane ? v[j] : v[J / 2 + j], 8);
+                        gate[j] = up_lane ? other : v[j];
+                        up[j] = up_lane ? v[J / 2 + j] : other;
+                    }
+                    glu_units<J / 2>(g.glu.word, [&](int j) { return gate[j]; }, [&](int j) { return up[j]; }, 1.f, units);
+#pragma unroll
+                    for (int j = 0; j < J / 2; ++j)
+                        park[(up_lane ? J / 2 + j : j) * 16 + (lane >> 4) * 8 + (lane & 7)] = from_float<Tout>(units[j]);
+                } else {
+                    if (g.has_bias)
+#pragma unroll
+                        for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], b);
+                    if (g.accumulate == EPI_RELU2)
+#pragma unroll
+                        for (int j = 0; j < J; ++j) v[j] = epilogue_act(v[j], EPI_RELU2);
+                    if (g.accumulate == EPI_ADD) {
+                        // (all the old values are requested before the first store: a load behind a store through the same pointer would wait)
+                        float old[J];
+#pragma unroll
+                        for (int j = 0; j < J; ++j) old[j] = n < g.N && t + j < g.M ? to_float(out[(size_t)(t + j) * g.ldo + n]) : 0.f;
+#pragma unroll
+                        for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], old[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; ++j) park[j * 32 + lane] = from_float<Tout>(v[j]);
+                }
+                __syncwarp();
+                if (vec) {
+                    const int pieces = width / PER;              // of a token's row: 2, 4 or 8
+                    for (int i = lane; i < J * pieces; i += 32) {
+                        const int j = i / pieces, c = i % pieces * PER;
+                        if (t + j < g.M)
+                            *reinterpret_cast<uint4*>(out + (size_t)(t + j) * g.ldo + column + c) = *reinterpret_cast<const uint4*>(park + j * width + c);
+                    }
+                } else {
+                    const int last = g.glu ? g.N >> 1 : g.N;
+                    for (int i = lane; i < J * width; i += 32) {
+                        const int j = i / width, c = i % width;
+                        if (t + j < g.M && column + c < last) out[(size_t)(t + j) * g.ldo + column + c] = park[i];
+                    }
+                }
+                __syncwarp();
+            };
+            int t = mine;
+            uint32_t sum16[16], sum8[8];
+#pragma unroll 1
+            for (; t + 16 <= mine_end; t += 16) finish(sum16, t);
+            if (t < mine_end) finish(sum8, t);
         } else if (lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 33); }
     }
     tcgen05_fence_before();
