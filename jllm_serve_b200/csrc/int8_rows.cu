@@ -20,29 +20,21 @@ namespace {
 constexpr float kTiny = 7.888609052210118e-31f;      // 2^-100
 constexpr int MOST_CHUNKS = 4, MOST_THREADS = 1024;   // what a row's threads hold: 32,768 values
 
-// The larger of two magnitudes; a NaN stays (fmaxf would drop it).
-__device__ __forceinline__ float mag_max(float a, float b) { return a >= b || a != a ? a : b; }
+// Magnitudes are compared as the bits of |v|: one integer instruction, and a NaN is larger than everything and stays.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Sum and largest magnitude over the threads of a row: a warp, or (BLOCK) the block's warps. `scratch` holds 64 floats.
-template <bool BLOCK>
-__device__ __forceinline__ void row_reduce(float& sum, float& m, float* scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        m = mag_max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
+// Sum and largest magnitude over the threads of a row: a warp, or (BLOCK) the block's warps. `scratch` holds 64 words.
+template <bool BLOCK, bool SUM>
+__device__ __forceinline__ void row_reduce(float& sum, uint32_t& m, uint32_t* scratch) {
+    if constexpr (SUM) sum = warp_sum(sum);
+    m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (BLOCK) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
         __syncthreads();               // (what a reduction in front of this one left has been read)
-        if (lane == 0) scratch[warp] = sum, scratch[32 + warp] = m;
+        if (lane == 0) scratch[warp] = m, scratch[32 + warp] = __float_as_uint(sum);
         __syncthreads();
-        sum = lane < warps ? scratch[lane] : 0.f;
-        m = lane < warps ? scratch[32 + lane] : 0.f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            m = mag_max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        }
+        m = __reduce_max_sync(0xffffffffu, lane < warps ? scratch[lane] : 0u);
+        if constexpr (SUM) sum = warp_sum(lane < warps ? __uint_as_float(scratch[32 + lane]) : 0.f);
     }
 }
 
@@ -92,27 +84,32 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8], in
             if (j < left) p[j] = __float2bfloat16_rn(v[j]);
     }
 }
-// ... rounded to 8 bits (q's rows begin at multiples of 16 bytes)
-__device__ __forceinline__ void store8(int8_t* p, const float (&v)[8], float inverse, int left) {
-    int q[8];
+// Four values rounded to 8 bits. |v * inverse| is at most 127 and a few roundings, so adding 1.5 * 2^23 rounds it to a whole number,
+// half to even, which then stands in the lowest byte (a conversion runs at a quarter of the rate and needs its result clamped).
+__device__ __forceinline__ uint32_t four_int8(const float* v, float inverse) {
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = inverse == 0.f ? 0 : max(-127, min(127, __float2int_rn(__fmul_rn(v[j], inverse))));
+    for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(__fadd_rn(__fmul_rn(v[j], inverse), 12582912.f));
+    const uint32_t q = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+    return inverse == 0.f ? 0u : q;
+}
+// ... eight of them stored (q's rows begin at multiples of 16 bytes)
+__device__ __forceinline__ void store8(int8_t* p, const float (&v)[8], float inverse, int left) {
+    const uint2 w = make_uint2(four_int8(v, inverse), four_int8(v + 4, inverse));
     if (left >= 8) {
-        uint2 w;
-        w.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
-        w.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
         *reinterpret_cast<uint2*>(p) = w;
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < left) p[j] = (int8_t)q[j];
+            if (j < left) p[j] = (int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
     }
 }
 
 struct RowScale {
     float scale, inverse;
 };
-__device__ __forceinline__ RowScale row_scale(float m) {
+__device__ __forceinline__ RowScale row_scale(uint32_t bits) {
+    const float m = __uint_as_float(bits);
     if (!(m < INFINITY)) return {__int_as_float(0x7fffffff), 0.f};
     if (m < kTiny) return {0.f, 0.f};
     return {__fdiv_rn(m, 127.f), __fdiv_rn(127.f, m)};
@@ -125,44 +122,46 @@ template <bool BLOCK> __device__ __forceinline__ int my_place() { return BLOCK ?
 template <typename T, int V, bool BLOCK>
 __global__ void quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
                                 int dim) {
-    __shared__ float scratch[64];
+    __shared__ uint32_t scratch[64];
     pdl_wait();
     pdl_trigger();
     const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8;
     if (r >= rows) return;
     const T* src = x + (size_t)r * ldx;
     int8_t* dst = q + (size_t)r * ldq;
-    float v[V][8], m = 0.f, unused = 0.f;
-    if constexpr (V <= MOST_CHUNKS) {
+    constexpr bool HELD = V <= MOST_CHUNKS;
+    float v[HELD ? V : 1][8], unused = 0.f;
+    uint32_t m = 0;
+    auto look = [&](const float (&c)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, magnitude(c[j]));
+    };
+    if constexpr (HELD) {
 #pragma unroll
         for (int c = 0; c < V; ++c)
             if (at + c * step < dim) load8(v[c], src + at + c * step, dim - at - c * step, vec);
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(v[c][j]));
-            }
-        row_reduce<BLOCK>(unused, m, scratch);
-        const RowScale s = row_scale(m);
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) store8(dst + at + c * step, v[c], s.inverse, dim - at - c * step);
-        if (at == 0) scale[r] = s.scale;
+            if (at + c * step < dim) look(v[c]);
     } else {
         for (int i = at; i < dim; i += step) {
             load8(v[0], src + i, dim - i, vec);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(v[0][j]));
+            look(v[0]);
         }
-        row_reduce<BLOCK>(unused, m, scratch);
-        const RowScale s = row_scale(m);
+    }
+    row_reduce<BLOCK, false>(unused, m, scratch);
+    const RowScale s = row_scale(m);
+    if constexpr (HELD) {
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) store8(dst + at + c * step, v[c], s.inverse, dim - at - c * step);
+    } else {
         for (int i = at; i < dim; i += step) {
             load8(v[0], src + i, dim - i, vec);
             store8(dst + i, v[0], s.inverse, dim - i);
         }
-        if (at == 0) scale[r] = s.scale;
     }
+    if (at == 0) scale[r] = s.scale;
 }
 
 struct NormArgs {
@@ -188,7 +187,7 @@ __device__ __forceinline__ void times_gain(float (&w)[8], const NormArgs& a, int
 
 template <typename Ty, int V, bool BLOCK>
 __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
-    __shared__ float scratch[64];
+    __shared__ uint32_t scratch[64];
     pdl_wait();
     pdl_trigger();
     const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8, dim = a.dim;
@@ -207,14 +206,15 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
             for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], b[j]);
         }
     };
-    float ss = 0.f, m = 0.f;
+    float ss = 0.f;
+    uint32_t top = 0;
     auto take = [&](float (&t)[8], int i) {      // t becomes w
         if (y) store8(total + i, t, dim - i, a.t_vec);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(t[j], t[j], ss);
         times_gain(t, a, i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(t[j]));
+        for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
     };
     constexpr bool HELD = V <= MOST_CHUNKS;
     float w[HELD ? V : 1][8];
@@ -231,7 +231,8 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
             take(w[0], i);
         }
     }
-    row_reduce<BLOCK>(ss, m, scratch);
+    row_reduce<BLOCK, true>(ss, top, scratch);
+    float m = __uint_as_float(top);
     const float* t_row = y ? total : x;          // (from here on t is read back: the thread's own writes)
     const bool t_vec = y ? a.t_vec : a.x_vec;
     if (ss > 1e-24f && ss < 1e30f && m >= kTiny && m < 1e30f) {
@@ -253,7 +254,7 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     // Squares or products left float32, or vanished in it, or the row is zeros or not numbers: once more with t scaled by powers of two.
     const float fs = ss < 1e30f ? (ss > 1e-24f ? 1.f : 1.2089258196146292e+24f) : 8.271806125530277e-25f;               // 2^80, 2^-80
     const float fm = m < 1e30f ? (m >= kTiny ? 1.f : 1.2676506002282294e+30f) : 7.52316384526264e-37f;                 // 2^100, 2^-120
-    ss = m = 0.f;
+    ss = 0.f, top = 0;
     for (int i = at; i < dim; i += step) {
         float t[8], u[8];
         load8(t, t_row + i, dim - i, t_vec);
@@ -265,9 +266,10 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
         }
         times_gain(t, a, i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = mag_max(m, fabsf(t[j]));
+        for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
     }
-    row_reduce<BLOCK>(ss, m, scratch);
+    row_reduce<BLOCK, true>(ss, top, scratch);
+    m = __uint_as_float(top);
     const double root = 1.0 / sqrt((double)ss / ((double)fs * (double)fs) / dim + (double)a.eps);
     const double most = root * ((double)m / (double)fm);             // (NaN where the row has one, or is 0 / 0)
     const bool whole = ss < INFINITY && most < (double)INFINITY;
@@ -283,32 +285,47 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     if (at == 0) a.scale[r] = !whole ? __int_as_float(0x7fffffff) : (inverse == 0.f ? 0.f : (float)(most / 127.0));
 }
 
+// Four 8-bit integers as floats: a byte under the exponent of 2^23 (with its sign bit turned: 128 more than it is), less that.
+__device__ __forceinline__ void four_floats(float* v, uint32_t q, float s) {
+    q ^= 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(q, 0x4b000000u, 0x7540 + j)), 8388736.f), s);
+}
+
+constexpr int VALUE_ROWS = 4;       // rows that a block of the kernel below goes through
 template <typename T>
 __global__ void __launch_bounds__(256)
 values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ scale, T* __restrict__ out, int ldo, bool vec, int rows, int dim) {
     pdl_wait();
     pdl_trigger();
-    const int chunks = (dim + 7) / 8;
-    const long long total = (long long)rows * chunks;
-    for (long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x; item < total; item += (long long)gridDim.x * blockDim.x) {
-        int r, c;
-        split_item(item, chunks, r, c);
-        const int left = dim - c * 8;
-        const int8_t* src = q + (size_t)r * ldq + c * 8;
-        const float s = scale[r];
-        float v[8];
-        if (left >= 8) {
-            const uint2 w = *reinterpret_cast<const uint2*>(src);
+    const int at = (blockIdx.x * 256 + threadIdx.x) * 8, left = dim - at;
+    if (left <= 0) return;
+    for (int group = blockIdx.y; group * VALUE_ROWS < rows; group += gridDim.y) {
+        uint2 w[VALUE_ROWS];
+        float s[VALUE_ROWS];
+        const int lo = group * VALUE_ROWS;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = __fmul_rn((float)(int8_t)(w.x >> (8 * j)), s);
-                v[4 + j] = __fmul_rn((float)(int8_t)(w.y >> (8 * j)), s);
+        for (int i = 0; i < VALUE_ROWS; ++i)
+            if (lo + i < rows) {
+                const int8_t* src = q + (size_t)(lo + i) * ldq + at;
+                s[i] = scale[lo + i];
+                if (left >= 8) {
+                    w[i] = *reinterpret_cast<const uint2*>(src);
+                } else {
+                    w[i] = make_uint2(0, 0);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < left) (j < 4 ? w[i].x : w[i].y) |= (uint32_t)(uint8_t)src[j] << (8 * (j & 3));
+                }
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < left ? __fmul_rn((float)src[j], s) : 0.f;
-        }
-        store8(out + (size_t)r * ldo + c * 8, v, left, vec);
+        for (int i = 0; i < VALUE_ROWS; ++i)
+            if (lo + i < rows) {
+                float v[8];
+                four_floats(v, w[i].x, s[i]);
+                four_floats(v + 4, w[i].y, s[i]);
+                store8(out + (size_t)(lo + i) * ldo + at, v, left, vec);
+            }
     }
 }
 
@@ -399,13 +416,13 @@ JLLM_EXPORT int jllm_int8_values(const Int8View* view, void* out, int out_dtype,
     JLLM_REQUIRE_ROWS("int8_values", v);
     JLLM_REQUIRE(ldo >= v.cols, "int8_values: ldo=%d for %d values", ldo, v.cols);
     if (v.rows == 0) return JLLM_OK;
-    const long long items = (long long)v.rows * ((v.cols + 7) / 8), most = (long long)(jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 1) * 16;
-    const int blocks = (int)((items + 255) / 256 > most ? most : (items + 255) / 256);
+    const int groups = (v.rows + VALUE_ROWS - 1) / VALUE_ROWS;
+    const dim3 blocks((v.cols + 2047) / 2048, groups < 65535 ? groups : 65535);
     if (out_dtype == JLLM_F32)
-        jllm_launch(values_kernel<float>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale, (float*)out, ldo,
+        jllm_launch(values_kernel<float>, blocks, dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale, (float*)out, ldo,
                     vec16(out, ldo, 4), v.rows, v.cols);
     else
-        jllm_launch(values_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale,
+        jllm_launch(values_kernel<__nv_bfloat16>, blocks, dim3(256), 0, stream, LAUNCH_DEPENDENT, v.data, v.stride, v.scale,
                     (__nv_bfloat16*)out, ldo, vec16(out, ldo, 2), v.rows, v.cols);
     return jllm_check_launch("int8_values");
 }
