@@ -8,10 +8,10 @@
 // k_blocks + kb) * 16 KB; its scales are filled up to whole tiles. The activations' tiles come by tiled TMA copies, which fill rows
 // beyond M and k beyond K with zeros.
 //
-// Two kernels. Few tokens (`swap`): the weight rows are the M side of the MMAs, the tokens the N side, and a cluster of blocks shares the
-// k blocks of 128 weight rows. Many tokens (`pair`): two SMs to a tile of 256 tokens x 64, 128 or 256 weight rows. Every wait is bounded
-// and raises the products' error word (codes 31-33 swap, 34-36 pair).
-#include "gemm_epilogue.cuh"
+// In both kernels the weight rows are the M side of the MMAs and the tokens the N side, so that tokens are filled up to a multiple of 16
+// or 32 and not of 128. Few tokens (`cluster`): a cluster of blocks shares the k blocks of 128 weight rows. Many tokens (`pair`): two SMs to
+// a tile of 256 weight rows x up to 256 tokens. Every wait is bounded and raises the products' error word (codes 31-33 cluster, 34-36 pair).
+#include "tcgen05_common.cuh"
 #include "int8_view.h"
 
 namespace {
@@ -71,18 +71,135 @@ __device__ __forceinline__ float scaled(uint32_t sum, float scale_a, float scale
     return __fmul_rn(__fmul_rn((float)(int)sum, scale_a), scale_w);
 }
 
+// What happens to the sums: the same in both kernels.
+struct Finish {
+    VecRef bias;
+    int has_bias, ldo, accumulate, M, N;
+    GluArgs glu;
+};
+// Results leave 16 bytes a lane: a warp parks its 32 weight rows x J tokens in shared memory and takes them back token by token. A lane
+// that stores its own values stores 2 bytes of every token's row, with all that a store costs (84 ns a token and block, now 25).
+template <typename Tout>
+struct TokenEpilogue {
+    const Finish& f;
+    Tout* out;
+    Tout* park;                // the warp's: 16 x 32 values, 16-byte aligned
+    const float* token_scales; // shared memory, of the tokens from `first` on, 16-byte aligned
+    int first, n, lane;        // n: this lane's weight row
+    float sw, b;               // its scale and its bias
+    bool vec;
+
+    __device__ __forceinline__ TokenEpilogue(const Finish& f_, Tout* out_, Tout* park_, const float* token_scales_, int n_, int lane_, float sw_)
+        : f(f_), out(out_), park(park_), token_scales(token_scales_), first(0), n(n_), lane(lane_), sw(sw_),
+          b(f_.has_bias && n_ < f_.N ? f_.bias[n_] : 0.f),
+          vec(n_ - lane_ + 32 <= f_.N && ((uintptr_t)out_ & 15u) == 0 && (((size_t)f_.ldo * sizeof(Tout)) & 15u) == 0) {}
+
+    // the sums of the tokens [t, t + J) for this lane's weight row; the whole warp calls it
+    template <int J>
+    __device__ __forceinline__ void operator()(const uint32_t (&sum)[J], int t) const {
+        constexpr int PER = 16 / sizeof(Tout);       // values of a 16-byte piece
+        float v[J];
+#pragma unroll
+        for (int j = 0; j < J; j += 4) {
+            const float4 sa = *reinterpret_cast<const float4*>(token_scales + (t - first) + j);
+            v[j] = scaled(sum[j], sa.x, sw);
+            v[j + 1] = scaled(sum[j + 1], sa.y, sw);
+            v[j + 2] = scaled(sum[j + 2], sa.z, sw);
+            v[j + 3] = scaled(sum[j + 3], sa.w, sw);
+        }
+        const bool add_behind = sizeof(Tout) == 4 && f.accumulate == EPI_ADD;      // (a bfloat16 sum is rounded once, so it is made here)
+        if (f.glu) {
+            // rows come in blocks of 16, 8 gate rows and the 8 up rows of the same hidden units: the gates' lanes take the first half of
+            // the tokens, the others the second
+            const bool up_lane = lane & 8;
+            float gate[J / 2], up[J / 2], units[J / 2];
+#pragma unroll
+            for (int j = 0; j < J / 2; ++j) {
+                const float other = __shfl_xor_sync(0xffffffffu, up_lane ? v[j] : v[J / 2 + j], 8);
+                gate[j] = up_lane ? other : v[j];
+                up[j] = up_lane ? v[J / 2 + j] : other;
+            }
+            glu_units<J / 2>(f.glu.word, [&](int j) { return gate[j]; }, [&](int j) { return up[j]; }, 1.f, units);
+#pragma unroll
+            for (int j = 0; j < J / 2; ++j) park[(up_lane ? J / 2 + j : j) * 16 + (lane >> 4) * 8 + (lane & 7)] = from_float<Tout>(units[j]);
+        } else {
+            if (f.has_bias)
+#pragma unroll
+                for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], b);
+            if (f.accumulate == EPI_RELU2)
+#pragma unroll
+                for (int j = 0; j < J; ++j) v[j] = epilogue_act(v[j], EPI_RELU2);
+            if (f.accumulate == EPI_ADD && !add_behind) {
+                // (all the old values are requested before the first store: a load behind a store through the same pointer would wait)
+                float old[J];
+#pragma unroll
+                for (int j = 0; j < J; ++j) old[j] = n < f.N && t + j < f.M ? to_float(out[(size_t)(t + j) * f.ldo + n]) : 0.f;
+#pragma unroll
+                for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], old[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) park[j * 32 + lane] = from_float<Tout>(v[j]);
+        }
+        __syncwarp();
+        if (f.glu) leave<J, 16, PER>(t, (n - lane) >> 1, f.N >> 1, false);
+        else leave<J, 32, PER>(t, n - lane, f.N, add_behind);
+        __syncwarp();
+    }
+
+    // parked rows of WIDTH values -> out[t + j, column + ...], only what lies in [M, last)
+    template <int J, int WIDTH, int PER>
+    __device__ __forceinline__ void leave(int t, int column, int last, bool add) const {
+        if (vec) {
+            constexpr int PIECES = WIDTH / PER, STEPS = (J * PIECES + 31) / 32;
+            uint4 piece[STEPS];
+            Tout* dst[STEPS];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int i = lane + 32 * s, j = i / PIECES, c = i % PIECES * PER;
+                dst[s] = i < J * PIECES && t + j < f.M ? out + (size_t)(t + j) * f.ldo + column + c : nullptr;
+                if (dst[s]) piece[s] = *reinterpret_cast<const uint4*>(park + j * WIDTH + c);
+            }
+            if (add) {
+                float4 old[STEPS];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+                    if (dst[s]) old[s] = *reinterpret_cast<const float4*>(dst[s]);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    piece[s].x = __float_as_uint(__fadd_rn(__uint_as_float(piece[s].x), old[s].x));
+                    piece[s].y = __float_as_uint(__fadd_rn(__uint_as_float(piece[s].y), old[s].y));
+                    piece[s].z = __float_as_uint(__fadd_rn(__uint_as_float(piece[s].z), old[s].z));
+                    piece[s].w = __float_as_uint(__fadd_rn(__uint_as_float(piece[s].w), old[s].w));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+                if (dst[s]) *reinterpret_cast<uint4*>(dst[s]) = piece[s];
+        } else {
+            const int c = lane & (WIDTH - 1);
+            if (column + c < last)
+#pragma unroll
+                for (int j = lane / WIDTH; j < J; j += 32 / WIDTH)
+                    if (t + j < f.M) {
+                        Tout* dst = out + (size_t)(t + j) * f.ldo + column + c;
+                        const Tout v = park[j * WIDTH + c];
+                        *dst = add ? from_float<Tout>(__fadd_rn(to_float(v), to_float(*dst))) : v;
+                    }
+        }
+    }
+};
+
 // ---- few tokens: a cluster of blocks to 128 weight rows --------------------------------------------------------------------
 // With few tokens the product is nothing but reading W once. Block p of a cluster streams its part of the tile's k blocks (one contiguous
 // 16 KB bulk copy each, requested before the kernel in front has finished: weights are nobody's output); the accumulator [128 weight
 // rows x tokens] lies in its tensor memory. Of the tokens every block finishes a share: the others send their parts of it (st.async,
 // which counts its bytes on the owner's mbarrier: one way through the cluster and no meeting), the owner adds them up, scales and stores.
-struct SwapArgs {
+struct ClusterArgs {
     const int8_t* w;
     const float *scale_w, *scale_a;
-    VecRef bias;
-    int has_bias, ldo, accumulate, M, N, k_blocks, ntok, stages, blocks, share;      // ntok: the MMAs' N; share: tokens a block finishes
+    Finish f;
+    int k_blocks, ntok, stages, blocks, share;      // ntok: the MMAs' N; share: tokens a block finishes
     uint32_t tmem_cols;
-    GluArgs glu;
     int* error_word;
 };
 
@@ -102,7 +219,7 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
 
 template <typename Tout>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ SwapArgs g, Tout* __restrict__ out) {
+gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ClusterArgs g, Tout* __restrict__ out) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) float token_scales[256];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -120,7 +237,7 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int tile = (int)blockIdx.x / blocks, rank = (int)blockIdx.x % blocks;      // (clusters lie along x: this is the rank)
     const int kb_lo = (int)((long long)g.k_blocks * rank / blocks), n_kb = (int)((long long)g.k_blocks * (rank + 1) / blocks) - kb_lo;
-    const int tokens = (g.M + 7) & ~7;                              // the accumulator's columns that anybody needs
+    const int tokens = (g.f.M + 7) & ~7;                              // the accumulator's columns that anybody needs
     const int mine = rank * share, mine_end = min(mine + share, tokens);
 
     if (threadIdx.x == 0) {
@@ -207,11 +324,12 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const int quad = warp & 3, row = quad * 32 + lane, n = tile * 128 + row;
         const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16);
         const float sw = g.scale_w[n];                        // (filled up to whole tiles)
-        const float b = g.has_bias && n < g.N ? g.bias[n] : 0.f;
+        // (parks in the ring, which is idle once every MMA is done)
+        const TokenEpilogue<Tout> finish(g.f, out, reinterpret_cast<Tout*>(aligned + (size_t)quad * 2048), token_scales, n, lane, sw);
         pdl_wait();          // the token scales, and what is added into, were written by the kernels before
         pdl_trigger();
         // (into shared memory while the weights come: asked for in front of every store they were 1 us for 8 tokens)
-        for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < g.M ? g.scale_a[i] : 0.f;
+        for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < g.f.M ? g.scale_a[i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
         ok = mbar_wait(acc_bar, 0, abort_flag);
@@ -241,87 +359,24 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag));
         if (ok) {
             const uint8_t* parts = aligned + parts_at + (size_t)row * 16;
-            // Results leave 16 bytes a lane: a warp parks its 32 weight rows x J tokens in the ring (idle by now: every MMA is done) and takes
-            // them back token by token. A lane that stores its own values stores 2 bytes of every token's row, with all that a store costs.
-            Tout* park = reinterpret_cast<Tout*>(aligned + (size_t)quad * 4096);
-            const int width = g.glu ? 16 : 32, column = g.glu ? (tile * 128 + quad * 32) >> 1 : tile * 128 + quad * 32;
-            const bool vec = tile * 128 + quad * 32 + 32 <= g.N && ((uintptr_t)out & 15u) == 0 && (((size_t)g.ldo * sizeof(Tout)) & 15u) == 0;
-            auto finish = [&](auto& sum, int t) {
-                constexpr int J = sizeof(sum) / 4, PER = 16 / sizeof(Tout);       // tokens; values of a 16-byte piece
+            auto add_up = [&](auto& sum, int t) {
                 tmem_ld(taddr + t, sum);
-                float v[J];
                 tmem_ld_wait();
                 for (int p = 0; p < blocks - 1; ++p) {
                     const uint8_t* src = parts + (size_t)p * part_bytes + (size_t)((t - mine) / 4) * 2048;
 #pragma unroll
-                    for (int q = 0; q < J / 4; ++q) {
+                    for (int q = 0; q < (int)(sizeof(sum) / 16); ++q) {
                         const uint4 x = *reinterpret_cast<const uint4*>(src + q * 2048);
                         sum[4 * q] += x.x, sum[4 * q + 1] += x.y, sum[4 * q + 2] += x.z, sum[4 * q + 3] += x.w;
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < J; j += 4) {
-                    const float4 sa = *reinterpret_cast<const float4*>(token_scales + t + j);
-                    v[j] = scaled(sum[j], sa.x, sw);
-                    v[j + 1] = scaled(sum[j + 1], sa.y, sw);
-                    v[j + 2] = scaled(sum[j + 2], sa.z, sw);
-                    v[j + 3] = scaled(sum[j + 3], sa.w, sw);
-                }
-                if (g.glu) {
-                    // rows come in blocks of 16, 8 gate rows and the 8 up rows of the same hidden units: the gates' lanes take the first half of
-                    // the tokens, the others the second
-                    const bool up_lane = lane & 8;
-                    float gate[J / 2], up[J / 2], units[J / 2];
-#pragma unroll
-                    for (int j = 0; j < J / 2; ++j) {
-                        const float other = __shfl_xor_sync(0xffffffffu, up_lane ? v[j] : v[J / 2 + j], 8);
-                        gate[j] = up_lane ? other : v[j];
-                        up[j] = up_lane ? v[J / 2 + j] : other;
-                    }
-                    glu_units<J / 2>(g.glu.word, [&](int j) { return gate[j]; }, [&](int j) { return up[j]; }, 1.f, units);
-#pragma unroll
-                    for (int j = 0; j < J / 2; ++j)
-                        park[(up_lane ? J / 2 + j : j) * 16 + (lane >> 4) * 8 + (lane & 7)] = from_float<Tout>(units[j]);
-                } else {
-                    if (g.has_bias)
-#pragma unroll
-                        for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], b);
-                    if (g.accumulate == EPI_RELU2)
-#pragma unroll
-                        for (int j = 0; j < J; ++j) v[j] = epilogue_act(v[j], EPI_RELU2);
-                    if (g.accumulate == EPI_ADD) {
-                        // (all the old values are requested before the first store: a load behind a store through the same pointer would wait)
-                        float old[J];
-#pragma unroll
-                        for (int j = 0; j < J; ++j) old[j] = n < g.N && t + j < g.M ? to_float(out[(size_t)(t + j) * g.ldo + n]) : 0.f;
-#pragma unroll
-                        for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], old[j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < J; ++j) park[j * 32 + lane] = from_float<Tout>(v[j]);
-                }
-                __syncwarp();
-                if (vec) {
-                    const int pieces = width / PER;              // of a token's row: 2, 4 or 8
-                    for (int i = lane; i < J * pieces; i += 32) {
-                        const int j = i / pieces, c = i % pieces * PER;
-                        if (t + j < g.M)
-                            *reinterpret_cast<uint4*>(out + (size_t)(t + j) * g.ldo + column + c) = *reinterpret_cast<const uint4*>(park + j * width + c);
-                    }
-                } else {
-                    const int last = g.glu ? g.N >> 1 : g.N;
-                    for (int i = lane; i < J * width; i += 32) {
-                        const int j = i / width, c = i % width;
-                        if (t + j < g.M && column + c < last) out[(size_t)(t + j) * g.ldo + column + c] = park[i];
-                    }
-                }
-                __syncwarp();
+                finish(sum, t);
             };
             int t = mine;
             uint32_t sum16[16], sum8[8];
 #pragma unroll 1
-            for (; t + 16 <= mine_end; t += 16) finish(sum16, t);
-            if (t < mine_end) finish(sum8, t);
+            for (; t + 16 <= mine_end; t += 16) add_up(sum16, t);
+            if (t < mine_end) add_up(sum8, t);
         } else if (lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 33); }
     }
     tcgen05_fence_before();
@@ -337,33 +392,48 @@ gemm_int8_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     }
 }
 
-struct SwapCut {
+struct ClusterCut {
     int blocks, share, ntok, stages;
     size_t smem;
 };
-SwapCut swap_cut(int blocks, int M, int k_blocks) {
-    SwapCut c{blocks, ((M + 7) / 8 + blocks - 1) / blocks * 8, (M + 15) / 16 * 16, 0, 0};
+ClusterCut cluster_cut(int blocks, int M, int k_blocks) {
+    ClusterCut c{blocks, ((M + 7) / 8 + blocks - 1) / blocks * 8, (M + 15) / 16 * 16, 0, 0};
     const size_t stage = TILE_BYTES + (size_t)c.ntok * BK, parts = (size_t)(blocks - 1) * c.share * 512;
     const size_t room = c.ntok <= 64 ? 104 * 1024 : SMEM_ROOM - 4096;
     c.stages = parts + 2 * stage > room ? 0 : (int)((room - parts) / stage);
     const int most = (k_blocks + blocks - 1) / blocks;
     if (c.stages > most) c.stages = most;
     c.smem = c.stages * stage + parts + 1024 + 8 * (2 * c.stages + 2) + 16;
+    // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: the blocks on an SM never ask for
+    // more than its 512 columns. Of 60 KB and more (less 128 columns each) there are at most three, of 114 KB one beside another; a block that
+    // takes all columns (of this file or another) has over 190 KB.
+    const size_t least = blocks == 1 ? 0 : c.ntok > 128 ? 114 * 1024 : 60 * 1024;
+    if (c.smem < least) c.smem = least;
     return c;
 }
 
-// ---- many tokens: two SMs to a tile of 256 tokens x BN weight rows ----------------------------------------------------------
-// A cluster of two blocks: each brings 128 tokens and half of the tile's weight rows, one lane of the first block issues MMAs of M 256
-// that read both blocks' shared memory, and each block ends up with its 128 tokens in its own tensor memory, where two accumulators let
-// a tile's epilogue run under the next tile's main loop. Every copy completes on the FIRST block's "full" barrier of the stage;
-// tcgen05.commit, multicast to both blocks, frees the stage in both. The pairs walk the tiles with m fastest.
-constexpr int STAGING_BYTES = 4 * STAGING_WARP_FLOATS * 4;
-template <int BN> struct PairShape {
-    static constexpr int W_BYTES = BN / 2 * BK, STAGE_BYTES = TILE_BYTES + W_BYTES;
-    static constexpr int STAGES = 196608 / STAGE_BYTES;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 1024 + 256 + STAGING_BYTES;
-    static_assert(STAGE_BYTES % 1024 == 0 && SMEM <= 227 * 1024, "swizzled tiles lie at multiples of 1,024 bytes");
+// ---- many tokens: two SMs to a tile of 256 weight rows x up to 256 tokens ------------------------------------------------------
+// A cluster of two blocks: each brings 128 weight rows and half of the tile's tokens, one lane of the first block issues MMAs of M 256
+// that read both blocks' shared memory, and each block ends up with its 128 weight rows in its own tensor memory, where two accumulators
+// let a tile's epilogue run under the next tile's main loop. Every copy completes on the FIRST block's "full" barrier of the stage;
+// tcgen05.commit, multicast to both blocks, frees the stage in both. The pairs walk the tiles with the tokens fastest: what is read
+// together shares its weights.
+constexpr int PARK_BYTES = 4 * 2048, SCALE_BYTES = 4 * 1024;
+constexpr size_t PAIR_ROOM = 200 * 1024;
+struct PairArgs {
+    const float *scale_w, *scale_a;
+    Finish f;
+    int k_blocks, ntok, groups, stages;       // ntok: tokens of a tile (a multiple of 32), groups of them
+    int* error_word;
 };
+int pair_stages(int ntok) {
+    const int stages = (int)(PAIR_ROOM / (TILE_BYTES + (size_t)ntok / 2 * BK));
+    return stages > 12 ? 12 : stages;
+}
+size_t pair_smem(int ntok) {
+    const int stages = pair_stages(ntok);
+    return (size_t)stages * (TILE_BYTES + (size_t)ntok / 2 * BK) + PARK_BYTES + SCALE_BYTES + 8 * (2 * stages + 4) + 16 + 1024;
+}
 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
@@ -382,37 +452,33 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
                  : "memory");
 }
 
-template <typename Tout, int BN>
+template <typename Tout>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                      const __grid_constant__ CUtensorMap map_out, int bulk_out, const float* __restrict__ scale_a,
-                      const float* __restrict__ scale_w, VecRef bias, int has_bias, Tout* __restrict__ out, int ldo, int accumulate, int M,
-                      int N, int k_blocks, GluArgs glu, int* __restrict__ error_word) {
-    using S = PairShape<BN>;
-    constexpr int STAGES = S::STAGES, STAGE_BYTES = S::STAGE_BYTES;
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ PairArgs g,
+                      Tout* __restrict__ out) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-    // the stages, the epilogue's staging (1024-byte aligned, as the stages are), the barriers: full[STAGES] (the first block's are used),
-    // empty[STAGES] (each block its own), acc_full[2] (each its own), acc_empty[2] (the first block's); then the TMEM base and the abort flag
-    const uint32_t bars = base + STAGES * STAGE_BYTES + STAGING_BYTES;
+    const int stages = g.stages;
+    const uint32_t stage_bytes = TILE_BYTES + (uint32_t)g.ntok / 2 * BK, ring = (uint32_t)stages * stage_bytes;
+    // the stages, the epilogue's rooms, the barriers: full[stages] (the first block's are used), empty[stages] (each block its own),
+    // acc_full[2] (each its own), acc_empty[2] (the first block's); then the TMEM base and the abort flag
+    const uint32_t bars = base + ring + PARK_BYTES + SCALE_BYTES;
     auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
-    auto acc_full_bar = [&](int b) { return bars + 8u * (2 * STAGES + b); };
-    auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
-    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + STAGES * STAGE_BYTES + STAGING_BYTES + 8 * (2 * STAGES + 4));
+    auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
+    auto acc_full_bar = [&](int b) { return bars + 8u * (2 * stages + b); };
+    auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * stages + 2 + b); };
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + ring + PARK_BYTES + SCALE_BYTES + 8 * (2 * stages + 4));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-    uint8_t* staging = aligned + STAGES * STAGE_BYTES;
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     uint32_t rank;                                    // 0: the pair's first block, which issues the MMAs
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int tiles_m = (M + 255) / 256, tiles = tiles_m * ((N + BN - 1) / BN);
-    const int packed_rows = (N + 127) & ~127;         // rows of the packed weight
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, k_blocks = g.k_blocks;
+    const int packed_tiles = (g.f.N + 127) >> 7, tiles = ((packed_tiles + 1) >> 1) * g.groups;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
@@ -423,9 +489,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2) {   // the same warp of both blocks allocates the columns in both
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(2 * BN)
-                     : "memory");
+    if (warp == 2) {   // the same warp of both blocks allocates all columns in both (one block per SM)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tcgen05_fence_before();
@@ -440,7 +505,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     auto give_up = [&](int code) {
         *abort_flag = 1;
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1u)), "r"(1) : "memory");
-        atomicExch(error_word, code);
+        atomicExch(g.error_word, code);
     };
 
     if (warp == 0) {
@@ -450,29 +515,30 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         uint32_t parity = 1, dst = base;
         bool ok = true;
         for (int tile = pair; ok && tile < tiles; tile += pairs) {
-            const int m0 = (tile % tiles_m) * 256 + (int)rank * 128, n0 = (tile / tiles_m) * BN, w0 = n0 + (int)rank * (BN / 2);
-            const bool mine = w0 < packed_rows;                            // this block's half of the weight rows exists
-            const uint32_t tx = 2 * TILE_BYTES + (n0 + BN / 2 < packed_rows ? 2 : 1) * S::W_BYTES;     // both blocks' bytes
-            int wy = (w0 >> 7) * k_blocks * 128 + (w0 & 127);              // row of the packed weight's k block
+            const int row = tile % g.groups * g.ntok + (int)rank * (g.ntok >> 1), wt = tile / g.groups * 2;
+            const bool mine = wt + (int)rank < packed_tiles;               // this block's half of the weight rows exists
+            const uint32_t tx = (wt + 1 < packed_tiles ? 2 : 1) * TILE_BYTES + (uint32_t)g.ntok * BK;     // both blocks' bytes
+            int wy = (wt + (int)rank) * k_blocks * 128;                    // row of the packed weight's k block
             for (int kb = 0; kb < k_blocks; ++kb, wy += 128) {
                 if (!warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
                 const uint32_t full0 = first_full + 8u * s;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full_bar(s), tx);
-                    tma_load_2d_pair(dst, &map_a, kb * BK, m0, full0);
-                    if (mine) tma_load_2d_pair(dst + TILE_BYTES, &map_w, 0, wy, full0);
+                    if (mine) tma_load_2d_pair(dst, &map_w, 0, wy, full0);
+                    tma_load_2d_pair(dst + TILE_BYTES, &map_a, kb * BK, row, full0);
                 }
                 __syncwarp();
-                dst += STAGE_BYTES;
-                if (++s == STAGES) { s = 0; parity ^= 1u; dst = base; }
+                dst += stage_bytes;
+                if (++s == stages) { s = 0; parity ^= 1u; dst = base; }
             }
         }
         if (!ok && lane == 0) give_up(34);
     } else if (warp == 1) {
         // ---------------- MMA issuer (the first block) ----------------
         if (rank == 0) {
-            const uint64_t desc_a0 = smem_desc_sw128(base), desc_b0 = smem_desc_sw128(base + TILE_BYTES);
-            uint64_t desc_a = desc_a0, desc_b = desc_b0;          // (a stage further is an addition to the address field)
+            const uint32_t idesc = idesc_i8(256, g.ntok);
+            const uint64_t desc_w0 = smem_desc_sw128(base), desc_b0 = smem_desc_sw128(base + TILE_BYTES);
+            uint64_t desc_w = desc_w0, desc_b = desc_b0;          // (a stage further is an addition to the address field)
             uint32_t local_tile = 0, parity = 0;
             int s = 0;
             bool ok = true;
@@ -480,20 +546,20 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 const uint32_t buf = local_tile & 1u;
                 if (!warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                 tcgen05_fence_after();
-                const uint32_t tmem_d = tmem_base + buf * BN;
+                const uint32_t tmem_d = tmem_base + buf * 256;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
                     tcgen05_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < BK / 32; ++k)
-                            mma_i8_pair(tmem_d, desc_a + 2 * k, desc_b + 2 * k, idesc_i8(256, BN), (kb > 0 || k > 0) ? 1u : 0u);
+                            mma_i8_pair(tmem_d, desc_w + 2 * k, desc_b + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
                         commit_pair(empty_bar(s));          // both blocks' stage is free when these MMAs have read it
                     }
                     __syncwarp();
-                    desc_a += STAGE_BYTES >> 4;
-                    desc_b += STAGE_BYTES >> 4;
-                    if (++s == STAGES) { s = 0; parity ^= 1u; desc_a = desc_a0; desc_b = desc_b0; }
+                    desc_w += stage_bytes >> 4;
+                    desc_b += stage_bytes >> 4;
+                    if (++s == stages) { s = 0; parity ^= 1u; desc_w = desc_w0; desc_b = desc_b0; }
                 }
                 if (ok && elect_one()) commit_pair(acc_full_bar(buf));
                 __syncwarp();
@@ -501,41 +567,36 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             if (!ok && lane == 0) give_up(35);
         }
     } else {
-        // ---------------- epilogue: warps 2..5 of both blocks, TMEM lanes 32 * (warp % 4) ----------------
+        // ---------------- epilogue: warps 2..5 of both blocks, TMEM lanes 32 * (warp % 4) = weight rows of the block's tile ----------------
         const int quad = warp & 3;
-        const TileEpilogue<Tout> ep{out, ldo, M, N, accumulate, has_bias, glu, bias, bulk_out ? &map_out : nullptr};
-        float* my_staging = reinterpret_cast<float*>(staging + quad * (bulk_out ? BULK_WARP_BYTES : STAGING_WARP_FLOATS * 4));
+        Tout* park = reinterpret_cast<Tout*>(aligned + ring + quad * 2048);
+        float* scales = reinterpret_cast<float*>(aligned + ring + PARK_BYTES + quad * 1024);      // (each warp keeps its own: nobody to wait for)
         uint32_t local_tile = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < tiles; tile += pairs, ++local_tile) {
-            const int row0 = (tile % tiles_m) * 256 + (int)rank * 128 + quad * 32, n0 = (tile / tiles_m) * BN;
+            const int first = tile % g.groups * g.ntok, end = min(first + g.ntok, g.f.M), wt = tile / g.groups * 2 + (int)rank;
+            const int n = wt * 128 + quad * 32 + lane;
+            const bool mine = wt < packed_tiles;
             const uint32_t buf = local_tile & 1u;
-            const float sa = row0 + lane < M ? scale_a[row0 + lane] : 0.f;
-            if (!mbar_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag)) { ok = false; break; }
+            for (int i = lane; i < g.ntok; i += 32) scales[i] = first + i < g.f.M ? g.scale_a[first + i] : 0.f;
+            TokenEpilogue<Tout> finish(g.f, out, park, scales, n, lane, mine ? g.scale_w[n] : 0.f);
+            finish.first = first;
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag))) { ok = false; break; }
             tcgen05_fence_after();
-            const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
-            const bool whole = ep.rows_whole(row0);
+            const uint32_t taddr = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
+            if (mine && n - lane < g.f.N)
 #pragma unroll 1
-            for (int c0 = 0; c0 < BN && n0 + c0 < N; c0 += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(taddr + c0, v);
-                tmem_ld_wait();
-                const float4* sw = reinterpret_cast<const float4*>(scale_w + n0 + c0);      // (filled up to whole tiles)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float4 f = sw[j];
-                    v[4 * j] = __float_as_uint(scaled(v[4 * j], sa, f.x));
-                    v[4 * j + 1] = __float_as_uint(scaled(v[4 * j + 1], sa, f.y));
-                    v[4 * j + 2] = __float_as_uint(scaled(v[4 * j + 2], sa, f.z));
-                    v[4 * j + 3] = __float_as_uint(scaled(v[4 * j + 3], sa, f.w));
+                for (int t = first; t < end; t += 16) {
+                    uint32_t sum[16];
+                    tmem_ld(taddr + (t - first), sum);
+                    tmem_ld_wait();
+                    finish(sum, t);
                 }
-                ep.store(v, row0, lane, n0 + c0, whole, my_staging);
-            }
             tcgen05_fence_before();          // this warp has read the accumulator
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(in_block(acc_empty_bar(buf), 0));
         }
-        ep.bulk_done(lane);
         if (!ok && lane == 0) give_up(36);
     }
     tcgen05_fence_before();
@@ -544,7 +605,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     cluster_wait();          // neither block leaves, or frees tensor memory, while the other may still reach into it
     if (warp == 2) {
         tcgen05_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
     }
 }
 
@@ -580,8 +641,8 @@ int byte_map_for(const void* ptr, long long rows, long long cols, long long ld, 
 }
 
 template <typename Tout>
-int launch_swap(const CUtensorMap& map_a, const SwapArgs& g, const SwapCut& c, int tiles, void* out, cudaStream_t stream) {
-    auto kern = gemm_int8_swap_kernel<Tout>;
+int launch_cluster(const CUtensorMap& map_a, const ClusterArgs& g, const ClusterCut& c, int tiles, void* out, cudaStream_t stream) {
+    auto kern = gemm_int8_cluster_kernel<Tout>;
     if (jllm_allow_smem((const void*)kern, c.smem) != cudaSuccess)
         return jllm_fail(JLLM_CUDA_ERROR, "gemm_int8: %zu bytes of shared memory refused", c.smem);
     cudaLaunchConfig_t cfg = {};
@@ -602,19 +663,22 @@ int launch_swap(const CUtensorMap& map_a, const SwapArgs& g, const SwapCut& c, i
         cfg.numAttrs = 2;
     }
     cudaLaunchKernelEx(&cfg, kern, map_a, g, static_cast<Tout*>(out));
-    return jllm_check_launch("gemm_int8_swap");
+    return jllm_check_launch("gemm_int8_cluster");
 }
 
-template <typename Tout, int BN>
+// pairs of blocks that the device runs at a time (with all the shared memory a pair may ask for), looked up once
+template <typename Tout>
 int resident_pairs() {
     static int pairs = -1;
     if (pairs >= 0) return pairs;
-    auto kern = gemm_int8_pair_kernel<Tout, BN>;
-    if (jllm_allow_smem((const void*)kern, PairShape<BN>::SMEM) != cudaSuccess) return 0;
+    auto kern = gemm_int8_pair_kernel<Tout>;
+    size_t smem = 0;
+    for (int ntok = 32; ntok <= 256; ntok += 32) smem = pair_smem(ntok) > smem ? pair_smem(ntok) : smem;
+    if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 2));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = PairShape<BN>::SMEM;
+    cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -630,105 +694,85 @@ int resident_pairs() {
     return pairs = n;
 }
 
-}  // namespace
-
-int* jllm_gemm_error_word();
-extern int g_plain_stores;
-
-namespace {
-
 struct Product {
     const int8_t *a, *w;
     int lda;
     const float *scale_a, *scale_w;
-    int k_blocks;
-    VecRef bias;
-    int has_bias;
+    int k_blocks, K;
     void* out;
-    int out_dtype, ldo, accumulate, M, N, K;
-    GluArgs glu;
+    int out_dtype;
+    Finish f;
     int* error_word;
     cudaStream_t stream;
 };
 
-int run_swap(const Product& p, int blocks) {
-    const SwapCut c = swap_cut(blocks, p.M, p.k_blocks);
-    JLLM_REQUIRE(blocks >= 1 && blocks <= 8 && blocks <= p.k_blocks && p.M <= 256 && c.stages >= 1,
-                 "gemm_int8: clusters of %d blocks do not take %d rows of %d k blocks", blocks, p.M, p.k_blocks);
+int run_cluster(const Product& p, int blocks) {
+    const int M = p.f.M;
+    JLLM_REQUIRE(blocks >= 1 && blocks <= 8 && blocks <= p.k_blocks && M <= 256 && cluster_cut(blocks, M, p.k_blocks).stages >= 1,
+                 "gemm_int8: clusters of %d blocks do not take %d rows of %d k blocks", blocks, M, p.k_blocks);
+    const ClusterCut c = cluster_cut(blocks, M, p.k_blocks);
     CUtensorMap map_a;
-    const int rc = byte_map_for(p.a, p.M, p.K, p.lda, c.ntok, true, &map_a);
+    const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, true, &map_a);
     if (rc != JLLM_OK) return rc;
     uint32_t cols = 32;
     while ((int)cols < c.ntok) cols <<= 1;
-    const SwapArgs g{p.w, p.scale_w, p.scale_a, p.bias, p.has_bias, p.ldo, p.accumulate, p.M, p.N, p.k_blocks, c.ntok, c.stages, c.blocks,
-                     c.share, cols, p.glu, p.error_word};
-    const int tiles = (p.N + 127) / 128;
-    return p.out_dtype == JLLM_F32 ? launch_swap<float>(map_a, g, c, tiles, p.out, p.stream)
-                                   : launch_swap<__nv_bfloat16>(map_a, g, c, tiles, p.out, p.stream);
-}
-
-template <typename Tout, int BN>
-int run_pair(const Product& p) {
-    const long long packed_rows = (long long)((p.N + 127) / 128) * p.k_blocks * 128;
-    JLLM_REQUIRE(packed_rows < (1LL << 31), "gemm_int8: a packed weight of %lld rows of 128 bytes is too long", packed_rows);
-    CUtensorMap map_a, map_w, map_out = {};
-    int rc = byte_map_for(p.a, p.M, p.K, p.lda, 128, true, &map_a);
-    if (rc != JLLM_OK) return rc;
-    rc = byte_map_for(p.w, packed_rows, 128, 128, BN / 2, false, &map_w);
-    if (rc != JLLM_OK) return rc;
-    const int bulk_out = p.out_dtype == JLLM_F32 && !p.glu && p.accumulate != EPI_RELU2 && p.ldo % 4 == 0 && ((uintptr_t)p.out % 16) == 0 && !g_plain_stores;
-    if (bulk_out) {
-        rc = tensor_map_out_f32(p.out, p.M, p.N, p.ldo, &map_out);
-        if (rc != JLLM_OK) return rc;
-    }
-    int pairs = resident_pairs<Tout, BN>();
-    JLLM_REQUIRE(pairs >= 1, "gemm_int8: the device runs no cluster of two blocks with %zu bytes of shared memory", PairShape<BN>::SMEM);
-    const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + BN - 1) / BN);
-    JLLM_REQUIRE(tiles < (1LL << 31) - 1024, "gemm_int8: %lld tiles", tiles);
-    if (pairs > tiles) pairs = (int)tiles;
-    jllm_launch(gemm_int8_pair_kernel<Tout, BN>, dim3(2 * pairs), dim3(THREADS), PairShape<BN>::SMEM, p.stream, LAUNCH_DEPENDENT, map_a, map_w,
-                map_out, bulk_out, p.scale_a, p.scale_w, p.bias, p.has_bias, (Tout*)p.out, p.ldo, p.accumulate, p.M, p.N, p.k_blocks, p.glu,
-                p.error_word);
-    return jllm_check_launch("gemm_int8_pair");
+    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, cols, p.error_word};
+    const int tiles = (p.f.N + 127) / 128;
+    return p.out_dtype == JLLM_F32 ? launch_cluster<float>(map_a, g, c, tiles, p.out, p.stream)
+                                   : launch_cluster<__nv_bfloat16>(map_a, g, c, tiles, p.out, p.stream);
 }
 
 template <typename Tout>
-int run_pair_width(const Product& p, int width) {
-    switch (width) {
-        case 256: return run_pair<Tout, 256>(p);
-        case 128: return run_pair<Tout, 128>(p);
-        case 64: return run_pair<Tout, 64>(p);
-        default: return jllm_fail(JLLM_BAD_ARGUMENT, "gemm_int8: tiles of 64, 128 or 256 weight rows, not %d", width);
-    }
+int run_pair(const Product& p, int ntok) {
+    JLLM_REQUIRE(ntok >= 32 && ntok <= 256 && ntok % 32 == 0, "gemm_int8: tiles of 32, 64 .. 256 tokens, not %d", ntok);
+    const long long packed_rows = (long long)((p.f.N + 127) / 128) * p.k_blocks * 128;
+    JLLM_REQUIRE(packed_rows < (1LL << 31), "gemm_int8: a packed weight of %lld rows of 128 bytes is too long", packed_rows);
+    CUtensorMap map_a, map_w;
+    int rc = byte_map_for(p.a, p.f.M, p.K, p.lda, ntok / 2, true, &map_a);
+    if (rc != JLLM_OK) return rc;
+    rc = byte_map_for(p.w, packed_rows, 128, 128, 128, false, &map_w);
+    if (rc != JLLM_OK) return rc;
+    int pairs = resident_pairs<Tout>();
+    JLLM_REQUIRE(pairs >= 1, "gemm_int8: the device runs no cluster of two blocks with %zu bytes of shared memory", pair_smem(ntok));
+    const int groups = (p.f.M + ntok - 1) / ntok;
+    const long long tiles = (long long)groups * ((p.f.N + 255) / 256);
+    JLLM_REQUIRE(tiles < (1LL << 31) - 1024, "gemm_int8: %lld tiles", tiles);
+    if (pairs > tiles) pairs = (int)tiles;
+    const PairArgs g{p.scale_w, p.scale_a, p.f, p.k_blocks, ntok, groups, pair_stages(ntok), p.error_word};
+    jllm_launch(gemm_int8_pair_kernel<Tout>, dim3(2 * pairs), dim3(THREADS), pair_smem(ntok), p.stream, LAUNCH_DEPENDENT, map_a, map_w, g,
+                static_cast<Tout*>(p.out));
+    return jllm_check_launch("gemm_int8_pair");
 }
 
-// Blocks of a cluster (swap), or minus the tile's weight rows (pair).
+// Blocks of a cluster, or minus the tokens of a pair's tile.
 int choose(int M, int N, int k_blocks, int sms) {
     const int tiles = (N + 127) / 128;
-    if (M <= 256) {
+    if (M <= 128) {
         int blocks = sms / tiles;
         if (blocks > 8) blocks = 8;
         if (blocks > k_blocks) blocks = k_blocks;
         if (blocks < 1) blocks = 1;
-        while (blocks > 1 && swap_cut(blocks, M, k_blocks).stages < 1) --blocks;
+        while (blocks > 1 && cluster_cut(blocks, M, k_blocks).stages < 1) --blocks;
         return blocks;
     }
-    const long long tiles_m = (M + 255) / 256, pairs = sms / 2 > 0 ? sms / 2 : 1;
+    const long long pair_tiles = (N + 255) / 256, pairs = sms / 2 > 0 ? sms / 2 : 1;
     int best = 256;
     double least = 1e30;
-    for (int width : {256, 128, 64}) {
-        const long long rounds = (tiles_m * ((N + width - 1) / width) + pairs - 1) / pairs;
-        const double cost = (double)rounds * (256 + width);
-        if (cost < least) least = cost, best = width;
+    for (int ntok = 256; ntok >= 32; ntok -= 32) {
+        const long long rounds = (pair_tiles * ((M + ntok - 1) / ntok) + pairs - 1) / pairs;
+        const double cost = (double)rounds * (256 + ntok);
+        if (cost < least) least = cost, best = ntok;
     }
     return -best;
 }
 
 }  // namespace
 
+int* jllm_gemm_error_word();
+
 // `rows`: the int8 activations [M, K], their rows at multiples of 16 bytes; `weight`: ops.pack_int8 of the [N, K] weight, its scales filled
 // up to a multiple of 128 and 16-byte aligned; out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a
-// cluster (swap), minus the weight rows of a tile (pair), 0 as the sizes have it.
+// cluster, minus the tokens of a pair's tile, 0 as the sizes have it.
 JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo,
                                int accumulate, int swiglu_word, int cut, cudaStream_t stream) {
     const int8_t *a = rows->data, *w_packed = weight->data;
@@ -747,9 +791,9 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     if (M == 0) return JLLM_OK;
     int* error_word = jllm_gemm_error_word();
     if (!error_word) return jllm_fail(JLLM_CUDA_ERROR, "gemm_int8: no error word");
-    const Product p{a, w_packed, lda, scale_a, scale_w, k_blocks, VecRef{bias, bias_dtype}, (int)(bias != nullptr), out, out_dtype, ldo, accumulate,
-                    M, N, K, glu, error_word, stream};
+    const Product p{a, w_packed, lda, scale_a, scale_w, k_blocks, K, out, out_dtype,
+                    Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, M, N, glu}, error_word, stream};
     if (cut == 0) cut = choose(M, N, k_blocks, jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 1);
-    if (cut > 0) return run_swap(p, cut);
-    return out_dtype == JLLM_F32 ? run_pair_width<float>(p, -cut) : run_pair_width<__nv_bfloat16>(p, -cut);
+    if (cut > 0) return run_cluster(p, cut);
+    return out_dtype == JLLM_F32 ? run_pair<float>(p, -cut) : run_pair<__nv_bfloat16>(p, -cut);
 }

@@ -302,7 +302,8 @@ def test_product_gated(ops, rows, hidden, kind):
                                                 (6, 256, 260, 4096), (7, 100, 256, 1025), (8, 256, 400, 3000), (8, 8, 384, 8192), (8, 1, 100, 1024), (7, 24, 64, 12000),
                                                 (-64, 1, 10, 20), (-64, 130, 250, 700), (-64, 700, 400, 333), (-64, 2048, 3000, 256),
                                                 (-128, 257, 129, 500), (-128, 256, 1000, 640), (-128, 1200, 4224, 300),
-                                                (-256, 300, 128, 200), (-256, 513, 700, 1111), (-256, 2100, 5000, 300), (-256, 5, 257, 150)])
+                                                (-32, 1, 3, 9), (-32, 300, 600, 1000), (-96, 500, 1111, 2000), (-160, 300, 2600, 513), (-160, 159, 129, 4096), (-192, 400, 900, 260),
+                                                (-224, 777, 1003, 2049), (-256, 300, 128, 200), (-256, 513, 700, 1111), (-256, 2100, 5000, 300), (-256, 5, 257, 150)])
 def test_product_cut_up(ops, cut, rows, width, dim):
     """Every way of cutting the work gives the same bits."""
     (a, sa), (w, sw) = integers(rows, dim, 11), integers(width, dim, 12)
@@ -430,7 +431,7 @@ def test_refusals(ops):
             lambda: ops.gemm_int8(a8, packed, out, accumulate=7),
             lambda: ops.gemm_int8(a8, packed, out, cut=2),                # one k block
             lambda: ops.gemm_int8(a8, packed, out, cut=9),
-            lambda: ops.gemm_int8(a8, packed, out, cut=-32),
+            lambda: ops.gemm_int8(a8, packed, out, cut=-48),
             lambda: ops.gemm_int8(ops.int8_rows(4, 48, DEV), packed, out),
             lambda: ops.gemm_int8(ops.Int8Rows(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4)), packed, out)):
         with pytest.raises(E):
