@@ -418,7 +418,8 @@ ClusterCut cluster_cut(int blocks, int M, int k_blocks) {
 // let a tile's epilogue run under the next tile's main loop. Every copy completes on the FIRST block's "full" barrier of the stage;
 // tcgen05.commit, multicast to both blocks, frees the stage in both. The pairs walk the tiles with the tokens fastest: what is read
 // together shares its weights.
-constexpr int PARK_BYTES = 4 * 2048, SCALE_BYTES = 4 * 1024;
+constexpr int PAIR_THREADS = 320, EPI_WARPS = 8;       // warps 2..9: two to each quarter of the weight rows, taking turns of 16 tokens
+constexpr int PARK_BYTES = EPI_WARPS * 2048, SCALE_BYTES = EPI_WARPS * 1024;
 constexpr size_t PAIR_ROOM = 200 * 1024;
 struct PairArgs {
     const float *scale_w, *scale_a;
@@ -453,7 +454,7 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
 }
 
 template <typename Tout>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ PairArgs g,
                       Tout* __restrict__ out) {
     extern __shared__ uint8_t smem_raw[];
@@ -484,7 +485,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full_bar(b), 1);
-            mbar_init(acc_empty_bar(b), 8);   // one arrival per epilogue warp of both blocks
+            mbar_init(acc_empty_bar(b), 2 * EPI_WARPS);   // one arrival per epilogue warp of both blocks
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -567,10 +568,10 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             if (!ok && lane == 0) give_up(35);
         }
     } else {
-        // ---------------- epilogue: warps 2..5 of both blocks, TMEM lanes 32 * (warp % 4) = weight rows of the block's tile ----------------
-        const int quad = warp & 3;
-        Tout* park = reinterpret_cast<Tout*>(aligned + ring + quad * 2048);
-        float* scales = reinterpret_cast<float*>(aligned + ring + PARK_BYTES + quad * 1024);      // (each warp keeps its own: nobody to wait for)
+        // ---------------- epilogue: warps 2..9 of both blocks, TMEM lanes 32 * (warp % 4) = weight rows of the block's tile ----------------
+        const int quad = warp & 3, turn = (warp - 2) >> 2;
+        Tout* park = reinterpret_cast<Tout*>(aligned + ring + (warp - 2) * 2048);
+        float* scales = reinterpret_cast<float*>(aligned + ring + PARK_BYTES + (warp - 2) * 1024);      // (each warp keeps its own: nobody to wait for)
         uint32_t local_tile = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < tiles; tile += pairs, ++local_tile) {
@@ -587,7 +588,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const uint32_t taddr = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
             if (mine && n - lane < g.f.N)
 #pragma unroll 1
-                for (int t = first; t < end; t += 16) {
+                for (int t = first + 16 * turn; t < end; t += 32) {
                     uint32_t sum[16];
                     tmem_ld(taddr + (t - first), sum);
                     tmem_ld_wait();
@@ -677,7 +678,7 @@ int resident_pairs() {
     if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 2));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(PAIR_THREADS);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -739,7 +740,7 @@ int run_pair(const Product& p, int ntok) {
     JLLM_REQUIRE(tiles < (1LL << 31) - 1024, "gemm_int8: %lld tiles", tiles);
     if (pairs > tiles) pairs = (int)tiles;
     const PairArgs g{p.scale_w, p.scale_a, p.f, p.k_blocks, ntok, groups, pair_stages(ntok), p.error_word};
-    jllm_launch(gemm_int8_pair_kernel<Tout>, dim3(2 * pairs), dim3(THREADS), pair_smem(ntok), p.stream, LAUNCH_DEPENDENT, map_a, map_w, g,
+    jllm_launch(gemm_int8_pair_kernel<Tout>, dim3(2 * pairs), dim3(PAIR_THREADS), pair_smem(ntok), p.stream, LAUNCH_DEPENDENT, map_a, map_w, g,
                 static_cast<Tout*>(p.out));
     return jllm_check_launch("gemm_int8_pair");
 }
