@@ -105,6 +105,46 @@ __device__ __forceinline__ void store8(int8_t* p, const float (&v)[8], float inv
     }
 }
 
+// Eight values as they lie in memory: what a row's threads hold until its scale is known.
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p, int left, bool vec) { load8(v, p, left, vec); }
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, magnitude(v[j]));
+        return m;
+    }
+    __device__ __forceinline__ void values(float (&out)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = v[j];
+    }
+};
+template <> struct Raw8<__nv_bfloat16> {
+    uint32_t w[4];             // two values each
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int left, bool vec) {
+        if (vec && left >= 8) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {
+            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = (2 * j < left ? (uint32_t)h[2 * j] : 0u) | (2 * j + 1 < left ? (uint32_t)h[2 * j + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int j = 1; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+        return max(m << 16, m & 0xffff0000u);
+    }
+    __device__ __forceinline__ void values(float (&out)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[2 * j] = __uint_as_float(w[j] << 16), out[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+};
+
 struct RowScale {
     float scale, inverse;
 };
@@ -130,23 +170,20 @@ __global__ void quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8
     const T* src = x + (size_t)r * ldx;
     int8_t* dst = q + (size_t)r * ldq;
     constexpr bool HELD = V <= MOST_CHUNKS;
-    float v[HELD ? V : 1][8], unused = 0.f;
+    Raw8<T> raw[HELD ? V : 1];
+    float unused = 0.f, v[8];
     uint32_t m = 0;
-    auto look = [&](const float (&c)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, magnitude(c[j]));
-    };
     if constexpr (HELD) {
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) load8(v[c], src + at + c * step, dim - at - c * step, vec);
+            if (at + c * step < dim) raw[c].load(src + at + c * step, dim - at - c * step, vec);
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) look(v[c]);
+            if (at + c * step < dim) m = max(m, raw[c].largest());
     } else {
         for (int i = at; i < dim; i += step) {
-            load8(v[0], src + i, dim - i, vec);
-            look(v[0]);
+            raw[0].load(src + i, dim - i, vec);
+            m = max(m, raw[0].largest());
         }
     }
     row_reduce<BLOCK, false>(unused, m, scratch);
@@ -154,11 +191,15 @@ __global__ void quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8
     if constexpr (HELD) {
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) store8(dst + at + c * step, v[c], s.inverse, dim - at - c * step);
+            if (at + c * step < dim) {
+                raw[c].values(v);
+                store8(dst + at + c * step, v, s.inverse, dim - at - c * step);
+            }
     } else {
         for (int i = at; i < dim; i += step) {
-            load8(v[0], src + i, dim - i, vec);
-            store8(dst + i, v[0], s.inverse, dim - i);
+            raw[0].load(src + i, dim - i, vec);
+            raw[0].values(v);
+            store8(dst + i, v, s.inverse, dim - i);
         }
     }
     if (at == 0) scale[r] = s.scale;
