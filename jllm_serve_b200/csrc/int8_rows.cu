@@ -11,14 +11,15 @@
 //
 // A thread takes V chunks of 8 neighbouring values, chunk i of a row being thread i % T's. V and T follow from the row's width alone, so
 // a row's sum has one order whatever else is in the batch. Rows of up to 512 values are a warp's each, wider ones a block's, beyond 32,768
-// values (`wide`) a thread's chunks are fetched again behind the reduction.
+// values (16,384 of a norm) a thread's chunks are fetched again behind the reduction.
 #include "head_rotate.cuh"
 #include "int8_view.h"
 
 namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;      // 2^-100
-constexpr int MOST_CHUNKS = 4, MOST_THREADS = 1024;   // what a row's threads hold: 32,768 values
+constexpr int MOST_CHUNKS = 4, MOST_THREADS = 1024;   // what a row's threads hold: 32,768 values; of a norm's, with its gains, half of that
+constexpr int NORM_THREADS = 512;
 
 // Magnitudes are compared as the bits of |v|: one integer instruction, and a NaN is larger than everything and stays.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -46,17 +47,6 @@ __device__ __forceinline__ void load8(float (&v)[8], const float* p, int left, b
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
-    }
-}
-__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* p, int left, bool vec) {
-    if (vec && left >= 8) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? to_float(p[j]) : 0.f;
     }
 }
 __device__ __forceinline__ void store8(float* p, const float (&v)[8], int left, bool vec) {
@@ -160,7 +150,7 @@ template <bool BLOCK> __device__ __forceinline__ int my_row() { return BLOCK ? b
 template <bool BLOCK> __device__ __forceinline__ int my_place() { return BLOCK ? threadIdx.x : threadIdx.x & 31; }
 
 template <typename T, int V, bool BLOCK>
-__global__ void quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
+__global__ void __launch_bounds__(MOST_THREADS) quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
                                 int dim) {
     __shared__ uint32_t scratch[64];
     pdl_wait();
@@ -209,7 +199,7 @@ struct NormArgs {
     const float* x;
     const void* y;
     float* total;           // may be x
-    VecRef gain;
+    const void* gain;
     int8_t* q;
     float* scale;
     int ldx, ldy, ldt, ldq, rows, dim;
@@ -217,65 +207,87 @@ struct NormArgs {
     bool x_vec, y_vec, t_vec, g_vec;
 };
 
-// w = t gain from t's eight values
-__device__ __forceinline__ void times_gain(float (&w)[8], const NormArgs& a, int i) {
-    float g[8];
-    if (a.gain.dtype == JLLM_F32) load8(g, static_cast<const float*>(a.gain.p) + i, a.dim - i, a.g_vec);
-    else load8(g, static_cast<const __nv_bfloat16*>(a.gain.p) + i, a.dim - i, a.g_vec);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = __fmul_rn(w[j], g[j]);
-}
-
-template <typename Ty, int V, bool BLOCK>
-__global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
+template <typename Ty, typename Tg, int V, bool BLOCK>
+__global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS) add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ uint32_t scratch[64];
+    const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8, dim = a.dim;
+    constexpr bool HELD = V <= MOST_CHUNKS;
+    const Tg* gains = static_cast<const Tg*>(a.gain);
+    // The gains are nobody's output: they are on their way while the kernel in front ends. (Four chunks of them, held beside the rest,
+    // leave too few blocks an SM: 2,048 x 12,288 took 39 us, with the gains asked for chunk by chunk 25.)
+    constexpr bool GAINS_HELD = V <= 2;
+    Raw8<Tg> gain[GAINS_HELD ? V : 1];
+    if constexpr (GAINS_HELD) {
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+            if (at + c * step < dim) gain[c].load(gains + at + c * step, dim - at - c * step, a.g_vec);
+    }
     pdl_wait();
     pdl_trigger();
-    const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8, dim = a.dim;
     if (r >= a.rows) return;
     const float* x = a.x + (size_t)r * a.ldx;
     const Ty* y = a.y ? static_cast<const Ty*>(a.y) + (size_t)r * a.ldy : nullptr;
     float* total = a.y ? a.total + (size_t)r * a.ldt : nullptr;
     int8_t* dst = a.q + (size_t)r * a.ldq;
-    // t = x + y of the chunk at i, left in `total`
-    auto fetch = [&](float (&t)[8], int i) {
-        load8(t, x + i, dim - i, a.x_vec);
-        if (y) {
-            float b[8];
-            load8(b, y + i, dim - i, a.y_vec);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], b[j]);
-        }
-    };
     float ss = 0.f;
     uint32_t top = 0;
-    auto take = [&](float (&t)[8], int i) {      // t becomes w
-        if (y) store8(total + i, t, dim - i, a.t_vec);
+    // the chunk at i: t = x + y, left in `total`; t becomes w = t gain
+    auto take = [&](float (&t)[8], const Raw8<Ty>& other, const Raw8<Tg>& gain, int i) {
+        float b[8];
+        if (y) {
+            other.values(b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = __fadd_rn(t[j], b[j]);
+            store8(total + i, t, dim - i, a.t_vec);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(t[j], t[j], ss);
-        times_gain(t, a, i);
+        gain.values(b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
+        for (int j = 0; j < 8; ++j) {
+            t[j] = __fmul_rn(t[j], b[j]);
+            top = max(top, magnitude(t[j]));
+        }
     };
-    constexpr bool HELD = V <= MOST_CHUNKS;
+    // w of the chunk at i once more (t scaled by f), from what the thread itself has left
+    auto again = [&](float (&t)[8], int i, float f) {
+        float b[8];
+        load8(t, (y ? total : x) + i, dim - i, y ? a.t_vec : a.x_vec);
+        Raw8<Tg> g;
+        g.load(gains + i, dim - i, a.g_vec);
+        g.values(b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(__fmul_rn(t[j], f), b[j]);
+    };
     float w[HELD ? V : 1][8];
+    Raw8<Ty> other[HELD ? V : 1];
     if constexpr (HELD) {
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) fetch(w[c], at + c * step);
+            if (at + c * step < dim) {
+                load8(w[c], x + at + c * step, dim - at - c * step, a.x_vec);
+                if (y) other[c].load(y + at + c * step, dim - at - c * step, a.y_vec);
+            }
 #pragma unroll
         for (int c = 0; c < V; ++c)
-            if (at + c * step < dim) take(w[c], at + c * step);
+            if (at + c * step < dim) {
+                if constexpr (GAINS_HELD) {
+                    take(w[c], other[c], gain[c], at + c * step);
+                } else {
+                    gain[0].load(gains + at + c * step, dim - at - c * step, a.g_vec);
+                    take(w[c], other[c], gain[0], at + c * step);
+                }
+            }
     } else {
         for (int i = at; i < dim; i += step) {
-            fetch(w[0], i);
-            take(w[0], i);
+            load8(w[0], x + i, dim - i, a.x_vec);
+            if (y) other[0].load(y + i, dim - i, a.y_vec);
+            gain[0].load(gains + i, dim - i, a.g_vec);
+            take(w[0], other[0], gain[0], i);
         }
     }
     row_reduce<BLOCK, true>(ss, top, scratch);
     float m = __uint_as_float(top);
-    const float* t_row = y ? total : x;          // (from here on t is read back: the thread's own writes)
-    const bool t_vec = y ? a.t_vec : a.x_vec;
     if (ss > 1e-24f && ss < 1e30f && m >= kTiny && m < 1e30f) {
         const float inverse = __fdiv_rn(127.f, m);
         if constexpr (HELD) {
@@ -284,8 +296,7 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
                 if (at + c * step < dim) store8(dst + at + c * step, w[c], inverse, dim - at - c * step);
         } else {
             for (int i = at; i < dim; i += step) {
-                load8(w[0], t_row + i, dim - i, t_vec);
-                times_gain(w[0], a, i);
+                again(w[0], i, 1.f);
                 store8(dst + i, w[0], inverse, dim - i);
             }
         }
@@ -297,15 +308,14 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     const float fm = m < 1e30f ? (m >= kTiny ? 1.f : 1.2676506002282294e+30f) : 7.52316384526264e-37f;                 // 2^100, 2^-120
     ss = 0.f, top = 0;
     for (int i = at; i < dim; i += step) {
-        float t[8], u[8];
-        load8(t, t_row + i, dim - i, t_vec);
+        float t[8];
+        load8(t, (y ? total : x) + i, dim - i, y ? a.t_vec : a.x_vec);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            u[j] = __fmul_rn(t[j], fs);
-            ss = fmaf(u[j], u[j], ss);
-            t[j] = __fmul_rn(t[j], fm);
+            const float u = __fmul_rn(t[j], fs);
+            ss = fmaf(u, u, ss);
         }
-        times_gain(t, a, i);
+        again(t, i, fm);
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
     }
@@ -317,10 +327,7 @@ __global__ void add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     const float inverse = whole && most >= (double)kTiny ? __fdiv_rn(127.f, m) : 0.f;
     for (int i = at; i < dim; i += step) {
         float t[8];
-        load8(t, t_row + i, dim - i, t_vec);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], fm);
-        times_gain(t, a, i);
+        again(t, i, fm);
         store8(dst + i, t, inverse, dim - i);
     }
     if (at == 0) a.scale[r] = !whole ? __int_as_float(0x7fffffff) : (inverse == 0.f ? 0.f : (float)(most / 127.0));
@@ -370,17 +377,17 @@ values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ s
     }
 }
 
-// The threads that share a row of `dim` values and the chunks each holds: two where 256 threads are enough, else four.
+// The threads that share a row of `dim` values and the chunks each holds: two where 512 threads are enough, else four.
 struct RowCut {
     int threads, chunks;
 };
-RowCut row_cut(int dim) {
+RowCut row_cut(int dim, int most) {
     const int all = (dim + 7) / 8;
     if (all <= 32) return {32, 1};
     if (all <= 64) return {32, 2};
-    const int chunks = all <= 512 ? 2 : MOST_CHUNKS;
+    const int chunks = all <= 1024 ? 2 : MOST_CHUNKS;
     const int threads = ((all + chunks - 1) / chunks + 31) / 32 * 32;
-    return threads <= MOST_THREADS ? RowCut{threads, chunks} : RowCut{MOST_THREADS, MOST_CHUNKS + 1};
+    return threads <= most ? RowCut{threads, chunks} : RowCut{MOST_THREADS, MOST_CHUNKS + 1};
 }
 constexpr int WARPS = 4;       // rows of a block whose warps have one each
 
@@ -396,7 +403,7 @@ bool vec16(const void* p, int ld, int size) { return (uintptr_t)p % 16 == 0 && (
 
 template <typename T>
 void launch_quantize(const void* x, int ldx, int8_t* q, int ldq, float* scale, int rows, int dim, cudaStream_t stream) {
-    const RowCut cut = row_cut(dim);
+    const RowCut cut = row_cut(dim, MOST_THREADS);
     const bool vec = vec16(x, ldx, sizeof(T));
 #define JLLM_GO(V, BLOCK)                                                                                                             \
     jllm_launch(quantize_kernel<T, V, BLOCK>, dim3(BLOCK ? rows : (rows + WARPS - 1) / WARPS), dim3(BLOCK ? cut.threads : 32 * WARPS), 0, \
@@ -404,11 +411,11 @@ void launch_quantize(const void* x, int ldx, int8_t* q, int ldq, float* scale, i
     JLLM_ROW_CUT(cut);
 #undef JLLM_GO
 }
-template <typename Ty>
+template <typename Ty, typename Tg>
 void launch_norm(const NormArgs& a, cudaStream_t stream) {
-    const RowCut cut = row_cut(a.dim);
+    const RowCut cut = row_cut(a.dim, NORM_THREADS);
 #define JLLM_GO(V, BLOCK)                                                                                                                  \
-    jllm_launch(add_rmsnorm_kernel<Ty, V, BLOCK>, dim3(BLOCK ? a.rows : (a.rows + WARPS - 1) / WARPS), dim3(BLOCK ? cut.threads : 32 * WARPS), 0, \
+    jllm_launch(add_rmsnorm_kernel<Ty, Tg, V, BLOCK>, dim3(BLOCK ? a.rows : (a.rows + WARPS - 1) / WARPS), dim3(BLOCK ? cut.threads : 32 * WARPS), 0, \
                 stream, LAUNCH_DEPENDENT, a)
     JLLM_ROW_CUT(cut);
 #undef JLLM_GO
@@ -443,11 +450,12 @@ JLLM_EXPORT int jllm_add_rmsnorm_int8(const float* x, int ldx, const void* y, in
     JLLM_REQUIRE(ldx >= v.cols && (!y || (ldy >= v.cols && ldt >= v.cols && total)), "add_rmsnorm_int8: ldx=%d ldy=%d ldt=%d for %d values", ldx,
                  ldy, ldt, v.cols);
     if (v.rows == 0) return JLLM_OK;
-    const NormArgs a{x, y, total, VecRef{gain, gain_dtype}, const_cast<int8_t*>(v.data), const_cast<float*>(v.scale), ldx, ldy, ldt, v.stride,
+    const NormArgs a{x, y, total, gain, const_cast<int8_t*>(v.data), const_cast<float*>(v.scale), ldx, ldy, ldt, v.stride,
                      v.rows, v.cols, eps, vec16(x, ldx, 4), vec16(y, ldy, y_dtype == JLLM_F32 ? 4 : 2), vec16(total, ldt, 4),
                      (uintptr_t)gain % 16 == 0};
-    if (y_dtype == JLLM_F32) launch_norm<float>(a, stream);
-    else launch_norm<__nv_bfloat16>(a, stream);
+    const bool g32 = gain_dtype == JLLM_F32;
+    if (y_dtype == JLLM_F32) g32 ? launch_norm<float, float>(a, stream) : launch_norm<float, __nv_bfloat16>(a, stream);
+    else g32 ? launch_norm<__nv_bfloat16, float>(a, stream) : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, stream);
     return jllm_check_launch("add_rmsnorm_int8");
 }
 
