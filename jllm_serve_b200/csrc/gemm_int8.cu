@@ -217,8 +217,9 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
     return false;
 }
 
+// (128 registers a thread: registers are dealt out for eight warps where there are six, and with more no second block fits beside one)
 template <typename Tout>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(256, 2)
 gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ClusterArgs g, Tout* __restrict__ out) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) float token_scales[256];
@@ -396,10 +397,12 @@ struct ClusterCut {
     int blocks, share, ntok, stages;
     size_t smem;
 };
-ClusterCut cluster_cut(int blocks, int M, int k_blocks) {
+// `deep`: the ring takes all shared memory of an SM, else half of it, so that a second block (of this product, or of the next one, whose first
+// weights then come while this one ends) fits beside.
+ClusterCut cluster_cut(int blocks, bool deep, int M, int k_blocks) {
     ClusterCut c{blocks, ((M + 7) / 8 + blocks - 1) / blocks * 8, (M + 15) / 16 * 16, 0, 0};
     const size_t stage = TILE_BYTES + (size_t)c.ntok * BK, parts = (size_t)(blocks - 1) * c.share * 512;
-    const size_t room = c.ntok <= 64 ? 104 * 1024 : SMEM_ROOM - 4096;
+    const size_t room = deep ? SMEM_ROOM - 4096 : 104 * 1024;
     c.stages = parts + 2 * stage > room ? 0 : (int)((room - parts) / stage);
     const int most = (k_blocks + blocks - 1) / blocks;
     if (c.stages > most) c.stages = most;
@@ -673,15 +676,13 @@ int launch_cluster(const CUtensorMap& map_a, const ClusterArgs& g, const Cluster
     return jllm_check_launch("gemm_int8_cluster");
 }
 
-// clusters of that many blocks that the device runs at a time with that much shared memory
+// clusters of that many blocks that the device runs at a time, one block an SM
 template <typename Tout>
-int resident_clusters(const ClusterCut& c, size_t smem) {
+int resident_clusters(const ClusterCut& c) {
     int n = 0;
-    ClusterCut one = c;
-    one.smem = smem;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = cluster_config<Tout>(one, 1, attr, nullptr);
-    if (jllm_allow_smem((const void*)gemm_int8_cluster_kernel<Tout>, smem) != cudaSuccess ||
+    const cudaLaunchConfig_t cfg = cluster_config<Tout>(c, 1, attr, nullptr);
+    if (jllm_allow_smem((const void*)gemm_int8_cluster_kernel<Tout>, c.smem) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, gemm_int8_cluster_kernel<Tout>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         return 0;
@@ -729,11 +730,11 @@ struct Product {
     cudaStream_t stream;
 };
 
-int run_cluster(const Product& p, int blocks) {
+int run_cluster(const Product& p, int blocks, bool deep) {
     const int M = p.f.M;
-    JLLM_REQUIRE(blocks >= 1 && blocks <= 8 && blocks <= p.k_blocks && M <= 256 && cluster_cut(blocks, M, p.k_blocks).stages >= 1,
+    JLLM_REQUIRE(blocks >= 1 && blocks <= 8 && blocks <= p.k_blocks && M <= 256 && cluster_cut(blocks, deep, M, p.k_blocks).stages >= 1,
                  "gemm_int8: clusters of %d blocks do not take %d rows of %d k blocks", blocks, M, p.k_blocks);
-    const ClusterCut c = cluster_cut(blocks, M, p.k_blocks);
+    const ClusterCut c = cluster_cut(blocks, deep, M, p.k_blocks);
     CUtensorMap map_a;
     const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, true, &map_a);
     if (rc != JLLM_OK) return rc;
@@ -767,32 +768,35 @@ int run_pair(const Product& p, int ntok) {
     return jllm_check_launch("gemm_int8_pair");
 }
 
-// What a product takes, about, in us (up to what both kernels take alike), fitted to 1,164 sizes from 1 to 2,048 rows against 256 to 34,816
-// weight rows of 256 to 17,408 values, launched back to back on weights larger than L2: what it chooses is 1.8% slower than the best
-// cut of each size in the geometric mean (up to 16 rows 2.5, 17 to 64 3.1, 65 to 128 4.3, 129 to 256 0.9, beyond 0.3%).
-//   clusters: a block's k blocks, each 0.22 us and 1.1 ns a token; all clusters at once with one block an SM, or (w = 0.63 a round) blocks side
-//   by side, or one batch behind the other; sending 0.18 us a block of the cluster and 11.5 ns a token sent;
-//   pairs: rounds of tiles, a k block 0.127 us and 0.31 ns a token; 1.2 us more from launch to first results;
-//   both: no faster than memory gives the weights.
-constexpr double MEMORY_BYTES_US = 8e6;
+// What a product takes, about, in us (up to what all ways take alike), fitted to 846 sizes of 1 to 256 rows against 128 to 34,816 weight
+// rows of 256 to 17,408 values, launched back to back on weights larger than L2: what it chooses is 2.1% slower than the best way of each
+// size in the geometric mean (up to 16 rows 2.2, 17 to 64 2.9, 65 to 128 2.0, 129 to 256 0.9%; the pairs of 558 sizes of 300 to 2,048 rows
+// 0.2%). Deep rings are 9% of that.
+//   clusters: a block's k blocks, each a ring's share of the 1.13 us that a copy is on its way, or 0.12 us and 0.55 ns a token; all clusters
+//   at once, one block an SM, or (half of that a round) two blocks side by side, or one batch behind the other; nothing of the next product
+//   beside it: 0.3 us; sending 0.15 us a block of the cluster and 10 ns a token sent;
+//   pairs: rounds of tiles, a k block 0.126 us and 0.2 ns a token; 1.55 us more from launch to first results;
+//   both: no faster than memory and L2 give the weights.
+constexpr int DEEP = 10;              // a cluster's cut: its blocks, and 10 more with all of an SM's shared memory
+constexpr double READ_BYTES_US = 1e7;
 double pair_cost(int M, int N, int k_blocks, int ntok, int pairs) {
     const long long tiles = (long long)((N + 255) / 256) * ((M + ntok - 1) / ntok), rounds = (tiles + pairs - 1) / pairs;
-    const double run = (double)rounds * (k_blocks < 3 ? 3 : k_blocks) * (0.127 + 0.00031 * ntok), read = (double)N * k_blocks * BK / MEMORY_BYTES_US;
-    return 1.2 + (run > read ? run : read) + 0.002 * ntok;
+    const double run = (double)rounds * (k_blocks < 3 ? 3 : k_blocks) * (0.126 + 0.0002 * ntok), read = (double)N * k_blocks * BK / READ_BYTES_US;
+    return 1.55 + (run > read ? run : read) + 0.0016 * ntok;
 }
 template <typename Tout>
-double cluster_cost(int M, int N, int k_blocks, int blocks) {
-    const ClusterCut c = cluster_cut(blocks, M, k_blocks);
+double cluster_cost(int M, int N, int k_blocks, int blocks, bool deep) {
+    const ClusterCut c = cluster_cut(blocks, deep, M, k_blocks);
     if (blocks > k_blocks || c.stages < 1) return 1e30;
-    const int tiles = (N + 127) / 128, alone = resident_clusters<Tout>(c, SMEM_ROOM), beside = resident_clusters<Tout>(c, c.smem);
-    if (alone < 1 || beside < 1) return 1e30;
-    const double each = (double)((k_blocks + blocks - 1) / blocks) * (0.22 + 0.0011 * c.ntok);
+    // (the driver counts one block an SM for whatever allocates tensor memory; two run where shared memory has room)
+    const int tiles = (N + 127) / 128, alone = resident_clusters<Tout>(c), beside = c.smem + 2048 <= 114 * 1024 ? 2 * alone : alone;
+    if (alone < 1) return 1e30;
+    const double flow = 0.12 + 0.00055 * c.ntok, lag = 1.13 / c.stages;
+    const double each = (double)((k_blocks + blocks - 1) / blocks) * (flow > lag ? flow : lag);
     const int waves = (tiles + alone - 1) / alone, batches = (tiles + beside - 1) / beside;
-    double run = each;
-    if (beside < 2 * alone) run = waves * (each + 0.5) - 0.5;
-    else if (waves > 1) run = 0.63 * waves * each + (batches - 1) * 0.5;
-    const double read = (double)N * k_blocks * BK / MEMORY_BYTES_US;
-    return (run > read ? run : read) + (blocks > 1 ? 0.18 * blocks + 0.0115 * (c.ntok - c.share) : 0.0) + 0.006 * c.share;
+    const double run = beside == alone ? waves * (each + 1.2) - 1.2 + 0.3 : (waves > 1 ? 0.5 * waves : 1.0) * each + (batches - 1) * 1.2;
+    const double read = (double)N * k_blocks * BK / READ_BYTES_US;
+    return (run > read ? run : read) + (blocks > 1 ? 0.15 * blocks + 0.01 * (c.ntok - c.share) : 0.0) + 0.007 * (c.share < c.ntok ? c.share : c.ntok);
 }
 
 // Blocks of a cluster, or minus the tokens of a pair's tile. (The driver is asked how many clusters fit once per size: the choice is kept.)
@@ -819,9 +823,9 @@ int choose(int M, int N, int k_blocks) {
     const auto it = known.find(key);
     if (it != known.end()) return it->second;
     int best = 1;
-    for (int blocks = 1; blocks <= 8; ++blocks) {
-        const double cost = cluster_cost<Tout>(M, N, k_blocks, blocks);
-        if (cost < least) least = cost, best = blocks;
+    for (int cut = 1; cut <= 2 * DEEP - 2; ++cut) {
+        const double cost = cut == DEEP - 1 || cut == DEEP ? 1e30 : cluster_cost<Tout>(M, N, k_blocks, cut % DEEP, cut > DEEP);
+        if (cost < least) least = cost, best = cut;
     }
     if (M >= 48) {
         const int pair = best_pair(least);
@@ -837,7 +841,7 @@ int* jllm_gemm_error_word();
 
 // `rows`: the int8 activations [M, K], their rows at multiples of 16 bytes; `weight`: ops.pack_int8 of the [N, K] weight, its scales filled
 // up to a multiple of 128 and 16-byte aligned; out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a
-// cluster, minus the tokens of a pair's tile, 0 as the sizes have it.
+// cluster (and 10 more: with all of an SM's shared memory), minus the tokens of a pair's tile, 0 as the sizes have it.
 JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo,
                                int accumulate, int swiglu_word, int cut, cudaStream_t stream) {
     const int8_t *a = rows->data, *w_packed = weight->data;
@@ -859,6 +863,7 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     const Product p{a, w_packed, lda, scale_a, scale_w, k_blocks, K, out, out_dtype,
                     Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, M, N, glu}, error_word, stream};
     if (cut == 0) cut = out_dtype == JLLM_F32 ? choose<float>(M, N, k_blocks) : choose<__nv_bfloat16>(M, N, k_blocks);
-    if (cut >= 0) return run_cluster(p, cut);
+    JLLM_REQUIRE(cut <= 2 * DEEP - 2, "gemm_int8: no cut %d", cut);
+    if (cut >= 0) return run_cluster(p, cut % DEEP, cut > DEEP);
     return out_dtype == JLLM_F32 ? run_pair<float>(p, -cut) : run_pair<__nv_bfloat16>(p, -cut);
 }

@@ -1711,7 +1711,7 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
     float32, so a row's result is the same bits in any batch. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or
     bfloat16; `accumulate` as the other products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`;
     no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. `cut` (tests): the blocks of a cluster that share 128
-    weight rows, or minus the tokens of a tile of 256 weight rows; 0: as the sizes have it."""
+    weight rows (and 10 more: with all of an SM's shared memory), or minus the tokens of a tile of 256 weight rows; 0: as the sizes have it."""
     name = "gemm_int8"
     word = glu_kind(swiglu) if swiglu else 0
     if bool(word) != w.glu or isinstance(swiglu, GluUnits):
