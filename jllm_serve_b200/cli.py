@@ -24,6 +24,7 @@ DEFAULTS: Dict[str, Tuple[str, str]] = {
     "model.random-weights": ("", "seed: make random weights for --model-config instead of reading a folder"),
     "model.config": ("", "a config.json to use with model.random-weights"),
     "backend.dtype": ("bf16", "bf16 | fp32 (true 32-bit, no tensor cores)"),
+    "backend.weights": ("", "int8: the layers' weights and rows in 8-bit integers (bf16 models of attention and dense feed-forward layers)"),
     "backend.ctx": ("0", "context length; 0 = the model's max_position_embeddings"),
     "backend.batch": ("512", "rows of one prompt portion (the reference's backend.batch)"),
     "backend.kv-block": ("16", "positions per cache page"),
@@ -51,7 +52,7 @@ DEFAULTS: Dict[str, Tuple[str, str]] = {
 
 ALIASES = {
     "model": "model.dir", "dir": "model.dir", "random-weights": "model.random-weights", "model-config": "model.config",
-    "dtype": "backend.dtype", "ctx": "backend.ctx", "batch": "backend.batch", "chunk": "backend.batch",
+    "dtype": "backend.dtype", "weights": "backend.weights", "ctx": "backend.ctx", "batch": "backend.batch", "chunk": "backend.batch",
     "page-size": "backend.kv-block", "num-pages": "backend.num-pages", "kv-share": "backend.kv-share",
     "max-batch-tokens": "engine.pass-budget",
     "max-running": "engine.max-running", "temp": "sampling.temperature", "temperature": "sampling.temperature",
@@ -146,6 +147,10 @@ class Settings:
     def validate(self) -> "Settings":
         if self.get("backend.dtype") not in ("bf16", "fp32", "bfloat16", "float32"):
             raise SettingsError(f"backend.dtype must be bf16 or fp32, got '{self.get('backend.dtype')}'")
+        if self.get("backend.weights") not in ("", "int8"):
+            raise SettingsError(f"backend.weights must be int8 or empty, got '{self.get('backend.weights')}'")
+        if self.get("backend.weights") == "int8" and self.get("backend.dtype") not in ("bf16", "bfloat16"):
+            raise SettingsError("backend.weights int8 goes with backend.dtype bf16")
         self.integer("backend.ctx", 0)
         self.integer("backend.batch", 1)
         self.integer("backend.kv-block", 1)
@@ -186,7 +191,7 @@ USAGE = """usage: jllm <command> [options]
   bench      measure prefill/decode throughput on a synthetic prompt
   config     print the effective configuration and where each value comes from
 options (override with --config <file> or flags):
-  --model <dir>   --random-weights <seed> --model-config <config.json>   --dtype bf16|fp32
+  --model <dir>   --random-weights <seed> --model-config <config.json>   --dtype bf16|fp32   --weights int8
   --ctx <n>  --batch <n>  --page-size <n>  --num-pages <n|auto>  --kv-share <0..1>  --max-batch-tokens <n>
   --max-running <n>
   --temp <t> --top-k <k> --top-p <p> --min-p <p> --seed <s> --max-tokens <n> --ignore-eos
@@ -200,7 +205,7 @@ def build_engine(s: Settings):
     from .engine import Engine
     batch = s.integer("backend.batch")
     budget = s.integer("engine.pass-budget") or batch + s.integer("engine.mixed-reserve")
-    kw = dict(dtype=s.get("backend.dtype"), ctx=s.integer("backend.ctx") or None,
+    kw = dict(dtype=s.get("backend.dtype"), weights=s.get("backend.weights") or None, ctx=s.integer("backend.ctx") or None,
               page_size=s.integer("backend.kv-block"), kv_share=s.number("backend.kv-share"),
               num_pages="auto" if s.get("backend.num-pages") == "auto" else (s.integer("backend.num-pages") or None),
               max_batch_tokens=budget, chunk=batch, min_chunk=s.integer("engine.min-chunk"),

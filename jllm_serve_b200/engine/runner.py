@@ -42,15 +42,22 @@ class ModelRunner:
                  dtype="bfloat16", device="cuda:0", page_size: int = 16, num_pages=None,
                  max_tokens: Optional[int] = None, max_batch_tokens: int = 2048, max_requests: int = 64,
                  ctx: Optional[int] = None, schedule=None, poison_freed_pages: bool = False,
-                 cuda_graphs: bool = True, kv_share: float = DEFAULT_SHARE):
+                 cuda_graphs: bool = True, kv_share: float = DEFAULT_SHARE, weights: Optional[str] = None):
         """Either `model_dir` (config.json + model.safetensors) or `config` + `seed` (random weights made on
         the device). The pool holds `num_pages` pages per group, or enough for `max_tokens` cached tokens, or,
         with `num_pages="auto"`, the share `kv_share` of the device memory that is free once the weights are
-        loaded (never more than `max_requests` full contexts need)."""
+        loaded (never more than `max_requests` full contexts need). `weights` "int8": the layers' weights are rounded to 8-bit integers
+        when they are loaded, one scale a row, and the rows that meet them at every step, one scale a token (bfloat16 models of
+        attention and dense feed-forward layers; embedding, head, norms and cache stay as they are)."""
         ops.require_device()
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
         self.dtype = _as_dtype(dtype)
+        if weights not in (None, "int8"):
+            raise ValueError(f"weights {weights!r} are not built (int8, or None: as the compute dtype)")
+        if weights == "int8" and self.dtype != torch.bfloat16:
+            raise ValueError("weights in 8-bit integers go with the compute dtype bfloat16")
+        self.weights = weights
         if model_dir is not None:
             spec, raw = load_config(model_dir)
         elif config is not None:
@@ -65,7 +72,7 @@ class ModelRunner:
         self.page_size = int(page_size)
         self.max_rows = int(max_batch_tokens)
         self.max_requests = int(max_requests)
-        rt = Runtime(self.device, self.dtype, self.ctx, self.max_rows, self.page_size)
+        rt = Runtime(self.device, self.dtype, self.ctx, self.max_rows, self.page_size, weights or "")
         wants = model_wants(entry, spec)
         self.notes: List[str] = []
         if model_dir is not None:
@@ -299,6 +306,7 @@ class ModelRunner:
         self.builder = None
         self.last_batch = None
         self.runtime._buffers.clear()
+        self.runtime._int8_rows.clear()
 
     def finish(self, request: Hashable) -> None:
         """The request is over: everything it holds is given back."""
@@ -320,6 +328,6 @@ class ModelRunner:
 
     def describe(self) -> str:
         core = self.spec.core
-        return (f"{core.description} | dtype={str(self.dtype).replace('torch.', '')} ctx={self.ctx} "
+        return (f"{core.description} | dtype={str(self.dtype).replace('torch.', '')}{' weights=int8' if self.weights else ''} ctx={self.ctx} "
                 f"page={self.page_size} pages={self.cache.num_pages} groups={len(self.cache.paged)} "
                 f"max_batch_tokens={self.max_rows}")

@@ -40,7 +40,7 @@ from ..cache.manager import PagedKeysValues
 from ..csrc import ops
 from ..weights.loader import TensorWant
 from .base import Mixer, register_mixer
-from .linear import Linear
+from .linear import Linear, layer_linear
 
 
 def _up8(n: int) -> int:
@@ -94,10 +94,10 @@ class GqaAttention(Mixer):
             if b:
                 b.append(torch.zeros((pad + self.gate_width + tail,), dtype=b[0].dtype, device=b[0].device))
             self.width = self.g_off + self.gate_width + tail
-        self.qkv = Linear(torch.cat(w, dim=0).contiguous(), torch.cat(b).contiguous() if b else None)
+        self.qkv = layer_linear(torch.cat(w, dim=0).contiguous(), torch.cat(b).contiguous() if b else None, runtime)
         self._q_only = None          # the query rows alone, made when a run first reads another run's cache
         del w, b
-        self.out = Linear(tensors.pop(prefix + names.o), tensors.pop(prefix + names.o_bias) if spec.out_bias else None)
+        self.out = layer_linear(tensors.pop(prefix + names.o), tensors.pop(prefix + names.o_bias) if spec.out_bias else None, runtime)
         self.sink = tensors.pop(prefix + names.sink) if spec.sink else None
         self.q_gain = tensors.pop(prefix + names.q_norm) if spec.qk_norm else None
         self.k_gain = tensors.pop(prefix + names.k_norm) if spec.qk_norm else None

@@ -35,9 +35,11 @@ class Runtime:
     max_positions: int                     # the context: positions 0 .. max_positions - 1 can be cached
     max_rows: int                          # most rows (tokens) in one step
     page_size: int
+    weights: str = ""                      # "int8": the products of the parts that know it run in 8-bit integers (parts/linear.py)
 
     def __post_init__(self):
         self._buffers: Dict[str, torch.Tensor] = {}
+        self._int8_rows: dict = {}
         self.notes: list = []              # what a part wants the user to know about how it was built
 
     def buffer(self, name: str, cols: int, dtype: Optional[torch.dtype] = None, rows: Optional[int] = None):
@@ -51,6 +53,17 @@ class Runtime:
             buf = torch.empty((rows or self.max_rows, cols), dtype=dtype, device=self.device)
             self._buffers[key] = buf
         return buf
+
+    def int8_rows(self, name: str, cols: int, rows: int):
+        """The first `rows` rows of a persistent buffer of rows in 8-bit integers, shared as `buffer` is."""
+        from ..csrc import ops
+        key = (name, cols, rows)
+        held = self._int8_rows.get(key)
+        if held is None:
+            whole = self._int8_rows.get((name, cols, None)) or ops.int8_rows(self.max_rows, cols, self.device)
+            self._int8_rows[(name, cols, None)] = whole
+            held = self._int8_rows[key] = whole[:rows]
+        return held
 
 
 class Part:

@@ -48,6 +48,10 @@ class PreNormBlock(Block):
                 raise ValueError("a convolution over the mixer's input is built for the pre_norm arrangement with an RMS norm")
             self.input_conv = tensors[prefix + spec.input_conv]
         self.scale = float(getattr(spec, "residual_scale", 1.0))
+        # products in 8-bit integers: the norms round their results themselves, and the second norm adds the mixer's result
+        self.int8 = runtime.weights == "int8"
+        if self.int8:
+            self.mixer.overwrite = True
         self._scaled_outside = set()
         for part in (self.mixer, self.feed_forward):
             if part is None or self.scale == 1.0:
@@ -56,6 +60,13 @@ class PreNormBlock(Block):
                 part.residual_scale = self.scale
             else:
                 self._scaled_outside.add(id(part))
+
+    @classmethod
+    def takes_int8(cls, spec) -> bool:
+        """Whether a layer of this spec runs with its products in 8-bit integers."""
+        return (cls is PreNormBlock and spec.norm.kind == "rmsnorm" and spec.mixer.kind == "gqa_attention" and not spec.mixer.wide
+                and spec.feed_forward is not None and spec.feed_forward.kind == "dense_glu" and not spec.input_conv
+                and float(getattr(spec, "residual_scale", 1.0)) == 1.0)
 
     @property
     def graph_safe(self) -> bool:
@@ -99,6 +110,8 @@ class PreNormBlock(Block):
             ops.add_scaled(x, y, self.scale)
 
     def forward(self, x, batch, cache) -> None:
+        if self.int8:
+            return self._forward_int8(x, batch, cache)
         xb = self.rt.buffer("normed", self.dim)[:x.shape[0]]
         if self.input_conv is not None:
             ops.norm_conv(x, self.mixer_norm.gain, self.mixer_norm.eps, self.input_conv, cache.block_states[0], batch, xb)
@@ -113,6 +126,15 @@ class PreNormBlock(Block):
         y = self._into(self.feed_forward, x)
         self.feed_forward.forward(xb, y, batch)
         self._settle(x, y)
+
+
+    def _forward_int8(self, x, batch, cache) -> None:
+        rows8 = self.rt.int8_rows("normed", self.dim, x.shape[0])
+        y = self.rt.buffer("mixer_result", self.dim)[:x.shape[0]]
+        self.mixer_norm.forward(x, rows8)
+        self.mixer.forward(rows8, y, batch, cache)
+        self.ffn_norm.forward(x, rows8, add=y)
+        self.feed_forward.forward(rows8, x, batch)
 
 
 register_block("pre_norm", PreNormBlock, replace=True)

@@ -6,6 +6,9 @@ reading bfloat16 and summing in float32. Weights are [out, in] row-major in the 
 (src/main/java/org/robomiri/jllm/cpu/CpuMatmul.java:390-396); for the tensor-core kernels a bfloat16 weight is
 PACKED once, when the part is built (`ops.pack_weight`: tiles of 128 rows x 64 k in the shared-memory image the
 tensor cores read, so a tile is one contiguous bulk copy), and the row-major copy is let go.
+
+With `Runtime.weights` "int8" the layers' products are `Int8Linear`s instead: weight and rows in 8-bit integers, a scale a weight row
+and a scale a token (`ops.gemm_int8`). Half the bytes of a bfloat16 weight, and twice the tensor cores' rate.
 """
 from __future__ import annotations
 
@@ -57,3 +60,37 @@ class Linear:
         else:
             weight = self.weight if self.weight is not None else self.packed.unpack()
             ops.gemm_plain(a, weight, out, self.bias, accumulate)
+
+
+class Int8Linear:
+    """`Linear` in 8-bit integers. The rows come in 8 bits from a norm that rounds them itself (`ops.Int8Rows`), or as a part's bfloat16
+    result, which is rounded here. `glu`: the weight's rows are all gate rows, then all up rows, for `forward(swiglu=...)`."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, runtime, glu: bool = False):
+        assert weight.dim() == 2
+        self.bias, self.rt = bias, runtime
+        self.out_features, self.in_features = weight.shape
+        self.packed = ops.quantize_weight_int8(weight, glu)
+
+    def rows(self, lo: int, hi: int) -> "Int8Linear":
+        """The product with rows [lo, hi) of the weight only."""
+        out = Int8Linear.__new__(Int8Linear)
+        out.bias, out.rt = (self.bias[lo:hi] if self.bias is not None else None), self.rt
+        out.out_features, out.in_features = hi - lo, self.in_features
+        out.packed = ops.pack_int8(self.packed.unpack()[lo:hi].contiguous(), self.packed.scale[lo:hi].contiguous())
+        return out
+
+    def forward(self, a, out: torch.Tensor, accumulate: bool = False, swiglu=False, relu2: bool = False) -> None:
+        """a [rows, in]: `ops.Int8Rows`, or float32 or bfloat16 rows; otherwise as `Linear.forward`."""
+        if a.shape[0] == 0:
+            return
+        if not isinstance(a, ops.Int8Rows):
+            rows8 = self.rt.int8_rows("product_input", self.in_features, a.shape[0])
+            ops.quantize_int8(a, rows8)
+            a = rows8
+        ops.gemm_int8(a, self.packed, out, self.bias, ops.EPILOGUE_RELU2 if relu2 else accumulate, swiglu)
+
+
+def layer_linear(weight: torch.Tensor, bias: torch.Tensor | None, runtime):
+    """The product of a layer's part with a weight [out, in], as the runtime has them."""
+    return Int8Linear(weight, bias, runtime) if runtime.weights == "int8" else Linear(weight, bias)

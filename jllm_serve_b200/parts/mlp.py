@@ -13,7 +13,7 @@ import torch
 from ..csrc import ops
 from ..weights.loader import TensorWant
 from .base import FeedForward, register_feed_forward
-from .linear import Linear
+from .linear import Int8Linear, Linear
 
 
 class DenseGlu(FeedForward):
@@ -28,6 +28,12 @@ class DenseGlu(FeedForward):
         self.glu = ops.glu_descriptor(self.activation, self.limit)
         self.overwrite = False                                      # True: the result replaces x instead of being added to it
         gate, up = tensors.pop(prefix + names[0]), tensors.pop(prefix + names[1])
+        if runtime.weights == "int8":
+            self.fused = spec.hidden % 8 == 0
+            self.gate_up = Int8Linear(torch.cat([gate, up], dim=0), None, runtime, glu=self.fused)
+            del gate, up
+            self.down = Int8Linear(tensors.pop(prefix + names[2]), None, runtime)
+            return
         # bfloat16: blocks of 8 gate rows followed by their 8 up rows, so that the product's epilogue holds a
         # gate value and its up value together and applies SwiGLU itself (no [rows, 2 hidden] round trip)
         self.fused = gate.dtype == torch.bfloat16 and dim % 8 == 0 and spec.hidden % 8 == 0

@@ -22,7 +22,10 @@ class RmsNorm(Norm):
     def wants(cls, spec, dim: int, prefix: str) -> dict:
         return {prefix + getattr(spec, "gain_name", "weight"): TensorWant((dim,), "vector", init="gain")}
 
-    def forward(self, x, out, row_index=None, rows=None):
+    def forward(self, x, out, row_index=None, rows=None, add=None):
+        """`out` may be `ops.Int8Rows`: the result in 8 bits, and `add` (float32 or bfloat16) is added to x in place first."""
+        if isinstance(out, ops.Int8Rows):
+            return ops.add_rmsnorm_int8(x, self.gain, self.eps, out, y=add)
         ops.rmsnorm(x, self.gain, self.eps, out, row_index, rows)
 
 

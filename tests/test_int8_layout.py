@@ -54,3 +54,12 @@ def test_refusals():
                  lambda: ops.pack_int8(zeros(1, ops.INT8_MAX_K + 1, dtype=torch.int8), zeros(1))):
         with pytest.raises(ops.KernelError):
             call()
+
+
+def test_settings_of_the_command_line(tmp_path):
+    from jllm_serve_b200.cli import Settings, SettingsError
+    load = lambda *args: Settings.load(list(args), env={}, cwd=tmp_path).validate()      # noqa: E731
+    assert load().get("backend.weights") == "" and load("--weights", "int8").get("backend.weights") == "int8"
+    for args in (("--weights", "int4"), ("--weights", "int8", "--dtype", "fp32")):
+        with pytest.raises(SettingsError):
+            load(*args)
