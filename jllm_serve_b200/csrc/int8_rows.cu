@@ -153,8 +153,8 @@ template <typename T, int V, bool BLOCK>
 __global__ void __launch_bounds__(MOST_THREADS) quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
                                 int dim) {
     __shared__ uint32_t scratch[64];
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8;
     if (r >= rows) return;
     const T* src = x + (size_t)r * ldx;
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS
         for (int c = 0; c < V; ++c)
             if (at + c * step < dim) gain[c].load(gains + at + c * step, dim - at - c * step, a.g_vec);
     }
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     if (r >= a.rows) return;
     const float* x = a.x + (size_t)r * a.ldx;
     const Ty* y = a.y ? static_cast<const Ty*>(a.y) + (size_t)r * a.ldy : nullptr;
@@ -344,8 +344,8 @@ constexpr int VALUE_ROWS = 4;       // rows that a block of the kernel below goe
 template <typename T>
 __global__ void __launch_bounds__(256)
 values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ scale, T* __restrict__ out, int ldo, bool vec, int rows, int dim) {
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     const int at = (blockIdx.x * 256 + threadIdx.x) * 8, left = dim - at;
     if (left <= 0) return;
     for (int group = blockIdx.y; group * VALUE_ROWS < rows; group += gridDim.y) {
