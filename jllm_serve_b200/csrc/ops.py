@@ -215,6 +215,7 @@ class _Signatures:
     jllm_quantize_int8 = [P, I, I, P, P]
     jllm_add_rmsnorm_int8 = [P, I, P, I, I, P, I, P, I, F, P, P]
     jllm_int8_values = [P, P, I, I, P]
+    jllm_pack_int8 = [P, ctypes.c_longlong, I, I, I, P, P]
     jllm_gemm_int8 = [P, P, P, I, P, I, I, I, I, I, P]
 
 
@@ -1566,13 +1567,14 @@ class _Int8View(ctypes.Structure):          # (Int8View in int8_view.h)
 class Int8Rows:
     """Rows of activations in 8-bit integers: row r stands for data[r] * scale[r]. data int8 [rows, cols], its rows beginning at
     multiples of 16 bytes (`int8_rows` makes such); scale float32 [rows]. A slice of rows is `rows8[lo:hi]`."""
-    __slots__ = ("data", "scale", "rows", "cols", "shape", "stride", "on_gpu", "_view", "view")
+    __slots__ = ("data", "scale", "rows", "cols", "shape", "width", "stride", "on_gpu", "_view", "view")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor):
         if data.dtype != torch.int8 or scale.dtype != torch.float32 or data.dim() != 2 or scale.shape != data.shape[:1]:
             _refuse("Int8Rows", f"int8 data [rows, cols] and a float32 scale for each row, got {data.dtype} {tuple(data.shape)} and {scale.dtype} {tuple(scale.shape)}")
         self.data, self.scale = data, scale
         self.rows, self.cols = self.shape = tuple(data.shape)
+        self.width = (self.cols,)
         self.on_gpu = data.is_cuda and scale.is_cuda and data.device == scale.device
         self.stride = data.stride(0) if self.rows > 1 else -(-self.cols // 16) * 16          # (a single row's stride says nothing)
         if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or self.stride < self.cols or self.stride % 16 or data.data_ptr() % 16
@@ -1597,6 +1599,8 @@ def int8_rows(rows: int, cols: int, device) -> Int8Rows:
 def _row_stride(name, what, t, shape):
     """The row stride of a [rows, cols] matrix with neighbouring values on the GPU."""
     if t.shape == shape and t.is_cuda:
+        if t.is_contiguous():
+            return shape[1]
         down, along = t.stride()
         if shape[0] <= 1:
             down = shape[1]
@@ -1621,7 +1625,7 @@ def add_rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, out: Int8R
     shape, or None (nothing is added, and there is no total); total float32 of x's shape, x itself by default (no other overlap of what
     is read and written); gain float32 or bfloat16 [dim]."""
     name = "add_rmsnorm_int8"
-    if (x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != out.shape[1:] or (gain.stride(0) != 1 and out.cols > 1)
+    if (x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != out.width or not gain.is_contiguous()
             or not gain.is_cuda or not out.on_gpu):
         _refuse(name, f"on the GPU, float32 rows and a float32 or bfloat16 gain of {out.cols} values, got {x.dtype} and {gain.dtype} {tuple(gain.shape)}")
     ldx = _row_stride(name, "x", x, out.shape)
@@ -1686,13 +1690,19 @@ def pack_int8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> Pac
     N, K = data.shape
     if K > INT8_MAX_K or (glu and N % 16):
         _refuse("pack_int8", f"at most {INT8_MAX_K} columns, and gate and up rows in eights, got {N} x {K}")
-    if glu:
-        data, scale = _glu_order(data), _glu_order(scale)
     T, KB = -(-N // 128), -(-K // 128)
-    padded = torch.zeros((T * 128, KB * 128), dtype=torch.int8, device=data.device)
-    padded[:N, :K] = data
-    tiles = padded.view(T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)                  # [T, KB, 128 rows, 8 chunks, 16]
-    packed = tiles.gather(3, _swizzle_index(data.device).expand(T, KB, 128, 8, 16)).contiguous().view(T, KB, 128, 128)
+    if glu:
+        scale = _glu_order(scale)
+    if data.is_cuda:
+        if data.stride(1) != 1 and K > 1:
+            data = data.contiguous()
+        packed = torch.empty((T, KB, 128, 128), dtype=torch.int8, device=data.device)
+        _call("jllm_pack_int8", data.data_ptr(), data.stride(0), N, K, int(glu), packed.data_ptr(), _stream())
+    else:                    # (without a GPU: what the layout is, for whoever looks at it)
+        padded = torch.zeros((T * 128, KB * 128), dtype=torch.int8, device=data.device)
+        padded[:N, :K] = _glu_order(data) if glu else data
+        tiles = padded.view(T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)                  # [T, KB, 128 rows, 8 chunks, 16]
+        packed = tiles.gather(3, _swizzle_index(data.device).expand(T, KB, 128, 8, 16)).contiguous().view(T, KB, 128, 128)
     scales = torch.zeros((T * 128,), dtype=torch.float32, device=data.device)
     scales[:N] = scale
     return PackedInt8(packed, scales, N, K, glu)
@@ -1721,7 +1731,7 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
     if bias is None:
         b, b_dtype = 0, F32
     else:
-        if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_cuda or (bias.stride(0) != 1 and w.rows > 1):
+        if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_cuda or not bias.is_contiguous():
             _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
         b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
     _call("jllm_gemm_int8", a.view, w.view, b, b_dtype, out.data_ptr(), _DT[out.dtype],

@@ -400,6 +400,18 @@ def test_operators_in_a_graph(ops):
     ops.check_kernel_errors()
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 1), (128, 128), (129, 127), (300, 500), (16, 1000), (2064, 336)])
+def test_packing_on_the_gpu_gives_the_layout(ops, rows, cols):
+    (w, scale) = integers(rows, cols + 5, 3)
+    for glu in ([False, True] if rows % 16 == 0 else [False]):
+        for first in (0, 3):                      # rows at any byte
+            want = ops.pack_int8(w[:, first:first + cols], scale, glu)
+            got = ops.pack_int8(w.to(DEV)[:, first:first + cols], scale.to(DEV), glu)
+            assert torch.equal(got.data.cpu(), want.data) and torch.equal(got.scales.cpu(), want.scales) and got.glu == glu
+    apart = w[:, :cols].T.contiguous().to(DEV).T
+    assert torch.equal(ops.pack_int8(apart, scale.to(DEV)).data.cpu(), ops.pack_int8(w[:, :cols], scale).data)
+
+
 def test_weight_in_8_bits(ops):
     w = rnd(300, 500)
     packed = ops.quantize_weight_int8(w.to(torch.bfloat16).to(DEV))
