@@ -204,7 +204,8 @@ struct ClusterArgs {
 };
 
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+    const unsigned long long began = now_ns();
+    for (uint32_t i = 1;; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -212,9 +213,8 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if ((i & 1023u) == 1023u && *abort_flag) return false;
+        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > WAIT_NS)) return false;
     }
-    return false;
 }
 
 // (128 registers a thread: registers are dealt out for eight warps where there are six, and with more no second block fits beside one)
@@ -283,7 +283,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         int s = 0;
         uint32_t parity = 0;                                   // the ring's second lap waits for the first lap's release
         for (int i = stages; i < n_kb; ++i) {
-            if (!warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
+            if (!timed_warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
             if (elect_one()) {
                 const uint32_t dst = base + (uint32_t)s * stage_bytes;
                 mbar_expect_tx(full_bar(s), stage_bytes);
@@ -303,7 +303,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         int s = 0;
         uint32_t parity = 0;
         for (int i = 0; i < n_kb; ++i) {
-            if (!warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
+            if (!timed_warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
             tcgen05_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -333,7 +333,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < g.f.M ? g.scale_a[i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
-        ok = mbar_wait(acc_bar, 0, abort_flag);
+        ok = timed_wait(acc_bar, 0, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         tcgen05_fence_after();
         if (ok)
@@ -524,7 +524,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const uint32_t tx = (wt + 1 < packed_tiles ? 2 : 1) * TILE_BYTES + (uint32_t)g.ntok * BK;     // both blocks' bytes
             int wy = (wt + (int)rank) * k_blocks * 128;                    // row of the packed weight's k block
             for (int kb = 0; kb < k_blocks; ++kb, wy += 128) {
-                if (!warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
+                if (!timed_warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
                 const uint32_t full0 = first_full + 8u * s;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full_bar(s), tx);
@@ -548,11 +548,11 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             bool ok = true;
             for (int tile = pair; ok && tile < tiles; tile += pairs, ++local_tile) {
                 const uint32_t buf = local_tile & 1u;
-                if (!warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                if (!timed_warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                 tcgen05_fence_after();
                 const uint32_t tmem_d = tmem_base + buf * 256;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
+                    if (!timed_warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
                     tcgen05_fence_after();
                     if (elect_one()) {
 #pragma unroll
@@ -586,7 +586,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             TokenEpilogue<Tout> finish(g.f, out, park, scales, n, lane, mine ? g.scale_w[n] : 0.f);
             finish.first = first;
             __syncwarp();
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, timed_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag))) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t taddr = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
             if (mine && n - lane < g.f.N)

@@ -63,6 +63,27 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
 }
 
+// The same with a limit in time: a try may last some microseconds while the thread sleeps, and four million of them minutes. Two seconds
+// are beyond every kernel here; who waits longer gives up, says so and leaves.
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ bool timed_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long began = now_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > WAIT_NS)) return false;
+    }
+}
+__device__ __forceinline__ bool timed_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, timed_wait(bar, parity, abort_flag));
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"

@@ -1,13 +1,14 @@
 """Times the hand-written kernels alone on the layer shapes of a model, against their rooflines.
 
-    python -m jllm_serve_b200.kernel_bench [--rows 8] [--prompt 2048] [--context 4096] [--repeat 20] [--only NAME] [--eager]
+    python -m jllm_serve_b200.kernel_bench [--rows 8] [--prompt 2048] [--context 4096] [--repeat 20] [--only NAME] [--eager] [--int8]
 
 Every kernel runs on random tensors of the shapes one layer of the Qwen3-8B configuration gives it
 (hidden 4096, 32/8 heads of 128, intermediate 12288), timed with CUDA events over `--repeat` calls (replayed
 as one CUDA graph unless `--eager`) that rotate through several copies of the weights, so every call streams
 them from HBM. It prints, per kernel,
 microseconds per call and the achieved GB/s (weight or cache bytes, the decode kernels) or TFLOP/s (the
-prefill kernels). With `--repeat 1` it is the small workload that profilers are pointed at.
+prefill kernels). With `--repeat 1` it is the small workload that profilers are pointed at. `--int8`: the layer's linears in 8-bit
+integers instead (products, norms and quantised rows of both steps).
 """
 from __future__ import annotations
 
@@ -42,6 +43,7 @@ def main() -> int:
     ap.add_argument("--all-kernels", action="store_true",
                     help="the products of the prefill step also on every product kernel that takes their shape, not only "
                          "on the one the dispatch chooses")
+    ap.add_argument("--int8", action="store_true", help="the layer's linears in 8-bit integers, and nothing else")
     args = ap.parse_args()
 
     from .csrc import ops
@@ -63,6 +65,12 @@ def main() -> int:
     def case(name, fn, copies, bytes_=0, flops=0):
         if args.only in name:
             cases.append((name, fn, copies, bytes_, flops))
+
+    if args.int8:
+        int8_cases(ops, case, args, dev, (M, T), D, (H + 2 * Hkv) * hd, F)
+        run_cases(cases, args)
+        ops.check_kernel_errors()
+        return 0
 
     # ---- decode: M rows ----
     a_d, a_f = torch.randn(M, D, device=dev).to(bf), torch.randn(M, F, device=dev).to(bf)
@@ -158,6 +166,39 @@ def main() -> int:
     xbp = torch.empty(T, D, device=dev, dtype=bf)
     case("prefill rmsnorm", lambda i: ops.rmsnorm(x_p, gp, 1e-6, xbp), 1, T * D * 6)
 
+    run_cases(cases, args)
+    ops.check_kernel_errors()
+    return 0
+
+
+def int8_cases(ops, case, args, dev, steps, D, qkv, F) -> None:
+    """The linears of one layer in 8-bit integers, at a decode step's rows and a prompt's."""
+    def weights(n, k, glu=False):
+        copies = max(2, int(300e6 // (n * k)) + 1) if args.repeat > 1 else 1
+        return [ops.quantize_weight_int8(torch.randn(n, k, device=dev) * k ** -0.5, glu) for _ in range(copies)]
+
+    named = {"qkv": weights(qkv, D), "o": weights(D, D), "gate_up + swiglu": weights(2 * F, D, True), "down": weights(D, F)}
+    for step, rows in zip(("decode", "prefill"), steps):
+        for what, ws in named.items():
+            n, k = ws[0].shape
+            a = ops.int8_rows(rows, k, dev)
+            ops.quantize_int8(torch.randn(rows, k, device=dev), a)
+            glu = ws[0].glu
+            out = torch.empty(rows, n // 2 if glu else n, device=dev, dtype=torch.bfloat16)
+            size = dict(bytes_=n * k) if step == "decode" else dict(flops=2 * rows * n * k)
+            case(f"{step} int8 gemm {what}", lambda i, a=a, ws=ws, out=out, glu=glu: ops.gemm_int8(a, ws[i], out, swiglu=glu), len(ws), **size)
+        copies = max(2, int(300e6 // (rows * D * 11)) + 1) if step == "prefill" and args.repeat > 1 else 1
+        xs = [torch.randn(rows, D, device=dev) for _ in range(copies)]
+        ys, ts, qs = [x.bfloat16() for x in xs], [torch.empty_like(x) for x in xs], [ops.int8_rows(rows, D, dev) for _ in xs]
+        gain = torch.ones(D, device=dev, dtype=torch.bfloat16)
+        case(f"{step} int8 rmsnorm with addition", lambda i, xs=xs, ys=ys, ts=ts, qs=qs: ops.add_rmsnorm_int8(xs[i], gain, 1e-6, qs[i], ys[i], ts[i]),
+             copies, rows * D * 11)
+        hs = [torch.randn(rows, F, device=dev).bfloat16() for _ in range(copies)]
+        h8 = [ops.int8_rows(rows, F, dev) for _ in hs]
+        case(f"{step} int8 quantise units", lambda i, hs=hs, h8=h8: ops.quantize_int8(hs[i], h8[i]), copies, rows * F * 3)
+
+
+def run_cases(cases, args) -> None:
     for name, fn, copies, bytes_, flops in cases:
         for i in range(3 if args.repeat > 1 else 0):
             fn(i % copies)
@@ -183,8 +224,6 @@ def main() -> int:
         us = s.elapsed_time(e) / args.repeat * 1e3
         rate = f"{bytes_ / us / 1e3:8.0f} GB/s" if bytes_ else f"{flops / us / 1e6:8.0f} TFLOP/s"
         print(f"{name:36s} {us:9.1f} us {rate}", flush=True)
-    ops.check_kernel_errors()
-    return 0
 
 
 if __name__ == "__main__":
