@@ -99,9 +99,7 @@ __device__ __forceinline__ long long jllm_page_of(const int* __restrict__ table,
 // wait with pdl_wait() until the predecessor has completed and its writes are visible. Every kernel calls
 // pdl_wait() before it reads anything a predecessor wrote or writes anything a predecessor may read, and
 // only then pdl_trigger(), so at most one successor is resident early. Without the launch attribute both
-// calls return at once. (The kernels of int8_rows.cu trigger first: the kernel behind them may then be resident while
-// the one in front of them runs. It still waits for them, and they have waited for that one; and a kernel that takes
-// tensor memory triggers when it has it, so nobody waits for what a later kernel holds.)
+// calls return at once.
 //
 // One thing limits this. An SM cannot change how its memory is split between shared memory and L1 while blocks
 // are resident on it. A kernel whose blocks arrive while a predecessor with a large shared-memory allocation (the

@@ -35,14 +35,6 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -85,12 +77,12 @@ struct TokenEpilogue {
     Tout* out;
     Tout* park;                // the warp's: 16 x 32 values, 16-byte aligned
     const float* token_scales; // shared memory, of the tokens from `first` on, 16-byte aligned
-    int first, n, lane;        // n: this lane's weight row
+    int first, end, n, lane;   // the group's tokens [first, end); n: this lane's weight row
     float sw, b;               // its scale and its bias
     bool vec;
 
     __device__ __forceinline__ TokenEpilogue(const Finish& f_, Tout* out_, Tout* park_, const float* token_scales_, int n_, int lane_, float sw_)
-        : f(f_), out(out_), park(park_), token_scales(token_scales_), first(0), n(n_), lane(lane_), sw(sw_),
+        : f(f_), out(out_), park(park_), token_scales(token_scales_), first(0), end(0), n(n_), lane(lane_), sw(sw_),
           b(f_.has_bias && n_ < f_.N ? f_.bias[n_] : 0.f),
           vec(n_ - lane_ + 32 <= f_.N && ((uintptr_t)out_ & 15u) == 0 && (((size_t)f_.ldo * sizeof(Tout)) & 15u) == 0) {}
 
@@ -133,7 +125,7 @@ struct TokenEpilogue {
                 // (all the old values are requested before the first store: a load behind a store through the same pointer would wait)
                 float old[J];
 #pragma unroll
-                for (int j = 0; j < J; ++j) old[j] = n < f.N && t + j < f.M ? to_float(out[(size_t)(t + j) * f.ldo + n]) : 0.f;
+                for (int j = 0; j < J; ++j) old[j] = n < f.N && t + j < end ? to_float(out[(size_t)(t + j) * f.ldo + n]) : 0.f;
 #pragma unroll
                 for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], old[j]);
             }
@@ -146,7 +138,7 @@ struct TokenEpilogue {
         __syncwarp();
     }
 
-    // parked rows of WIDTH values -> out[t + j, column + ...], only what lies in [M, last)
+    // parked rows of WIDTH values -> out[t + j, column + ...], only what lies in [end, last)
     template <int J, int WIDTH, int PER>
     __device__ __forceinline__ void leave(int t, int column, int last, bool add) const {
         if (vec) {
@@ -156,7 +148,7 @@ struct TokenEpilogue {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 const int i = lane + 32 * s, j = i / PIECES, c = i % PIECES * PER;
-                dst[s] = i < J * PIECES && t + j < f.M ? out + (size_t)(t + j) * f.ldo + column + c : nullptr;
+                dst[s] = i < J * PIECES && t + j < end ? out + (size_t)(t + j) * f.ldo + column + c : nullptr;
                 if (dst[s]) piece[s] = *reinterpret_cast<const uint4*>(park + j * WIDTH + c);
             }
             if (add) {
@@ -180,7 +172,7 @@ struct TokenEpilogue {
             if (column + c < last)
 #pragma unroll
                 for (int j = lane / WIDTH; j < J; j += 32 / WIDTH)
-                    if (t + j < f.M) {
+                    if (t + j < end) {
                         Tout* dst = out + (size_t)(t + j) * f.ldo + column + c;
                         const Tout v = park[j * WIDTH + c];
                         *dst = add ? from_float<Tout>(__fadd_rn(to_float(v), to_float(*dst))) : v;
@@ -199,6 +191,7 @@ struct ClusterArgs {
     const float *scale_w, *scale_a;
     Finish f;
     int k_blocks, ntok, stages, blocks, share;      // ntok: the MMAs' N; share: tokens a block finishes
+    int groups, span;                               // groups of `span` tokens
     uint32_t tmem_cols;
     int* error_word;
 };
@@ -236,9 +229,11 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
-    const int tile = (int)blockIdx.x / blocks, rank = (int)blockIdx.x % blocks;      // (clusters lie along x: this is the rank)
+    // a cluster's 128 weight rows and its group of tokens, the groups fastest: what runs together shares its weights
+    const int unit = (int)blockIdx.x / blocks, rank = (int)blockIdx.x % blocks;      // (clusters lie along x: this is the rank)
+    const int tile = unit / g.groups, first = unit % g.groups * g.span, here = min(g.span, g.f.M - first);
     const int kb_lo = (int)((long long)g.k_blocks * rank / blocks), n_kb = (int)((long long)g.k_blocks * (rank + 1) / blocks) - kb_lo;
-    const int tokens = (g.f.M + 7) & ~7;                              // the accumulator's columns that anybody needs
+    const int tokens = (here + 7) & ~7;                               // the accumulator's columns that anybody needs
     const int mine = rank * share, mine_end = min(mine + share, tokens);
 
     if (threadIdx.x == 0) {
@@ -278,7 +273,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         pdl_trigger();
         if (elect_one())
             for (int i = 0; i < early; ++i)
-                tma_load_2d(base + (uint32_t)i * stage_bytes + TILE_BYTES, &map_a, (kb_lo + i) * BK, 0, full_bar(i));
+                tma_load_2d(base + (uint32_t)i * stage_bytes + TILE_BYTES, &map_a, (kb_lo + i) * BK, first, full_bar(i));
         __syncwarp();
         int s = 0;
         uint32_t parity = 0;                                   // the ring's second lap waits for the first lap's release
@@ -288,11 +283,13 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 const uint32_t dst = base + (uint32_t)s * stage_bytes;
                 mbar_expect_tx(full_bar(s), stage_bytes);
                 bulk_copy(dst, w + (size_t)i * TILE_BYTES, TILE_BYTES, full_bar(s));
-                tma_load_2d(dst + TILE_BYTES, &map_a, (kb_lo + i) * BK, 0, full_bar(s));
+                tma_load_2d(dst + TILE_BYTES, &map_a, (kb_lo + i) * BK, first, full_bar(s));
             }
             __syncwarp();
             if (++s == stages) { s = 0; parity ^= 1u; }
         }
+        // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
+        for (int i = max(0, n_kb - stages); ok && i < n_kb; ++i) ok = timed_warp_wait(empty_bar(i % stages), (uint32_t)(i / stages) & 1u, abort_flag);
         if (!ok && lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 31); }
         if (blocks > 1) cluster_wait();
     } else if (warp == 1) {
@@ -326,11 +323,13 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16);
         const float sw = g.scale_w[n];                        // (filled up to whole tiles)
         // (parks in the ring, which is idle once every MMA is done)
-        const TokenEpilogue<Tout> finish(g.f, out, reinterpret_cast<Tout*>(aligned + (size_t)quad * 2048), token_scales, n, lane, sw);
+        TokenEpilogue<Tout> finish(g.f, out, reinterpret_cast<Tout*>(aligned + (size_t)quad * 2048), token_scales, n, lane, sw);
+        finish.first = first;
+        finish.end = first + here;
         pdl_wait();          // the token scales, and what is added into, were written by the kernels before
         pdl_trigger();
         // (into shared memory while the weights come: asked for in front of every store they were 1 us for 8 tokens)
-        for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < g.f.M ? g.scale_a[i] : 0.f;
+        for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < here ? g.scale_a[first + i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
         ok = timed_wait(acc_bar, 0, abort_flag);
@@ -371,7 +370,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                         sum[4 * q] += x.x, sum[4 * q + 1] += x.y, sum[4 * q + 2] += x.z, sum[4 * q + 3] += x.w;
                     }
                 }
-                finish(sum, t);
+                finish(sum, first + t);
             };
             int t = mine;
             uint32_t sum16[16], sum8[8];
@@ -386,21 +385,25 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(g.tmem_cols) : "memory");
     }
-    // A block whose wait ran out stays until the others have left (their waits are bounded) or come here: they may still send to it.
-    if (blocks > 1 && *abort_flag) {
+    // No block leaves while words that it sent are on their way, or before everything sent to it is there (also where a wait ran out): its
+    // memory is the next block's at once.
+    if (blocks > 1) {
         cluster_arrive();
         cluster_wait();
     }
 }
 
 struct ClusterCut {
-    int blocks, share, ntok, stages;
+    int blocks, share, ntok, stages, groups, span;
     size_t smem;
 };
 // `deep`: the ring takes all shared memory of an SM, else half of it, so that a second block (of this product, or of the next one, whose first
 // weights then come while this one ends) fits beside.
-ClusterCut cluster_cut(int blocks, bool deep, int M, int k_blocks) {
-    ClusterCut c{blocks, ((M + 7) / 8 + blocks - 1) / blocks * 8, (M + 15) / 16 * 16, 0, 0};
+ClusterCut cluster_cut(int blocks, bool deep, int groups, int M, int k_blocks) {
+    const int span = ((M + groups - 1) / groups + 15) / 16 * 16;          // (the last group may be short, or there are fewer)
+    ClusterCut c{blocks, (span / 8 + blocks - 1) / blocks * 8, span, 0, (M + span - 1) / span, span, 0};
+    if (span > 256) return c;
+    if (groups == 1) c.share = ((M + 7) / 8 + blocks - 1) / blocks * 8;
     const size_t stage = TILE_BYTES + (size_t)c.ntok * BK, parts = (size_t)(blocks - 1) * c.share * 512;
     const size_t room = deep ? SMEM_ROOM - 4096 : 104 * 1024;
     c.stages = parts + 2 * stage > room ? 0 : (int)((room - parts) / stage);
@@ -413,204 +416,6 @@ ClusterCut cluster_cut(int blocks, bool deep, int M, int k_blocks) {
     const size_t least = blocks == 1 ? 0 : c.ntok > 128 ? 114 * 1024 : 60 * 1024;
     if (c.smem < least) c.smem = least;
     return c;
-}
-
-// ---- many tokens: two SMs to a tile of 256 weight rows x up to 256 tokens ------------------------------------------------------
-// A cluster of two blocks: each brings 128 weight rows and half of the tile's tokens, one lane of the first block issues MMAs of M 256
-// that read both blocks' shared memory, and each block ends up with its 128 weight rows in its own tensor memory, where two accumulators
-// let a tile's epilogue run under the next tile's main loop. Every copy completes on the FIRST block's "full" barrier of the stage;
-// tcgen05.commit, multicast to both blocks, frees the stage in both. The pairs walk the tiles with the tokens fastest: what is read
-// together shares its weights.
-constexpr int PAIR_THREADS = 320, EPI_WARPS = 8;       // warps 2..9: two to each quarter of the weight rows, taking turns of 16 tokens
-constexpr int PARK_BYTES = EPI_WARPS * 2048, SCALE_BYTES = EPI_WARPS * 1024;
-constexpr size_t PAIR_ROOM = 200 * 1024;
-struct PairArgs {
-    const float *scale_w, *scale_a;
-    Finish f;
-    int k_blocks, ntok, groups, stages;       // ntok: tokens of a tile (a multiple of 32), groups of them
-    int* error_word;
-};
-int pair_stages(int ntok) {
-    const int stages = (int)(PAIR_ROOM / (TILE_BYTES + (size_t)ntok / 2 * BK));
-    return stages > 12 ? 12 : stages;
-}
-size_t pair_smem(int ntok) {
-    const int stages = pair_stages(ntok);
-    return (size_t)stages * (TILE_BYTES + (size_t)ntok / 2 * BK) + PARK_BYTES + SCALE_BYTES + 8 * (2 * stages + 4) + 16 + 1024;
-}
-
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// a tiled copy into THIS block's shared memory that completes on a barrier that may be the partner's
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar)
-        : "memory");
-}
-// arrives, when the MMAs issued so far are done, on the barrier at this offset in both blocks of the pair
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3)
-                 : "memory");
-}
-
-template <typename Tout>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
-gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ PairArgs g,
-                      Tout* __restrict__ out) {
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-    const int stages = g.stages;
-    const uint32_t stage_bytes = TILE_BYTES + (uint32_t)g.ntok / 2 * BK, ring = (uint32_t)stages * stage_bytes;
-    // the stages, the epilogue's rooms, the barriers: full[stages] (the first block's are used), empty[stages] (each block its own),
-    // acc_full[2] (each its own), acc_empty[2] (the first block's); then the TMEM base and the abort flag
-    const uint32_t bars = base + ring + PARK_BYTES + SCALE_BYTES;
-    auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
-    auto acc_full_bar = [&](int b) { return bars + 8u * (2 * stages + b); };
-    auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * stages + 2 + b); };
-    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + ring + PARK_BYTES + SCALE_BYTES + 8 * (2 * stages + 4));
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-
-    const int warp = uniform_warp(), lane = threadIdx.x & 31;
-    uint32_t rank;                                    // 0: the pair's first block, which issues the MMAs
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, k_blocks = g.k_blocks;
-    const int packed_tiles = (g.f.N + 127) >> 7, tiles = ((packed_tiles + 1) >> 1) * g.groups;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
-            mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(acc_full_bar(b), 1);
-            mbar_init(acc_empty_bar(b), 2 * EPI_WARPS);   // one arrival per epilogue warp of both blocks
-        }
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 2) {   // the same warp of both blocks allocates all columns in both (one block per SM)
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
-    tcgen05_fence_before();
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();          // the partner's barriers are set up and its tensor memory is there before anything reaches them
-    tcgen05_fence_after();
-    const uint32_t tmem_base = *tmem_base_slot;
-    pdl_wait();
-    pdl_trigger();
-
-    auto give_up = [&](int code) {
-        *abort_flag = 1;
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1u)), "r"(1) : "memory");
-        atomicExch(g.error_word, code);
-    };
-
-    if (warp == 0) {
-        // ---------------- producer (both blocks) ----------------
-        const uint32_t first_full = in_block(full_bar(0), 0);
-        int s = 0;
-        uint32_t parity = 1, dst = base;
-        bool ok = true;
-        for (int tile = pair; ok && tile < tiles; tile += pairs) {
-            const int row = tile % g.groups * g.ntok + (int)rank * (g.ntok >> 1), wt = tile / g.groups * 2;
-            const bool mine = wt + (int)rank < packed_tiles;               // this block's half of the weight rows exists
-            const uint32_t tx = (wt + 1 < packed_tiles ? 2 : 1) * TILE_BYTES + (uint32_t)g.ntok * BK;     // both blocks' bytes
-            int wy = (wt + (int)rank) * k_blocks * 128;                    // row of the packed weight's k block
-            for (int kb = 0; kb < k_blocks; ++kb, wy += 128) {
-                if (!timed_warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
-                const uint32_t full0 = first_full + 8u * s;
-                if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(full_bar(s), tx);
-                    if (mine) tma_load_2d_pair(dst, &map_w, 0, wy, full0);
-                    tma_load_2d_pair(dst + TILE_BYTES, &map_a, kb * BK, row, full0);
-                }
-                __syncwarp();
-                dst += stage_bytes;
-                if (++s == stages) { s = 0; parity ^= 1u; dst = base; }
-            }
-        }
-        if (!ok && lane == 0) give_up(34);
-    } else if (warp == 1) {
-        // ---------------- MMA issuer (the first block) ----------------
-        if (rank == 0) {
-            const uint32_t idesc = idesc_i8(256, g.ntok);
-            const uint64_t desc_w0 = smem_desc_sw128(base), desc_b0 = smem_desc_sw128(base + TILE_BYTES);
-            uint64_t desc_w = desc_w0, desc_b = desc_b0;          // (a stage further is an addition to the address field)
-            uint32_t local_tile = 0, parity = 0;
-            int s = 0;
-            bool ok = true;
-            for (int tile = pair; ok && tile < tiles; tile += pairs, ++local_tile) {
-                const uint32_t buf = local_tile & 1u;
-                if (!timed_warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                tcgen05_fence_after();
-                const uint32_t tmem_d = tmem_base + buf * 256;
-                for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!timed_warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
-                    tcgen05_fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < BK / 32; ++k)
-                            mma_i8_pair(tmem_d, desc_w + 2 * k, desc_b + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                        commit_pair(empty_bar(s));          // both blocks' stage is free when these MMAs have read it
-                    }
-                    __syncwarp();
-                    desc_w += stage_bytes >> 4;
-                    desc_b += stage_bytes >> 4;
-                    if (++s == stages) { s = 0; parity ^= 1u; desc_w = desc_w0; desc_b = desc_b0; }
-                }
-                if (ok && elect_one()) commit_pair(acc_full_bar(buf));
-                __syncwarp();
-            }
-            if (!ok && lane == 0) give_up(35);
-        }
-    } else {
-        // ---------------- epilogue: warps 2..9 of both blocks, TMEM lanes 32 * (warp % 4) = weight rows of the block's tile ----------------
-        const int quad = warp & 3, turn = (warp - 2) >> 2;
-        Tout* park = reinterpret_cast<Tout*>(aligned + ring + (warp - 2) * 2048);
-        float* scales = reinterpret_cast<float*>(aligned + ring + PARK_BYTES + (warp - 2) * 1024);      // (each warp keeps its own: nobody to wait for)
-        uint32_t local_tile = 0;
-        bool ok = true;
-        for (int tile = pair; ok && tile < tiles; tile += pairs, ++local_tile) {
-            const int first = tile % g.groups * g.ntok, end = min(first + g.ntok, g.f.M), wt = tile / g.groups * 2 + (int)rank;
-            const int n = wt * 128 + quad * 32 + lane;
-            const bool mine = wt < packed_tiles;
-            const uint32_t buf = local_tile & 1u;
-            for (int i = lane; i < g.ntok; i += 32) scales[i] = first + i < g.f.M ? g.scale_a[first + i] : 0.f;
-            TokenEpilogue<Tout> finish(g.f, out, park, scales, n, lane, mine ? g.scale_w[n] : 0.f);
-            finish.first = first;
-            __syncwarp();
-            if (!__all_sync(0xffffffffu, timed_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag))) { ok = false; break; }
-            tcgen05_fence_after();
-            const uint32_t taddr = tmem_base + buf * 256 + ((uint32_t)(quad * 32) << 16);
-            if (mine && n - lane < g.f.N)
-#pragma unroll 1
-                for (int t = first + 16 * turn; t < end; t += 32) {
-                    uint32_t sum[16];
-                    tmem_ld(taddr + (t - first), sum);
-                    tmem_ld_wait();
-                    finish(sum, t);
-                }
-            tcgen05_fence_before();          // this warp has read the accumulator
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(in_block(acc_empty_bar(buf), 0));
-        }
-        if (!ok && lane == 0) give_up(36);
-    }
-    tcgen05_fence_before();
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();          // neither block leaves, or frees tensor memory, while the other may still reach into it
-    if (warp == 2) {
-        tcgen05_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
-    }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
@@ -676,46 +481,25 @@ int launch_cluster(const CUtensorMap& map_a, const ClusterArgs& g, const Cluster
     return jllm_check_launch("gemm_int8_cluster");
 }
 
-// clusters of that many blocks that the device runs at a time, one block an SM
+// clusters of that many blocks that the device runs at a time, one block an SM; asked once per device
 template <typename Tout>
-int resident_clusters(const ClusterCut& c) {
+int resident_clusters(int blocks) {
+    static int known[64][9] = {};          // (one more than the answer)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (known[dev][blocks]) return known[dev][blocks] - 1;
     int n = 0;
+    ClusterCut one{};
+    one.blocks = blocks, one.smem = SMEM_ROOM;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = cluster_config<Tout>(c, 1, attr, nullptr);
-    if (jllm_allow_smem((const void*)gemm_int8_cluster_kernel<Tout>, c.smem) != cudaSuccess ||
+    const cudaLaunchConfig_t cfg = cluster_config<Tout>(one, 1, attr, nullptr);
+    if (jllm_allow_smem((const void*)gemm_int8_cluster_kernel<Tout>, SMEM_ROOM) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, gemm_int8_cluster_kernel<Tout>, &cfg) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    return n;
-}
-
-// pairs of blocks that the device runs at a time (with all the shared memory a pair may ask for), looked up once
-template <typename Tout>
-int resident_pairs() {
-    static int pairs = -1;
-    if (pairs >= 0) return pairs;
-    auto kern = gemm_int8_pair_kernel<Tout>;
-    size_t smem = 0;
-    for (int ntok = 32; ntok <= 256; ntok += 32) smem = pair_smem(ntok) > smem ? pair_smem(ntok) : smem;
-    if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess) return 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (jllm_device_sm_count() > 0 ? jllm_device_sm_count() : 2));
-    cfg.blockDim = dim3(PAIR_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = 0;
     }
-    return pairs = n;
+    known[dev][blocks] = n + 1;
+    return n;
 }
 
 struct Product {
@@ -730,106 +514,76 @@ struct Product {
     cudaStream_t stream;
 };
 
-int run_cluster(const Product& p, int blocks, bool deep) {
+// What stands for a cut in one number: the blocks of a cluster, 10 more with a deep ring, 100 more for each group of tokens
+constexpr int DEEP = 10, GROUP = 100;
+struct Cut {
+    int blocks, groups;
+    bool deep;
+};
+Cut cut_of(int code, int M) {
+    const int groups = code / GROUP;
+    return {code % DEEP, groups > 0 ? groups : (M + 255) / 256, code % GROUP > DEEP};
+}
+
+int run_cluster(const Product& p, int code) {
     const int M = p.f.M;
-    JLLM_REQUIRE(blocks >= 1 && blocks <= 8 && blocks <= p.k_blocks && M <= 256 && cluster_cut(blocks, deep, M, p.k_blocks).stages >= 1,
-                 "gemm_int8: clusters of %d blocks do not take %d rows of %d k blocks", blocks, M, p.k_blocks);
-    const ClusterCut c = cluster_cut(blocks, deep, M, p.k_blocks);
+    const Cut cut = cut_of(code, M);
+    JLLM_REQUIRE(code > 0 && code % GROUP < 2 * DEEP && cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= p.k_blocks && cut.groups <= M,
+                 "gemm_int8: no cut %d for %d rows of %d k blocks", code, M, p.k_blocks);
+    const ClusterCut c = cluster_cut(cut.blocks, cut.deep, cut.groups, M, p.k_blocks);
+    JLLM_REQUIRE(c.stages >= 1, "gemm_int8: clusters of %d blocks do not take %d rows in %d groups", cut.blocks, M, cut.groups);
+    const long long units = (long long)((p.f.N + 127) / 128) * c.groups;
+    JLLM_REQUIRE(units * c.blocks < (1LL << 31) && (long long)(c.groups + 1) * c.span < (1LL << 31), "gemm_int8: %lld tiles of %d rows", units, M);
     CUtensorMap map_a;
     const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, true, &map_a);
     if (rc != JLLM_OK) return rc;
     uint32_t cols = 32;
     while ((int)cols < c.ntok) cols <<= 1;
-    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, cols, p.error_word};
-    const int tiles = (p.f.N + 127) / 128;
-    return p.out_dtype == JLLM_F32 ? launch_cluster<float>(map_a, g, c, tiles, p.out, p.stream)
-                                   : launch_cluster<__nv_bfloat16>(map_a, g, c, tiles, p.out, p.stream);
+    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, c.groups, c.span, cols, p.error_word};
+    return p.out_dtype == JLLM_F32 ? launch_cluster<float>(map_a, g, c, (int)units, p.out, p.stream)
+                                   : launch_cluster<__nv_bfloat16>(map_a, g, c, (int)units, p.out, p.stream);
 }
 
-template <typename Tout>
-int run_pair(const Product& p, int ntok) {
-    JLLM_REQUIRE(ntok >= 32 && ntok <= 256 && ntok % 32 == 0, "gemm_int8: tiles of 32, 64 .. 256 tokens, not %d", ntok);
-    const long long packed_rows = (long long)((p.f.N + 127) / 128) * p.k_blocks * 128;
-    JLLM_REQUIRE(packed_rows < (1LL << 31), "gemm_int8: a packed weight of %lld rows of 128 bytes is too long", packed_rows);
-    CUtensorMap map_a, map_w;
-    int rc = byte_map_for(p.a, p.f.M, p.K, p.lda, ntok / 2, true, &map_a);
-    if (rc != JLLM_OK) return rc;
-    rc = byte_map_for(p.w, packed_rows, 128, 128, 128, false, &map_w);
-    if (rc != JLLM_OK) return rc;
-    int pairs = resident_pairs<Tout>();
-    JLLM_REQUIRE(pairs >= 1, "gemm_int8: the device runs no cluster of two blocks with %zu bytes of shared memory", pair_smem(ntok));
-    const int groups = (p.f.M + ntok - 1) / ntok;
-    const long long tiles = (long long)groups * ((p.f.N + 255) / 256);
-    JLLM_REQUIRE(tiles < (1LL << 31) - 1024, "gemm_int8: %lld tiles", tiles);
-    if (pairs > tiles) pairs = (int)tiles;
-    const PairArgs g{p.scale_w, p.scale_a, p.f, p.k_blocks, ntok, groups, pair_stages(ntok), p.error_word};
-    jllm_launch(gemm_int8_pair_kernel<Tout>, dim3(2 * pairs), dim3(PAIR_THREADS), pair_smem(ntok), p.stream, LAUNCH_DEPENDENT, map_a, map_w, g,
-                static_cast<Tout*>(p.out));
-    return jllm_check_launch("gemm_int8_pair");
-}
-
-// What a product takes, about, in us (up to what all ways take alike), fitted to 846 sizes of 1 to 256 rows against 128 to 34,816 weight
-// rows of 256 to 17,408 values, launched back to back on weights larger than L2: what it chooses is 2.1% slower than the best way of each
-// size in the geometric mean (up to 16 rows 2.2, 17 to 64 2.9, 65 to 128 2.0, 129 to 256 0.9%; the pairs of 558 sizes of 300 to 2,048 rows
-// 0.2%). Deep rings are 9% of that.
-//   clusters: a block's k blocks, each a ring's share of the 1.13 us that a copy is on its way, or 0.12 us and 0.55 ns a token; all clusters
-//   at once, one block an SM, or (half of that a round) two blocks side by side, or one batch behind the other; nothing of the next product
-//   beside it: 0.3 us; sending 0.15 us a block of the cluster and 10 ns a token sent;
-//   pairs: rounds of tiles, a k block 0.126 us and 0.2 ns a token; 1.55 us more from launch to first results;
-//   both: no faster than memory and L2 give the weights.
-constexpr int DEEP = 10;              // a cluster's cut: its blocks, and 10 more with all of an SM's shared memory
+// @COST
 constexpr double READ_BYTES_US = 1e7;
-double pair_cost(int M, int N, int k_blocks, int ntok, int pairs) {
-    const long long tiles = (long long)((N + 255) / 256) * ((M + ntok - 1) / ntok), rounds = (tiles + pairs - 1) / pairs;
-    const double run = (double)rounds * (k_blocks < 3 ? 3 : k_blocks) * (0.126 + 0.0002 * ntok), read = (double)N * k_blocks * BK / READ_BYTES_US;
-    return 1.55 + (run > read ? run : read) + 0.0016 * ntok;
-}
 template <typename Tout>
-double cluster_cost(int M, int N, int k_blocks, int blocks, bool deep) {
-    const ClusterCut c = cluster_cut(blocks, deep, M, k_blocks);
-    if (blocks > k_blocks || c.stages < 1) return 1e30;
+double cluster_cost(int M, int N, int k_blocks, const Cut& cut) {
+    const ClusterCut c = cluster_cut(cut.blocks, cut.deep, cut.groups, M, k_blocks);
+    if (cut.blocks > k_blocks || c.stages < 1) return 1e30;
     // (the driver counts one block an SM for whatever allocates tensor memory; two run where shared memory has room)
-    const int tiles = (N + 127) / 128, alone = resident_clusters<Tout>(c), beside = c.smem + 2048 <= 114 * 1024 ? 2 * alone : alone;
+    const long long units = (long long)((N + 127) / 128) * c.groups;
+    const int alone = resident_clusters<Tout>(cut.blocks), beside = c.smem + 2048 <= 114 * 1024 ? 2 * alone : alone;
     if (alone < 1) return 1e30;
     const double flow = 0.12 + 0.00055 * c.ntok, lag = 1.13 / c.stages;
-    const double each = (double)((k_blocks + blocks - 1) / blocks) * (flow > lag ? flow : lag);
-    const int waves = (tiles + alone - 1) / alone, batches = (tiles + beside - 1) / beside;
+    const double each = (double)((k_blocks + cut.blocks - 1) / cut.blocks) * (flow > lag ? flow : lag);
+    const double waves = (double)((units + alone - 1) / alone), batches = (double)((units + beside - 1) / beside);
     const double run = beside == alone ? waves * (each + 1.2) - 1.2 + 0.3 : (waves > 1 ? 0.5 * waves : 1.0) * each + (batches - 1) * 1.2;
     const double read = (double)N * k_blocks * BK / READ_BYTES_US;
-    return (run > read ? run : read) + (blocks > 1 ? 0.15 * blocks + 0.01 * (c.ntok - c.share) : 0.0) + 0.007 * (c.share < c.ntok ? c.share : c.ntok);
+    return (run > read ? run : read) + (cut.blocks > 1 ? 0.15 * cut.blocks + 0.01 * (c.ntok - c.share) : 0.0) + 0.007 * (c.share < c.ntok ? c.share : c.ntok);
 }
 
-// Blocks of a cluster, or minus the tokens of a pair's tile. (The driver is asked how many clusters fit once per size: the choice is kept.)
+// The cut for a product. (Worked out once per size: the choice is kept.)
 template <typename Tout>
 int choose(int M, int N, int k_blocks) {
-    const int pairs = resident_pairs<Tout>();
-    auto best_pair = [&](double& least) {
-        int best = 0;
-        for (int ntok = 256; pairs > 0 && ntok >= 32; ntok -= 32) {
-            if (ntok >= M + 32) continue;
-            const double cost = pair_cost(M, N, k_blocks, ntok, pairs);
-            if (cost < least) least = cost, best = -ntok;
-        }
-        return best;
-    };
-    double least = 1e30;
-    if (M > 256) return best_pair(least);
     static std::mutex mu;
-    static std::unordered_map<unsigned long long, int> known;
+    static std::unordered_map<MapKey, int, MapKeyHash> known;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
-    const unsigned long long key = (((unsigned long long)N << 11 | (unsigned)k_blocks) << 9 | (unsigned)M) << 6 | (unsigned)(dev & 63);
+    const MapKey key{nullptr, M, N, k_blocks, dev};
     std::lock_guard<std::mutex> lock(mu);
     const auto it = known.find(key);
     if (it != known.end()) return it->second;
-    int best = 1;
-    for (int cut = 1; cut <= 2 * DEEP - 2; ++cut) {
-        const double cost = cut == DEEP - 1 || cut == DEEP ? 1e30 : cluster_cost<Tout>(M, N, k_blocks, cut % DEEP, cut > DEEP);
-        if (cost < least) least = cost, best = cut;
-    }
-    if (M >= 48) {
-        const int pair = best_pair(least);
-        if (pair) best = pair;
+    int best = 1 + GROUP * ((M + 255) / 256);
+    double least = 1e30;
+    for (int span = 16; span <= 256; span += 16) {
+        if (M <= 256 && span < (M + 15) / 16 * 16) continue;         // (few tokens are one group: another would read the weights again)
+        const int groups = (M + span - 1) / span;
+        for (int ring = 0; ring < 2; ++ring)
+            for (int blocks = 1; blocks <= 8; ++blocks) {
+                const double cost = cluster_cost<Tout>(M, N, k_blocks, {blocks, groups, ring == 1});
+                if (cost < least) least = cost, best = blocks + DEEP * ring + GROUP * groups;
+            }
+        if (M <= 256) break;
     }
     if (known.size() >= 4096) known.clear();
     return known[key] = best;
@@ -841,7 +595,7 @@ int* jllm_gemm_error_word();
 
 // `rows`: the int8 activations [M, K], their rows at multiples of 16 bytes; `weight`: ops.pack_int8 of the [N, K] weight, its scales filled
 // up to a multiple of 128 and 16-byte aligned; out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a
-// cluster (and 10 more: with all of an SM's shared memory), minus the tokens of a pair's tile, 0 as the sizes have it.
+// cluster, 10 more with a ring of all of an SM's shared memory, 100 more for each group of tokens; 0 as the sizes have it.
 JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo,
                                int accumulate, int swiglu_word, int cut, cudaStream_t stream) {
     const int8_t *a = rows->data, *w_packed = weight->data;
@@ -863,7 +617,5 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     const Product p{a, w_packed, lda, scale_a, scale_w, k_blocks, K, out, out_dtype,
                     Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, M, N, glu}, error_word, stream};
     if (cut == 0) cut = out_dtype == JLLM_F32 ? choose<float>(M, N, k_blocks) : choose<__nv_bfloat16>(M, N, k_blocks);
-    JLLM_REQUIRE(cut <= 2 * DEEP - 2, "gemm_int8: no cut %d", cut);
-    if (cut >= 0) return run_cluster(p, cut % DEEP, cut > DEEP);
-    return out_dtype == JLLM_F32 ? run_pair<float>(p, -cut) : run_pair<__nv_bfloat16>(p, -cut);
+    return run_cluster(p, cut);
 }

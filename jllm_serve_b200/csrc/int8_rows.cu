@@ -154,14 +154,12 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
 template <bool BLOCK> __device__ __forceinline__ int my_row() { return BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); }
 template <bool BLOCK> __device__ __forceinline__ int my_place() { return BLOCK ? threadIdx.x : threadIdx.x & 31; }
 
-// The kernel behind one of these may come to the SMs before the kernel in front has ended (it waits for this one, and this one for that): a
-// product then has its first weights under way while its rows are made. A decode step of an 8B model, one request: 2.25 -> 2.00 ms.
 template <typename T, int V, bool BLOCK>
 __global__ void __launch_bounds__(MOST_THREADS) quantize_kernel(const T* __restrict__ x, int ldx, bool vec, int8_t* __restrict__ q, int ldq, float* __restrict__ scale, int rows,
                                 int dim) {
     __shared__ uint32_t scratch[64];
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     const int r = my_row<BLOCK>(), at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8;
     if (r >= rows) return;
     const T* src = x + (size_t)r * ldx;
@@ -229,8 +227,8 @@ __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS
         for (int c = 0; c < V; ++c)
             if (at + c * step < dim) gain[c].load(gains + at + c * step, dim - at - c * step, a.g_vec);
     }
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     if (r >= a.rows) return;
     const float* x = a.x + (size_t)r * a.ldx;
     const Ty* y = a.y ? static_cast<const Ty*>(a.y) + (size_t)r * a.ldy : nullptr;
@@ -351,8 +349,8 @@ constexpr int VALUE_ROWS = 4;       // rows that a block of the kernel below goe
 template <typename T>
 __global__ void __launch_bounds__(256)
 values_kernel(const int8_t* __restrict__ q, int ldq, const float* __restrict__ scale, T* __restrict__ out, int ldo, bool vec, int rows, int dim) {
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     const int at = (blockIdx.x * 256 + threadIdx.x) * 8, left = dim - at;
     if (left <= 0) return;
     for (int group = blockIdx.y; group * VALUE_ROWS < rows; group += gridDim.y) {

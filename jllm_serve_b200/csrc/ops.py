@@ -1196,7 +1196,7 @@ def bounds_errors() -> dict:
 
 # Which kernel a code in an error word is from: the products share one word, the attention kernels another.
 WAIT_KERNELS = {"products": ((1, 3, "gemm_tcgen05"), (11, 13, "gemm_stream"), (14, 16, "gemm_stream (clusters)"), (21, 23, "gemm_pair"),
-                             (31, 33, "gemm_int8 (clusters)"), (34, 36, "gemm_int8 (pairs)")),
+                             (31, 33, "gemm_int8")),
                 "attention": ((21, 23, "attention_prefill_tc"), (31, 33, "attention_prefill_pair"), (41, 43, "attention_prefill_latent"),
                               (51, 52, "attention_decode_ring"))}
 
@@ -1721,7 +1721,7 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
     float32, so a row's result is the same bits in any batch. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or
     bfloat16; `accumulate` as the other products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`;
     no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. `cut` (tests): the blocks of a cluster that share 128
-    weight rows (and 10 more: with all of an SM's shared memory), or minus the tokens of a tile of 256 weight rows; 0: as the sizes have it."""
+    weight rows, 10 more with a ring of all of an SM's shared memory, 100 more for each group of tokens; 0: as the sizes have it."""
     name = "gemm_int8"
     word = glu_kind(swiglu) if swiglu else 0
     if bool(word) != w.glu or isinstance(swiglu, GluUnits):

@@ -298,14 +298,15 @@ def test_product_gated(ops, rows, hidden, kind):
     ops.check_kernel_errors()
 
 
-@pytest.mark.parametrize("cut,rows,width,dim", [(1, 1, 128, 128), (1, 256, 300, 1300), (2, 3, 200, 300), (3, 17, 129, 1000), (4, 40, 1003, 2049), (15, 200, 70, 900),
-                                                (16, 256, 260, 4096), (17, 100, 256, 1025), (18, 256, 400, 3000), (8, 8, 384, 8192), (8, 1, 100, 1024), (11, 1, 700, 4096), (11, 256, 129, 500), (12, 40, 1003, 2049), (13, 64, 400, 2500),
-                                                (14, 250, 130, 3000), (16, 16, 384, 8192), (18, 256, 200, 1024), (18, 7, 1400, 2300), (2, 144, 300, 256), (12, 160, 129, 129),
-                                                (7, 24, 64, 12000),
-                                                (-64, 1, 10, 20), (-64, 130, 250, 700), (-64, 700, 400, 333), (-64, 2048, 3000, 256),
-                                                (-128, 257, 129, 500), (-128, 256, 1000, 640), (-128, 1200, 4224, 300),
-                                                (-32, 1, 3, 9), (-32, 300, 600, 1000), (-96, 500, 1111, 2000), (-160, 300, 2600, 513), (-160, 159, 129, 4096), (-192, 400, 900, 260),
-                                                (-224, 777, 1003, 2049), (-256, 300, 128, 200), (-256, 513, 700, 1111), (-256, 2100, 5000, 300), (-256, 5, 257, 150)])
+@pytest.mark.parametrize("cut,rows,width,dim", [
+    (1, 1, 128, 128), (11, 256, 300, 1300), (2, 3, 200, 300), (3, 17, 129, 1000), (4, 40, 1003, 2049), (15, 200, 70, 900), (16, 256, 260, 4096),
+    (17, 100, 256, 1025), (18, 256, 400, 3000), (8, 8, 384, 8192), (8, 1, 100, 1024), (11, 1, 700, 4096), (11, 256, 129, 500), (12, 40, 1003, 2049),
+    (13, 64, 400, 2500), (14, 250, 130, 3000), (16, 16, 384, 8192), (18, 256, 200, 1024), (18, 7, 1400, 2300), (2, 144, 300, 256), (12, 160, 129, 129),
+    (7, 24, 64, 12000),
+    # groups of tokens: even ones, a short last one, fewer than were asked for, one token in the last
+    (201, 32, 10, 20), (202, 130, 250, 700), (211, 300, 2600, 513), (301, 257, 129, 500), (312, 700, 400, 333), (401, 777, 1003, 2049),
+    (512, 513, 700, 1111), (812, 2048, 3000, 256), (911, 2100, 5000, 300), (713, 100, 300, 900), (1201, 777, 1003, 2049), (3002, 500, 257, 640),
+    (1001, 161, 128, 200), (218, 500, 130, 1500), (1712, 4100, 130, 300)])
 def test_product_cut_up(ops, cut, rows, width, dim):
     """Every way of cutting the work gives the same bits."""
     (a, sa), (w, sw) = integers(rows, dim, 11), integers(width, dim, 12)
@@ -448,7 +449,8 @@ def test_refusals(ops):
             lambda: ops.gemm_int8(a8, packed, out, cut=10),
             lambda: ops.gemm_int8(a8, packed, out, cut=19),
             lambda: ops.gemm_int8(a8, packed, out, cut=21),
-            lambda: ops.gemm_int8(a8, packed, out, cut=-48),
+            lambda: ops.gemm_int8(a8, packed, out, cut=501),              # more groups than rows
+            lambda: ops.gemm_int8(a8, packed, out, cut=-64),
             lambda: ops.gemm_int8(ops.int8_rows(4, 48, DEV), packed, out),
             lambda: ops.gemm_int8(ops.Int8Rows(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4)), packed, out)):
         with pytest.raises(E):
