@@ -8,9 +8,9 @@
 // k_blocks + kb) * 16 KB; its scales are filled up to whole tiles. The activations' tiles come by tiled TMA copies, which fill rows
 // beyond M and k beyond K with zeros.
 //
-// In both kernels the weight rows are the M side of the MMAs and the tokens the N side, so that tokens are filled up to a multiple of 16
-// or 32 and not of 128. Few tokens (`cluster`): a cluster of blocks shares the k blocks of 128 weight rows. Many tokens (`pair`): two SMs to
-// a tile of 256 weight rows x up to 256 tokens. Every wait is bounded and raises the products' error word (codes 31-33 cluster, 34-36 pair).
+// The weight rows are the M side of the MMAs and the tokens the N side, so that tokens are filled up to a multiple of 16 and not of 128. A cluster of
+// one to eight blocks has 128 weight rows and a group of up to 256 tokens, each block a part of the k blocks. Every wait is bounded and raises
+// the products' error word (codes 31-33).
 #include "tcgen05_common.cuh"
 #include "int8_view.h"
 
@@ -181,11 +181,19 @@ struct TokenEpilogue {
     }
 };
 
-// ---- few tokens: a cluster of blocks to 128 weight rows --------------------------------------------------------------------
+// ---- a cluster of blocks to 128 weight rows and a group of tokens --------------------------------------------------------------
 // With few tokens the product is nothing but reading W once. Block p of a cluster streams its part of the tile's k blocks (one contiguous
 // 16 KB bulk copy each, requested before the kernel in front has finished: weights are nobody's output); the accumulator [128 weight
 // rows x tokens] lies in its tensor memory. Of the tokens every block finishes a share: the others send their parts of it (st.async,
-// which counts its bytes on the owner's mbarrier: one way through the cluster and no meeting), the owner adds them up, scales and stores.
+// which counts its bytes on the owner's mbarrier: one way through the cluster), the owner adds them up, scales and stores.
+// Bound by memory where the weight is large: one row against 24,576 x 4,096 17.3 us (5.8 TB/s, 0.89 of the
+// measured copy), 4,096 x 12,288 10.7 (4.7), 64 rows of it 11.1;
+// below that by the way from launch to last store (about 3 us beside the stream: 5.5 us for the 16.8 MB of 4,096 x 4,096).
+// With many tokens it is what an SM takes in: a ring of 200 KB (or two of 100 KB: two blocks an SM, the one's epilogue under the other's main
+// loop) against the 1 to 2 us that a copy is on its way when all SMs ask. 2,048 rows of 24,576 x 4,096, gated: 173 us alone (2.4 POP/s), 199 one behind the other under the
+// power limit. (Pairs of
+// SMs with `cta_group::2`, which take in a third less, took 130 us for it (147 under the limit), and 29 where 300 rows take 40 here. In a model's prompt steps one of them stopped
+// once in some thousands of passes and no wait gave up; the cause was not found by reading, so they are gone.)
 struct ClusterArgs {
     const int8_t* w;
     const float *scale_w, *scale_a;
@@ -544,7 +552,11 @@ int run_cluster(const Product& p, int code) {
                                    : launch_cluster<__nv_bfloat16>(map_a, g, c, (int)units, p.out, p.stream);
 }
 
-// @COST
+// What a product takes, about, in us (up to what all ways take alike), fitted to products launched back to back on weights larger than L2.
+// Up to 256 rows (one group; 846 sizes of 1 to 256 rows against 128 to 34,816 weight rows of 256 to 17,408 values: what is chosen is 2.1% slower than
+// the best way of each size in the geometric mean): a block's k blocks, each a ring's share of the 1.13 us that a copy is on its way, or 0.12 us and
+// 0.55 ns a token; all clusters at once, one block an SM, or (half of that a round) two blocks side by side, or one batch behind the other; nothing
+// of the next product beside it: 0.3 us; sending 0.15 us a block of the cluster and 10 ns a token sent; no faster than memory and L2 give the weights.
 constexpr double READ_BYTES_US = 1e7;
 template <typename Tout>
 double cluster_cost(int M, int N, int k_blocks, const Cut& cut) {
@@ -560,6 +572,33 @@ double cluster_cost(int M, int N, int k_blocks, const Cut& cut) {
     const double run = beside == alone ? waves * (each + 1.2) - 1.2 + 0.3 : (waves > 1 ? 0.5 * waves : 1.0) * each + (batches - 1) * 1.2;
     const double read = (double)N * k_blocks * BK / READ_BYTES_US;
     return (run > read ? run : read) + (cut.blocks > 1 ? 0.15 * cut.blocks + 0.01 * (c.ntok - c.share) : 0.0) + 0.007 * (c.share < c.ntok ? c.share : c.ntok);
+}
+
+// More rows (groups of them; 162 sizes of 300 to 2,048 rows against 1,024 to 24,576 weight rows of 1,024 to 12,288 values: 1.6%): all SMs take in at once.
+// One block an SM: rounds of k blocks, each the ring's share of 1.06 us, or 0.135 us and 0.27 ns a token, and 1.9 us and 10 ns a token to begin and
+// end. Two blocks side by side: the SM's share of all k blocks at 0.215 us and 0.25 ns a token (or a ring's share of 1.45 us), an end that shows
+// once, 2 us a batch. Sending 0.55 us a block of the cluster and 43 ns a token.
+template <typename Tout>
+double groups_cost(int M, int N, int k_blocks, const Cut& cut) {
+    const ClusterCut c = cluster_cut(cut.blocks, cut.deep, cut.groups, M, k_blocks);
+    if (cut.blocks > k_blocks || c.stages < 1) return 1e30;
+    const long long units = (long long)((N + 127) / 128) * c.groups;
+    const int alone = resident_clusters<Tout>(cut.blocks), sms = resident_clusters<Tout>(1), beside = c.smem + 2048 <= 114 * 1024 ? 2 * alone : alone;
+    if (alone < 1 || sms < 1) return 1e30;
+    const int each_kb = (k_blocks + cut.blocks - 1) / cut.blocks, mine = c.share < c.ntok ? c.share : c.ntok;
+    const double flow = 0.135 + 0.00027 * c.ntok, lag = 1.06 / c.stages, each = each_kb * (flow > lag ? flow : lag), end = 0.0104 * mine;
+    const double waves = (double)((units + alone - 1) / alone), batches = (double)((units + beside - 1) / beside);
+    double run = waves * (each + 1.9 + end);
+    if (beside > alone) {
+        const double two = 0.215 + 0.00025 * c.ntok, two_lag = 1.45 / (2 * c.stages);
+        run = each + end;
+        if (waves > 1) {
+            const double shared = (double)(units * cut.blocks) / sms * each_kb * (two > two_lag ? two : two_lag);
+            run = (run > shared ? run : shared) + end;
+        }
+        run += (batches - 1) * 2.0;
+    }
+    return run + (cut.blocks > 1 ? 0.55 * cut.blocks + 0.043 * (c.ntok - c.share) : 0.0);
 }
 
 // The cut for a product. (Worked out once per size: the choice is kept.)
@@ -580,7 +619,8 @@ int choose(int M, int N, int k_blocks) {
         const int groups = (M + span - 1) / span;
         for (int ring = 0; ring < 2; ++ring)
             for (int blocks = 1; blocks <= 8; ++blocks) {
-                const double cost = cluster_cost<Tout>(M, N, k_blocks, {blocks, groups, ring == 1});
+                const Cut cut{blocks, groups, ring == 1};
+                const double cost = M <= 256 ? cluster_cost<Tout>(M, N, k_blocks, cut) : groups_cost<Tout>(M, N, k_blocks, cut);
                 if (cost < least) least = cost, best = blocks + DEEP * ring + GROUP * groups;
             }
         if (M <= 256) break;
