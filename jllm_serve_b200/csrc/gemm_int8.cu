@@ -58,12 +58,12 @@ __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
     return r;
 }
 
-// The result from the exact sum: the same operations in the same order in both kernels.
+// The result from the exact sum: the same operations in the same order for every cut.
 __device__ __forceinline__ float scaled(uint32_t sum, float scale_a, float scale_w) {
     return __fmul_rn(__fmul_rn((float)(int)sum, scale_a), scale_w);
 }
 
-// What happens to the sums: the same in both kernels.
+// What happens to the sums.
 struct Finish {
     VecRef bias;
     int has_bias, ldo, accumulate, M, N;
@@ -186,14 +186,14 @@ struct TokenEpilogue {
 // 16 KB bulk copy each, requested before the kernel in front has finished: weights are nobody's output); the accumulator [128 weight
 // rows x tokens] lies in its tensor memory. Of the tokens every block finishes a share: the others send their parts of it (st.async,
 // which counts its bytes on the owner's mbarrier: one way through the cluster), the owner adds them up, scales and stores.
-// Bound by memory where the weight is large: one row against 24,576 x 4,096 17.3 us (5.8 TB/s, 0.89 of the
-// measured copy), 4,096 x 12,288 10.7 (4.7), 64 rows of it 11.1;
-// below that by the way from launch to last store (about 3 us beside the stream: 5.5 us for the 16.8 MB of 4,096 x 4,096).
+// Bound by memory where the weight is large: one row against 24,576 x 4,096 17.3 us (5.8 TB/s, 0.89 of the measured copy), 4,096 x 12,288
+// 10.7 (4.7), 64 rows of it 11.1; below that by the way from launch to last store (about 3 us beside the stream: 5.5 us for the 16.8 MB of
+// 4,096 x 4,096).
 // With many tokens it is what an SM takes in: a ring of 200 KB (or two of 100 KB: two blocks an SM, the one's epilogue under the other's main
-// loop) against the 1 to 2 us that a copy is on its way when all SMs ask. 2,048 rows of 24,576 x 4,096, gated: 173 us alone (2.4 POP/s), 199 one behind the other under the
-// power limit. (Pairs of
-// SMs with `cta_group::2`, which take in a third less, took 130 us for it (147 under the limit), and 29 where 300 rows take 40 here. In a model's prompt steps one of them stopped
-// once in some thousands of passes and no wait gave up; the cause was not found by reading, so they are gone.)
+// loop) against the 1 to 2 us that a copy is on its way when all SMs ask. 2,048 rows of 24,576 x 4,096, gated: 173 us alone (2.4 POP/s), 199
+// one behind the other under the power limit. (Pairs of SMs with `cta_group::2`, which take in a third less, took 130 us for it, 147 under the
+// limit, and 29 where 300 rows take 40 here. Models that ran them stopped now and then without a wait that gave up. The cause is not known, and
+// that it lies in the pairs is not shown; they are gone because they could not be cleared.)
 struct ClusterArgs {
     const int8_t* w;
     const float *scale_w, *scale_a;
