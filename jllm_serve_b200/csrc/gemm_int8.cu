@@ -9,8 +9,10 @@
 // beyond M and k beyond K with zeros.
 //
 // The weight rows are the M side of the MMAs and the tokens the N side, so that tokens are filled up to a multiple of 16 and not of 128. A cluster of
-// one to eight blocks has 128 weight rows and a group of up to 256 tokens, each block a part of the k blocks. Every wait is bounded and raises
-// the products' error word (codes 31-33).
+// one to eight blocks has 128 weight rows and a group of up to 256 tokens, each block a part of the k blocks. The waits on barriers in shared
+// memory end by the clock and raise the products' error word (31: the producer, 32: the MMAs, 33: the epilogue; the first one stays). Without a
+// limit, as in every kernel, are the waits of the hardware itself: for the grid in front, for tensor memory, for the cluster's barrier (which
+// every block reaches on every path).
 #include "tcgen05_common.cuh"
 #include "int8_view.h"
 
@@ -202,9 +204,13 @@ struct ClusterArgs {
     int groups, span;                               // groups of `span` tokens
     uint32_t tmem_cols;
     int* error_word;
+    unsigned long long limit;                       // what a wait may last, ns
+    int starve;                                     // (a test of the waits: jllm_gemm_int8_starve_next)
 };
+// STARVE_*: what never happens in the starved product
+enum : int { STARVE_NOTHING = 0, STARVE_COPY = 1, STARVE_RELEASE = 2, STARVE_PARTS = 3 };
 
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit) {
     const unsigned long long began = now_ns();
     for (uint32_t i = 1;; ++i) {
         uint32_t ok;
@@ -214,8 +220,12 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > WAIT_NS)) return false;
+        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > limit)) return false;
     }
+}
+// What is still on its way when a wait has run out: waited for whatever the others do, until `limit` after `began`.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, unsigned long long began, unsigned long long limit) {
+    while (!mbar_try_wait(bar, parity) && now_ns() - began < limit) {}
 }
 
 // (128 registers a thread: registers are dealt out for eight warps where there are six, and with more no second block fits beside one)
@@ -235,6 +245,14 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const uint32_t acc_bar = bars + 16u * stages, parts_bar = acc_bar + 8u;
     uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + bars_at + 8 * (2 * stages + 2));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
+    volatile int* requested = abort_flag + 1;          // k blocks whose copies, and whose MMAs, are under way or done
+    volatile int* multiplied = abort_flag + 2;
+    // Who waits for another role of the block waits twice as long as that one does for its copies, so that the code names what is missing.
+    auto give_up = [&](int code) {
+        atomicCAS(g.error_word, 0, code);
+        __threadfence();               // (before anybody follows the flag and has a code of his own)
+        *abort_flag = 1;
+    };
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     // a cluster's 128 weight rows and its group of tokens, the groups fastest: what runs together shares its weights
@@ -247,13 +265,13 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
+            mbar_init(empty_bar(s), g.starve == STARVE_RELEASE && s == 0 ? 2 : 1);
         }
         mbar_init(acc_bar, 1);
         mbar_init(parts_bar, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        mbar_expect_tx(parts_bar, (uint32_t)(blocks - 1) * (uint32_t)max(0, mine_end - mine) * 512u);
+        mbar_expect_tx(parts_bar, (uint32_t)(blocks - 1) * (uint32_t)max(0, mine_end - mine) * 512u + (g.starve == STARVE_PARTS ? 16u : 0u));
     }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(g.tmem_cols)
@@ -273,7 +291,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         const int early = min(stages, n_kb);
         if (elect_one())
             for (int i = 0; i < early; ++i) {
-                mbar_expect_tx(full_bar(i), stage_bytes);
+                mbar_expect_tx(full_bar(i), stage_bytes + (g.starve == STARVE_COPY && rank == 0 && i == 0 ? 16u : 0u));
                 bulk_copy(base + (uint32_t)i * stage_bytes, w + (size_t)i * TILE_BYTES, TILE_BYTES, full_bar(i));
             }
         __syncwarp();
@@ -283,10 +301,10 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             for (int i = 0; i < early; ++i)
                 tma_load_2d(base + (uint32_t)i * stage_bytes + TILE_BYTES, &map_a, (kb_lo + i) * BK, first, full_bar(i));
         __syncwarp();
-        int s = 0;
+        int s = 0, i = early;
         uint32_t parity = 0;                                   // the ring's second lap waits for the first lap's release
-        for (int i = stages; i < n_kb; ++i) {
-            if (!timed_warp_wait(empty_bar(s), parity, abort_flag)) { ok = false; break; }
+        for (; i < n_kb; ++i) {
+            if (!timed_warp_wait(empty_bar(s), parity, abort_flag, 2 * g.limit)) { ok = false; break; }
             if (elect_one()) {
                 const uint32_t dst = base + (uint32_t)s * stage_bytes;
                 mbar_expect_tx(full_bar(s), stage_bytes);
@@ -297,18 +315,22 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             if (++s == stages) { s = 0; parity ^= 1u; }
         }
         // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
-        for (int i = max(0, n_kb - stages); ok && i < n_kb; ++i) ok = timed_warp_wait(empty_bar(i % stages), (uint32_t)(i / stages) & 1u, abort_flag);
-        if (!ok && lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 31); }
+        for (int j = max(0, n_kb - stages); ok && j < n_kb; ++j)
+            ok = timed_warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * g.limit);
+        if (lane == 0) {
+            *requested = i;
+            if (!ok) give_up(31);
+        }
         if (blocks > 1) cluster_wait();
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         const uint32_t idesc = idesc_i8(128, g.ntok);
         const uint64_t desc_w0 = smem_desc_sw128(base), desc_b0 = smem_desc_sw128(base + TILE_BYTES);
         uint64_t desc_w = desc_w0, desc_b = desc_b0;          // (a stage further is an addition to the address field)
-        int s = 0;
+        int s = 0, i = 0;
         uint32_t parity = 0;
-        for (int i = 0; i < n_kb; ++i) {
-            if (!timed_warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
+        for (; i < n_kb; ++i) {
+            if (!timed_warp_wait(full_bar(s), parity, abort_flag, g.limit)) { ok = false; break; }
             tcgen05_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -320,10 +342,12 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             desc_b += stage_bytes >> 4;
             if (++s == stages) { s = 0; parity ^= 1u; desc_w = desc_w0; desc_b = desc_b0; }
         }
-        if (ok) {
-            if (elect_one()) tcgen05_commit(acc_bar);
-        } else if (lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 32); }
+        if (ok && elect_one()) tcgen05_commit(acc_bar);
         __syncwarp();
+        if (lane == 0) {
+            *multiplied = i;
+            if (!ok) give_up(32);
+        }
         if (blocks > 1) cluster_wait();
     } else {
         // ---------------- epilogue: warps 2..5, TMEM lanes 32 * (warp % 4) = weight rows of the tile ----------------
@@ -340,7 +364,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < here ? g.scale_a[first + i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
-        ok = timed_wait(acc_bar, 0, abort_flag);
+        ok = timed_wait(acc_bar, 0, abort_flag, 2 * g.limit);
         ok = __all_sync(0xffffffffu, ok);
         tcgen05_fence_after();
         if (ok)
@@ -364,7 +388,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 for (; t + 16 <= t1; t += 16) send(v16, t);
                 if (t < t1) send(v8, t);
             }
-        if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag));
+        if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag, 2 * g.limit));
         if (ok) {
             const uint8_t* parts = aligned + parts_at + (size_t)row * 16;
             auto add_up = [&](auto& sum, int t) {
@@ -385,19 +409,28 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 #pragma unroll 1
             for (; t + 16 <= mine_end; t += 16) add_up(sum16, t);
             if (t < mine_end) add_up(sum8, t);
-        } else if (lane == 0) { *abort_flag = 1; atomicExch(g.error_word, 33); }
+        } else if (lane == 0) give_up(33);
     }
     tcgen05_fence_before();
     __syncthreads();
+    const bool gave_up = *abort_flag;
+    const unsigned long long ended = gave_up ? now_ns() : 0;
+    if (gave_up) {
+        // (where no wait ran out these have been waited for: the copies by the MMAs, the MMAs by the epilogue and the producer)
+        for (int j = max(0, *requested - stages); j < *requested; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, ended, g.limit);
+        if (const int j = *multiplied - 1; j >= 0) drain(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, ended, g.limit);
+    }
     if (warp == 2) {
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(g.tmem_cols) : "memory");
     }
-    // No block leaves while words that it sent are on their way, or before everything sent to it is there (also where a wait ran out): its
-    // memory is the next block's at once.
+    // No block leaves before everything sent to it is there: its memory is the next block's at once. A block whose epilogue went through has
+    // waited for its parts; one that gave up, or whose neighbours did, waits for them here, behind the barrier that all sends are made in front
+    // of, for as long as a wait may last (parts that were never sent do not come; one that was sent takes microseconds).
     if (blocks > 1) {
         cluster_arrive();
         cluster_wait();
+        if (gave_up) drain(parts_bar, 0, now_ns(), g.limit);
     }
 }
 
@@ -510,6 +543,13 @@ int resident_clusters(int blocks) {
     return n;
 }
 
+// A test of the waits: what the next product of this thread is to miss, and how long its waits last.
+struct Starve {
+    int what;
+    unsigned long long limit;
+};
+thread_local Starve g_starve_next = {STARVE_NOTHING, WAIT_NS};
+
 struct Product {
     const int8_t *a, *w;
     int lda;
@@ -520,6 +560,7 @@ struct Product {
     Finish f;
     int* error_word;
     cudaStream_t stream;
+    Starve starve;
 };
 
 // What stands for a cut in one number: the blocks of a cluster, 10 more with a deep ring, 100 more for each group of tokens
@@ -542,12 +583,15 @@ int run_cluster(const Product& p, int code) {
     JLLM_REQUIRE(c.stages >= 1, "gemm_int8: clusters of %d blocks do not take %d rows in %d groups", cut.blocks, M, cut.groups);
     const long long units = (long long)((p.f.N + 127) / 128) * c.groups;
     JLLM_REQUIRE(units * c.blocks < (1LL << 31) && (long long)(c.groups + 1) * c.span < (1LL << 31), "gemm_int8: %lld tiles of %d rows", units, M);
+    JLLM_REQUIRE(p.starve.what == STARVE_NOTHING || (units * c.blocks <= 64 && (p.starve.what != STARVE_PARTS || c.blocks > 1)),
+                 "gemm_int8: the starved product of the wait test has at most 64 blocks, and a cluster where parts are missed");
     CUtensorMap map_a;
     const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, true, &map_a);
     if (rc != JLLM_OK) return rc;
     uint32_t cols = 32;
     while ((int)cols < c.ntok) cols <<= 1;
-    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, c.groups, c.span, cols, p.error_word};
+    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, c.groups, c.span, cols, p.error_word,
+                        p.starve.limit, p.starve.what};
     return p.out_dtype == JLLM_F32 ? launch_cluster<float>(map_a, g, c, (int)units, p.out, p.stream)
                                    : launch_cluster<__nv_bfloat16>(map_a, g, c, (int)units, p.out, p.stream);
 }
@@ -633,6 +677,15 @@ int choose(int M, int N, int k_blocks) {
 
 int* jllm_gemm_error_word();
 
+// A test of the bounded waits: the NEXT product of this thread has waits of `limit_us` microseconds, and with `what` 1 a copy's barrier that
+// expects more than comes, with 2 a stage that is never released, with 3 a part that no block of the cluster sends (0: the limit alone). It
+// returns, raises the error word and leaves the device usable.
+JLLM_EXPORT int jllm_gemm_int8_starve_next(int what, int limit_us) {
+    JLLM_REQUIRE(what >= STARVE_NOTHING && what <= STARVE_PARTS && limit_us >= 1 && limit_us <= 1000000, "gemm_int8_starve_next: %d, %d us", what, limit_us);
+    g_starve_next = {what, limit_us * 1000ull};
+    return JLLM_OK;
+}
+
 // `rows`: the int8 activations [M, K], their rows at multiples of 16 bytes; `weight`: ops.pack_int8 of the [N, K] weight, its scales filled
 // up to a multiple of 128 and 16-byte aligned; out [M, N] (or [M, N / 2] with swiglu) float32 or bfloat16. `cut` (tests): blocks of a
 // cluster, 10 more with a ring of all of an SM's shared memory, 100 more for each group of tokens; 0 as the sizes have it.
@@ -642,6 +695,8 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     const float *scale_a = rows->scale, *scale_w = weight->scale;
     const int M = rows->rows, K = rows->cols, lda = rows->stride, N = weight->rows, k_blocks = weight->stride;
     const GluArgs glu = glu_args(swiglu_word, nullptr);
+    const Starve starve = g_starve_next;
+    g_starve_next = {STARVE_NOTHING, WAIT_NS};
     JLLM_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= MAX_K && weight->cols == K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d) against a weight of %d",
                  M, N, K, MAX_K, weight->cols);
     JLLM_REQUIRE(lda >= K && lda % 16 == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)w_packed % 16) == 0 && ((uintptr_t)scale_w % 16) == 0,
@@ -655,7 +710,7 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     int* error_word = jllm_gemm_error_word();
     if (!error_word) return jllm_fail(JLLM_CUDA_ERROR, "gemm_int8: no error word");
     const Product p{a, w_packed, lda, scale_a, scale_w, k_blocks, K, out, out_dtype,
-                    Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, M, N, glu}, error_word, stream};
+                    Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, M, N, glu}, error_word, stream, starve};
     if (cut == 0) cut = out_dtype == JLLM_F32 ? choose<float>(M, N, k_blocks) : choose<__nv_bfloat16>(M, N, k_blocks);
     return run_cluster(p, cut);
 }

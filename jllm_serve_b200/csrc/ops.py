@@ -217,6 +217,7 @@ class _Signatures:
     jllm_int8_values = [P, P, I, I, P]
     jllm_pack_int8 = [P, ctypes.c_longlong, I, I, I, P, P]
     jllm_gemm_int8 = [P, P, P, I, P, I, I, I, I, I, P]
+    jllm_gemm_int8_starve_next = [I, I]
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -1736,3 +1737,10 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
         b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
     _call("jllm_gemm_int8", a.view, w.view, b, b_dtype, out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows)), int(accumulate), word, cut, _stream())
+
+
+def gemm_int8_starve_next(what: str, limit_us: int = 2000) -> None:
+    """A test of the bounded waits: the next `gemm_int8` has waits of `limit_us` microseconds and misses a "copy", a "release" of a stage or
+    the "parts" of its cluster's other blocks ("nothing": the limit alone); it returns and raises the error word that `check_kernel_errors` reads."""
+    if library().jllm_gemm_int8_starve_next(("nothing", "copy", "release", "parts").index(what), int(limit_us)):
+        _refuse("gemm_int8_starve_next", f"a limit of 1 to 1,000,000 us, got {limit_us}")

@@ -71,17 +71,17 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-__device__ __forceinline__ bool timed_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool timed_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS) {
     if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long began = now_ns();
     for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > WAIT_NS)) return false;
+        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > limit)) return false;
     }
 }
-__device__ __forceinline__ bool timed_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool timed_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, timed_wait(bar, parity, abort_flag));
+    return __all_sync(0xffffffffu, timed_wait(bar, parity, abort_flag, limit));
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
