@@ -329,6 +329,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         uint64_t desc_w = desc_w0, desc_b = desc_b0;          // (a stage further is an addition to the address field)
         int s = 0, i = 0;
         uint32_t parity = 0;
+        pdl_wait();          // (the copies are complete no sooner, and the time that the kernel in front still takes is not this wait's)
         for (; i < n_kb; ++i) {
             if (!timed_warp_wait(full_bar(s), parity, abort_flag, g.limit)) { ok = false; break; }
             tcgen05_fence_after();

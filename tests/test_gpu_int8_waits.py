@@ -60,6 +60,26 @@ def test_a_short_limit_does_not_disturb_a_product_that_misses_nothing(ops):
         assert torch.equal(out.cpu(), want)
 
 
+@pytest.mark.parametrize("cut", [1, 4, 11, 12])
+def test_what_the_kernel_in_front_takes_is_not_waited_for(ops, cut):
+    """A row of 2^27 values takes one block some 16 ms, and lets the product's blocks begin at once: a limit of 1 ms counts from there on."""
+    a8, packed, want = product(ops, 20, 256, 1024)
+    out = torch.empty(20, 256, device=DEV)
+    ops.gemm_int8(a8, packed, out, cut=cut)
+    row, row8 = torch.ones(1, 1 << 27, dtype=torch.bfloat16, device=DEV), ops.int8_rows(1, 1 << 27, DEV)
+    began, ended = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    out.zero_()
+    began.record()
+    ops.quantize_int8(row, row8)
+    ops.gemm_int8_starve_next("nothing", 1000)
+    ops.gemm_int8(a8, packed, out, cut=cut)
+    ended.record()
+    torch.cuda.synchronize()
+    assert began.elapsed_time(ended) > 4.0
+    ops.check_kernel_errors()
+    assert torch.equal(out.cpu(), want)
+
+
 def test_refusals(ops):
     for limit in (0, -1, 2000000):
         with pytest.raises(ops.KernelError):
