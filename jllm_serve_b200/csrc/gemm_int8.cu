@@ -304,7 +304,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         int s = 0, i = early;
         uint32_t parity = 0;                                   // the ring's second lap waits for the first lap's release
         for (; i < n_kb; ++i) {
-            if (!timed_warp_wait(empty_bar(s), parity, abort_flag, 2 * g.limit)) { ok = false; break; }
+            if (!warp_wait(empty_bar(s), parity, abort_flag, 2 * g.limit)) { ok = false; break; }
             if (elect_one()) {
                 const uint32_t dst = base + (uint32_t)s * stage_bytes;
                 mbar_expect_tx(full_bar(s), stage_bytes);
@@ -316,7 +316,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
         for (int j = max(0, n_kb - stages); ok && j < n_kb; ++j)
-            ok = timed_warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * g.limit);
+            ok = warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * g.limit);
         if (lane == 0) {
             *requested = i;
             if (!ok) give_up(31);
@@ -331,7 +331,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         uint32_t parity = 0;
         pdl_wait();          // (the copies are complete no sooner, and the time that the kernel in front still takes is not this wait's)
         for (; i < n_kb; ++i) {
-            if (!timed_warp_wait(full_bar(s), parity, abort_flag, g.limit)) { ok = false; break; }
+            if (!warp_wait(full_bar(s), parity, abort_flag, g.limit)) { ok = false; break; }
             tcgen05_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -365,7 +365,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < here ? g.scale_a[first + i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
-        ok = timed_wait(acc_bar, 0, abort_flag, 2 * g.limit);
+        ok = mbar_wait(acc_bar, 0, abort_flag, 2 * g.limit);
         ok = __all_sync(0xffffffffu, ok);
         tcgen05_fence_after();
         if (ok)

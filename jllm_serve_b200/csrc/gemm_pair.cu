@@ -309,16 +309,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const long long tile_last_kb = (long long)(tile - whole_tiles + 1) * k_blocks - 1;
             const int others = (int)(((tile_last_kb + 1) * dealt + sk_kb - 1) / sk_kb - 1) - pair;
             if (warp == 2 && lane == 0) {
-                int seen = 0;
-                for (uint32_t tries = 0; seen < others && tries < SPIN_LIMIT; ++tries) {
-                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-                    if (seen < others) {
-                        if ((tries & 255u) == 255u && *abort_flag) break;
-                        __nanosleep(32);
-                    }
-                }
-                if (seen >= others) *counter = 0;                     // back to zero for the next product
-                *parts_flag = seen >= others;
+                const bool all = counter_wait(counter, others, abort_flag);
+                if (all) *counter = 0;                                // back to zero for the next product
+                *parts_flag = all;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (!*parts_flag) { ok = false; break; }

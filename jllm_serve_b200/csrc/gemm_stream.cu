@@ -176,6 +176,7 @@ gemm_stream_kernel(const __grid_constant__ CUtensorMap map_a, const __nv_bfloat1
             int s = 0;
             uint32_t parity = 0, segment = 0;
             long long g = run_lo;
+            pdl_wait();          // (the copies are complete no sooner)
             while (ok && g < run_hi) {
                 const int kb0 = (int)(g % k_blocks);
                 const long long seg_end = min(run_hi, g + (k_blocks - kb0));      // the tile's k blocks that are this block's
@@ -306,15 +307,7 @@ gemm_stream_kernel(const __grid_constant__ CUtensorMap map_a, const __nv_bfloat1
                 if (warp == 2 && lane == 0) {
                     __threadfence();
                     atomicAdd(&counters[tile], 1);
-                    int seen = has_share ? 0 : parts;
-                    for (uint32_t spin = 0; seen < parts && spin < SPIN_LIMIT; ++spin) {
-                        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counters + tile) : "memory");
-                        if (seen < parts) {
-                            if ((spin & 255u) == 255u && *abort_flag) break;
-                            __nanosleep(32);
-                        }
-                    }
-                    *last_flag = seen >= parts;
+                    *last_flag = !has_share || counter_wait(counters + tile, parts, abort_flag);
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (!*last_flag) { ok = false; break; }
@@ -478,6 +471,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __nv_bfloat
         bool ok = true;
         int s = 0;
         uint32_t parity = 0;
+        pdl_wait();          // (the copies are complete no sooner)
         for (int i = 0; i < n_kb; ++i) {
             if (!warp_wait(full_bar(s), parity, abort_flag)) { ok = false; break; }
             tcgen05_fence_after();

@@ -56,8 +56,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     int stream, float* __restrict__ partials, int* __restrict__ counters, int* __restrict__ error_word,
                     int starve) {
     // `starve` (a test of the bounded waits, never set otherwise): the first stage's barrier expects 16 bytes more than
-    // the copies bring, so it never completes, and every wait gives up after 1,024 tries instead of 4 million.
-    const uint32_t spin = starve ? 1024u : SPIN_LIMIT;
+    // the copies bring, so it never completes, and (1) every wait gives up after 1,024 tries too or (2) by the clock alone.
+    const uint32_t tries = starve == 1 ? 1024u : 0xffffffffu;
     constexpr int STAGES = stages_for(BN), B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     constexpr uint32_t IDESC = idesc_for(BN);
     static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256, "tile width");
@@ -169,7 +169,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 const uint32_t tx = A_BYTES + bytes0 + bytes1;
                 uint32_t extra = starve ? 16u : 0u;         // the wait test: the first barrier expects too much
                 for (int kb = lo; kb < hi; ++kb, src += 8192) {
-                    if (!warp_wait(empty_bar(s), parity, abort_flag, spin)) { ok = false; break; }
+                    if (!warp_wait(empty_bar(s), parity, abort_flag, WAIT_NS, tries)) { ok = false; break; }
                     if (elect_one()) {
                         mbar_expect_tx(full_bar(s), tx + extra);
                         tma_load_2d(dst, &map_a, kb * BK, m0, full_bar(s));
@@ -196,11 +196,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             int tile, lo, hi;
             for (; ok && next_unit(walk, tile, lo, hi); ++local_tile) {
                 const uint32_t buf = local_tile & 1u;
-                if (!warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag, spin)) { ok = false; break; }
+                if (!warp_wait(acc_empty_bar(buf), ((local_tile >> 1) & 1u) ^ 1u, abort_flag, WAIT_NS, tries)) { ok = false; break; }
                 tcgen05_fence_after();
                 const uint32_t tmem_d = tmem_base + buf * BN;
                 for (int kb = lo; kb < hi; ++kb) {
-                    if (!warp_wait(full_bar(s), parity, abort_flag, spin)) { ok = false; break; }
+                    if (!warp_wait(full_bar(s), parity, abort_flag, WAIT_NS, tries)) { ok = false; break; }
                     tcgen05_fence_after();
                     if (elect_one()) {
 #pragma unroll
@@ -229,7 +229,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         for (; ok && next_unit(walk, tile, k_lo, k_hi); ++local_tile) {
             const int m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * BN;
             const uint32_t buf = local_tile & 1u;
-            if (!mbar_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag, spin)) { ok = false; break; }
+            if (!mbar_wait(acc_full_bar(buf), (local_tile >> 1) & 1u, abort_flag, WAIT_NS, tries)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
             // bias / residual / SwiGLU and the store of 32 columns of this thread's row
@@ -279,16 +279,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             const long long tile_last_kb = (long long)(tile - whole_tiles + 1) * k_blocks - 1;
             const int others = (int)(((tile_last_kb + 1) * dealt + sk_kb - 1) / sk_kb - 1) - (int)blockIdx.x;
             if (warp == 2 && lane == 0) {
-                int seen = 0;
-                for (uint32_t tries = 0; seen < others && tries < spin; ++tries) {
-                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counters + tile) : "memory");
-                    if (seen < others) {
-                        if ((tries & 255u) == 255u && *abort_flag) break;
-                        __nanosleep(32);
-                    }
-                }
-                if (seen >= others) counters[tile] = 0;               // back to zero for the next product
-                *last_flag = seen >= others;
+                const bool all = counter_wait(counters + tile, others, abort_flag);
+                if (all) counters[tile] = 0;                          // back to zero for the next product
+                *last_flag = all;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (!*last_flag) { ok = false; break; }
@@ -363,12 +356,12 @@ JLLM_EXPORT int jllm_gemm_tcgen05_error() {
 }
 
 // A test of the bounded waits: the NEXT product launched through jllm_gemm_tcgen05 by this thread starves (its first
-// barrier expects more bytes than arrive and its waits give up after 1,024 tries): it must return, raise the error
+// barrier expects more bytes than arrive and its waits give up after 1,024 tries, or by the clock alone): it must return, raise the error
 // word and leave the device usable. The test keeps that product to a single tile.
 namespace {
 thread_local int g_starve_next = 0;
 }
-JLLM_EXPORT void jllm_gemm_tcgen05_starve_next() { g_starve_next = 1; }
+JLLM_EXPORT void jllm_gemm_tcgen05_starve_next(int by_clock) { g_starve_next = by_clock ? 2 : 1; }
 
 // A test's switch: float32 outputs are stored (and added into) by the epilogue warps' own loads and stores, as where
 // the output's rows allow no tensor map, instead of by bulk copies. For the paired product too.

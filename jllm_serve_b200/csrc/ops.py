@@ -144,7 +144,7 @@ class _Signatures:
     jllm_gemm_stream = [P, I, P, I, P, I, P, I, I, I, I, I, I, I, P, P, ctypes.c_longlong, I, I, P]
     jllm_gemm_stream_cluster = [I, I, I, I]
     jllm_gemm_tcgen05_error = []
-    jllm_gemm_tcgen05_starve_next = []
+    jllm_gemm_tcgen05_starve_next = [I]
     jllm_attention_plain = [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P, I, F, P]
     jllm_attention_decode = [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, F, I, P, P]
     jllm_attention_decode_flat = [P, I, P, P, P, I, P, P, P, I, I, I, I, I, I, I, F, I, P, F, P]
@@ -1236,10 +1236,11 @@ def attention_decode_separate_combine(on: bool) -> None:
     library().jllm_attention_decode_separate_combine(int(bool(on)))
 
 
-def gemm_tcgen05_starve_next() -> None:
+def gemm_tcgen05_starve_next(by_clock: bool = False) -> None:
     """A test of the bounded waits: the next tcgen05 product (one tile) is given a barrier that never completes and
-    waits that give up after 1,024 tries; it returns and raises the error word that `check_kernel_errors` reads."""
-    library().jllm_gemm_tcgen05_starve_next()
+    waits that give up after 1,024 tries (`by_clock`: after their two seconds, as every kernel's do); it returns and raises the error
+    word that `check_kernel_errors` reads."""
+    library().jllm_gemm_tcgen05_starve_next(int(by_clock))
 
 
 def gemm_tcgen05_error() -> int:

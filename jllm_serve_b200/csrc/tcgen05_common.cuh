@@ -11,8 +11,6 @@
 
 namespace tc {
 
-constexpr uint32_t SPIN_LIMIT = 1u << 22;
-
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -35,14 +33,43 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait: false if the phase did not complete within the limit or another role gave up already.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          uint32_t limit = SPIN_LIMIT) {
-    for (uint32_t i = 0; i < limit; ++i) {
+// Waits end by the clock: a try may last some microseconds while the thread sleeps, so a count of tries says little about time (four million
+// of them were minutes). Two seconds are beyond every kernel here; who waits longer gives up, says so in an error word and leaves. What the
+// kernel in front still takes must not be waited for here: a role that waits for copies waits for that kernel (pdl_wait) first.
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// False if the phase did not complete within the limit (or that many tries: a test's) or another role gave up already.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS,
+                                          uint32_t tries = 0xffffffffu) {
+    unsigned long long began = 0;
+    for (uint32_t i = 0; i < tries; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 1023u) == 1023u && *abort_flag) return false;
+        if ((i & 63u) == 63u) {             // (the clock is far away: waits that are over soon do without it)
+            const unsigned long long now = now_ns();
+            if (began == 0) began = now;
+            if (*abort_flag || now - began > limit) return false;
+        }
     }
     return false;
+}
+// The same for a counter in global memory that other blocks of the grid raise to `want`.
+__device__ __forceinline__ bool counter_wait(const int* counter, int want, volatile int* abort_flag) {
+    unsigned long long began = 0;
+    for (uint32_t i = 0;; ++i) {
+        int seen;
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+        if (seen >= want) return true;
+        if ((i & 255u) == 255u) {
+            const unsigned long long now = now_ns();
+            if (began == 0) began = now;
+            if (*abort_flag || now - began > WAIT_NS) return false;
+        }
+        __nanosleep(32);
+    }
 }
 // ---- a warp that only issues (copies, MMAs) --------------------------------------------------------------------------
 // tcgen05.mma, tcgen05.commit and the bulk copies take their operands from the warp's uniform registers. Issued under `if (lane == 0)`
@@ -58,30 +85,10 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 // mbar_wait by a whole warp
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit = SPIN_LIMIT) {
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS,
+                                          uint32_t tries = 0xffffffffu) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
-}
-
-// The same with a limit in time: a try may last some microseconds while the thread sleeps, and four million of them minutes. Two seconds
-// are beyond every kernel here; who waits longer gives up, says so and leaves.
-constexpr unsigned long long WAIT_NS = 2000000000ull;
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ bool timed_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long began = now_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > limit)) return false;
-    }
-}
-__device__ __forceinline__ bool timed_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit = WAIT_NS) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, timed_wait(bar, parity, abort_flag, limit));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit, tries));
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
