@@ -211,8 +211,8 @@ struct ClusterArgs {
 enum : int { STARVE_NOTHING = 0, STARVE_COPY = 1, STARVE_RELEASE = 2, STARVE_PARTS = 3 };
 
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit) {
-    const unsigned long long began = now_ns();
-    for (uint32_t i = 1;; ++i) {
+    unsigned long long began = 0;
+    for (uint32_t i = 0;; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -220,8 +220,16 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if ((i & 15u) == 0u && (*abort_flag || now_ns() - began > limit)) return false;
+        if ((i & 63u) == 63u) {
+            const unsigned long long now = now_ns();
+            if (began == 0) began = now;
+            if (*abort_flag || now - began > limit) return false;
+        }
     }
+}
+// (the bytes alone, no arrival)
+__device__ __forceinline__ void mbar_expect_more(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // What is still on its way when a wait has run out: waited for whatever the others do, until `limit` after `began`.
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, unsigned long long began, unsigned long long limit) {
@@ -245,8 +253,6 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const uint32_t acc_bar = bars + 16u * stages, parts_bar = acc_bar + 8u;
     uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + bars_at + 8 * (2 * stages + 2));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
-    volatile int* requested = abort_flag + 1;          // k blocks whose copies, and whose MMAs, are under way or done
-    volatile int* multiplied = abort_flag + 2;
     // Who waits for another role of the block waits twice as long as that one does for its copies, so that the code names what is missing.
     auto give_up = [&](int code) {
         atomicCAS(g.error_word, 0, code);
@@ -265,13 +271,20 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), g.starve == STARVE_RELEASE && s == 0 ? 2 : 1);
+            mbar_init(empty_bar(s), 1);
         }
         mbar_init(acc_bar, 1);
         mbar_init(parts_bar, 1);
         *abort_flag = 0;
+        if (g.starve != STARVE_NOTHING) {
+            if (g.starve == STARVE_RELEASE) {
+                asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(empty_bar(0)) : "memory");
+                mbar_init(empty_bar(0), 2);
+            } else if (g.starve == STARVE_PARTS) mbar_expect_more(parts_bar, 16);
+            else if (rank == 0) mbar_expect_more(full_bar(0), 16);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        mbar_expect_tx(parts_bar, (uint32_t)(blocks - 1) * (uint32_t)max(0, mine_end - mine) * 512u + (g.starve == STARVE_PARTS ? 16u : 0u));
+        mbar_expect_tx(parts_bar, (uint32_t)(blocks - 1) * (uint32_t)max(0, mine_end - mine) * 512u);
     }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"(g.tmem_cols)
@@ -285,13 +298,14 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (blocks > 1) cluster_arrive();          // (waited for in front of the first send: every block runs and has its barriers)
 
     bool ok = true;
+    int issued = 0;                            // k blocks whose copies (warp 0), or whose MMAs (warp 1), are under way or done
     if (warp == 0) {
         // ---------------- producer: weights by bulk copy, activations by TMA ----------------
         const int8_t* w = g.w + ((size_t)tile * g.k_blocks + kb_lo) * TILE_BYTES;
         const int early = min(stages, n_kb);
         if (elect_one())
             for (int i = 0; i < early; ++i) {
-                mbar_expect_tx(full_bar(i), stage_bytes + (g.starve == STARVE_COPY && rank == 0 && i == 0 ? 16u : 0u));
+                mbar_expect_tx(full_bar(i), stage_bytes);
                 bulk_copy(base + (uint32_t)i * stage_bytes, w + (size_t)i * TILE_BYTES, TILE_BYTES, full_bar(i));
             }
         __syncwarp();
@@ -317,10 +331,8 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
         for (int j = max(0, n_kb - stages); ok && j < n_kb; ++j)
             ok = warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * g.limit);
-        if (lane == 0) {
-            *requested = i;
-            if (!ok) give_up(31);
-        }
+        issued = i;
+        if (!ok && lane == 0) give_up(31);
         if (blocks > 1) cluster_wait();
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
@@ -345,10 +357,8 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         if (ok && elect_one()) tcgen05_commit(acc_bar);
         __syncwarp();
-        if (lane == 0) {
-            *multiplied = i;
-            if (!ok) give_up(32);
-        }
+        issued = i;
+        if (!ok && lane == 0) give_up(32);
         if (blocks > 1) cluster_wait();
     } else {
         // ---------------- epilogue: warps 2..5, TMEM lanes 32 * (warp % 4) = weight rows of the tile ----------------
@@ -413,13 +423,14 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         } else if (lane == 0) give_up(33);
     }
     tcgen05_fence_before();
-    __syncthreads();
-    const bool gave_up = *abort_flag;
-    const unsigned long long ended = gave_up ? now_ns() : 0;
+    const bool gave_up = __syncthreads_or(!ok);
     if (gave_up) {
         // (where no wait ran out these have been waited for: the copies by the MMAs, the MMAs by the epilogue and the producer)
-        for (int j = max(0, *requested - stages); j < *requested; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, ended, g.limit);
-        if (const int j = *multiplied - 1; j >= 0) drain(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, ended, g.limit);
+        const unsigned long long began = now_ns();
+        if (warp == 0)
+            for (int j = max(0, issued - stages); j < issued; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, began, g.limit);
+        if (warp == 1 && issued > 0) drain(empty_bar((issued - 1) % stages), (uint32_t)((issued - 1) / stages) & 1u, began, g.limit);
+        __syncthreads();
     }
     if (warp == 2) {
         tcgen05_fence_after();
