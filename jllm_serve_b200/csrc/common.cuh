@@ -298,15 +298,29 @@ struct ScoreCap {
 };
 inline ScoreCap score_cap(float cap, float scale) { return cap > 0.f ? ScoreCap{scale / cap, cap * 1.4426950408889634f} : ScoreCap{0.f, 0.f}; }
 
+// Minimum and maximum; KEEPS_NAN: of what is not a number such a one (fminf and fmaxf give the other operand).
+template <bool KEEPS_NAN> __device__ __forceinline__ float lower_of(float a, float b) {
+    if constexpr (!KEEPS_NAN) return fminf(a, b);
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <bool KEEPS_NAN> __device__ __forceinline__ float higher_of(float a, float b) {
+    if constexpr (!KEEPS_NAN) return fmaxf(a, b);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // N gated units whose activation is one word's, as a product's epilogue has them: the activation is chosen ONCE, in front of the loop
 // (a choice per unit makes a chain of branches of it, and a thread's units wait for one another).
-template <int N, typename Gate, typename Up>
+template <int N, bool KEEPS_NAN = false, typename Gate, typename Up>
 __device__ __forceinline__ void glu_units(int word, Gate gate, Up up, float factor, float (&out)[N]) {
     if ((word & 3) == GLU_SWISH_CLAMPED) {
         const float limit = __int_as_float(word & ~3);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float g = fminf(gate(j), limit), u = fminf(fmaxf(up(j), -limit), limit);
+            const float g = lower_of<KEEPS_NAN>(gate(j), limit), u = lower_of<KEEPS_NAN>(higher_of<KEEPS_NAN>(up(j), -limit), limit);
             out[j] = __fmul_rn(__fdividef(g, 1.f + __expf(-kSwishAlpha * g)) * (u + 1.f), factor);
         }
     } else if (word == GLU_GELU_TANH) {

@@ -113,7 +113,7 @@ struct TokenEpilogue {
                 gate[j] = up_lane ? other : v[j];
                 up[j] = up_lane ? v[J / 2 + j] : other;
             }
-            glu_units<J / 2>(f.glu.word, [&](int j) { return gate[j]; }, [&](int j) { return up[j]; }, 1.f, units);
+            glu_units<J / 2, true>(f.glu.word, [&](int j) { return gate[j]; }, [&](int j) { return up[j]; }, 1.f, units);
 #pragma unroll
             for (int j = 0; j < J / 2; ++j) park[(up_lane ? J / 2 + j : j) * 16 + (lane >> 4) * 8 + (lane & 7)] = from_float<Tout>(units[j]);
         } else {
@@ -122,7 +122,10 @@ struct TokenEpilogue {
                 for (int j = 0; j < J; ++j) v[j] = __fadd_rn(v[j], b);
             if (f.accumulate == EPI_RELU2)
 #pragma unroll
-                for (int j = 0; j < J; ++j) v[j] = epilogue_act(v[j], EPI_RELU2);
+                for (int j = 0; j < J; ++j) {
+                    const float z = v[j] < 0.f ? 0.f : v[j];              // (what is not a number stays so: a maximum would drop it)
+                    v[j] = __fmul_rn(z, z);
+                }
             if (f.accumulate == EPI_ADD && !add_behind) {
                 // (all the old values are requested before the first store: a load behind a store through the same pointer would wait)
                 float old[J];
