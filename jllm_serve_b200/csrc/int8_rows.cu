@@ -212,6 +212,61 @@ struct NormArgs {
     bool x_vec, y_vec, t_vec, g_vec;
 };
 
+// A row whose squares or products left float32, or vanished in it, or that is zeros or not numbers, in two more passes. First the largest
+// magnitudes of t and of w = t gain, which 64 bits hold exactly whatever the two are (of w the upper half: its exponent is what is wanted, and
+// an infinity or a NaN shows); then sum and maximum of both, divided by the powers of two that they lie at. A thread reads what it has left
+// itself. (A function of its own: nothing of it costs the other rows a register.)
+template <typename Tg, bool BLOCK>
+__device__ __noinline__ void norm_beyond_float32(const NormArgs& a, int r, uint32_t* scratch) {
+    const int at = my_place<BLOCK>() * 8, step = (BLOCK ? blockDim.x : 32) * 8, dim = a.dim;
+    const float* t_row = a.y ? a.total + (size_t)r * a.ldt : a.x + (size_t)r * a.ldx;
+    const bool t_vec = a.y ? a.t_vec : a.x_vec;
+    const Tg* gains = static_cast<const Tg*>(a.gain);
+    // f(t, gain) of the chunk at i in place of t
+    auto chunk = [&](float (&t)[8], int i, auto&& f) {
+        float b[8];
+        load8(t, t_row + i, dim - i, t_vec);
+        Raw8<Tg> g;
+        g.load(gains + i, dim - i, a.g_vec);
+        g.values(b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = f(t[j], b[j]);
+    };
+    float t[8], unused = 0.f, ss = 0.f;
+    uint32_t top_t = 0, top_w = 0, top = 0;
+    for (int i = at; i < dim; i += step)
+        chunk(t, i, [&](float v, float g) {
+            top_t = max(top_t, magnitude(v));
+            top_w = max(top_w, (uint32_t)__double2hiint(__dmul_rn((double)v, (double)g)) & 0x7fffffffu);
+            return v;
+        });
+    row_reduce<BLOCK, false>(unused, top_t, scratch);
+    row_reduce<BLOCK, false>(unused, top_w, scratch);
+    const bool finite = top_t < 0x7f800000u && top_w < 0x7ff00000u;
+    // 2^-exponent of a float64's upper half (1 of zero): in 64 bits even the smallest float32 has an exponent of its own
+    auto down = [&](uint32_t high) { return high != 0 && finite ? __hiloint2double((int)((2046u - (high >> 20)) << 20), 0) : 1.0; };
+    const double ft = down((uint32_t)__double2hiint((double)__uint_as_float(top_t)) & 0x7fffffffu), fw = down(top_w);
+    auto scaled_w = [&](float v, float g) { return (float)((double)v * (double)g * fw); };
+    for (int i = at; i < dim; i += step)
+        chunk(t, i, [&](float v, float g) {
+            const float u = (float)((double)v * ft);
+            ss = fmaf(u, u, ss);
+            top = max(top, magnitude(scaled_w(v, g)));
+            return v;
+        });
+    row_reduce<BLOCK, true>(ss, top, scratch);
+    const float m = __uint_as_float(top);
+    const double root = 1.0 / sqrt((double)ss / ft / ft / dim + (double)a.eps);
+    const double most = root * ((double)m / fw);                     // (NaN where the row is 0 / 0)
+    const bool whole = finite && most < 127.0 * 3.4028234e38;        // (the scale is a number of float32)
+    const float inverse = whole && most >= (double)kTiny ? __fdiv_rn(127.f, m) : 0.f;
+    for (int i = at; i < dim; i += step) {
+        chunk(t, i, scaled_w);
+        store8(a.q + (size_t)r * a.ldq + i, t, inverse, dim - i);
+    }
+    if (at == 0) a.scale[r] = !whole ? __int_as_float(0x7fffffff) : (inverse == 0.f ? 0.f : (float)(most / 127.0));
+}
+
 template <typename Ty, typename Tg, int V, bool BLOCK>
 __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS) add_rmsnorm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ uint32_t scratch[64];
@@ -254,16 +309,6 @@ __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS
             top = max(top, magnitude(t[j]));
         }
     };
-    // w of the chunk at i once more (t scaled by f), from what the thread itself has left
-    auto again = [&](float (&t)[8], int i, float f) {
-        float b[8];
-        load8(t, (y ? total : x) + i, dim - i, y ? a.t_vec : a.x_vec);
-        Raw8<Tg> g;
-        g.load(gains + i, dim - i, a.g_vec);
-        g.values(b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(__fmul_rn(t[j], f), b[j]);
-    };
     float w[HELD ? V : 1][8];
     Raw8<Ty> other[HELD ? V : 1];
     if constexpr (HELD) {
@@ -293,7 +338,7 @@ __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS
     }
     row_reduce<BLOCK, true>(ss, top, scratch);
     float m = __uint_as_float(top);
-    if (ss > 1e-24f && ss < 1e30f && m >= kTiny && m < 1e30f) {
+    if (ss > 1e-24f && ss < 1e30f && m >= kTiny && m < 1e20f) {       // (root below 1e17: the scale stays in float32)
         const float inverse = __fdiv_rn(127.f, m);
         if constexpr (HELD) {
 #pragma unroll
@@ -301,41 +346,20 @@ __global__ void __launch_bounds__(V <= MOST_CHUNKS ? NORM_THREADS : MOST_THREADS
                 if (at + c * step < dim) store8(dst + at + c * step, w[c], inverse, dim - at - c * step);
         } else {
             for (int i = at; i < dim; i += step) {
-                again(w[0], i, 1.f);
-                store8(dst + i, w[0], inverse, dim - i);
+                // w once more, from what the thread itself has left
+                float t[8], b[8];
+                load8(t, (y ? total : x) + i, dim - i, y ? a.t_vec : a.x_vec);
+                gain[0].load(gains + i, dim - i, a.g_vec);
+                gain[0].values(b);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(t[j], b[j]);
+                store8(dst + i, t, inverse, dim - i);
             }
         }
         if (at == 0) a.scale[r] = __fmul_rn(rms_scale(ss, dim, a.eps), __fdiv_rn(m, 127.f));
         return;
     }
-    // Squares or products left float32, or vanished in it, or the row is zeros or not numbers: once more with t scaled by powers of two.
-    const float fs = ss < 1e30f ? (ss > 1e-24f ? 1.f : 1.2089258196146292e+24f) : 8.271806125530277e-25f;               // 2^80, 2^-80
-    const float fm = m < 1e30f ? (m >= kTiny ? 1.f : 1.2676506002282294e+30f) : 7.52316384526264e-37f;                 // 2^100, 2^-120
-    ss = 0.f, top = 0;
-    for (int i = at; i < dim; i += step) {
-        float t[8];
-        load8(t, (y ? total : x) + i, dim - i, y ? a.t_vec : a.x_vec);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float u = __fmul_rn(t[j], fs);
-            ss = fmaf(u, u, ss);
-        }
-        again(t, i, fm);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(t[j]));
-    }
-    row_reduce<BLOCK, true>(ss, top, scratch);
-    m = __uint_as_float(top);
-    const double root = 1.0 / sqrt((double)ss / ((double)fs * (double)fs) / dim + (double)a.eps);
-    const double most = root * ((double)m / (double)fm);             // (NaN where the row has one, or is 0 / 0)
-    const bool whole = ss < INFINITY && most < (double)INFINITY;
-    const float inverse = whole && most >= (double)kTiny ? __fdiv_rn(127.f, m) : 0.f;
-    for (int i = at; i < dim; i += step) {
-        float t[8];
-        again(t, i, fm);
-        store8(dst + i, t, inverse, dim - i);
-    }
-    if (at == 0) a.scale[r] = !whole ? __int_as_float(0x7fffffff) : (inverse == 0.f ? 0.f : (float)(most / 127.0));
+    norm_beyond_float32<Tg, BLOCK>(a, r, scratch);
 }
 
 // Four 8-bit integers as floats: a byte under the exponent of 2^23 (with its sign bit turned: 128 more than it is), less that.

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_int8 import integers, on_gpu, rnd
+from tests.test_gpu_int8 import check_norm, integers, on_gpu, rnd
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -47,3 +47,38 @@ def test_not_a_number_stays_one_through_every_epilogue(ops, rows, dtype):
         units = torch.ones(rows, width // 2, dtype=dtype, device=DEV)
         ops.gemm_int8(a8, up, units, swiglu=ops.glu_descriptor(kind, 3.0))
         assert torch.equal(torch.isnan(units.cpu()), want), kind
+
+
+@pytest.mark.parametrize("dim", [48, 500, 4100, 17000])
+def test_norm_of_rows_whose_products_leave_float32(ops, dim):
+    spread = torch.exp(rnd(5, dim, seed=4))
+    def norm(x, gain, eps):                                      # noqa: E306
+        out = ops.int8_rows(x.shape[0], dim, DEV)
+        ops.add_rmsnorm_int8(x.to(DEV), gain.to(DEV), eps, out)
+        return out
+    # no gain against values of any size: rows of zeros; less of it than float32 says exactly: zeros too, or (what a row of results below
+    # 2^-100 may keep) numbers, which are then no further off than the step of their 8 bits and the spacing of float32 down there
+    x = rnd(5, dim) * torch.tensor([[1.0], [3e8], [1e20], [1e30], [5e37]])
+    for gain in (torch.zeros(dim), torch.zeros(dim).bfloat16(), torch.full((dim,), 1e-42), rnd(dim, seed=9) * 1e-38):
+        out = norm(x, gain, 1e-6)
+        v = x.double() / torch.sqrt((x.double() ** 2).mean(dim=1, keepdim=True) + 1e-6) * gain.double()
+        got, scale = out.data.cpu().double(), out.scale.cpu().double()
+        kept = scale.gt(0)
+        assert torch.isfinite(scale).all() and got[~kept & gain.eq(0).all()].eq(0).all() and float(v.abs().max()) < 2.0 ** -100
+        off = (got * scale[:, None] - v).abs()
+        assert (off <= torch.where(kept, 0.51 * v.abs().amax(dim=1) / 127 + 127 * 2.0 ** -149, v.abs().amax(dim=1))[:, None]).all()
+    # large gains against small values that reach over many powers of two: each value keeps its bits
+    x = rnd(5, dim) * spread ** 4 * torch.tensor([[1e-3], [1e-6], [1e-9], [1e-20], [1e-30]])
+    gain = 1e37 * (1 + 0.3 * rnd(dim, seed=2).clamp(-2, 2))
+    check_norm(norm(x, gain, 0.0), x, gain, 0.0, dim)
+    # small gains, and values below what a square says in float32
+    x = rnd(5, dim) * torch.tensor([[1.0], [1e-10], [1e-25], [1e-33], [1e-36]])
+    gain = 1e-25 * (1 + 0.3 * rnd(dim, seed=2))
+    check_norm(norm(x, gain, 0.0), x, gain, 0.0, dim)
+    gain = 1 + 0.3 * rnd(dim, seed=2)
+    check_norm(norm(x, gain, 0.0), x, gain, 0.0, dim)
+    # what leaves float32 as a value is not a number in 8 bits
+    gain = torch.ones(dim)
+    gain[dim // 2] = math.inf
+    out = norm(rnd(5, dim) + 3, gain, 1e-6)
+    assert torch.isnan(out.scale).all() and out.data.eq(0).all()
