@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_int8 import check_norm, integers, on_gpu, rnd
+from tests.test_gpu_int8 import check_norm, integers, on_gpu, plain_int8, rnd, same
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -82,3 +82,17 @@ def test_norm_of_rows_whose_products_leave_float32(ops, dim):
     gain[dim // 2] = math.inf
     out = norm(rnd(5, dim) + 3, gain, 1e-6)
     assert torch.isnan(out.scale).all() and out.data.eq(0).all()
+
+
+@pytest.mark.parametrize("dim", [32768, 32769, 40003])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("first", [0, 1])
+def test_quantize_rows_too_wide_to_be_held(ops, dim, dtype, first):
+    wide = (rnd(4, dim + 8) * torch.exp(rnd(4, 1, seed=3))).to(dtype)
+    wide[1, first + dim - 1], wide[2] = math.nan, 0.0
+    x = wide[:, first:first + dim]                               # (rows that begin at any value)
+    out = ops.int8_rows(4, dim, DEV)
+    ops.quantize_int8(wide.to(DEV)[:, first:first + dim], out)
+    want_q, want_scale = plain_int8(x.float())
+    assert torch.isnan(want_scale[1]) and want_scale[2] == 0
+    assert torch.equal(out.data.cpu(), want_q) and same(out.scale.cpu(), want_scale)
