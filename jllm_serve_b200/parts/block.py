@@ -127,10 +127,9 @@ class PreNormBlock(Block):
         self.feed_forward.forward(xb, y, batch)
         self._settle(x, y)
 
-
     def _forward_int8(self, x, batch, cache) -> None:
         rows8 = self.rt.int8_rows("normed", self.dim, x.shape[0])
-        y = self.rt.buffer("mixer_result", self.dim)[:x.shape[0]]
+        y = self.rt.buffer("mixer_result", self.dim, torch.float32)[:x.shape[0]]     # (added to the residual unrounded, as without 8 bits)
         self.mixer_norm.forward(x, rows8)
         self.mixer.forward(rows8, y, batch, cache)
         self.ffn_norm.forward(x, rows8, add=y)

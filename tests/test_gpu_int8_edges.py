@@ -96,3 +96,19 @@ def test_quantize_rows_too_wide_to_be_held(ops, dim, dtype, first):
     want_q, want_scale = plain_int8(x.float())
     assert torch.isnan(want_scale[1]) and want_scale[2] == 0
     assert torch.equal(out.data.cpu(), want_q) and same(out.scale.cpu(), want_scale)
+
+
+def test_a_layer_adds_its_mixers_result_unrounded(tmp_path):
+    """The residual stream is float32 and so is what is added to it, as in a bfloat16 model."""
+    from jllm_serve_b200.engine import Engine
+    from tests.tiny import TINY_A, make_model_folder
+    with Engine(make_model_folder(TINY_A, 3, tmp_path), weights="int8", page_size=8, max_tokens_cached=128, max_batch_tokens=64, max_running=2,
+                ctx=64) as engine:
+        block = engine.runner.model.blocks[0]
+        x = rnd(10, block.dim).to(DEV)
+        y = (1 + 2.0 ** -12 * rnd(10, block.dim, seed=1)).to(DEV)
+        block.mixer.forward = lambda rows8, out, batch, cache: out.copy_(y)
+        block.feed_forward.forward = lambda rows8, out, batch: None
+        want = x + y
+        block.forward(x, None, None)
+        assert torch.equal(x, want)
