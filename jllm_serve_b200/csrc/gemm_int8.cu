@@ -456,7 +456,7 @@ struct ClusterCut {
 // `deep`: the ring takes all shared memory of an SM, else half of it, so that a second block (of this product, or of the next one, whose first
 // weights then come while this one ends) fits beside.
 ClusterCut cluster_cut(int blocks, bool deep, int groups, int M, int k_blocks) {
-    const int span = ((M + groups - 1) / groups + 15) / 16 * 16;          // (the last group may be short, or there are fewer)
+    const int span = (int)((((long long)M + groups - 1) / groups + 15) / 16 * 16);          // (the last group may be short, or there are fewer)
     ClusterCut c{blocks, (span / 8 + blocks - 1) / blocks * 8, span, 0, (M + span - 1) / span, span, 0};
     if (span > 256) return c;
     if (groups == 1) c.share = ((M + 7) / 8 + blocks - 1) / blocks * 8;
@@ -712,7 +712,7 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     const GluArgs glu = glu_args(swiglu_word, nullptr);
     const Starve starve = g_starve_next;
     g_starve_next = {STARVE_NOTHING, WAIT_NS};
-    JLLM_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= MAX_K && weight->cols == K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d) against a weight of %d",
+    JLLM_REQUIRE(M >= 0 && M <= INT8_MOST && N >= 1 && K >= 1 && K <= MAX_K && weight->cols == K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d) against a weight of %d",
                  M, N, K, MAX_K, weight->cols);
     JLLM_REQUIRE(lda >= K && lda % 16 == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)w_packed % 16) == 0 && ((uintptr_t)scale_w % 16) == 0,
                  "gemm_int8: rows and weights begin at multiples of 16 bytes (lda=%d, K=%d)", lda, K);

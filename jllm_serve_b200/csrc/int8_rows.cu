@@ -478,7 +478,8 @@ void launch_norm(const NormArgs& a, cudaStream_t stream) {
 
 // What all three ask of the int8 rows
 #define JLLM_REQUIRE_ROWS(name, v)                                                                                                 \
-    JLLM_REQUIRE((v).rows >= 0 && (v).cols > 0 && (v).stride >= (v).cols && vec16((v).data, (v).stride, 1),                         \
+    JLLM_REQUIRE((v).rows >= 0 && (v).cols > 0 && (v).stride >= (v).cols && vec16((v).data, (v).stride, 1) && (v).rows <= INT8_MOST && \
+                     (v).cols <= INT8_MOST,                                                                                         \
                  name ": %d int8 rows of %d values begin at multiples of 16 bytes (stride %d)", (v).rows, (v).cols, (v).stride)
 
 // x [rows, cols] float32 or bfloat16 (row stride ldx) -> the int8 rows of `view`.

@@ -1555,6 +1555,7 @@ def decode_splits(rows, kv_heads, kv_bucket, heads, head_dim, scratch, places: i
 
 # ---- linears in 8-bit integers ---------------------------------------------------------------------------
 
+INT8_MOST = 0x7fffffff - 8191      # rows, and values of a row: the kernels count them in 32 bits and step past the end by up to 8,192
 INT8_MAX_K = 131071      # a product's sum of k products of two 8-bit integers stays exact in 32 bits up to here
 
 
@@ -1580,8 +1581,8 @@ class Int8Rows:
         self.on_gpu = data.is_cuda and scale.is_cuda and data.device == scale.device
         self.stride = data.stride(0) if self.rows > 1 else -(-self.cols // 16) * 16          # (a single row's stride says nothing)
         if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or self.stride < self.cols or self.stride % 16 or data.data_ptr() % 16
-                or (self.rows > 1 and scale.stride(0) != 1) or max(self.stride, self.rows) > 0x7fffffff):
-            _refuse("Int8Rows", f"rows of neighbouring values that begin at multiples of 16 bytes, got strides {data.stride()}, {scale.stride()} at {data.data_ptr():#x}")
+                or (self.rows > 1 and scale.stride(0) != 1) or self.stride > 0x7fffffff or max(self.shape) > INT8_MOST):
+            _refuse("Int8Rows", f"at most {INT8_MOST} rows of as many neighbouring values that begin at multiples of 16 bytes, got {self.shape}, strides {data.stride()}, {scale.stride()} at {data.data_ptr():#x}")
         # what the launchers are told of the rows, laid out once
         self._view = _Int8View(data.data_ptr(), scale.data_ptr(), self.rows, self.cols, self.stride)
         self.view = ctypes.addressof(self._view)

@@ -1,0 +1,21 @@
+"""What the 8-bit operators refuse and how they hand their arguments on, at the edges (CPU)."""
+import pytest
+import torch
+
+from jllm_serve_b200.csrc import ops
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 2 ** 31 - 16), (1, 2 ** 31 - 8176), (2 ** 31 - 1, 16), (2 ** 31 - 8191, 1)])
+def test_rows_that_32_bits_do_not_count_are_refused(rows, cols):
+    """A thread steps from its last value past the row's end by as much as the row's threads hold: that has to stay below 2^31."""
+    data = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device="meta")[:, :cols]
+    with pytest.raises(ops.KernelError):
+        ops.Int8Rows(data, torch.empty(rows, device="meta"))
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 2 ** 31 - 8192), (2 ** 31 - 8192, 16)])
+def test_the_largest_rows(rows, cols):
+    rows8 = ops.Int8Rows(torch.empty((rows, cols), dtype=torch.int8, device="meta"), torch.empty(rows, device="meta"))
+    assert rows8.shape == (rows, cols)
+    # the furthest that the kernels' 32-bit counters go: a row's step, four rows of one group, a group of tokens
+    assert cols - 1 + 1024 * 8 <= 2 ** 31 - 1 and rows + 255 <= 2 ** 31 - 1
