@@ -23,9 +23,13 @@ class RmsNorm(Norm):
         return {prefix + getattr(spec, "gain_name", "weight"): TensorWant((dim,), "vector", init="gain")}
 
     def forward(self, x, out, row_index=None, rows=None, add=None):
-        """`out` may be `ops.Int8Rows`: the result in 8 bits, and `add` (float32 or bfloat16) is added to x in place first."""
+        """`out` may be `ops.Int8Rows`: the result of every row of x in 8 bits, and `add` (float32 or bfloat16) is added to x in place first."""
         if isinstance(out, ops.Int8Rows):
+            if row_index is not None or rows is not None:
+                raise ops.KernelError("a norm in 8 bits takes every row of x as it lies")
             return ops.add_rmsnorm_int8(x, self.gain, self.eps, out, y=add)
+        if add is not None:
+            raise ops.KernelError("an addition in front of the norm is built for results in 8 bits")
         ops.rmsnorm(x, self.gain, self.eps, out, row_index, rows)
 
 

@@ -19,3 +19,16 @@ def test_the_largest_rows(rows, cols):
     assert rows8.shape == (rows, cols)
     # the furthest that the kernels' 32-bit counters go: a row's step, four rows of one group, a group of tokens
     assert cols - 1 + 1024 * 8 <= 2 ** 31 - 1 and rows + 255 <= 2 ** 31 - 1
+
+
+def test_a_norm_does_not_drop_what_it_cannot_do():
+    from types import SimpleNamespace
+
+    from jllm_serve_b200.parts.norm import RmsNorm
+    norm = RmsNorm(SimpleNamespace(eps=1e-6), 16, {"n.weight": torch.ones(16)}, "n.", None)
+    x, rows8 = torch.zeros(2, 16), ops.int8_rows(2, 16, "cpu")
+    for call in (lambda: norm.forward(x, torch.empty(2, 16), add=x),                      # no sum in front of a bfloat16 result
+                 lambda: norm.forward(x, rows8, row_index=torch.zeros(2, dtype=torch.int32)),
+                 lambda: norm.forward(x, rows8, rows=1)):
+        with pytest.raises(ops.KernelError, match="8 bits"):
+            call()
