@@ -1626,7 +1626,8 @@ def add_rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, out: Int8R
     """out = rmsnorm(x + y) * gain in 8 bits (as `quantize_int8` has them; a row of results below 2^-100 may keep its numbers), total =
     x + y: the residual's addition, the norm behind it and the rounding in one pass. x float32 [rows, dim]; y float32 or bfloat16 of x's
     shape, or None (nothing is added, and there is no total); total float32 of x's shape, x itself by default (no other overlap of what
-    is read and written); gain float32 or bfloat16 [dim]."""
+    is read and written); gain float32 or bfloat16 [dim], a weight: it is read before what is in front on the stream has ended, so not
+    what a kernel right in front writes."""
     name = "add_rmsnorm_int8"
     if (x.dtype != torch.float32 or gain.dtype not in _DT or gain.shape != out.width or not gain.is_contiguous()
             or not gain.is_cuda or not out.on_gpu):
@@ -1707,7 +1708,9 @@ def pack_int8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> Pac
         tiles = padded.view(T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)                  # [T, KB, 128 rows, 8 chunks, 16]
         packed = tiles.gather(3, _swizzle_index(data.device).expand(T, KB, 128, 8, 16)).contiguous().view(T, KB, 128, 128)
     scales = torch.zeros((T * 128,), dtype=torch.float32, device=data.device)
-    scales[:N] = scale
+    # (neighbouring values are copied, others moved by a kernel: a product right behind that kernel may read its weight's scales before it
+    # waits for it)
+    scales[:N] = scale.contiguous()
     return PackedInt8(packed, scales, N, K, glu)
 
 
@@ -1723,7 +1726,8 @@ def gemm_int8(a: Int8Rows, w: PackedInt8, out: torch.Tensor, bias: torch.Tensor 
     """out (+)= a @ w^T (+ bias): the integers' sums are exact, the result is sum * scale of the token * scale of the weight row in
     float32, so a row's result is the same bits in any batch. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or
     bfloat16; `accumulate` as the other products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`;
-    no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. `cut` (tests): the blocks of a cluster that share 128
+    no bias, nothing added): out[r, j] = act(gate_j) * up_j, [rows, w.rows / 2]. The weight, its scales and the bias are read before what is
+    in front on the stream has ended: not what a kernel right in front writes. `cut` (tests): the blocks of a cluster that share 128
     weight rows, 10 more with a ring of all of an SM's shared memory, 100 more for each group of tokens; 0: as the sizes have it."""
     name = "gemm_int8"
     word = glu_kind(swiglu) if swiglu else 0

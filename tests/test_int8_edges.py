@@ -32,3 +32,18 @@ def test_a_norm_does_not_drop_what_it_cannot_do():
                  lambda: norm.forward(x, rows8, rows=1)):
         with pytest.raises(ops.KernelError, match="8 bits"):
             call()
+
+
+def test_scales_of_any_stride_are_packed_by_a_copy():
+    """What lies apart is brought together first, so that nothing but a copy writes the packed weight's scales."""
+    w, scale = torch.ones(5, 8, dtype=torch.int8), torch.arange(10.0)[::2]
+    seen = []
+
+    class Watch(torch.utils._python_dispatch.TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if "copy_" in str(func):
+                seen.append((args[0].shape, args[1].is_contiguous()))
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        packed = ops.pack_int8(w, scale)
+    assert torch.equal(packed.scale, scale) and ((5,), True) in [(tuple(s), c) for s, c in seen]
