@@ -51,14 +51,6 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// the address, in the cluster's shared window, of `addr` (an address in this block's shared memory) in block `rank`
-__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 
 // The result from the exact sum: the same operations in the same order for every cut.
 __device__ __forceinline__ float scaled(uint32_t sum, float scale_a, float scale_w) {
@@ -143,7 +135,7 @@ struct TokenEpilogue {
         __syncwarp();
     }
 
-    // parked rows of WIDTH values -> out[t + j, column + ...], only what lies in [end, last)
+    // parked rows of WIDTH values -> out[t + j, column ...], of tokens in front of `end` and columns in front of `last` (`vec`: all are)
     template <int J, int WIDTH, int PER>
     __device__ __forceinline__ void leave(int t, int column, int last, bool add) const {
         if (vec) {
@@ -476,11 +468,11 @@ ClusterCut cluster_cut(int blocks, bool deep, int groups, int M, int k_blocks) {
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
 
-// A [rows, cols] matrix of bytes with row stride ld, read in boxes of box_rows x 128, with the 128-byte swizzle or as it lies.
-int byte_map_for(const void* ptr, long long rows, long long cols, long long ld, int box_rows, bool swizzle, CUtensorMap* out) {
+// A [rows, cols] matrix of bytes with row stride ld, read in boxes of box_rows x 128 with the 128-byte swizzle.
+int byte_map_for(const void* ptr, long long rows, long long cols, long long ld, int box_rows, CUtensorMap* out) {
     static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
     static std::mutex mu;
-    const MapKey key{ptr, rows, cols, ld, box_rows * 2 + (swizzle ? 1 : 0)};
+    const MapKey key{ptr, rows, cols, ld, box_rows};
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
     if (it != cache.end()) {
@@ -495,7 +487,7 @@ int byte_map_for(const void* ptr, long long rows, long long cols, long long ld, 
     const cuuint32_t elem[2] = {1, 1};
     CUtensorMap map;
     const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return jllm_fail(JLLM_CUDA_ERROR, "gemm_int8: cuTensorMapEncodeTiled failed (%d) for [%lld, %lld] bytes, ld %lld", (int)r, rows, cols, ld);
@@ -505,7 +497,6 @@ int byte_map_for(const void* ptr, long long rows, long long cols, long long ld, 
     return JLLM_OK;
 }
 
-template <typename Tout>
 cudaLaunchConfig_t cluster_config(const ClusterCut& c, int tiles, cudaLaunchAttribute* attr, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * c.blocks);
@@ -527,7 +518,7 @@ int launch_cluster(const CUtensorMap& map_a, const ClusterArgs& g, const Cluster
     if (jllm_allow_smem((const void*)kern, c.smem) != cudaSuccess)
         return jllm_fail(JLLM_CUDA_ERROR, "gemm_int8: %zu bytes of shared memory refused", c.smem);
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = cluster_config<Tout>(c, tiles, attr, stream);
+    cudaLaunchConfig_t cfg = cluster_config(c, tiles, attr, stream);
     if (jllm_launch_overlaps(c.smem, LAUNCH_DEPENDENT)) {
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -548,7 +539,7 @@ int resident_clusters(int blocks) {
     ClusterCut one{};
     one.blocks = blocks, one.smem = SMEM_ROOM;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = cluster_config<Tout>(one, 1, attr, nullptr);
+    const cudaLaunchConfig_t cfg = cluster_config(one, 1, attr, nullptr);
     if (jllm_allow_smem((const void*)gemm_int8_cluster_kernel<Tout>, SMEM_ROOM) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, gemm_int8_cluster_kernel<Tout>, &cfg) != cudaSuccess) {
         cudaGetLastError();
@@ -601,7 +592,7 @@ int run_cluster(const Product& p, int code) {
     JLLM_REQUIRE(p.starve.what == STARVE_NOTHING || (units * c.blocks <= 64 && (p.starve.what != STARVE_PARTS || c.blocks > 1)),
                  "gemm_int8: the starved product of the wait test has at most 64 blocks, and a cluster where parts are missed");
     CUtensorMap map_a;
-    const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, true, &map_a);
+    const int rc = byte_map_for(p.a, M, p.K, p.lda, c.ntok, &map_a);
     if (rc != JLLM_OK) return rc;
     uint32_t cols = 32;
     while ((int)cols < c.ntok) cols <<= 1;
