@@ -195,15 +195,17 @@ struct ClusterArgs {
     const int8_t* w;
     const float *scale_w, *scale_a;
     Finish f;
-    int k_blocks, ntok, stages, blocks, share;      // ntok: the MMAs' N; share: tokens a block finishes
+    int k_blocks, ntok, ring, blocks, share;        // ntok: the MMAs' N; share: tokens a block finishes; ring: below
     int groups, span;                               // groups of `span` tokens
     uint32_t tmem_cols;
     int* error_word;
-    unsigned long long limit;                       // what a wait may last, ns
-    int starve;                                     // (a test of the waits: jllm_gemm_int8_starve_next)
 };
-// STARVE_*: what never happens in the starved product
+// The ring's stages, and of a test of the waits (jllm_gemm_int8_starve_next) what never happens in it and its limit in us (0: WAIT_NS), in one
+// word: an argument more is a line more of the arguments, and a product of few rows waits 0.1 us for it.
 enum : int { STARVE_NOTHING = 0, STARVE_COPY = 1, STARVE_RELEASE = 2, STARVE_PARTS = 3 };
+constexpr int ring_word(int stages, int starve, int limit_us) { return stages | starve << 8 | limit_us << 10; }
+constexpr int MOST_LIMIT_US = 1000000;
+static_assert(ring_word(255, STARVE_PARTS, MOST_LIMIT_US) > 0, "20 bits of a limit");
 
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit) {
     unsigned long long began = 0;
@@ -239,7 +241,8 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     __shared__ __align__(16) float token_scales[256];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-    const int stages = g.stages, blocks = g.blocks, share = g.share;
+    const int stages = g.ring & 255, starve = g.ring >> 8 & 3, blocks = g.blocks, share = g.share;
+    const unsigned long long limit = g.ring >> 10 ? (g.ring >> 10) * 1000ull : WAIT_NS;
     const uint32_t stage_bytes = TILE_BYTES + (uint32_t)g.ntok * BK, parts_at = (uint32_t)stages * stage_bytes;
     const uint32_t part_bytes = (uint32_t)share * 128 * 4;         // one block's part of a share, [share / 4][128 rows][4 tokens]
     const uint32_t bars_at = parts_at + (uint32_t)(blocks - 1) * part_bytes, bars = base + bars_at;
@@ -271,11 +274,11 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         mbar_init(acc_bar, 1);
         mbar_init(parts_bar, 1);
         *abort_flag = 0;
-        if (g.starve != STARVE_NOTHING) {
-            if (g.starve == STARVE_RELEASE) {
+        if (starve != STARVE_NOTHING) {
+            if (starve == STARVE_RELEASE) {
                 asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(empty_bar(0)) : "memory");
                 mbar_init(empty_bar(0), 2);
-            } else if (g.starve == STARVE_PARTS) mbar_expect_more(parts_bar, 16);
+            } else if (starve == STARVE_PARTS) mbar_expect_more(parts_bar, 16);
             else if (rank == 0) mbar_expect_more(full_bar(0), 16);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -313,7 +316,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         int s = 0, i = early;
         uint32_t parity = 0;                                   // the ring's second lap waits for the first lap's release
         for (; i < n_kb; ++i) {
-            if (!warp_wait(empty_bar(s), parity, abort_flag, 2 * g.limit)) { ok = false; break; }
+            if (!warp_wait(empty_bar(s), parity, abort_flag, 2 * limit)) { ok = false; break; }
             if (elect_one()) {
                 const uint32_t dst = base + (uint32_t)s * stage_bytes;
                 mbar_expect_tx(full_bar(s), stage_bytes);
@@ -325,7 +328,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
         for (int j = max(0, n_kb - stages); ok && j < n_kb; ++j)
-            ok = warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * g.limit);
+            ok = warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * limit);
         issued = i;
         if (!ok && lane == 0) give_up(31);
         if (blocks > 1) cluster_wait();
@@ -338,7 +341,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         uint32_t parity = 0;
         pdl_wait();          // (the copies are complete no sooner, and the time that the kernel in front still takes is not this wait's)
         for (; i < n_kb; ++i) {
-            if (!warp_wait(full_bar(s), parity, abort_flag, g.limit)) { ok = false; break; }
+            if (!warp_wait(full_bar(s), parity, abort_flag, limit)) { ok = false; break; }
             tcgen05_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -370,7 +373,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         for (int i = threadIdx.x - 64; i < 256; i += 128) token_scales[i] = i < here ? g.scale_a[first + i] : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (blocks > 1) cluster_wait();
-        ok = mbar_wait(acc_bar, 0, abort_flag, 2 * g.limit);
+        ok = mbar_wait(acc_bar, 0, abort_flag, 2 * limit);
         ok = __all_sync(0xffffffffu, ok);
         tcgen05_fence_after();
         if (ok)
@@ -394,7 +397,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 for (; t + 16 <= t1; t += 16) send(v16, t);
                 if (t < t1) send(v8, t);
             }
-        if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag, 2 * g.limit));
+        if (ok && blocks > 1 && mine < mine_end) ok = __all_sync(0xffffffffu, wait_cluster(parts_bar, 0, abort_flag, 2 * limit));
         if (ok) {
             const uint8_t* parts = aligned + parts_at + (size_t)row * 16;
             auto add_up = [&](auto& sum, int t) {
@@ -423,8 +426,8 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         // (where no wait ran out these have been waited for: the copies by the MMAs, the MMAs by the epilogue and the producer)
         const unsigned long long began = now_ns();
         if (warp == 0)
-            for (int j = max(0, issued - stages); j < issued; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, began, g.limit);
-        if (warp == 1 && issued > 0) drain(empty_bar((issued - 1) % stages), (uint32_t)((issued - 1) / stages) & 1u, began, g.limit);
+            for (int j = max(0, issued - stages); j < issued; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, began, limit);
+        if (warp == 1 && issued > 0) drain(empty_bar((issued - 1) % stages), (uint32_t)((issued - 1) / stages) & 1u, began, limit);
         __syncthreads();
     }
     if (warp == 2) {
@@ -437,7 +440,7 @@ gemm_int8_cluster_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (blocks > 1) {
         cluster_arrive();
         cluster_wait();
-        if (gave_up) drain(parts_bar, 0, now_ns(), g.limit);
+        if (gave_up) drain(parts_bar, 0, now_ns(), limit);
     }
 }
 
@@ -551,10 +554,9 @@ int resident_clusters(int blocks) {
 
 // A test of the waits: what the next product of this thread is to miss, and how long its waits last.
 struct Starve {
-    int what;
-    unsigned long long limit;
+    int what, limit_us;
 };
-thread_local Starve g_starve_next = {STARVE_NOTHING, WAIT_NS};
+thread_local Starve g_starve_next = {STARVE_NOTHING, 0};
 
 struct Product {
     const int8_t *a, *w;
@@ -596,8 +598,8 @@ int run_cluster(const Product& p, int code) {
     if (rc != JLLM_OK) return rc;
     uint32_t cols = 32;
     while ((int)cols < c.ntok) cols <<= 1;
-    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, c.stages, c.blocks, c.share, c.groups, c.span, cols, p.error_word,
-                        p.starve.limit, p.starve.what};
+    const ClusterArgs g{p.w, p.scale_w, p.scale_a, p.f, p.k_blocks, c.ntok, ring_word(c.stages, p.starve.what, p.starve.limit_us), c.blocks, c.share,
+                        c.groups, c.span, cols, p.error_word};
     return p.out_dtype == JLLM_F32 ? launch_cluster<float>(map_a, g, c, (int)units, p.out, p.stream)
                                    : launch_cluster<__nv_bfloat16>(map_a, g, c, (int)units, p.out, p.stream);
 }
@@ -687,8 +689,8 @@ int* jllm_gemm_error_word();
 // expects more than comes, with 2 a stage that is never released, with 3 a part that no block of the cluster sends (0: the limit alone). It
 // returns, raises the error word and leaves the device usable.
 JLLM_EXPORT int jllm_gemm_int8_starve_next(int what, int limit_us) {
-    JLLM_REQUIRE(what >= STARVE_NOTHING && what <= STARVE_PARTS && limit_us >= 1 && limit_us <= 1000000, "gemm_int8_starve_next: %d, %d us", what, limit_us);
-    g_starve_next = {what, limit_us * 1000ull};
+    JLLM_REQUIRE(what >= STARVE_NOTHING && what <= STARVE_PARTS && limit_us >= 1 && limit_us <= MOST_LIMIT_US, "gemm_int8_starve_next: %d, %d us", what, limit_us);
+    g_starve_next = {what, limit_us};
     return JLLM_OK;
 }
 
@@ -702,7 +704,7 @@ JLLM_EXPORT int jllm_gemm_int8(const Int8View* rows, const Int8View* weight, con
     const int M = rows->rows, K = rows->cols, lda = rows->stride, N = weight->rows, k_blocks = weight->stride;
     const GluArgs glu = glu_args(swiglu_word, nullptr);
     const Starve starve = g_starve_next;
-    g_starve_next = {STARVE_NOTHING, WAIT_NS};
+    g_starve_next = {STARVE_NOTHING, 0};
     JLLM_REQUIRE(M >= 0 && M <= INT8_MOST && N >= 1 && K >= 1 && K <= MAX_K && weight->cols == K, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d) against a weight of %d",
                  M, N, K, MAX_K, weight->cols);
     JLLM_REQUIRE(lda >= K && lda % 16 == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)w_packed % 16) == 0 && ((uintptr_t)scale_w % 16) == 0,
