@@ -186,11 +186,13 @@ struct TokenEpilogue {
 // Bound by memory where the weight is large: one row against 24,576 x 4,096 17.3 us (5.8 TB/s, 0.89 of the measured copy), 4,096 x 12,288
 // 10.7 (4.7), 64 rows of it 11.1; below that by the way from launch to last store (about 3 us beside the stream: 5.5 us for the 16.8 MB of
 // 4,096 x 4,096).
-// With many tokens it is what an SM takes in: a ring of 200 KB (or two of 100 KB: two blocks an SM, the one's epilogue under the other's main
-// loop) against the 1 to 2 us that a copy is on its way when all SMs ask. 2,048 rows of 24,576 x 4,096, gated: 173 us alone (2.4 POP/s), 199
-// one behind the other under the power limit. (Pairs of SMs with `cta_group::2`, which take in a third less, took 130 us for it, 147 under the
-// limit, and 29 where 300 rows take 40 here. Models that ran them stopped now and then without a wait that gave up. The cause is not known, and
-// that it lies in the pairs is not shown; they are gone because they could not be cleared.)
+// With many tokens neither the tensor pipe nor what an SM takes in is full. 300 rows of 24,576 x 4,096, gated, take 40 us: the pipe is active for
+// a third of it, 10 TB/s come from L2; 2,048 rows take 176 us alone (2.3 POP/s; 203 one behind the other under the power limit): 53% and
+// 14 TB/s. A block has one tile, and barriers, tensor memory, the first copies and the epilogue are paid for each: with the cut held some 16 and
+// 45 us of these do not depend on k. A ring of 200 KB, or two of 100 KB (two blocks an SM: the one's epilogue under the other's main loop), stands
+// against the 1 to 2 us that a copy is on its way when all SMs ask. (Pairs of SMs with `cta_group::2` took 130 us for the 2,048 rows, 147 under the
+// limit, and 29 for the 300. Models that ran them stopped now and then, and none of this product's waits gave up. The cause is not known, and that
+// it lies in the pairs is not shown; they are gone because they could not be cleared.)
 struct ClusterArgs {
     const int8_t* w;
     const float *scale_w, *scale_a;
@@ -604,11 +606,13 @@ int run_cluster(const Product& p, int code) {
                                    : launch_cluster<__nv_bfloat16>(map_a, g, c, (int)units, p.out, p.stream);
 }
 
-// What a product takes, about, in us (up to what all ways take alike), fitted to products launched back to back on weights larger than L2.
+// A count that puts the cuts in order. Its terms follow what a product does and its constants are fitted so that the least count is a fast cut, to
+// products launched back to back on weights larger than L2; a constant is no duration and a count no time (300 plain rows of 24,576 x 4,096
+// count 28 and take 37 us, 2,048 count 133 and take 174).
 // Up to 256 rows (one group; 846 sizes of 1 to 256 rows against 128 to 34,816 weight rows of 256 to 17,408 values: what is chosen is 2.1% slower than
-// the best way of each size in the geometric mean): a block's k blocks, each a ring's share of the 1.13 us that a copy is on its way, or 0.12 us and
-// 0.55 ns a token; all clusters at once, one block an SM, or (half of that a round) two blocks side by side, or one batch behind the other; nothing
-// of the next product beside it: 0.3 us; sending 0.15 us a block of the cluster and 10 ns a token sent; no faster than memory and L2 give the weights.
+// the best way of each size in the geometric mean): a block's k blocks, each 1.13 shared by the ring's stages (a copy's way) or 0.12 and 0.00055 a
+// token (the MMAs); all clusters at once, one block an SM, or (half of that a round) two blocks side by side, or one batch behind the other; 0.3 where
+// nothing of the next product lies beside it; sending 0.15 a block of the cluster and 0.01 a token sent; the weights' bytes by READ_BYTES_US at least.
 constexpr double READ_BYTES_US = 1e7;
 template <typename Tout>
 double cluster_cost(int M, int N, int k_blocks, const Cut& cut) {
@@ -627,9 +631,9 @@ double cluster_cost(int M, int N, int k_blocks, const Cut& cut) {
 }
 
 // More rows (groups of them; 162 sizes of 300 to 2,048 rows against 1,024 to 24,576 weight rows of 1,024 to 12,288 values: 1.6%): all SMs take in at once.
-// One block an SM: rounds of k blocks, each the ring's share of 1.06 us, or 0.135 us and 0.27 ns a token, and 1.9 us and 10 ns a token to begin and
-// end. Two blocks side by side: the SM's share of all k blocks at 0.215 us and 0.25 ns a token (or a ring's share of 1.45 us), an end that shows
-// once, 2 us a batch. Sending 0.55 us a block of the cluster and 43 ns a token.
+// One block an SM: rounds of k blocks, each 1.06 shared by the stages or 0.135 and 0.00027 a token, and 1.9 and 0.0104 a token to begin and end. Two
+// blocks side by side: the SM's share of all k blocks at 0.215 and 0.00025 a token (or 1.45 shared by both rings), an end that shows once, 2 a batch.
+// Sending 0.55 a block of the cluster and 0.043 a token.
 template <typename Tout>
 double groups_cost(int M, int N, int k_blocks, const Cut& cut) {
     const ClusterCut c = cluster_cut(cut.blocks, cut.deep, cut.groups, M, k_blocks);

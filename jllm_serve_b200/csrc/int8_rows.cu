@@ -9,8 +9,8 @@
 // What a row cannot say in 8 bits: a row whose largest magnitude is below 2^-100 is zeros with scale 0 (127 / m would leave
 // float32; of the norm's results such a row may keep its numbers), a row that holds an infinity or a NaN has the scale NaN and zeros, so that what is made of it is NaN and not a wrong number.
 //
-// Memory bounds them: 2,048 x 4,096 with bfloat16 added 15.8 us for 92 MB (5.8 TB/s, 0.89 of the measured copy), 2,048 x 12,288 quantised 14.0 us
-// for 75 MB (5.4 TB/s), 544 x 5,120 added 6.9 us for 31 MB; of a few rows what shows is a launch, one round trip to memory and the meeting (1.3 to
+// Memory bounds them: 2,048 x 4,096 with bfloat16 added 15.9 us for 92 MB (5.8 TB/s, 0.88 of the measured copy), 2,048 x 12,288 quantised 14.1 us
+// for 75 MB (5.4 TB/s), 544 x 4,096 added 5.9 us for 25 MB; of a few rows what shows is a launch, one round trip to memory and the meeting (1.3 to
 // 2.2 us). What made them so: one reduction where three passes took 63 us; values rounded by an addition and magnitudes compared as integers
 // (the quarter-rate conversions bounded 2,048 x 12,288 at 22 us); the gains under way before the wait (10.5 -> 6.9 us at 544 rows).
 //

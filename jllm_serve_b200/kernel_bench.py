@@ -172,21 +172,24 @@ def main() -> int:
 
 
 def int8_cases(ops, case, args, dev, steps, D, qkv, F) -> None:
-    """The linears of one layer in 8-bit integers, at a decode step's rows and a prompt's."""
+    """The linears of one layer in 8-bit integers, at a decode step's rows and a prompt's, with the results that a layer gives them: qkv and
+    the units in bfloat16, O's in float32 for the norm behind it, down's added into the float32 residual."""
     def weights(n, k, glu=False):
         copies = max(2, int(300e6 // (n * k)) + 1) if args.repeat > 1 else 1
         return [ops.quantize_weight_int8(torch.randn(n, k, device=dev) * k ** -0.5, glu) for _ in range(copies)]
 
-    named = {"qkv": weights(qkv, D), "o": weights(D, D), "gate_up + swiglu": weights(2 * F, D, True), "down": weights(D, F)}
+    named = {"qkv": weights(qkv, D), "o (float32)": weights(D, D), "gate_up + swiglu": weights(2 * F, D, True), "down (+= residual)": weights(D, F)}
     for step, rows in zip(("decode", "prefill"), steps):
         for what, ws in named.items():
             n, k = ws[0].shape
             a = ops.int8_rows(rows, k, dev)
             ops.quantize_int8(torch.randn(rows, k, device=dev), a)
             glu = ws[0].glu
-            out = torch.empty(rows, n // 2 if glu else n, device=dev, dtype=torch.bfloat16)
+            add = what.startswith("down")
+            out = torch.zeros(rows, n // 2 if glu else n, device=dev, dtype=torch.float32 if add or what.startswith("o ") else torch.bfloat16)
             size = dict(bytes_=n * k) if step == "decode" else dict(flops=2 * rows * n * k)
-            case(f"{step} int8 gemm {what}", lambda i, a=a, ws=ws, out=out, glu=glu: ops.gemm_int8(a, ws[i], out, swiglu=glu), len(ws), **size)
+            case(f"{step} int8 gemm {what}", lambda i, a=a, ws=ws, out=out, glu=glu, add=add: ops.gemm_int8(a, ws[i], out, accumulate=add, swiglu=glu),
+                 len(ws), **size)
         copies = max(2, int(300e6 // (rows * D * 11)) + 1) if step == "prefill" and args.repeat > 1 else 1
         xs = [torch.randn(rows, D, device=dev) for _ in range(copies)]
         ys, ts, qs = [x.bfloat16() for x in xs], [torch.empty_like(x) for x in xs], [ops.int8_rows(rows, D, dev) for _ in xs]

@@ -8,7 +8,7 @@ PACKED once, when the part is built (`ops.pack_weight`: tiles of 128 rows x 64 k
 tensor cores read, so a tile is one contiguous bulk copy), and the row-major copy is let go.
 
 With `Runtime.weights` "int8" the layers' products are `Int8Linear`s instead: weight and rows in 8-bit integers, a scale a weight row
-and a scale a token (`ops.gemm_int8`). Half the bytes of a bfloat16 weight, and twice the tensor cores' rate.
+and a scale a token (`ops.gemm_int8`). Half the bytes of a bfloat16 weight, on tensor cores of twice the rate.
 """
 from __future__ import annotations
 
