@@ -48,7 +48,8 @@ class ModelRunner:
         with `num_pages="auto"`, the share `kv_share` of the device memory that is free once the weights are
         loaded (never more than `max_requests` full contexts need). `weights` "int8": the layers' weights are rounded to 8-bit integers
         when they are loaded, one scale a row, and the rows that meet them at every step, one scale a token (bfloat16 models of
-        attention and dense feed-forward layers; embedding, head, norms and cache stay as they are)."""
+        attention and dense feed-forward layers; embedding, head, norms and cache stay as they are, and between a layer's products the
+        attention's result and the gated units are bfloat16 before their 8 bits, what is added to the residual float32)."""
         ops.require_device()
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
