@@ -1,0 +1,25 @@
+// What a launcher is told of rows, of a packed weight and of groups of rows: laid out once by whoever holds them, and not argument by argument
+// at every call.
+#pragma once
+#include <stdint.h>
+
+// Rows of activations: bfloat16 (scale null), or e4m3 with a float32 scale for each 128 values of a row.
+struct BlockRows {
+    const void* data;
+    const float* scale;
+    long long stride;            // bytes from row to row
+    int rows, cols, scale_ld;
+};
+// A packed weight of `groups` matrices [rows, cols]: the tiles, and of e4m3 the scales of every eight rows and 128 k.
+struct BlockWeight {
+    const void* data;
+    const float* scale;
+    int groups, rows, cols, k_blocks, scale_ld, glu;
+};
+// The pairs (row, choice) in the order of their groups: group g's are order[offsets[g]] .. order[offsets[g + 1] - 1]; place is the way back.
+struct RowGroupsView {
+    int *offsets, *order, *place;
+    int rows, top, groups;
+};
+// The kernels count rows, pairs and values in 32 bits and step past the end by up to a block's 8,192 values.
+constexpr int BLOCK_MOST = 0x7fffffff - 8191;

@@ -218,6 +218,12 @@ class _Signatures:
     jllm_pack_int8 = [P, ctypes.c_longlong, I, I, I, P, P]
     jllm_gemm_int8 = [P, P, P, I, P, I, I, I, I, I, P]
     jllm_gemm_int8_starve_next = [I, I]
+    jllm_quantize_fp8 = [P, I, ctypes.c_longlong, P, P]
+    jllm_fp8_values = [P, P, I, ctypes.c_longlong, P]
+    jllm_gemm_grouped = [P, P, P, I, P, I, P, I, I, I, I, I, P]
+    jllm_gemm_grouped_starve_next = [I, I]
+    jllm_group_rows = [P, I, P, P]
+    jllm_combine_groups = [P, I, I, P, P, I, P, I, I, I, I, P]
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -1197,7 +1203,7 @@ def bounds_errors() -> dict:
 
 # Which kernel a code in an error word is from: the products share one word, the attention kernels another.
 WAIT_KERNELS = {"products": ((1, 3, "gemm_tcgen05"), (11, 13, "gemm_stream"), (14, 16, "gemm_stream (clusters)"), (21, 23, "gemm_pair"),
-                             (31, 33, "gemm_int8")),
+                             (31, 33, "gemm_int8"), (41, 43, "gemm_grouped")),
                 "attention": ((21, 23, "attention_prefill_tc"), (31, 33, "attention_prefill_pair"), (41, 43, "attention_prefill_latent"),
                               (51, 52, "attention_decode_ring"))}
 
@@ -1750,3 +1756,296 @@ def gemm_int8_starve_next(what: str, limit_us: int = 2000) -> None:
     the "parts" of its cluster's other blocks ("nothing": the limit alone); it returns and raises the error word that `check_kernel_errors` reads."""
     if library().jllm_gemm_int8_starve_next(("nothing", "copy", "release", "parts").index(what), int(limit_us)):
         _refuse("gemm_int8_starve_next", f"a limit of 1 to 1,000,000 us, got {limit_us}")
+
+
+# ---- products in 8-bit floating point, and of ragged groups of rows (routed experts) --------------------------
+
+BLOCK = 128                        # values that share a scale; of a weight 128 x 128
+BLOCK_MOST = 0x7fffffff - 8191     # rows, pairs and values of a row: the kernels count them in 32 bits and step past the end by up to 8,192
+MOST_GROUPS = 1024
+
+
+class _BlockRows(ctypes.Structure):          # (fp8_view.h)
+    _fields_ = [("data", c_void_p), ("scale", c_void_p), ("stride", ctypes.c_longlong), ("rows", c_int), ("cols", c_int), ("scale_ld", c_int)]
+
+
+class _BlockWeight(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("scale", c_void_p), ("groups", c_int), ("rows", c_int), ("cols", c_int), ("k_blocks", c_int),
+                ("scale_ld", c_int), ("glu", c_int)]
+
+
+class _RowGroupsView(ctypes.Structure):
+    _fields_ = [("offsets", c_void_p), ("order", c_void_p), ("place", c_void_p), ("rows", c_int), ("top", c_int), ("groups", c_int)]
+
+
+def _on_current_device(name, *tensors):
+    """The launchers run on the current device's current stream: what they are given lies there."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if not t.is_cuda or t.device.index != here:
+            _refuse(name, f"everything lies on the current CUDA device, got {t.device}")
+
+
+class Fp8Rows:
+    """Rows of activations in 8-bit floating point: value j of row r stands for data[r, j] * scale[r, j // 128]. data float8_e4m3fn [rows, cols],
+    its rows beginning at multiples of 16 bytes; scales float32 [rows, blocks filled up to a multiple of four], 16-byte aligned (`fp8_rows` makes
+    such). `scale` are the blocks that the columns have. A slice of rows is `rows8[lo:hi]`."""
+    __slots__ = ("data", "scales", "scale", "rows", "cols", "shape", "blocks", "on_gpu", "_view", "view")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        if data.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32 or data.dim() != 2 or scales.dim() != 2 or scales.shape[0] != data.shape[0]:
+            _refuse("Fp8Rows", f"e4m3 data [rows, cols] and float32 scales [rows, blocks], got {data.dtype} {tuple(data.shape)} and {scales.dtype} {tuple(scales.shape)}")
+        self.data, self.scales = data, scales
+        self.rows, self.cols = self.shape = tuple(data.shape)
+        self.blocks = -(-self.cols // BLOCK)
+        self.on_gpu = data.is_cuda and scales.is_cuda and data.device == scales.device
+        stride = data.stride(0) if self.rows > 1 else -(-self.cols // 16) * 16              # (a single row's stride says nothing)
+        ld = scales.shape[1]
+        if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or stride < self.cols or stride % 16 or data.data_ptr() % 16 or max(self.shape) > BLOCK_MOST
+                or ld % 4 or ld < self.blocks or not scales.is_contiguous() or scales.data_ptr() % 16):
+            _refuse("Fp8Rows", f"neighbouring values that begin at multiples of 16 bytes and scales in whole fours, got {self.shape}, strides {data.stride()}, "
+                               f"scales {tuple(scales.shape)}, {scales.stride()} at {data.data_ptr():#x}, {scales.data_ptr():#x}")
+        self.scale = scales[:, :self.blocks]
+        # what the launchers are told of the rows, laid out once
+        self._view = _BlockRows(data.data_ptr(), scales.data_ptr(), stride, self.rows, self.cols, ld)
+        self.view = ctypes.addressof(self._view)
+
+    def __getitem__(self, rows: slice) -> "Fp8Rows":
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            _refuse("Fp8Rows", "a slice of neighbouring rows is what can be taken")
+        return Fp8Rows(self.data[rows], self.scales[rows])
+
+
+def fp8_rows(rows: int, cols: int, device) -> Fp8Rows:
+    """Room for `rows` rows of `cols` values in 8 bits (what `quantize_fp8` writes). (The bytes that fill a row up to 16 are there, and nobody's.)"""
+    if rows < 0 or cols < 1 or max(rows, cols) > BLOCK_MOST:
+        _refuse("fp8_rows", f"up to {BLOCK_MOST} rows of as many values, got {rows} x {cols}")
+    data = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((rows, -(-cols // (4 * BLOCK)) * 4), dtype=torch.float32, device=device)
+    return Fp8Rows(data[:, :cols], scales)
+
+
+def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
+    """out = the rows of x in 8-bit floating point: of every 128 neighbouring values scale = max(m, 2^-100) / 448 with m their largest magnitude, q =
+    x / scale rounded once to e4m3, half to even. x float32 or bfloat16 [rows, cols], any row stride. 128 values that hold an infinity or a NaN become
+    zeros with scale NaN (what is computed from them is then NaN)."""
+    name = "quantize_fp8"
+    if x.dtype not in _DT:
+        _refuse(name, f"float32 or bfloat16 rows, got {x.dtype}")
+    _on_current_device(name, x, out.data, out.scales)
+    _call("jllm_quantize_fp8", x.data_ptr(), _DT[x.dtype], _row_stride(name, "x", x, out.shape), out.view, _stream())
+
+
+def fp8_values(rows8: Fp8Rows, out: torch.Tensor) -> torch.Tensor:
+    """out = the values that the rows stand for, data * scale, float32 or bfloat16; returns out."""
+    name = "fp8_values"
+    if out.dtype not in _DT:
+        _refuse(name, f"float32 or bfloat16 values, got {out.dtype}")
+    _on_current_device(name, out, rows8.data, rows8.scales)
+    _call("jllm_fp8_values", rows8.view, out.data_ptr(), _DT[out.dtype], _row_stride(name, "out", out, rows8.shape), _stream())
+    return out
+
+
+class PackedBlocks:
+    """One weight [rows, cols], or one for each of `groups`, in the layout the tensor cores stream: tiles of 128 rows x 128 bytes of k (64 bfloat16
+    or 128 e4m3), each the 16 KB image of its 128-byte-swizzled shared-memory form, rows and k filled up with zeros. Of e4m3 weights `scales` [groups,
+    eights of rows, k blocks filled up to a multiple of four]: every eight rows' scales (they lie in one block of 128 rows). `glu`: the rows are blocks of
+    8 gate rows and their 8 up rows."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor | None, groups: int, rows: int, cols: int, glu: bool = False):
+        self.data, self.scales, self.groups, self.rows, self.cols, self.glu = data, scales, groups, rows, cols, glu
+        self.shape, self.tiles, self.k_blocks = (rows, cols), data.shape[1], data.shape[2]
+        self.fp8 = scales is not None
+        self._view = _BlockWeight(data.data_ptr(), _p(scales), groups, rows, cols, self.k_blocks, scales.shape[2] if self.fp8 else 0, int(glu))
+        self.view = ctypes.addressof(self._view)
+
+    def unpack(self) -> torch.Tensor:
+        """The [groups, rows, cols] values again (e4m3 without their scales), rows in the order they were packed in (tests)."""
+        G, T, KB = self.data.shape[:3]
+        idx = _swizzle_index(self.data.device).expand(G * T, KB, 128, 8, 16)
+        plain = self.data.view(G * T, KB, 128, 8, 16).gather(3, idx).permute(0, 2, 1, 3, 4).reshape(G, T * 128, KB * 128)
+        plain = plain.contiguous().view(torch.float8_e4m3fn if self.fp8 else torch.bfloat16)
+        return plain[:, :self.rows, :self.cols].contiguous()
+
+
+def _pack_bytes(name, w: torch.Tensor, glu: bool) -> torch.Tensor:
+    """[groups, rows, cols] values -> [groups, tiles, k blocks, 128, 128] bytes."""
+    G, N, K = w.shape
+    if glu and N % 16:
+        _refuse(name, f"gate and up rows in eights, got {N}")
+    if G * N == 0 or K == 0 or max(N, K * w.element_size()) > BLOCK_MOST or G > MOST_GROUPS:
+        _refuse(name, f"1 to {MOST_GROUPS} weights of up to {BLOCK_MOST} rows and bytes a row, got {tuple(w.shape)}")
+    w = w.contiguous().view(torch.int8)
+    K = w.shape[2]
+    T, KB = -(-N // 128), -(-K // 128)
+    if not w.is_cuda:            # (without a GPU: what the layout is, for whoever looks at it)
+        padded = torch.zeros((G, T * 128, KB * 128), dtype=torch.int8)
+        padded[:, :N, :K] = torch.stack([_glu_order(one) for one in w]) if glu else w
+        tiles = padded.view(G * T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)
+        return tiles.gather(3, _swizzle_index(w.device).expand(G * T, KB, 128, 8, 16)).contiguous().view(G, T, KB, 128, 128)
+    _on_current_device(name, w)
+    packed = torch.empty((G, T, KB, 128, 128), dtype=torch.int8, device=w.device)
+    for g in range(G):
+        _call("jllm_pack_int8", w[g].data_ptr(), K, N, K, int(glu), packed[g].data_ptr(), _stream())
+    return packed
+
+
+def pack_fp8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> PackedBlocks:
+    """Packs an e4m3 weight [rows, cols] with a float32 scale for every 128 x 128 block ([rows / 128, cols / 128], rounded up) for `gemm_fp8`, or
+    the weights [groups, rows, cols] of as many groups for `gemm_grouped` (done once, at load). `glu`: the rows are all gate rows, then all up rows (a
+    multiple of 8 each), and are laid out for a product with `swiglu`; the blocks are those of the rows as they are given."""
+    name = "pack_fp8"
+    if data.dim() == 2 and scale.dim() == 2:
+        data, scale = data[None], scale[None]
+    blocks = (data.shape[0], -(-data.shape[-2] // BLOCK), -(-data.shape[-1] // BLOCK)) if data.dim() == 3 else ()
+    if data.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32 or scale.shape != blocks or data.device != scale.device:
+        _refuse(name, f"e4m3 weights [groups, rows, cols] and a float32 scale for each 128 x 128 of them, got {data.dtype} {tuple(data.shape)} and {scale.dtype} {tuple(scale.shape)}")
+    G, N, K = data.shape
+    packed = _pack_bytes(name, data, glu)
+    T, KB = packed.shape[1:3]
+    first = torch.arange(0, -(-N // 8) * 8, 8, device=data.device)                       # the first row of every eight, as they lie in the tiles
+    if glu:
+        half = N // 2
+        first = torch.stack([first[:half // 8], first[:half // 8] + half], dim=1).reshape(-1)
+    scales = torch.zeros((G, T * 16, -(-KB // 4) * 4), dtype=torch.float32, device=data.device)
+    scales[:, :first.numel(), :KB] = scale[:, first // BLOCK]
+    return PackedBlocks(packed, scales, G, N, K, glu)
+
+
+def pack_grouped(weight: torch.Tensor, glu: bool = False) -> PackedBlocks:
+    """Packs the bfloat16 weights [groups, rows, cols] of as many groups for `gemm_grouped` (done once, at load); cols a multiple of 8. `glu` as in
+    `pack_fp8`."""
+    if weight.dim() != 3 or weight.dtype != torch.bfloat16 or weight.shape[2] % 8:
+        _refuse("pack_grouped", f"bfloat16 weights [groups, rows, cols], cols a multiple of 8, got {weight.dtype} {tuple(weight.shape)}")
+    return PackedBlocks(_pack_bytes("pack_grouped", weight, glu), None, *weight.shape, glu)
+
+
+def quantize_weight_fp8(weight: torch.Tensor, glu: bool = False) -> PackedBlocks:
+    """A float32 or bfloat16 weight [rows, cols], or [groups, rows, cols], rounded to e4m3 with a scale for every 128 x 128 block (the largest magnitude over
+    448), and packed."""
+    if weight.dtype not in _DT or weight.dim() not in (2, 3) or not weight.numel():
+        _refuse("quantize_weight_fp8", f"a float32 or bfloat16 weight [rows, cols] or [groups, rows, cols], got {weight.dtype} {tuple(weight.shape)}")
+    if weight.dim() == 2:
+        weight = weight[None]
+    G, N, K = weight.shape
+    data = torch.empty((G, N, K), dtype=torch.float8_e4m3fn, device=weight.device)
+    scale = torch.empty((G, -(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=weight.device)
+    for g in range(G):                            # (a weight at a time: the blocks are float32 beside it)
+        padded = torch.nn.functional.pad(weight[g].float(), (0, -K % BLOCK, 0, -N % BLOCK))
+        blocks = padded.view(scale.shape[1], BLOCK, scale.shape[2], BLOCK)
+        scale[g] = blocks.abs().amax(dim=(1, 3)).clamp(min=2.0 ** -100) / 448.0
+        data[g] = (blocks / scale[g][:, None, :, None]).clamp(-448.0, 448.0).view(padded.shape)[:N, :K].to(torch.float8_e4m3fn)
+    return pack_fp8(data, scale, glu)
+
+
+def _product_words(name, w: PackedBlocks, swiglu) -> int:
+    word = glu_kind(swiglu) if swiglu else 0
+    if bool(word) != w.glu or isinstance(swiglu, GluUnits):
+        _refuse(name, "a gated unit without weights of its own goes with a weight packed for it, and only with one")
+    return word
+
+
+def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate=False, swiglu=False, cut: int = 0) -> None:
+    """out (+)= a @ w^T (+ bias) in 8-bit floating point: the tensor cores sum the products of 128 k in float32, both blocks' scales multiply each such sum
+    and the sums over the blocks are float32. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or bfloat16; `accumulate` as the other
+    products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`; no bias, nothing added): out[r, j] = act(gate_j) * up_j,
+    [rows, w.rows / 2]. The weight, its scales and the bias are read before what is in front on the stream has ended: not what a kernel right in front
+    writes. `cut` (tests): tokens of a span x 1,000, 128-row tiles of a unit x 100, blocks an SM x 10, blocks of a cluster; 0: as the sizes have it."""
+    name = "gemm_fp8"
+    word = _product_words(name, w, swiglu)
+    if not w.fp8 or w.groups != 1 or a.cols != w.cols or out.dtype not in _DT:
+        _refuse(name, f"e4m3 rows and one e4m3 weight of {w.cols} columns and a float32 or bfloat16 result, got {a.cols} columns, {w.groups} weights and {out.dtype}")
+    _on_current_device(name, a.data, a.scales, w.data, out)
+    if bias is None:
+        b, b_dtype = 0, F32
+    else:
+        if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_contiguous():
+            _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
+        _on_current_device(name, bias)
+        b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
+    _call("jllm_gemm_grouped", a.view, w.view, 0, 0, b, b_dtype, out.data_ptr(), _DT[out.dtype],
+          _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows)), int(accumulate), word, cut, _stream())
+
+
+class RowGroups:
+    """The (row, choice) pairs of a step in the order of the groups (experts) they ask: group g's pairs are order[offsets[g]] .. order[offsets[g + 1] - 1],
+    each r * top + c of its row r and choice c, in ascending order; `order` is -1 behind the last pair. place[r, c] is where the pair (r, c) lies, -1 if it
+    asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs."""
+    __slots__ = ("offsets", "order", "place", "rows", "top", "groups", "pairs", "_view", "view")
+
+    def __init__(self, offsets, order, place, rows, top, groups):
+        self.offsets, self.order, self.place, self.rows, self.top, self.groups = offsets, order, place, rows, top, groups
+        self.pairs = rows * top
+        self._view = _RowGroupsView(offsets.data_ptr(), order.data_ptr(), place.data_ptr(), rows, top, groups)
+        self.view = ctypes.addressof(self._view)
+
+    def first(self, rows: int) -> "RowGroups":
+        """The same room for a step of fewer rows (to be filled anew)."""
+        if not 0 <= rows <= self.rows:
+            _refuse("RowGroups", f"0 to {self.rows} rows, got {rows}")
+        return RowGroups(self.offsets, self.order[:rows * self.top], self.place[:rows], rows, self.top, self.groups)
+
+
+def row_groups(rows: int, top: int, groups: int, device) -> RowGroups:
+    """Room for the groups of `rows` rows that choose `top` of `groups` each."""
+    if rows < 0 or top < 1 or rows * top > BLOCK_MOST or not 1 <= groups <= MOST_GROUPS:
+        _refuse("row_groups", f"up to {BLOCK_MOST} pairs and 1 to {MOST_GROUPS} groups, got {rows} x {top} and {groups}")
+    offsets = torch.zeros((groups + 1,), dtype=torch.int32, device=device)
+    return RowGroups(offsets, torch.full((rows * top,), -1, dtype=torch.int32, device=device),
+                     torch.full((rows, top), -1, dtype=torch.int32, device=device), rows, top, groups)
+
+
+def group_rows(choice: torch.Tensor, groups: RowGroups) -> None:
+    """Fills `groups` from choice int32 [rows, top], any row stride: the group that each row asks with each of its choices; anything outside [0, groups) asks
+    nobody (the rows that fill a batch up, an entry without weights)."""
+    name = "group_rows"
+    if choice.dtype != torch.int32 or choice.shape != groups.place.shape:
+        _refuse(name, f"int32 choices {tuple(groups.place.shape)}, got {choice.dtype} {tuple(choice.shape)}")
+    _on_current_device(name, choice, groups.offsets)
+    _call("jllm_group_rows", choice.data_ptr(), _row_stride(name, "choice", choice, (groups.rows, groups.top)), groups.view, _stream())
+
+
+def gemm_grouped(a, w: PackedBlocks, groups: RowGroups, out: torch.Tensor, swiglu=False, by_pair: bool = False, cut: int = 0) -> None:
+    """out[p] = a[row of pair p] @ (the weight of p's group)^T for all pairs of `groups`, in the groups' order. a: the rows that asked [groups.rows, w.cols]
+    (fetched where they lie), or with `by_pair` a row for each pair, in the groups' order already; bfloat16 against bfloat16 weights (rows beginning at
+    multiples of 16 bytes), `Fp8Rows` against e4m3 ones. out [groups.pairs, w.rows] (with `swiglu`, of weights packed with `glu`, half as many columns:
+    act(gate) * up) float32 or bfloat16, any row stride; rows behind the last pair stay as they were. Only weights that are asked are read. `cut` (tests) as
+    in `gemm_fp8`, without clusters."""
+    name = "gemm_grouped"
+    word = _product_words(name, w, swiglu)
+    rows = groups.pairs if by_pair else groups.rows
+    if w.groups != groups.groups or isinstance(a, Fp8Rows) != w.fp8 or tuple(a.shape) != (rows, w.cols) or out.dtype not in _DT:
+        _refuse(name, f"{rows} rows of {w.cols} {'e4m3' if w.fp8 else 'bfloat16'} values, {groups.groups} weights and a float32 or bfloat16 result, got "
+                      f"{type(a).__name__} {tuple(a.shape)}, {w.groups} weights and {out.dtype}")
+    if w.fp8:
+        _on_current_device(name, a.data, a.scales, w.data, groups.offsets, out)
+        view = a.view
+    else:
+        _on_current_device(name, a, w.data, groups.offsets, out)
+        stride = _row_stride(name, "a", a, (rows, w.cols))
+        if a.dtype != torch.bfloat16 or a.data_ptr() % 16 or stride % 8:
+            _refuse(name, f"bfloat16 rows that begin at multiples of 16 bytes, got {a.dtype}, stride {stride} at {a.data_ptr():#x}")
+        held = _BlockRows(a.data_ptr(), 0, 2 * stride, rows, w.cols, 0)
+        view = ctypes.addressof(held)
+    _call("jllm_gemm_grouped", view, w.view, groups.view, int(by_pair), 0, F32, out.data_ptr(), _DT[out.dtype],
+          _row_stride(name, "out", out, (groups.pairs, w.rows // 2 if word else w.rows)), 0, word, cut, _stream())
+
+
+def combine_groups(answers: torch.Tensor, groups: RowGroups, share: torch.Tensor, out: torch.Tensor, accumulate: bool = False) -> None:
+    """out[r] (+)= sum over row r's choices c, in their order, of share[r, c] * answers[place[r, c]] in float32; a choice that asks nobody adds nothing (its
+    share is not read). answers [groups.pairs, dim] and out [groups.rows, dim] float32 or bfloat16, share float32 [rows, top]; any row strides."""
+    name = "combine_groups"
+    if answers.dtype not in _DT or out.dtype not in _DT or share.dtype != torch.float32 or answers.dim() != 2:
+        _refuse(name, f"float32 or bfloat16 answers and result and float32 shares, got {answers.dtype}, {out.dtype} and {share.dtype}")
+    _on_current_device(name, answers, groups.offsets, share, out)
+    dim = answers.shape[1]
+    _call("jllm_combine_groups", answers.data_ptr(), _DT[answers.dtype], _row_stride(name, "answers", answers, (groups.pairs, dim)), groups.view,
+          share.data_ptr(), _row_stride(name, "share", share, (groups.rows, groups.top)), out.data_ptr(), _DT[out.dtype],
+          _row_stride(name, "out", out, (groups.rows, dim)), dim, int(bool(accumulate)), _stream())
+
+
+def gemm_grouped_starve_next(what: str, limit_us: int = 2000) -> None:
+    """A test of the bounded waits: the next `gemm_grouped` or `gemm_fp8` has waits of `limit_us` microseconds and misses a "copy", a "release" of a stage or
+    the "parts" of its cluster's other blocks ("nothing": the limit alone); it returns and raises the error word that `check_kernel_errors` reads."""
+    if library().jllm_gemm_grouped_starve_next(("nothing", "copy", "release", "parts").index(what), int(limit_us)):
+        _refuse("gemm_grouped_starve_next", f"a limit of 1 to 1,000,000 us, got {limit_us}")
