@@ -32,7 +32,6 @@ using namespace tc;
 
 constexpr int TILE_BYTES = 128 * 128;
 constexpr int MAX_GROUPS = 1024;
-constexpr size_t SMEM_ROOM = 224 * 1024;
 
 struct Finish {
     VecRef bias;
@@ -119,6 +118,30 @@ __device__ __forceinline__ void mbar_expect_more(uint32_t bar, uint32_t bytes) {
 // What is still on its way when a wait has run out: waited for whatever the others do, until `limit` after `began`.
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, unsigned long long began, unsigned long long limit) {
     while (!mbar_try_wait(bar, parity) && now_ns() - began < limit) {}
+}
+
+// Units in front of every group, by the whole block (a lane has 32 neighbouring groups at most); a __syncthreads has to follow.
+template <int NT, int MT>
+__device__ __forceinline__ void list_units(const Args& g, int* before, int* at) {
+    pdl_wait();          // (the offsets are the kernel in front's)
+    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = g.offsets[i];
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x, each = (g.groups + 31) / 32, lo = min(lane * each, g.groups), hi = min(lo + each, g.groups), tiles = (g.tiles + MT - 1) / MT;
+    int sum = 0;
+    for (int i = lo; i < hi; ++i) sum += (at[i + 1] - at[i] + NT - 1) / NT * tiles;
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int left = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += left;
+    }
+    run -= sum;
+    for (int i = lo; i < hi; ++i) {
+        before[i] = run;
+        run += (at[i + 1] - at[i] + NT - 1) / NT * tiles;
+    }
+    if (lane == 31) before[g.groups] = run;
 }
 
 // The list of units, in the order that the blocks walk it: groups, of a group the tiles, of a tile the spans (which share its weights).
@@ -282,29 +305,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (g.offsets) {
-        // units in front of every group: a lane has 32 neighbouring groups at most
-        pdl_wait();          // (the offsets are the kernel in front's)
-        for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = g.offsets[i];
-        __syncthreads();
-        if (warp == 0) {
-            const int each = (g.groups + 31) / 32, lo = min(lane * each, g.groups), hi = min(lo + each, g.groups), tiles = (g.tiles + MT - 1) / MT;
-            int sum = 0;
-            for (int i = lo; i < hi; ++i) sum += (at[i + 1] - at[i] + NT - 1) / NT * tiles;
-            int run = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int left = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += left;
-            }
-            run -= sum;
-            for (int i = lo; i < hi; ++i) {
-                before[i] = run;
-                run += (at[i + 1] - at[i] + NT - 1) / NT * tiles;
-            }
-            if (lane == 31) before[g.groups] = run;
-        }
-    }
+    if (g.offsets) list_units<NT, MT>(g, before, at);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -610,6 +611,351 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
 }
 
+// ---- many rows to a group: the rows are the M side -------------------------------------------------------------------------------
+// A unit is 128 pairs (the M side) x two tiles of the weight (256 columns). A thread of the epilogue has one pair and the 128 columns of one tile: the
+// pair's scale is a register, a tile's scale is one number (of gate and up rows three: a block of 128 up rows may end inside the tile), so a k
+// block costs one packed multiply-add for two values and nothing is shared between threads.
+constexpr int WIDE_ROWS = 128, WIDE_COLUMNS = 256, WIDE_THREADS = 384, WIDE_PARK = 20;      // (park: rows of 16 values, 20 apart: no two lanes' rows share a bank)
+constexpr uint32_t WIDE_STAGE = 3 * TILE_BYTES;
+// 384 threads are launched with 168 registers; the copying and issuing warps give of theirs what the sums need
+constexpr int WIDE_LAUNCHED = 168, WIDE_FEW = 72, WIDE_MANY = 216;
+static_assert(128 * WIDE_FEW + 256 * WIDE_MANY <= WIDE_THREADS * WIDE_LAUNCHED, "what a block was launched with");
+
+// 16 results of a pair (this lane's) -> out, columns from c0 on, through the warp's shared memory, so that a row's results leave together.
+template <typename Tout>
+__device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, float* park, const float (&v)[16], size_t p0, int rows, int c0, int last, bool vec, int lane) {
+    constexpr int PER = 16 / sizeof(Tout), PIECES = 16 / PER;
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(park + lane * WIDE_PARK + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    __syncwarp();
+    if (vec && c0 + 16 <= last) {
+#pragma unroll
+        for (int i = lane; i < 32 * PIECES; i += 32) {
+            const int j = i / PIECES, c = i % PIECES * PER;
+            if (j >= rows) continue;
+            Tout* dst = out + (p0 + j) * f.ldo + c0 + c;
+            float x[PER];
+#pragma unroll
+            for (int q = 0; q < PER; q += 4) *reinterpret_cast<float4*>(x + q) = *reinterpret_cast<const float4*>(park + j * WIDE_PARK + c + q);
+            __align__(16) Tout w[PER];
+            if (f.accumulate == EPI_ADD) {
+                *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(dst);
+#pragma unroll
+                for (int q = 0; q < PER; ++q) x[q] = __fadd_rn(x[q], to_float(w[q]));
+            }
+#pragma unroll
+            for (int q = 0; q < PER; ++q) w[q] = from_float<Tout>(x[q]);
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
+        }
+    } else {
+        const int c = lane & 15;
+        if (c0 + c < last)
+            for (int j = lane >> 4; j < rows; j += 2) {
+                Tout* dst = out + (p0 + j) * f.ldo + c0 + c;
+                const float x = park[j * WIDE_PARK + c];
+                *dst = from_float<Tout>(f.accumulate == EPI_ADD ? __fadd_rn(x, to_float(*dst)) : x);
+            }
+    }
+}
+
+template <bool FP8, bool GLU, typename Tout>
+__global__ void __launch_bounds__(WIDE_THREADS, 1)
+gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Args g, Tout* __restrict__ out) {
+    constexpr int NT = WIDE_ROWS, MT = 2, BUFFERS = 2, COLUMNS = BUFFERS * WIDE_COLUMNS, EPILOGUE = 8;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int before[MAX_GROUPS + 1], at[MAX_GROUPS + 1];
+    __shared__ __align__(16) float parks[EPILOGUE][32 * WIDE_PARK];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_word;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int stages = g.stages, n_kb = g.k_blocks;
+    const unsigned long long limit = g.limit_us ? g.limit_us * 1000ull : WAIT_NS;
+    const uint32_t bars = base + (uint32_t)stages * WIDE_STAGE;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
+    auto sums_bar = [&](int b) { return bars + 16u * stages + 8u * b; };
+    auto taken_bar = [&](int b) { return bars + 16u * stages + 8u * (BUFFERS + b); };
+    volatile int* abort_flag = &abort_word;
+    auto give_up = [&](int code) {
+        atomicCAS(g.error_word, 0, code);
+        __threadfence();               // (before anybody follows the flag and has a code of his own)
+        *abort_flag = 1;
+    };
+    const int warp = uniform_warp(), lane = threadIdx.x & 31, blocks = (int)gridDim.x;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1 + (g.starve == STARVE_RELEASE && s == 0));
+        }
+        for (int b = 0; b < BUFFERS; ++b) {
+            mbar_init(sums_bar(b), 1);
+            mbar_init(taken_bar(b), EPILOGUE);
+        }
+        abort_word = 0;
+        if (g.starve == STARVE_COPY && blockIdx.x == 0) mbar_expect_more(full_bar(0), 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"((uint32_t)COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (g.offsets) list_units<NT, MT>(g, before, at);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+
+    Units<NT, MT> units(g, before, at);
+    bool ok = true;
+    int issued = 0;                            // k blocks whose copies (warp 0), or whose MMAs (warp 1), are under way or done
+    if (warp < 4) {
+        if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WIDE_FEW));
+        if (warp == 0) {
+            // ---------------- producer ----------------
+            int s = 0;
+            uint32_t parity = 1;                                   // (the first lap finds every stage free)
+            bool waited = false;
+            for (int u = (int)blockIdx.x; u < units.total && ok; u += blocks) {
+                const Unit unit = units(u);
+                const int halves_here = min(MT, g.tiles - unit.tile);
+                const uint8_t* w = g.w + (size_t)((size_t)unit.e * g.tiles + unit.tile) * n_kb * TILE_BYTES;
+                const size_t next_tile = (size_t)n_kb * TILE_BYTES;
+                const uint32_t bytes = (uint32_t)halves_here * TILE_BYTES + (uint32_t)unit.width * 128;
+                auto weights = [&](int i, int s_) {
+                    mbar_expect_tx(full_bar(s_), bytes);
+                    for (int h = 0; h < halves_here; ++h)
+                        bulk_copy(base + (uint32_t)s_ * WIDE_STAGE + h * TILE_BYTES, w + h * next_tile + (size_t)i * TILE_BYTES, TILE_BYTES, full_bar(s_));
+                };
+                // (of one group the first weights are known in front of the wait, and nobody's output)
+                int early = 0;
+                if (!waited) {
+                    early = g.offsets ? 0 : min(stages, n_kb);
+                    if (elect_one())
+                        for (int i = 0; i < early; ++i) weights(i, i);
+                    __syncwarp();
+                    pdl_wait();
+                    pdl_trigger();
+                    waited = true;
+                }
+                int row[4] = {0, 0, 0, 0};                         // this lane's four of the unit's rows (filled up with its last)
+                if (g.order && lane * 4 < unit.width)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) row[q] = g.order[unit.first + min(lane * 4 + q, unit.here - 1)] / g.top;
+                for (int i = 0; i < n_kb; ++i) {
+                    if (!warp_wait(empty_bar(s), parity, abort_flag, 2 * limit)) { ok = false; break; }
+                    if (i >= early && elect_one()) weights(i, s);
+                    __syncwarp();
+                    const uint32_t dst = base + (uint32_t)s * WIDE_STAGE + MT * TILE_BYTES;
+                    const int x = i * 128;               // (rows are bytes to the tensor map)
+                    if (g.order) {
+                        if (lane * 4 < unit.width) tma_gather4(dst + lane * 512, &map_a, x, row, full_bar(s));
+                    } else if (elect_one()) {
+                        for (int t = 0; t < unit.width; t += 16) tma_load_2d(dst + t * 128, &map_a, x, unit.first + t, full_bar(s));
+                    }
+                    __syncwarp();
+                    ++issued;
+                    if (++s == stages) { s = 0; parity ^= 1u; }
+                }
+            }
+            if (!waited) {
+                pdl_wait();
+                pdl_trigger();
+            }
+            // (the last lap's releases have arrived too before the block may leave: none is on its way to memory that is somebody else's by then)
+            for (int j = max(0, issued - stages); ok && j < issued; ++j)
+                ok = warp_wait(empty_bar(j % stages), (uint32_t)(j / stages) & 1u, abort_flag, 2 * limit);
+            if (!ok && lane == 0) give_up(41);
+        } else if (warp == 1) {
+            // ---------------- MMA issuer ----------------
+            const uint64_t desc_w0 = smem_desc_sw128(base), desc_a0 = smem_desc_sw128(base + MT * TILE_BYTES);
+            uint64_t desc_w = desc_w0, desc_a = desc_a0;          // (a stage further is an addition to the address field)
+            int s = 0, buffer = 0;
+            uint32_t parity = 0, taken = 1;                        // (the first lap finds every buffer free)
+            pdl_wait();          // (the copies are complete no sooner, and the time that the kernel in front still takes is not this wait's)
+            for (int u = (int)blockIdx.x; u < units.total && ok; u += blocks) {
+                const Unit unit = units(u);
+                const uint32_t kind = idesc<FP8>(128 * min(MT, g.tiles - unit.tile));
+                for (int i = 0; i < n_kb; ++i) {
+                    if ((FP8 || i == 0) && !warp_wait(taken_bar(buffer), taken, abort_flag, 2 * limit)) { ok = false; break; }
+                    if (!warp_wait(full_bar(s), parity, abort_flag, limit)) { ok = false; break; }
+                    tcgen05_fence_after();
+                    if (elect_one()) {
+                        const uint32_t d = tmem_base + (uint32_t)(buffer * WIDE_COLUMNS);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t more = (!FP8 && i > 0) || k > 0;
+                            if constexpr (FP8) mma_f8(d, desc_a + 2 * k, desc_w + 2 * k, kind, more);
+                            else tcgen05_mma_bf16(d, desc_a + 2 * k, desc_w + 2 * k, kind, more);
+                        }
+                        tcgen05_commit(empty_bar(s));
+                        if (FP8 || i == n_kb - 1) tcgen05_commit(sums_bar(buffer));
+                    }
+                    __syncwarp();
+                    ++issued;
+                    if (FP8 || i == n_kb - 1)
+                        if (++buffer == BUFFERS) { buffer = 0; taken ^= 1u; }
+                    desc_w += WIDE_STAGE >> 4;
+                    desc_a += WIDE_STAGE >> 4;
+                    if (++s == stages) { s = 0; parity ^= 1u; desc_w = desc_w0; desc_a = desc_a0; }
+                }
+            }
+            if (!ok && lane == 0) give_up(42);
+        }
+    } else {
+        // ---------------- epilogue: TMEM lanes 32 * (warp % 4) = the unit's pairs, warps 4..7 its first tile, 8..11 its second ----------------
+        if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WIDE_MANY));
+        const int quad = warp & 3, half = (warp - 4) >> 2, token = quad * 32 + lane;
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128);
+        float* park = parks[warp - 4];
+        const bool vec = ((uintptr_t)out & 15u) == 0 && (((size_t)g.f.ldo * sizeof(Tout)) & 15u) == 0;
+        const int last = GLU ? g.f.N >> 1 : g.f.N;
+        pdl_wait();          // the token scales, and what is added into, were written by the kernels before
+        int buffer = 0;
+        uint32_t parity = 0;
+        for (int u = (int)blockIdx.x; u < units.total && ok; u += blocks) {
+            const Unit unit = units(u);
+            const int tile = unit.tile + half, rows = min(32, unit.here - quad * 32), c_tile = tile * (GLU ? 64 : 128);
+            const bool mine = tile < g.tiles && rows > 0;
+            const size_t p0 = (size_t)(unit.first + quad * 32);
+            // 32 columns of this lane's pair (a quarter of the tile) to results
+            auto finish = [&](float (&v)[32], int c) {
+                if constexpr (GLU) {
+                    float units16[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float eight[8];
+                        glu_units<8, true>(g.f.glu, [&](int q) { return v[16 * h + q]; }, [&](int q) { return v[16 * h + 8 + q]; }, 1.f, eight);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) units16[8 * h + q] = eight[q];
+                    }
+                    if (c_tile + 16 * c < last) leave_rows<Tout>(g.f, out, park, units16, p0, rows, c_tile + 16 * c, last, vec, lane);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c0 = c_tile + 32 * c + 16 * h;
+                        if (c0 >= last) break;
+                        float x[16];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            x[q] = v[16 * h + q];
+                            if (g.f.has_bias && c0 + q < last) x[q] = __fadd_rn(x[q], g.f.bias[c0 + q]);
+                            if (g.f.accumulate == EPI_RELU2) {
+                                const float z = x[q] < 0.f ? 0.f : x[q];              // (what is not a number stays so: a maximum would drop it)
+                                x[q] = __fmul_rn(z, z);
+                            }
+                        }
+                        leave_rows<Tout>(g.f, out, park, x, p0, rows, c0, last, vec, lane);
+                    }
+                }
+            };
+            if constexpr (FP8) {
+                uint64_t sums[64];
+#pragma unroll
+                for (int j = 0; j < 64; ++j) sums[j] = 0;
+                const int t_row = token < unit.here ? (g.order ? g.order[unit.first + token] / g.top : unit.first + token) : -1;
+                const float* sa_row = g.scale_a + (size_t)max(t_row, 0) * g.sa_ld;
+                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld;
+                // of gate and up rows in eights: the gates' scale, and the up rows' in front of and behind the edge of their block
+                const int edge = GLU ? (128 - ((last + c_tile) & 127)) >> 3 : 0;
+                float4 sa4 = make_float4(0.f, 0.f, 0.f, 0.f), sa_next = sa4, sw4[GLU ? 3 : 1], sw_next[GLU ? 3 : 1];
+                auto ask = [&](int kb) {
+                    if (t_row >= 0) sa_next = *reinterpret_cast<const float4*>(sa_row + kb);
+                    sw_next[0] = *reinterpret_cast<const float4*>(sw_row + kb);
+                    if constexpr (GLU) {
+                        sw_next[1] = *reinterpret_cast<const float4*>(sw_row + g.sw_ld + kb);
+                        sw_next[2] = *reinterpret_cast<const float4*>(sw_row + 15 * g.sw_ld + kb);
+                    }
+                };
+                ask(0);
+                for (int kb = 0; kb < n_kb; ++kb) {
+                    if ((kb & 3) == 0) {
+                        sa4 = sa_next;
+#pragma unroll
+                        for (int q = 0; q < (GLU ? 3 : 1); ++q) sw4[q] = sw_next[q];
+                        if (kb + 4 < n_kb) ask(kb + 4);
+                    }
+                    const int at4 = kb & 3;
+                    auto of4 = [&](const float4& f4) { return at4 == 0 ? f4.x : at4 == 1 ? f4.y : at4 == 2 ? f4.z : f4.w; };
+                    const float sa = of4(sa4);
+                    uint64_t scale[GLU ? 3 : 1];
+#pragma unroll
+                    for (int q = 0; q < (GLU ? 3 : 1); ++q) {
+                        const uint32_t both = __float_as_uint(__fmul_rn(sa, of4(sw4[q])));
+                        scale[q] = pair_of(both, both);
+                    }
+                    ok = __all_sync(0xffffffffu, mbar_wait(sums_bar(buffer), parity, abort_flag, 2 * limit));
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint32_t from = taddr + (uint32_t)(buffer * WIDE_COLUMNS);
+                    uint32_t v[2][16];
+                    tmem_ld(from, v[0]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        if (c < 7) tmem_ld(from + 16 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const uint64_t x = pair_of(v[c & 1][2 * q], v[c & 1][2 * q + 1]);
+                            const uint64_t by = !GLU || q < 4 ? scale[0] : c < edge ? scale[GLU ? 1 : 0] : scale[GLU ? 2 : 0];
+                            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[8 * c + q]) : "l"(x), "l"(by));
+                        }
+                        if (c < 7) tmem_ld_wait();
+                    }
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken_bar(buffer));
+                    if (++buffer == BUFFERS) { buffer = 0; parity ^= 1u; }
+                }
+                if (ok && mine)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) halves(sums[16 * c + q], v[2 * q], v[2 * q + 1]);
+                        finish(v, c);
+                    }
+            } else {
+                ok = __all_sync(0xffffffffu, mbar_wait(sums_bar(buffer), parity, abort_flag, 2 * limit));
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint32_t from = taddr + (uint32_t)(buffer * WIDE_COLUMNS);
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(from + 32 * c, r);
+                    tmem_ld_wait();
+                    if (c == 3) {           // the buffer is the next unit's as soon as its last values are read
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(taken_bar(buffer));
+                    }
+                    float v[32];
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(r[q]);
+                    if (mine) finish(v, c);
+                }
+                if (++buffer == BUFFERS) { buffer = 0; parity ^= 1u; }
+            }
+        }
+        if (!ok && lane == 0) give_up(43);
+    }
+    tcgen05_fence_before();
+    const bool gave_up = __syncthreads_or(!ok);
+    if (gave_up) {
+        // (where no wait ran out these have been waited for: the copies by the MMAs, the MMAs by the epilogue and the producer)
+        const unsigned long long began = now_ns();
+        if (warp == 0)
+            for (int j = max(0, issued - stages); j < issued; ++j) drain(full_bar(j % stages), (uint32_t)(j / stages) & 1u, began, limit);
+        if (warp == 1 && issued > 0) drain(empty_bar((issued - 1) % stages), (uint32_t)((issued - 1) / stages) & 1u, began, limit);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)COLUMNS) : "memory");
+    }
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------------
 
 // Rows of `bytes` bytes, `ld` bytes apart, read in boxes of box_rows x 128 bytes with the 128-byte swizzle (box_rows 1: gathers of four).
@@ -656,72 +1002,98 @@ struct Product {
     cudaStream_t stream;
 };
 
-template <bool FP8, int NT, int MT, typename Tout>
-int launch(const Product& p, const Cut& cut) {
-    using S = Shape<FP8, NT, MT>;
-    auto kern = gemm_grouped_kernel<FP8, NT, MT, Tout>;
+// What a kernel is to the launcher: pairs and tiles of a unit, a stage's bytes, buffers and columns of tensor memory, threads.
+struct Kind {
+    int nt, mt;
+    uint32_t stage;
+    int buffers, columns, threads;
+    bool clusters;
+};
+
+template <typename Tout>
+int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind, size_t own, const Product& p, const Cut& cut) {
     Args g = p.args;
-    const int sms = jllm_device_sm_count(), tiles = (g.tiles + MT - 1) / MT;
-    if (sms <= 0) return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: the device does not say how many SMs it has");
-    // (of groups: every group that has pairs ends one span of fewer than NT)
-    const long long spans = g.offsets ? (long long)p.pairs / NT + (g.groups < p.pairs ? g.groups : p.pairs) : ((long long)g.rows + NT - 1) / NT;
-    JLLM_REQUIRE(spans * tiles * cut.blocks < BLOCK_MOST, "gemm_grouped: %lld units of work", spans * tiles);
+    const int sms = jllm_device_sm_count(), tiles = (g.tiles + kind.mt - 1) / kind.mt;
+    if (sms <= 0 || own == 0) return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: the device does not say how many SMs it has, or what the kernel holds");
+    // (of groups: every group that has pairs ends one span that is not full)
+    const long long spans = g.offsets ? (long long)p.pairs / kind.nt + (g.groups < p.pairs ? g.groups : p.pairs) : ((long long)g.rows + kind.nt - 1) / kind.nt;
+    const long long units = spans * tiles;
+    JLLM_REQUIRE(units * cut.blocks < BLOCK_MOST, "gemm_grouped: %lld units of work", units);
     g.blocks = cut.blocks;
     g.share = cut.blocks > 1 ? ((g.rows + 7) / 8 + cut.blocks - 1) / cut.blocks * 8 : 0;
-    JLLM_REQUIRE(cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= g.k_blocks && (cut.blocks == 1 || (FP8 && NT <= 64 && MT == 1 && !g.offsets && g.rows <= NT)),
+    JLLM_REQUIRE(cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= g.k_blocks && (cut.blocks == 1 || (kind.clusters && !g.offsets && g.rows <= kind.nt)),
                  "gemm_grouped: no clusters of %d blocks for such a product", cut.blocks);
-    const size_t parts = (size_t)(cut.blocks - 1) * g.share * 512, least = 1024 + 8 * (2 * S::BUFFERS + 1) + 64;
-    // An SM has 228 KB, a block 227, of both 1 KB for the system and what the kernel holds by itself.
-    static const size_t own = [&] {
-        cudaFuncAttributes a{};
-        return cudaFuncGetAttributes(&a, (const void*)kern) == cudaSuccess ? a.sharedSizeBytes : (size_t)1 << 20;
-    }();
-    const size_t room = (cut.per_sm == 1 ? 227 * 1024 : 113 * 1024) - own;
-    JLLM_REQUIRE((cut.per_sm == 1 || cut.per_sm == 2) && S::COLUMNS * cut.per_sm <= 512 && own + least + parts + 2 * (S::STAGE + 16) <= room + own && own < 64 * 1024,
+    // An SM has 228 KB, a block 227 at most; each block's last KB is the system's, `own` what the kernel holds by itself.
+    const size_t parts = (size_t)(cut.blocks - 1) * g.share * 512, fixed = 1024 + 8 * (2 * kind.buffers + 1) + 64, each = kind.stage + 16;
+    const size_t all = cut.per_sm == 1 ? 227 * 1024 : 113 * 1024;
+    JLLM_REQUIRE((cut.per_sm == 1 || cut.per_sm == 2) && kind.columns * cut.per_sm <= 512 && own + fixed + parts + 2 * each <= all,
                  "gemm_grouped: %d blocks of such a product on an SM", cut.per_sm);
-    int stages = (int)((room - least - parts) / (S::STAGE + 16));
-    // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: of clusters' blocks no more are on an SM
-    // than its 512 columns allow (two of 256 at 113 KB; a block that takes more columns, of this file or another, leaves no room beside it).
-    if (cut.blocks == 1) {
-        const long long most = (long long)((spans * tiles + sms * cut.per_sm - 1) / (sms * cut.per_sm)) * g.k_blocks;
-        if (!g.offsets && stages > most) stages = most < 2 ? 2 : (int)most;
+    int stages = (int)((all - own - fixed - parts) / each);
+    if (!g.offsets && cut.blocks == 1) {
+        // (no more than a block has k blocks)
+        const long long most = (units + (long long)sms * cut.per_sm - 1) / ((long long)sms * cut.per_sm) * g.k_blocks;
+        if (stages > most) stages = most < 2 ? 2 : (int)most;
     }
     g.stages = stages;
-    size_t smem = stages * (size_t)(S::STAGE + 16) + parts + least;
-    if (cut.blocks > 1 && own + smem < 100 * 1024) smem = 100 * 1024 - own;
+    // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: a cluster's block takes all of an SM's
+    // shared memory, so none that holds columns is beside it.
+    const size_t smem = stages * each + parts + fixed;
     if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess)
         return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: %zu bytes of shared memory refused", smem);
-    cudaLaunchConfig_t cfg = {};
-    const long long grid = cut.blocks > 1 ? spans * tiles * cut.blocks : spans * tiles < (long long)sms * cut.per_sm ? spans * tiles : (long long)sms * cut.per_sm;
+    const long long at_once = (long long)sms * cut.per_sm, grid = cut.blocks > 1 ? units * cut.blocks : units < at_once ? units : at_once;
     JLLM_REQUIRE(g.starve == STARVE_NOTHING || (grid <= 64 && (g.starve != STARVE_PARTS || cut.blocks > 1)),
                  "gemm_grouped: the starved product of the wait test has at most 64 blocks, and a cluster where parts are missed");
+    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(S::THREADS);
+    cfg.blockDim = dim3(kind.threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = p.stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cut.blocks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (jllm_launch_overlaps(smem, LAUNCH_DEPENDENT)) {
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = 1;
-        cfg.numAttrs = 2;
+    int n = 0;
+    if (cut.blocks > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cut.blocks;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
     }
+    if (jllm_launch_overlaps(smem, LAUNCH_DEPENDENT)) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
     cudaLaunchKernelEx(&cfg, kern, *p.map, g, static_cast<Tout*>(p.out));
     return jllm_check_launch("gemm_grouped");
 }
 
+// What a kernel holds of shared memory by itself; 0 if the driver does not say, or if its threads are launched with fewer registers than `least`.
+size_t own_smem(const void* kern, int least = 0) {
+    cudaFuncAttributes a{};
+    if (cudaFuncGetAttributes(&a, kern) == cudaSuccess) return a.numRegs >= least ? a.sharedSizeBytes : 0;
+    cudaGetLastError();
+    return 0;
+}
+
+template <bool FP8, int NT, typename Tout>
+int launch_narrow(const Product& p, const Cut& cut) {
+    using S = Shape<FP8, NT, 1>;
+    auto kern = gemm_grouped_kernel<FP8, NT, 1, Tout>;
+    static const size_t own = own_smem((const void*)kern);
+    return launch<Tout>(kern, Kind{NT, 1, S::STAGE, S::BUFFERS, S::COLUMNS, S::THREADS, FP8}, own, p, cut);
+}
+template <bool FP8, bool GLU, typename Tout>
+int launch_wide(const Product& p, const Cut& cut) {
+    auto kern = gemm_grouped_wide_kernel<FP8, GLU, Tout>;
+    static const size_t own = own_smem((const void*)kern, FP8 ? WIDE_LAUNCHED : 0);          // (what the warps hand over has to be there)
+    return launch<Tout>(kern, Kind{WIDE_ROWS, 2, WIDE_STAGE, 2, 512, WIDE_THREADS, false}, own, p, cut);
+}
+
 template <bool FP8, typename Tout>
 int launch_cut(const Product& p, const Cut& cut) {
-    if (cut.nt == 16 && cut.mt == 1) return launch<FP8, 16, 1, Tout>(p, cut);
-    if (cut.nt == 32 && cut.mt == 1) return launch<FP8, 32, 1, Tout>(p, cut);
-    if (cut.nt == 64 && cut.mt == 1) return launch<FP8, 64, 1, Tout>(p, cut);
-    if (cut.nt == 128 && cut.mt == 1) return launch<FP8, 128, 1, Tout>(p, cut);
-    if (cut.nt == 128 && cut.mt == 2) return launch<FP8, 128, 2, Tout>(p, cut);
+    if (cut.nt == 16 && cut.mt == 1) return launch_narrow<FP8, 16, Tout>(p, cut);
+    if (cut.nt == 32 && cut.mt == 1) return launch_narrow<FP8, 32, Tout>(p, cut);
+    if (cut.nt == 64 && cut.mt == 1) return launch_narrow<FP8, 64, Tout>(p, cut);
+    if (cut.nt == WIDE_ROWS && cut.mt == 2) return p.args.f.glu ? launch_wide<FP8, true, Tout>(p, cut) : launch_wide<FP8, false, Tout>(p, cut);
     return jllm_fail(JLLM_BAD_ARGUMENT, "gemm_grouped: no kernel for spans of %d pairs and %d tiles", cut.nt, cut.mt);
 }
 
@@ -736,7 +1108,7 @@ Cut choose(bool fp8, int groups, int pairs, int tiles, int k_blocks) {
             if (cut.blocks > 8) cut.blocks = 8;
             while (cut.blocks > 1 && k_blocks / cut.blocks < 2) --cut.blocks;
         }
-        if (cut.nt == 128 && (tiles + 1) / 2 * ((mean + 127) / 128) >= sms) cut.mt = 2;
+        if (cut.nt == 128) cut.mt = 2;
     } else {
         cut.nt = mean <= 6 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : 128;
         if (cut.nt == 128) cut.mt = 2;

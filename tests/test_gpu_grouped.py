@@ -159,7 +159,7 @@ def test_rows_of_other_strides_and_slices(ops):
 
 # ---- products in 8 bits ----
 
-CUTS = [16111, 16121, 32111, 64111, 128111, 128211]
+CUTS = [16111, 16121, 32111, 64111, 128211]
 
 
 def run_product(ops, rows, n, k, *, bias=None, accumulate=False, glu=False, dtype=torch.float32, cut=0, seed=0):
