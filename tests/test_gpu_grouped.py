@@ -209,7 +209,7 @@ def test_product_of_every_cut(ops, rows, n, k, cut):
 @pytest.mark.parametrize("nt", [16, 32, 64])
 @pytest.mark.parametrize("blocks", [2, 3, 4, 5, 8])
 def test_product_of_clusters(ops, nt, blocks):
-    for rows in sorted({1, 8, 9, nt - 1, nt}):
+    for rows in sorted({1, 8, 9, nt - 1, nt, nt + 1, 3 * nt}):
         run_product(ops, rows, 260, 1930, cut=nt * 1000 + 110 + blocks, seed=blocks)
         run_product(ops, rows, 272, 1800, glu=True, dtype=torch.bfloat16, cut=nt * 1000 + 110 + blocks, seed=rows)
 
