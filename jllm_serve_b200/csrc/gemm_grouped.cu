@@ -46,9 +46,11 @@ struct Args {
     const int *offsets, *order;           // null: one group of `rows`; null: a pair's row is the pair
     int sw_ld, sa_ld;
     int groups, top, rows, tiles, k_blocks;
+    int spans, span;                      // of one group: spans of so many rows
     int row_bytes, row_step;              // of `a`: bytes that count, and 16-byte pieces from row to row
     Finish f;
     int stages, blocks, share;            // blocks of a cluster, tokens that each of them finishes
+    int box;                              // rows that one copy brings, of rows that lie together: a copy costs some 30 ns, whatever it brings
     int starve, limit_us;                 // a test of the waits (below); 0, 0
     int* error_word;
 };
@@ -119,7 +121,10 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity, unsigned lo
 // ---- what a kernel is made of: rows and tiles of a unit, buffers of sums in tensor memory (in 8 bits one k block's, else a unit's), warps ----
 template <bool FP8, int NT>
 struct Narrow {
-    static constexpr int ROWS = NT, TILES = 1, COLUMNS = NT, BUFFERS = FP8 ? 4 : 2, TMEM = BUFFERS * NT < 32 ? 32 : BUFFERS * NT;
+    // (in 8 bits a buffer has two k blocks' sums: what barriers and waits cost is paid for two;
+    // and there are as many as half of tensor memory holds, so that the ring does not wait while the first scales come)
+    static constexpr int ROWS = NT, TILES = 1, TOGETHER = FP8 ? 2 : 1, COLUMNS = TOGETHER * NT, BUFFERS = FP8 ? 256 / COLUMNS : 2,
+                         TMEM = BUFFERS * COLUMNS < 32 ? 32 : BUFFERS * COLUMNS;
     // four warps have the tile's weight rows; with 32 rows and more two sets of them share the rows
     static constexpr int SETS = NT >= 32 ? 2 : 1, EPILOGUE = 4 * SETS, FIRST = 2, THREADS = 32 * (FIRST + EPILOGUE);
     static constexpr int GATHER = 0, GATHER_WARPS = 1, GATHER_ROWS = NT;          // the producer fetches rows itself
@@ -127,7 +132,7 @@ struct Narrow {
 };
 template <bool FP8>
 struct Wide {
-    static constexpr int ROWS = 128, TILES = 2, COLUMNS = 256, BUFFERS = 2, TMEM = BUFFERS * COLUMNS;
+    static constexpr int ROWS = 128, TILES = 2, TOGETHER = 1, COLUMNS = 256, BUFFERS = 2, TMEM = BUFFERS * COLUMNS;
     // four warps have the rows; four sets of them share the 256 columns
     static constexpr int SETS = 4, EPILOGUE = 4 * SETS, FIRST = 4, THREADS = 32 * (FIRST + EPILOGUE);
     static constexpr int GATHER = 2, GATHER_WARPS = 2, GATHER_ROWS = 64;
@@ -189,25 +194,32 @@ struct Units {
     int e = 0;                            // the group of the unit that was asked for last (units are asked for in ascending order)
 
     __device__ __forceinline__ Units(const Args& g_, const int* before_, const int* at_) : g(g_), before(before_), at(at_) {
-        total = g.offsets ? before[g.groups] : (g.tiles + S::TILES - 1) / S::TILES * ((g.rows + S::ROWS - 1) / S::ROWS);
+        total = g.offsets ? before[g.groups] : (g.tiles + S::TILES - 1) / S::TILES * g.spans;
     }
     // the whole warp calls it
     __device__ __forceinline__ Unit operator()(int u) {
-        int count = g.rows, first = 0, r = u;
-        if (g.offsets) {
-            const int lane = threadIdx.x & 31;
-            for (;;) {                    // (before[groups] = total > u: it ends)
-                const int i = e + 1 + lane;
-                const unsigned behind = __ballot_sync(0xffffffffu, i <= g.groups && before[i] <= u);
-                e += __popc(behind);
-                if (behind != 0xffffffffu) break;
-            }
-            first = at[e], count = at[e + 1] - first, r = u - before[e];
+        if (!g.offsets) {
+            const int t = u / g.spans, first = (u - t * g.spans) * g.span;
+            return {0, t * S::TILES, first, min(g.span, g.rows - first), g.span};
         }
+        const int lane = threadIdx.x & 31;
+        for (;;) {                    // (before[groups] = total > u: it ends)
+            const int i = e + 1 + lane;
+            const unsigned behind = __ballot_sync(0xffffffffu, i <= g.groups && before[i] <= u);
+            e += __popc(behind);
+            if (behind != 0xffffffffu) break;
+        }
+        const int first = at[e], count = at[e + 1] - first, r = u - before[e];
         const int spans = (count + S::ROWS - 1) / S::ROWS, width = ((count + spans - 1) / spans + 15) & ~15, s = r % spans;
         return {e, r / spans * S::TILES, first + s * width, min(width, count - s * width), width};
     }
 };
+// The same unit in registers that the compiler knows to be the warp's: what the issuing instructions take from the warp's uniform registers is
+// otherwise moved there piece by piece (a k block's two copies 390 cycles for 150).
+__device__ __forceinline__ Unit uniform(const Unit& u) {
+    auto one = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    return {one(u.e), one(u.tile), one(u.first), one(u.here), one(u.width)};
+}
 // (a cluster's blocks have one unit, and k blocks [lo, lo + n) of it; a block by itself has all of them)
 struct Share {
     int unit, step, rank, kb_lo, n_kb;
@@ -277,42 +289,54 @@ __device__ __forceinline__ bool produce(const CUtensorMap* map_a, const Args& g,
     uint32_t parity = 1;                                   // (the first lap finds every stage free)
     [[maybe_unused]] Fetch<S> fetch;
     for (int u = share.unit; u < units.total && ok; u += share.step) {
-        const Unit unit = units(u);
-        const int tiles_here = min(S::TILES, g.tiles - unit.tile);
+        const Unit unit = uniform(units(u));
+        const bool both = S::TILES == 2 && unit.tile + 1 < g.tiles;
         const uint8_t* w = g.w + ((size_t)((size_t)unit.e * g.tiles + unit.tile) * g.k_blocks + share.kb_lo) * TILE_BYTES;
         const size_t next_tile = (size_t)g.k_blocks * TILE_BYTES;
-        const uint32_t bytes = (uint32_t)tiles_here * TILE_BYTES + (g.order ? 0u : (uint32_t)unit.width * 128u);
-        auto weights = [&](int i, int s_) {
+        const uint32_t bytes = (both ? 2u : 1u) * TILE_BYTES + (g.order ? 0u : (uint32_t)((unit.width + g.box - 1) / g.box * g.box) * 128u);
+        auto weights = [&](int s_) {
             mbar_expect_tx(ring.full(s_), bytes);
-            for (int h = 0; h < tiles_here; ++h) bulk_copy(ring.stage(s_) + h * TILE_BYTES, w + h * next_tile + (size_t)i * TILE_BYTES, TILE_BYTES, ring.full(s_));
+            bulk_copy(ring.stage(s_), w, TILE_BYTES, ring.full(s_));
+            if (both) bulk_copy(ring.stage(s_) + TILE_BYTES, w + next_tile, TILE_BYTES, ring.full(s_));
+        };
+        auto rows = [&](int s_, int kb) {
+            tma_load_2d(ring.rows(s_), map_a, kb * 128, unit.first, ring.full(s_));
+            for (int t = g.box; t < unit.width; t += g.box) tma_load_2d(ring.rows(s_) + t * 128, map_a, kb * 128, unit.first + t, ring.full(s_));
         };
         // (of one group the first weights are known in front of the wait, and nobody's output)
-        int early = 0;
+        int i = 0;
         if (!waited) {
-            early = g.offsets ? 0 : min(ring.stages, share.n_kb);
-            if (elect_one())
-                for (int i = 0; i < early; ++i) weights(i, i);
-            __syncwarp();
+            if (!g.offsets) {
+                const int early = min(ring.stages, share.n_kb);
+                for (; i < early; ++i, w += TILE_BYTES)
+                    if (elect_one()) weights(i);
+                __syncwarp();
+                pdl_wait();
+                for (i = 0; i < early; ++i)
+                    if (elect_one()) rows(i, share.kb_lo + i);
+                __syncwarp();
+                issued = early;
+                s = early == ring.stages ? 0 : early, parity = early == ring.stages ? 0u : 1u;
+            }
             pdl_wait();
             pdl_trigger();
             waited = true;
         }
         if constexpr (S::GATHER == 0)
             if (g.order) fetch.begin(g, unit, 0);
-        for (int i = 0; i < share.n_kb; ++i) {
+        for (; i < share.n_kb; ++i, w += TILE_BYTES) {
             if (!warp_wait(ring.empty(s), parity, abort_flag, 2 * limit)) { ok = false; break; }
-            if (i >= early && elect_one()) weights(i, s);
-            __syncwarp();
             const int kb = share.kb_lo + i;
-            if (g.order) {
-                if constexpr (S::GATHER == 0) {
+            if (elect_one()) {
+                weights(s);
+                if (!g.order) rows(s, kb);
+            }
+            __syncwarp();
+            if constexpr (S::GATHER == 0)
+                if (g.order) {
                     fetch.ask(g, ring, s, 0, kb);
                     fetch.asked(ring);
                 }
-            } else if (elect_one()) {
-                for (int t = 0; t < unit.width; t += 16) tma_load_2d(ring.rows(s) + t * 128, map_a, kb * 128, unit.first + t, ring.full(s));
-            }
-            __syncwarp();
             ++issued;
             if (++s == ring.stages) { s = 0; parity ^= 1u; }
         }
@@ -363,14 +387,16 @@ __device__ __forceinline__ bool multiply(const Args& g, const Ring<S>& ring, Uni
     uint32_t parity = 0, taken = 1;                        // (the first lap finds every buffer free)
     pdl_wait();          // (the copies are complete no sooner, and the time that the kernel in front still takes is not this wait's)
     for (int u = share.unit; u < units.total && ok; u += share.step) {
-        const Unit unit = units(u);
+        const Unit unit = uniform(units(u));
         const uint32_t kind = idesc<FP8>(ROWS_ARE_M ? 128 * min(S::TILES, g.tiles - unit.tile) : unit.width);
         for (int i = 0; i < share.n_kb; ++i) {
-            if ((FP8 || i == 0) && !warp_wait(ring.taken(buffer), taken, abort_flag, 2 * limit)) { ok = false; break; }
+            const int kb = share.kb_lo + i, at = FP8 ? kb % S::TOGETHER : 0;
+            const bool opens = i == 0 || (FP8 && at == 0), closes = i == share.n_kb - 1 || (FP8 && at == S::TOGETHER - 1);
+            if (opens && !warp_wait(ring.taken(buffer), taken, abort_flag, 2 * limit)) { ok = false; break; }
             if (!warp_wait(ring.full(s), parity, abort_flag, limit)) { ok = false; break; }
             tcgen05_fence_after();
             if (elect_one()) {
-                const uint32_t d = tmem_base + (uint32_t)(buffer * S::COLUMNS);
+                const uint32_t d = tmem_base + (uint32_t)(buffer * S::COLUMNS + at * (S::COLUMNS / S::TOGETHER));
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t m = (ROWS_ARE_M ? desc_r : desc_w) + 2 * k, n = (ROWS_ARE_M ? desc_w : desc_r) + 2 * k;
@@ -379,11 +405,11 @@ __device__ __forceinline__ bool multiply(const Args& g, const Ring<S>& ring, Uni
                     else tcgen05_mma_bf16(d, m, n, kind, more);
                 }
                 tcgen05_commit(ring.empty(s));
-                if (FP8 || i == share.n_kb - 1) tcgen05_commit(ring.sums(buffer));
+                if (closes) tcgen05_commit(ring.sums(buffer));
             }
             __syncwarp();
             ++issued;
-            if (FP8 || i == share.n_kb - 1)
+            if (closes)
                 if (++buffer == S::BUFFERS) { buffer = 0; taken ^= 1u; }
             desc_w += S::STAGE >> 4;
             desc_r += S::STAGE >> 4;
@@ -530,7 +556,7 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
     uint8_t* aligned = smem_raw + (ring.base - smem_u32(smem_raw));
     const int blocks = g.blocks, rank = share.rank, n_kb = share.n_kb, kb_lo = share.kb_lo;
     const uint32_t parts_at = (uint32_t)g.stages * S::STAGE, part_bytes = (uint32_t)g.share * 128 * 4;      // [share / 4][128 rows][4 tokens]
-    ring.bars = ring.base + parts_at + (uint32_t)(blocks - 1) * part_bytes;
+    ring.bars = ring.base + parts_at + (blocks > 1 ? (uint32_t)blocks * part_bytes : 0u);
     int* before = reinterpret_cast<int*>(aligned + (ring.parts() + 8 - ring.base));
     int* at = before + g.groups + 1;
     const unsigned long long limit = g.limit_us ? g.limit_us * 1000ull : WAIT_NS;
@@ -560,6 +586,18 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
         const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)t0;
         float* park = parks[warp - S::FIRST];
         const bool lines = ((uintptr_t)out & 15u) == 0 && (((size_t)g.f.ldo * sizeof(Tout)) & 15u) == 0;
+        float4 sw_next[CLASSES];
+        [[maybe_unused]] auto ask_weights = [&](const Unit& unit, int kb) {
+            const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + unit.tile) * 16 * g.sw_ld + kb;
+            sw_next[0] = *reinterpret_cast<const float4*>(sw_row);
+            if constexpr (CLASSES == 3) {
+                sw_next[1] = *reinterpret_cast<const float4*>(sw_row + g.sw_ld);
+                sw_next[2] = *reinterpret_cast<const float4*>(sw_row + 15 * g.sw_ld);
+            }
+        };
+        // (of one group the first weight and its scales are known in front of the wait, and nobody's output)
+        if constexpr (FP8)
+            if (!g.offsets && thread < NT && share.unit < units.total) ask_weights(units(share.unit), kb_lo & ~3);
         pdl_wait();          // the rows' scales, and what is added into, were written by the kernels before
         int buffer = 0, lap = 0;
         uint32_t parity = 0;
@@ -592,22 +630,12 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                 const int kind = GLU && (eight & 1) ? ((eight >> 1) < edge ? 1 : 2) : 0;
                 const bool has = thread < unit.here;
                 const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? g.order[unit.first + thread] / g.top : unit.first + thread) : 0) * g.sa_ld;
-                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + unit.tile) * 16 * g.sw_ld;
-                float4 sa_next = make_float4(0.f, 0.f, 0.f, 0.f), sw_next[CLASSES];
-                auto ask = [&](int kb) {
-                    if (thread < NT) {
-                        if (has) sa_next = *reinterpret_cast<const float4*>(sa_row + kb);
-                        sw_next[0] = *reinterpret_cast<const float4*>(sw_row + kb);
-                        if constexpr (CLASSES == 3) {
-                            sw_next[1] = *reinterpret_cast<const float4*>(sw_row + g.sw_ld + kb);
-                            sw_next[2] = *reinterpret_cast<const float4*>(sw_row + 15 * g.sw_ld + kb);
-                        }
-                    }
-                };
-                ask(kb_lo & ~3);
-                for (int i = 0; i < n_kb; ++i) {
-                    const int kb = kb_lo + i;
-                    if (i == 0 || (kb & 3) == 0) {
+                float4 sa_next = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (has) sa_next = *reinterpret_cast<const float4*>(sa_row + (kb_lo & ~3));
+                if (thread < NT && (g.offsets || u != share.unit)) ask_weights(unit, kb_lo & ~3);
+#pragma unroll 1
+                for (int kb = kb_lo, end = kb_lo + n_kb; kb < end;) {
+                    if (kb == kb_lo || (kb & 3) == 0) {
                         // the scales of four k blocks: asked for four blocks ahead, then shared
                         lap ^= 1;
                         if (thread < NT)
@@ -619,29 +647,47 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                                 scales[lap][3][q][thread] = __fmul_rn(sa_next.w, sw_next[q].w);
                             }
                         asm volatile("bar.sync 1, %0;" ::"n"(32 * S::EPILOGUE) : "memory");
-                        if ((kb & ~3) + 4 < kb_lo + n_kb) ask((kb & ~3) + 4);
+                        if (thread < NT && (kb & ~3) + 4 < end) {
+                            if (has) sa_next = *reinterpret_cast<const float4*>(sa_row + (kb & ~3) + 4);
+                            ask_weights(unit, (kb & ~3) + 4);
+                        }
                     }
-                    const float* by = &scales[lap][kb & 3][kind][t0];
+                    const int first = kb & 1, behind = min((kb | 1) + 1, end) - (kb & ~1);          // of the buffer's two k blocks
+                    const float* by = &scales[lap][kb & 2][kind][t0];
+                    constexpr int NEXT = CLASSES * (NT + 4);                                          // floats from k block to k block
+                    kb = (kb | 1) + 1;
                     if (ok) {
                         ok = __all_sync(0xffffffffu, mbar_wait(ring.sums(buffer), parity, abort_flag, 2 * limit));
                         if (!ok && lane == 0) give_up(43);
                     }
                     if (ok) {
                         tcgen05_fence_after();
-                        const uint32_t from = taddr + (uint32_t)(buffer * NT);
-#pragma unroll
-                        for (int c = 0; c < CHUNKS; ++c) {
-                            if (t0 + 16 * c >= unit.width) break;
-                            uint32_t v[16];
-                            tmem_ld(from + 16 * c, v);
-                            ulonglong2 s4[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) s4[q] = *reinterpret_cast<const ulonglong2*>(by + 16 * c + 4 * q);
-                            tmem_ld_wait();
+                        const uint32_t from = taddr + (uint32_t)(buffer * S::COLUMNS);
+                        auto add = [&](const uint32_t* v, const float* s, int c) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q) {
-                                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[8 * c + 2 * q]) : "l"(pair_of(v[4 * q], v[4 * q + 1])), "l"(s4[q].x));
-                                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[8 * c + 2 * q + 1]) : "l"(pair_of(v[4 * q + 2], v[4 * q + 3])), "l"(s4[q].y));
+                                const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(s + 4 * q);
+                                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[8 * c + 2 * q]) : "l"(pair_of(v[4 * q], v[4 * q + 1])), "l"(s4.x));
+                                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[8 * c + 2 * q + 1]) : "l"(pair_of(v[4 * q + 2], v[4 * q + 3])), "l"(s4.y));
+                            }
+                        };
+                        if (t0 < unit.width) {
+                            if constexpr (CHUNKS == 1) {
+                                uint32_t v[2][16];
+                                if (first == 0) tmem_ld(from, v[0]);
+                                if (behind == 2) tmem_ld(from + NT, v[1]);
+                                tmem_ld_wait();
+                                if (first == 0) add(v[0], by, 0);
+                                if (behind == 2) add(v[1], by + NEXT, 0);
+                            } else {
+#pragma unroll 1
+                                for (int j = first; j < behind; ++j) {
+                                    uint32_t v[32];
+                                    tmem_ld_32x32b_x32(from + j * NT, v);
+                                    tmem_ld_wait();
+#pragma unroll
+                                    for (int c = 0; c < CHUNKS; ++c) add(v + 16 * c, by + j * NEXT + 16 * c, c);
+                                }
                             }
                         }
                         tcgen05_fence_before();
@@ -650,71 +696,71 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                     }
                     if (++buffer == S::BUFFERS) { buffer = 0; parity ^= 1u; }
                 }
-                int mine_lo = 0, mine_end = unit.here;
+                // the unit's pairs that this warp finishes, 16 at a time: its own, or of a cluster's block its share's
+                int t = t0, end = min(t0 + MINE, unit.here), step = 16;
                 if (blocks > 1) {
-                    // (one unit a cluster)
-                    const int tokens = (unit.here + 7) & ~7, part = g.share;
-                    mine_lo = rank * part;
-                    const int all_end = min(mine_lo + part, tokens);
-                    mine_end = min(all_end, unit.here);
-                    if (thread == 0) mbar_expect_tx(ring.parts(), (uint32_t)(blocks - 1) * (uint32_t)max(0, all_end - mine_lo) * 512u);
+                    // (one unit a cluster) every block sends what it has of a token to the block that finishes it, itself among them
+                    const int tokens = (unit.here + 7) & ~7, part = g.share, lo = rank * part;
+                    if (thread == 0) mbar_expect_tx(ring.parts(), (uint32_t)blocks * (uint32_t)max(0, min(part, tokens - lo)) * 512u);
                     cluster_wait();
                     if (ok) {
+                        int to = t0 / part, begins = to * part;
+                        const uint32_t mine = ring.base + parts_at + (uint32_t)rank * part_bytes + (uint32_t)row * 16;
 #pragma unroll
                         for (int q = 0; q < MINE / 4; ++q) {
-                            const int t = t0 + 4 * q, p = t / part;
-                            if (t < tokens && p != rank) {
+                            const int tq = t0 + 4 * q;
+                            if (tq >= begins + part) ++to, begins += part;
+                            if (tq < tokens) {
                                 float v[4];
                                 halves(sums[2 * q], v[0], v[1]);
                                 halves(sums[2 * q + 1], v[2], v[3]);
-                                // of block p's blocks - 1 parts this block's is number `rank`, or rank - 1 if p is below it
-                                const uint32_t dst = in_block(ring.base + parts_at + (uint32_t)(rank - (rank > p ? 1 : 0)) * part_bytes + (uint32_t)((t - p * part) / 4) * 2048u + (uint32_t)row * 16, p);
                                 asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
-                                             ::"r"(dst), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-                                               "r"(__float_as_uint(v[3])), "r"(in_block(ring.parts(), p))
+                                             ::"r"(in_block(mine + (uint32_t)(tq - begins) * 512u, to)), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])),
+                                               "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(in_block(ring.parts(), to))
                                              : "memory");
                             }
                         }
-                        if (mine_lo < all_end) ok = __all_sync(0xffffffffu, wait_cluster(ring.parts(), 0, abort_flag, 2 * limit));
+                        if (lo < tokens) ok = __all_sync(0xffffffffu, wait_cluster(ring.parts(), 0, abort_flag, 2 * limit));
                         if (!ok && lane == 0) give_up(43);
                     }
-                    if (ok) {
-                        const uint8_t* parts = aligned + parts_at + (size_t)row * 16;
-#pragma unroll
-                        for (int q = 0; q < MINE / 4; ++q)
-                            if (t0 + 4 * q >= mine_lo && t0 + 4 * q < all_end)
-                                for (int p = 0; p < blocks - 1; ++p) {
-                                    const float4 x = *reinterpret_cast<const float4*>(parts + (size_t)p * part_bytes + (size_t)((t0 + 4 * q - mine_lo) / 4) * 2048);
-                                    float v[4];
-                                    halves(sums[2 * q], v[0], v[1]);
-                                    halves(sums[2 * q + 1], v[2], v[3]);
-                                    sums[2 * q] = pair_of(__float_as_uint(v[0] + x.x), __float_as_uint(v[1] + x.y));
-                                    sums[2 * q + 1] = pair_of(__float_as_uint(v[2] + x.z), __float_as_uint(v[3] + x.w));
-                                }
-                    }
+                    t = lo + (t0 / MINE) * 16, end = min(lo + part, unit.here), step = 16 * S::SETS;
                 }
                 if (ok)
 #pragma unroll 1
-                    for (int c = 0; c < CHUNKS; ++c) {
-                        const int t = t0 + 16 * c, lo = max(0, mine_lo - t), hi = min(16, mine_end - t);
-                        if (lo >= hi) continue;
-#pragma unroll
-                        for (int cc = 0; cc < CHUNKS; ++cc)          // (registers are not indexed: one of these runs)
-                            if (cc == c)
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) {
-                                    float a, b;
-                                    halves(sums[8 * cc + q], a, b);
-                                    park[(2 * q) * 32 + lane] = finished(a);
-                                    park[(2 * q + 1) * 32 + lane] = finished(b);
+                    for (; t < end; t += step) {
+                        if (blocks > 1) {
+                            const uint8_t* parts = aligned + parts_at + (size_t)(t - rank * g.share) * 512 + (size_t)row * 16;
+#pragma unroll 1
+                            for (int q = 0; q < 4 && t + 4 * q < end; ++q) {
+                                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                                for (int p = 0; p < blocks; ++p) {          // (in the blocks' order)
+                                    const float4 x = *reinterpret_cast<const float4*>(parts + (size_t)p * part_bytes + q * 2048);
+                                    v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
                                 }
-                        finish(t, lo, hi);
+                                park[(4 * q) * 32 + lane] = finished(v.x);
+                                park[(4 * q + 1) * 32 + lane] = finished(v.y);
+                                park[(4 * q + 2) * 32 + lane] = finished(v.z);
+                                park[(4 * q + 3) * 32 + lane] = finished(v.w);
+                            }
+                        } else {
+#pragma unroll
+                            for (int cc = 0; cc < CHUNKS; ++cc)          // (registers are not indexed: one of these runs)
+                                if (t == t0 + 16 * cc)
+#pragma unroll
+                                    for (int q = 0; q < 8; ++q) {
+                                        float a, b;
+                                        halves(sums[8 * cc + q], a, b);
+                                        park[(2 * q) * 32 + lane] = finished(a);
+                                        park[(2 * q + 1) * 32 + lane] = finished(b);
+                                    }
+                        }
+                        finish(t, 0, min(16, end - t));
                     }
             } else {
                 ok = __all_sync(0xffffffffu, mbar_wait(ring.sums(buffer), parity, abort_flag, 2 * limit));
                 if (!ok) break;
                 tcgen05_fence_after();
-                const uint32_t from = taddr + (uint32_t)(buffer * NT);
+                const uint32_t from = taddr + (uint32_t)(buffer * S::COLUMNS);
                 const int chunks = min(CHUNKS, (unit.here - t0 + 15) >> 4);
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
@@ -1007,7 +1053,7 @@ Cut cut_of(int code) { return {code / 1000, code / 100 % 10, code % 10, code / 1
 
 struct Product {
     Args args;
-    const CUtensorMap* map;
+    const BlockRows* rows;
     int pairs, out_dtype;
     void* out;
     cudaStream_t stream;
@@ -1033,11 +1079,12 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
     g.blocks = cut.blocks;
     // (of the rows of a span, as the units have them)
     const int span = (int)(((g.rows + spans - 1) / spans + 15) / 16 * 16), most_rows = g.rows < span ? g.rows : span;
+    g.spans = (int)spans, g.span = span;
     g.share = cut.blocks > 1 ? ((most_rows + 7) / 8 + cut.blocks - 1) / cut.blocks * 8 : 0;
     JLLM_REQUIRE(cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= g.k_blocks && (cut.blocks == 1 || (kind.clusters && !g.offsets)),
                  "gemm_grouped: no clusters of %d blocks for such a product", cut.blocks);
     // An SM has 228 KB, a block 227 at most; each block's last KB is the system's, `own` what the kernel holds by itself.
-    const size_t lists = g.offsets ? 8 * (size_t)(g.groups + 1) : 0, parts = (size_t)(cut.blocks - 1) * g.share * 512, fixed = kind.fixed + lists, each = kind.stage + 16;
+    const size_t lists = g.offsets ? 8 * (size_t)(g.groups + 1) : 0, parts = cut.blocks > 1 ? (size_t)cut.blocks * g.share * 512 : 0, fixed = kind.fixed + lists, each = kind.stage + 16;
     const size_t own = kind.own;
     const size_t all = cut.per_sm == 1 ? 227 * 1024 : 113 * 1024;
     JLLM_REQUIRE((cut.per_sm == 1 || cut.per_sm == 2) && kind.tmem * cut.per_sm <= 512 && own + fixed + parts + (FETCHED + 1) * each <= all,
@@ -1049,6 +1096,11 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
         if (stages > most) stages = most < 2 ? 2 : (int)most;
     }
     g.stages = stages;
+    // (a span's rows in one copy; of groups some of the next group's come along, of wide ones at most 63)
+    g.box = !g.offsets ? span : kind.rows < 64 ? kind.rows : 64;
+    CUtensorMap map;
+    const int rc = rows_map_for(p.rows->data, p.rows->rows, g.row_bytes, p.rows->stride, g.box, &map);
+    if (rc != JLLM_OK) return rc;
     // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: of a cluster's blocks, which have 256
     // columns at most, no more than two are on an SM (113 KB), nor one beside blocks of another product that together want more than the rest.
     const size_t smem = stages * each + parts + fixed;
@@ -1076,7 +1128,7 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    cudaLaunchKernelEx(&cfg, kern, *p.map, g, static_cast<Tout*>(p.out));
+    cudaLaunchKernelEx(&cfg, kern, map, g, static_cast<Tout*>(p.out));
     return jllm_check_launch("gemm_grouped");
 }
 
@@ -1188,14 +1240,11 @@ JLLM_EXPORT int jllm_gemm_grouped(const BlockRows* rows, const BlockWeight* weig
     int* error_word = jllm_gemm_error_word();
     if (!error_word) return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: no error word");
     const bool gather = groups && !by_pair;
-    CUtensorMap map;
-    const int rc = rows_map_for(rows->data, M, (long long)K * bytes, rows->stride, 16, &map);
-    if (rc != JLLM_OK) return rc;
     Product p;
     p.args = Args{static_cast<const uint8_t*>(weight->data), static_cast<const uint8_t*>(rows->data), weight->scale, rows->scale, groups ? groups->offsets : nullptr, gather ? groups->order : nullptr,
-                  weight->scale_ld, rows->scale_ld, weight->groups, groups ? groups->top : 1, M, (N + 127) / 128, weight->k_blocks, K * bytes, (int)(rows->stride / 16),
-                  Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, N, swiglu_word}, 0, 1, 0, starve.what, starve.limit_us, error_word};
-    p.map = &map, p.pairs = (int)pairs, p.out_dtype = out_dtype, p.out = out, p.stream = stream;
+                  weight->scale_ld, rows->scale_ld, weight->groups, groups ? groups->top : 1, M, (N + 127) / 128, weight->k_blocks, 0, 0, K * bytes, (int)(rows->stride / 16),
+                  Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, N, swiglu_word}, 0, 1, 0, 16, starve.what, starve.limit_us, error_word};
+    p.rows = rows, p.pairs = (int)pairs, p.out_dtype = out_dtype, p.out = out, p.stream = stream;
     const Cut cut = cut_code ? cut_of(cut_code) : choose(fp8, groups ? weight->groups : 1, (int)pairs, p.args.tiles, weight->k_blocks);
     return fp8 ? launch_product<true>(p, cut) : launch_product<false>(p, cut);
 }
