@@ -1,131 +1,177 @@
 // Around the products of ragged groups: the (row, choice) pairs of a step in the order of the experts they ask (group_rows), and of every row's
 // answers the sum with the router's weights (combine_groups).
 //
-// group_rows is a stable counting sort of pairs by expert, in ONE launch: a cluster of up to eight blocks, every warp a run of neighbouring pairs.
-// (1) a warp counts its run's experts, 32 pairs at a time (lanes of the same expert find one another, the first of them adds their number: no
-// atomics, and the order is the pairs'); (2) the counts of a block's warps, then of the cluster's blocks (through distributed shared memory), then
-// of the experts in front become each warp's first place for each expert; (3) a warp walks its run again and places its pairs. Latency bounds it: two
-// walks over what is in L2, three meetings.
+// group_rows is a stable counting sort of pairs by expert. A block has a run of neighbouring pairs and every warp of it a part of the run.
+// (1) a warp counts its pairs' experts, 32 pairs at a time (lanes of the same expert find one another by votes on its bits, the first of them adds their
+// number: no atomics, and the order is the pairs'), and each pair keeps its number among its warp's of that expert; (2) the warps' counts, and the
+// experts' in front, become each warp's first place for each expert; (3) every pair has its place, and the block's pairs leave in their experts' order.
+// Up to 2,048 pairs are one block and one launch. Of more, a launch in front counts every block's pairs by expert, and (2) adds up the blocks in front.
+// Latency bounds the small ones; of 131,072 pairs a cluster of eight blocks took 23 us for the votes and scattered words of 8 SMs.
 //
 // combine_groups reads every answer once and writes every row once: memory bounds it. The sum runs over a row's choices in their order in float32,
 // whatever place the pairs have: equal bits in every batch.
 #include "common.cuh"
 #include "fp8_view.h"
-#include "tcgen05_common.cuh"
 
 namespace {
 
-constexpr int MAX_GROUPS = 1024, MOST_WARPS = 32;
+constexpr int MAX_GROUPS = 1024, MOST_WARPS = 32, HELD = 2, MOST_BLOCKS = GROUP_BLOCKS;
+static_assert(32 * HELD * MOST_WARPS <= 1 << 11 && MAX_GROUPS <= 1 << 10, "a pair and its expert share a word");
 
-__device__ __forceinline__ int of_block(const int* p, uint32_t rank) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(tc::in_block(tc::smem_u32(p), rank)) : "memory");
-    return v;
+__device__ __forceinline__ int expert_of(const int* choice, int ld, int top, int groups, long long p) {
+    size_t at = (size_t)p;
+    if (ld != top) {
+        int row, c;
+        split_item(p, top, row, c);
+        at = (size_t)row * ld + c;
+    }
+    const int e = choice[at];
+    return e >= 0 && e < groups ? e : -1;
 }
 
-// `run`: pairs of a warp, a multiple of 32. Shared memory: counts [warps][groups], then the block's [groups].
-__global__ void __launch_bounds__(MOST_WARPS * 32) group_rows_kernel(const int* __restrict__ choice, int ld, int top, long long pairs, int groups, int run, int* __restrict__ offsets,
-                                                                     int* __restrict__ order, int* __restrict__ place) {
-    extern __shared__ int counts[];
-    __shared__ int sums[MOST_WARPS + 1];
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x, rank = blockIdx.x;
-    int *mine = counts + warp * groups, *block_count = counts + warps * groups;
-    for (int i = threadIdx.x; i < warps * groups; i += blockDim.x) counts[i] = 0;
+// counts[block][expert] of the pairs [block * of_block, ...)
+__global__ void __launch_bounds__(1024) count_rows_kernel(const int* __restrict__ choice, int ld, int top, long long pairs, int groups, int of_block, int* __restrict__ counts) {
+    __shared__ int mine[MAX_GROUPS];
+    for (int e = threadIdx.x; e < groups; e += blockDim.x) mine[e] = 0;
     pdl_wait();
     pdl_trigger();
     __syncthreads();
-    const long long first = ((long long)rank * warps + warp) * run, end = first + run < pairs ? first + run : pairs;
-    auto expert = [&](long long p) {
-        if (p >= end) return -1;
-        int row, c;
-        split_item(p, top, row, c);
-        const int e = choice[(size_t)row * ld + c];
-        return e >= 0 && e < groups ? e : -1;
-    };
-    for (long long p = first + lane; p - lane < end; p += 32) {
-        const int e = expert(p);
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[e] += __popc(same);
-        __syncwarp();
+    const long long first = (long long)blockIdx.x * of_block, end = first + of_block < pairs ? first + of_block : pairs;
+    for (long long p = first + threadIdx.x; p < end; p += blockDim.x) {
+        const int e = expert_of(choice, ld, top, groups, p);
+        if (e >= 0) atomicAdd(&mine[e], 1);          // (sums of whole numbers: their order does not matter)
     }
     __syncthreads();
-    // a warp's first place among its block's pairs of an expert, and the block's count
-    for (int e = threadIdx.x; e < groups; e += blockDim.x) {
-        int sum = 0;
-        for (int w = 0; w < warps; ++w) {
-            const int c = counts[w * groups + e];
-            counts[w * groups + e] = sum;
-            sum += c;
+    for (int e = threadIdx.x; e < groups; e += blockDim.x) counts[(size_t)blockIdx.x * groups + e] = mine[e];
+}
+
+// `run`: pairs of a warp, a multiple of 32. Shared memory: counts [warps][groups], the block's first places in the order and in itself and all
+// blocks' counts [groups] each, and of runs that are held the block's pairs (11 bits) with their experts (10).
+__global__ void __launch_bounds__(MOST_WARPS * 32) group_rows_kernel(const int* __restrict__ choice, int ld, int top, long long pairs, int groups, int run, const int* __restrict__ block_counts,
+                                                                     int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ place) {
+    extern __shared__ int counts[];
+    __shared__ unsigned long long sums[MOST_WARPS + 1];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x, rank = blockIdx.x;
+    int *mine = counts + warp * groups, *block_first = counts + warps * groups, *local_first = block_first + groups, *all_of = local_first + groups;
+    uint32_t* sorted = reinterpret_cast<uint32_t*>(all_of + groups);
+    for (int i = threadIdx.x; i < warps * groups; i += blockDim.x) counts[i] = 0;
+    pdl_wait();
+    pdl_trigger();
+    const long long block_at = (long long)rank * warps * run, first = block_at + (long long)warp * run, end = first + run < pairs ? first + run : pairs;
+    auto expert = [&](long long p) { return p < end ? expert_of(choice, ld, top, groups, p) : -1; };
+    const bool held = run <= 32 * HELD;
+    int e_of[HELD], number[HELD];
+    if (held)
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) e_of[i] = 32 * i < run ? expert(first + 32 * i + lane) : -1;
+    __syncthreads();
+    // the 32 pairs' numbers among the warp's of their experts so far
+    auto count = [&](int e) {
+        unsigned same = __ballot_sync(0xffffffffu, e >= 0);          // (lanes without an expert do not count)
+        for (int bit = 1; bit < groups; bit <<= 1) {
+            const unsigned set = __ballot_sync(0xffffffffu, e & bit);
+            same &= e & bit ? set : ~set;
         }
-        block_count[e] = sum;
+        const int before = __popc(same & ((1u << lane) - 1u)), so_far = e >= 0 ? mine[e] : 0;
+        __syncwarp();
+        if (e >= 0 && before == 0) mine[e] = so_far + __popc(same);
+        __syncwarp();
+        return so_far + before;
+    };
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (32 * i < run) number[i] = count(e_of[i]);
+    } else {
+        for (long long p = first + lane; p - lane < end; p += 32) count(expert(p));
     }
     __syncthreads();
-    if (blocks > 1) {
-        tc::cluster_arrive();
-        tc::cluster_wait();
-    }
-    // the experts in front: thread t has `each` neighbouring experts
+    // thread t has `each` neighbouring experts: the warps' counts become their first numbers in the block, and (two sums in one: all blocks' pairs above, the
+    // block's below) the experts in front are added up
     const int each = (groups + blockDim.x - 1) / blockDim.x, e0 = min((int)threadIdx.x * each, groups), e1 = min(e0 + each, groups);
-    int total = 0;
+    unsigned long long total = 0;
     for (int e = e0; e < e1; ++e) {
-        int all = 0;
-        for (int b = 0; b < blocks; ++b) all += of_block(block_count + e, b);
-        total += all;
+        int here = 0;
+        for (int w = 0; w < warps; w += 8) {          // (a multiple of eight warps)
+            int c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = counts[(w + i) * groups + e];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                counts[(w + i) * groups + e] = here;
+                here += c[i];
+            }
+        }
+        int all = here, below = 0;
+        if (blocks > 1) {
+            all = 0;
+#pragma unroll 8
+            for (int b = 0; b < blocks; ++b) {
+                const int c = block_counts[(size_t)b * groups + e];
+                all += c;
+                below += b < rank ? c : 0;
+            }
+        }
+        block_first[e] = below, local_first[e] = here, all_of[e] = all;
+        total += (unsigned long long)all << 32 | (unsigned)here;
     }
-    int upto = total;
+    unsigned long long upto = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int left = __shfl_up_sync(0xffffffffu, upto, o);
+        const unsigned long long left = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += left;
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
     if (warp == 0) {
-        const int s = lane < warps ? sums[lane] : 0;
-        int run_sum = s;
+        const unsigned long long s = lane < warps ? sums[lane] : 0;
+        unsigned long long so_far = s;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int left = __shfl_up_sync(0xffffffffu, run_sum, o);
-            if (lane >= o) run_sum += left;
+            const unsigned long long left = __shfl_up_sync(0xffffffffu, so_far, o);
+            if (lane >= o) so_far += left;
         }
-        if (lane < warps) sums[lane] = run_sum - s;
-        if (lane == 31) sums[MOST_WARPS] = run_sum;
+        if (lane < warps) sums[lane] = so_far - s;
+        if (lane == 31) sums[MOST_WARPS] = so_far;
     }
     __syncthreads();
-    int at = sums[warp] + upto - total;
+    const unsigned long long in_front = sums[warp] + upto - total;
+    int at = (int)(in_front >> 32), in_block = (int)(uint32_t)in_front;
     for (int e = e0; e < e1; ++e) {
         if (rank == 0) offsets[e] = at;
-        int below = 0, all = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const int c = of_block(block_count + e, b);
-            if (b < rank) below += c;
-            all += c;
-        }
-        for (int w = 0; w < warps; ++w) counts[w * groups + e] += at + below;
-        at += all;
+        const int here = local_first[e];
+        block_first[e] += at, local_first[e] = in_block;
+        at += all_of[e], in_block += here;
     }
-    const int routed = sums[MOST_WARPS];
+    const int routed = (int)(sums[MOST_WARPS] >> 32), routed_here = (int)(uint32_t)sums[MOST_WARPS];
     if (rank == 0 && threadIdx.x == 0) offsets[groups] = routed;
     __syncthreads();
-    for (long long p = first + lane; p - lane < end; p += 32) {
-        const int e = expert(p);
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        int to = -1;
-        if (e >= 0) to = mine[e] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (e >= 0 && (same & ((1u << lane) - 1u)) == 0) mine[e] += __popc(same);
-        __syncwarp();
-        if (p < end) {
-            place[p] = to;
-            if (to >= 0) order[to] = (int)p;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (32 * i < run) {
+                const long long p = first + 32 * i + lane;
+                const int e = e_of[i], n = e >= 0 ? mine[e] + number[i] : 0;
+                if (p < end) place[p] = e >= 0 ? block_first[e] + n : -1;
+                if (e >= 0) sorted[local_first[e] + n] = (uint32_t)(p - block_at) | (uint32_t)e << 11;
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < routed_here; i += blockDim.x) {
+            const int e = (int)(sorted[i] >> 11);
+            order[block_first[e] + i - local_first[e]] = (int)(block_at + (sorted[i] & 0x7ffu));
+        }
+    } else {
+        // (the counts have become first numbers: counting on from them gives the pairs theirs)
+        for (long long p = first + lane; p - lane < end; p += 32) {
+            const int e = expert(p), n = count(e);
+            if (p < end) {
+                place[p] = e >= 0 ? block_first[e] + n : -1;
+                if (e >= 0) order[block_first[e] + n] = (int)p;
+            }
         }
     }
     // the pairs without an expert leave the end of the order empty
     for (long long p = routed + (long long)rank * blockDim.x + threadIdx.x; p < pairs; p += (long long)blocks * blockDim.x) order[p] = -1;
-    if (blocks > 1) {          // (nobody's counts are gone while others read them)
-        tc::cluster_arrive();
-        tc::cluster_wait();
-    }
 }
 
 // A thread has 16 bytes of answers (PER values) of a row; `vec`: 16-byte accesses are allowed.
@@ -211,34 +257,21 @@ JLLM_EXPORT int jllm_group_rows(const int* choice, int ld, const RowGroupsView* 
     const long long pairs = (long long)g->rows * g->top;
     JLLM_REQUIRE(g->rows >= 0 && g->top >= 1 && pairs <= BLOCK_MOST && g->groups >= 1 && g->groups <= MAX_GROUPS && ld >= g->top,
                  "group_rows: %d rows of %d choices (%d apart) among %d groups (1 to %d)", g->rows, g->top, ld, g->groups, MAX_GROUPS);
-    // a run of 32 pairs a warp while eight blocks hold them, longer ones beyond
-    const long long runs = (pairs + 31) / 32;
-    const int blocks = runs <= MOST_WARPS ? 1 : runs <= 2 * MOST_WARPS ? 2 : runs <= 4 * MOST_WARPS ? 4 : 8;
-    int warps = runs < MOST_WARPS ? (int)(runs < 1 ? 1 : runs) : MOST_WARPS;
-    // (a warp's counts lie in shared memory: 227 KB hold 32 warps of 1,024 groups; few pairs leave few warps to walk many groups)
-    if (warps < 8) warps = 8;
+    // 32 or 64 pairs a warp while MOST_BLOCKS blocks hold them, longer runs beyond
+    constexpr int FULL = 32 * HELD * MOST_WARPS;
+    const int blocks = pairs <= FULL ? 1 : pairs <= (long long)FULL * MOST_BLOCKS ? (int)((pairs + FULL - 1) / FULL) : MOST_BLOCKS;
+    const int warps = pairs <= 8 * 32 ? 8 : pairs <= 16 * 32 ? 16 : MOST_WARPS;
     const int run = (int)(((pairs + (long long)blocks * warps - 1) / ((long long)blocks * warps) + 31) / 32 * 32);
-    const size_t smem = (size_t)(warps + 1) * g->groups * sizeof(int);
-    auto kern = group_rows_kernel;
-    if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess) return jllm_fail(JLLM_CUDA_ERROR, "group_rows: %zu bytes of shared memory refused", smem);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = blocks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (jllm_launch_overlaps(smem, LAUNCH_DEPENDENT)) {
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = 1;
-        cfg.numAttrs = 2;
+    const size_t smem = ((size_t)(warps + 3) * g->groups + (run <= 32 * HELD ? (size_t)warps * run : 0)) * sizeof(int);
+    if (jllm_allow_smem((const void*)group_rows_kernel, smem) != cudaSuccess) return jllm_fail(JLLM_CUDA_ERROR, "group_rows: %zu bytes of shared memory refused", smem);
+    if (blocks > 1) {
+        JLLM_REQUIRE(g->counts, "group_rows: no room for the blocks' counts");
+        jllm_launch(count_rows_kernel, dim3(blocks), dim3(1024), 0, stream, LAUNCH_DEPENDENT, choice, ld, g->top, pairs, g->groups, warps * run, g->counts);
+        const int rc = jllm_check_launch("group_rows");
+        if (rc != JLLM_OK) return rc;
     }
-    cudaLaunchKernelEx(&cfg, kern, choice, ld, g->top, pairs, g->groups, run, g->offsets, g->order, g->place);
+    jllm_launch(group_rows_kernel, dim3(blocks), dim3(warps * 32), smem, stream, LAUNCH_DEPENDENT, choice, ld, g->top, pairs, g->groups, run, (const int*)g->counts, g->offsets, g->order,
+                g->place);
     return jllm_check_launch("group_rows");
 }
 

@@ -2,10 +2,10 @@
 // largest magnitude of the 128, rounded to float32, and q = v / scale rounded to e4m3, half to even (448 is e4m3's largest value, so nothing is
 // cut off). 128 values that hold an infinity or a NaN have the scale NaN and zeros, so that what is made of them is NaN and not a wrong number.
 //
-// The quotient is rounded ONCE. t = v * (1 / scale) is off by less than 2 units in its last place, so rounding t is rounding the quotient wherever t
-// is further than that from a tie between two e4m3 values; near a tie (about one value in 10^5 of float32 rows; of bfloat16 rows, whose 8
-// bits make exact ties common, one in some hundreds) the sign of v - tie * scale decides, which one fused multiply-add gives exactly enough
-// (its product is exact and its result has the sign of the exact difference).
+// The quotient is rounded ONCE. v (1 / scale) is within 2^-23 of it; both v ((1 / scale) (1 - 2^-22)) and v ((1 / scale) (1 + 2^-22)) are rounded to
+// e4m3, and where they agree that is the quotient's value, which lies between them. Where they do not (next to a tie between two e4m3 values: about one
+// value in 10^5 of float32 rows; of bfloat16 rows, whose 8 bits make exact ties common, one in some hundreds) the sign of v - tie * scale decides,
+// which one fused multiply-add gives (its product is exact, and its result has the sign of the exact difference).
 //
 // Memory bounds it. 16 lanes have a block of 128 values, 8 neighbouring values a lane, so a maximum is four exchanges and nothing meets beyond a
 // half warp; a thread has several blocks' values under way at a time.
@@ -16,29 +16,58 @@ namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;      // 2^-100
 constexpr float kMost = 448.f;
-constexpr int THREADS = 256, AT_A_TIME = 4;
+constexpr int THREADS = 256, AT_A_TIME = 4;      // blocks of a half warp: neighbours in a row
 
-// Eight values from p on (`left` of them exist); `vec`: 16-byte accesses are allowed.
-__device__ __forceinline__ void load8(float (&v)[8], const float* p, int left, bool vec) {
-    if (vec && left >= 8) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
+// Eight neighbouring values of a lane, as they are stored.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
     }
-}
-__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* p, int left, bool vec) {
-    if (vec && left >= 8) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    // (`left` of them exist; `vec`: 16-byte accesses are allowed)
+    __device__ __forceinline__ void load(const float* p, int left, bool vec) {
+        if (vec && left >= 8) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? __bfloat162float(p[j]) : 0.f;
+            for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+        }
     }
-}
+    // the bits of the largest magnitude of 16 lanes' values (a NaN is larger than everything and stays)
+    __device__ __forceinline__ uint32_t most() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    }
+    __device__ __forceinline__ float value(int j) const { return v[j]; }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int left, bool vec) {
+        if (vec && left >= 8) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = (2 * j < left ? q[2 * j] : 0u) | (2 * j + 1 < left ? (uint32_t)q[2 * j + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ uint32_t most() const {
+        uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return max(m << 16, m & 0xffff0000u);
+    }
+    __device__ __forceinline__ float value(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
+};
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -51,78 +80,67 @@ __device__ __forceinline__ void from_e4m3x2(uint32_t two, float& lo, float& hi) 
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
 }
 
-// v / scale, moved off a tie between two e4m3 values where the quotient is not one: what rounds half to even then rounds the quotient.
-__device__ __forceinline__ float quotient(float v, float scale, float inverse) {
-    const float t = v * inverse;
-    const uint32_t bits = __float_as_uint(t) & 0x7fffffffu;
-    // e4m3 values from 2^-6 on have 3 bits behind the leading one: ties are where the 20 bits below are 0x80000. Smaller values lie 2^-9 apart,
-    // ties are the odd multiples of 2^-10.
-    float tie;
-    if (bits >= 0x3c800000u) {          // 2^-6
-        const uint32_t below = bits & 0xfffffu;
-        if (below - 0x7fffcu > 8u) return t;
-        tie = __uint_as_float((bits & ~0xfffffu) | 0x80000u);
-    } else {
-        const float steps = __uint_as_float(bits) * 1024.f, odd = 2.f * floorf(0.5f * steps) + 1.f;      // (the tie of this e4m3 step)
-        if (fabsf(steps - odd) > 1e-4f) return t;
-        tie = odd * 0.0009765625f;
-    }
-    // |v| against tie * scale
-    const float beyond = __fmaf_rn(-tie, scale, fabsf(v));
-    const float moved = beyond == 0.f ? tie : __uint_as_float(__float_as_uint(tie) + (beyond > 0.f ? 1 : -1));
-    return copysignf(moved, v);
+// Which of two neighbouring e4m3 values `lo` and `hi` (bytes of the same sign; the same one twice: that one) v / scale rounds to: |v| against tie * scale,
+// the tie between them; from the tie itself to the even one. `a`, `b`: their magnitudes.
+__device__ __forceinline__ uint32_t nearer(float v, float scale, uint32_t lo, uint32_t hi, float a, float b) {
+    const float beyond = __fmaf_rn(-0.5f * (a + b), scale, fabsf(v));
+    const uint32_t less = min(lo, hi), more = max(lo, hi);          // (bytes of a sign are ordered as their magnitudes)
+    return beyond > 0.f || (beyond == 0.f && (less & 1u)) ? more : less;
+}
+__device__ __forceinline__ uint32_t nearer_two(float v0, float v1, float scale, uint32_t lo, uint32_t hi) {
+    float a0, a1, b0, b1;
+    from_e4m3x2(lo & 0x7f7fu, a0, a1);
+    from_e4m3x2(hi & 0x7f7fu, b0, b1);
+    return nearer(v0, scale, lo & 0xffu, hi & 0xffu, a0, b0) | nearer(v1, scale, lo >> 8, hi >> 8, a1, b1) << 8;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) quantize_fp8_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
-                                                               int ld_scale, int rows, int cols, int blocks, bool vec) {
+                                                               int ld_scale, int rows, int cols, int blocks, int chunks, int per, bool vec) {
     pdl_wait();
     pdl_trigger();
     const int lane16 = threadIdx.x & 15;
-    const long long items = (long long)rows * blocks, step = (long long)gridDim.x * (THREADS / 16);
-    for (long long item = (long long)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);; item += AT_A_TIME * step) {
+    const long long items = (long long)rows * chunks, step = (long long)gridDim.x * (THREADS / 16);
+    for (long long item = (long long)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);; item += step) {
         // (whole warps go on together: the exchanges below are theirs)
         if (!__any_sync(0xffffffffu, item < items)) return;
-        float v[AT_A_TIME][8];
-        int row[AT_A_TIME], block[AT_A_TIME], left[AT_A_TIME];
+        int row = 0, first = 0;
+        split_item(item, chunks, row, first);
+        first *= per;
+        const int here = item < items ? min(per, blocks - first) : 0;          // blocks of this half warp
+        const T* src = x + (size_t)row * ldx + first * 128 + lane16 * 8;
+        const int left = cols - first * 128 - lane16 * 8;                      // values from there on
+        Eight<T> v[AT_A_TIME];
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a) {
-            const long long mine = item + a * step;
-            left[a] = 0;
-            row[a] = block[a] = 0;
-            if (mine < items) {
-                split_item(mine, blocks, row[a], block[a]);
-                left[a] = min(8, max(0, cols - block[a] * 128 - lane16 * 8));
-            } else {
-                row[a] = -1;
-            }
-            if (left[a] > 0) load8(v[a], x + (size_t)row[a] * ldx + block[a] * 128 + lane16 * 8, left[a], vec);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[a][j] = 0.f;
+            v[a].zero();
+            if (a < here && left > 128 * a) v[a].load(src + 128 * a, left - 128 * a, vec);
         }
+        uint8_t* dst = q + (size_t)row * ldq + first * 128 + lane16 * 8;
+        float* dst_scale = scale + (size_t)row * ld_scale + first;
+        const int room = ((cols + 15) & ~15) - first * 128 - lane16 * 8;
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a) {
-            uint32_t m = 0;                        // (magnitudes as bits: a NaN is larger than everything and stays)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[a][j]) & 0x7fffffffu);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const uint32_t m = v[a].most();
+            if (a >= here) continue;
             const bool bad = m >= 0x7f800000u;
             const float s = __fdiv_rn(fmaxf(__uint_as_float(bad ? 0u : m), kTiny), kMost), inverse = __frcp_rn(s);
-            if (row[a] < 0) continue;
-            if (lane16 == 0) scale[(size_t)row[a] * ld_scale + block[a]] = bad ? __uint_as_float(0x7fc00000u) : s;
-            uint32_t lo = 0, hi = 0;
-            if (!bad) {
-                float t[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = quotient(v[a][j], s, inverse);
-                lo = e4m3x2(t[0], t[1]) | e4m3x2(t[2], t[3]) << 16;
-                hi = e4m3x2(t[4], t[5]) | e4m3x2(t[6], t[7]) << 16;
-            }
+            if (lane16 == 0) dst_scale[a] = bad ? __uint_as_float(0x7fc00000u) : s;
             // (rows begin at multiples of 16 bytes and have room up to the next one: what is behind the last value is zero)
-            const int at = block[a] * 128 + lane16 * 8;
-            if (at < ((cols + 15) & ~15)) *reinterpret_cast<uint2*>(q + (size_t)row[a] * ldq + at) = make_uint2(lo, hi);
+            if (room <= 128 * a) continue;
+            const float below = inverse * (1.f - 2.384185791015625e-7f), above = inverse * (1.f + 2.384185791015625e-7f);      // 2^-22
+            uint32_t lo[4], hi[4], differ = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = e4m3x2(v[a].value(2 * j) * below, v[a].value(2 * j + 1) * below);
+                hi[j] = e4m3x2(v[a].value(2 * j) * above, v[a].value(2 * j + 1) * above);
+                differ |= lo[j] ^ hi[j];
+            }
+            if (differ)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (lo[j] != hi[j]) lo[j] = nearer_two(v[a].value(2 * j), v[a].value(2 * j + 1), s, lo[j], hi[j]);
+            *reinterpret_cast<uint2*>(dst + 128 * a) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
         }
     }
 }
@@ -152,24 +170,29 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8], in
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) fp8_values_kernel(const uint8_t* __restrict__ q, long long ldq, const float* __restrict__ scale, int ld_scale, T* __restrict__ out,
-                                                             long long ldo, int rows, int cols, int eights, bool vec) {
+                                                             long long ldo, int rows, int cols, int blocks, int chunks, int per, bool vec) {
     pdl_wait();
     pdl_trigger();
-    const long long items = (long long)rows * eights, step = (long long)gridDim.x * THREADS;
-    for (long long item = (long long)blockIdx.x * THREADS + threadIdx.x; item < items; item += AT_A_TIME * step) {
+    const int lane16 = threadIdx.x & 15;
+    const long long items = (long long)rows * chunks, step = (long long)gridDim.x * (THREADS / 16);
+    for (long long item = (long long)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4); item < items; item += step) {
+        int row, first;
+        split_item(item, chunks, row, first);
+        first *= per;
+        const int here = min(per, blocks - first), left = cols - first * 128 - lane16 * 8;
+        const uint8_t* src = q + (size_t)row * ldq + first * 128 + lane16 * 8;
+        T* dst = out + (size_t)row * ldo + first * 128 + lane16 * 8;
         uint2 w[AT_A_TIME];
         float s[AT_A_TIME];
-        int row[AT_A_TIME], at[AT_A_TIME];
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a)
-            if (item + a * step < items) {
-                split_item(item + a * step, eights, row[a], at[a]);
-                w[a] = *reinterpret_cast<const uint2*>(q + (size_t)row[a] * ldq + at[a] * 8);
-                s[a] = scale[(size_t)row[a] * ld_scale + at[a] / 16];
+            if (a < here && left > 128 * a) {
+                w[a] = *reinterpret_cast<const uint2*>(src + 128 * a);
+                s[a] = scale[(size_t)row * ld_scale + first + a];
             }
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a)
-            if (item + a * step < items) {
+            if (a < here && left > 128 * a) {
                 float v[8];
                 from_e4m3x2(w[a].x & 0xffffu, v[0], v[1]);
                 from_e4m3x2(w[a].x >> 16, v[2], v[3]);
@@ -177,7 +200,7 @@ __global__ void __launch_bounds__(THREADS) fp8_values_kernel(const uint8_t* __re
                 from_e4m3x2(w[a].y >> 16, v[6], v[7]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], s[a]);
-                store8(out + (size_t)row[a] * ldo + at[a] * 8, v, cols - at[a] * 8, vec);
+                store8(dst + 128 * a, v, left - 128 * a, vec);
             }
     }
 }
@@ -187,6 +210,12 @@ int grid_for(long long items, int per_block) {
     const long long all = (items + per_block - 1) / per_block, most = (long long)jllm_device_sm_count() * 8;
     return (int)(all < most ? all : most > 0 ? most : 1);
 }
+
+// A row's blocks in equal chunks of up to AT_A_TIME.
+struct Chunks {
+    int blocks, chunks, per;
+    explicit Chunks(int cols) : blocks((cols + 127) / 128), chunks((blocks + AT_A_TIME - 1) / AT_A_TIME), per((blocks + chunks - 1) / chunks) {}
+};
 
 int check(const char* name, const BlockRows* r) {
     JLLM_REQUIRE((r->scale || r->rows == 0) && r->rows >= 0 && r->rows <= BLOCK_MOST && r->cols >= 1 && r->cols <= BLOCK_MOST && r->stride % 16 == 0 && r->stride >= r->cols &&
@@ -202,17 +231,18 @@ JLLM_EXPORT int jllm_quantize_fp8(const void* x, int dtype, long long ldx, const
     if (rc != JLLM_OK) return rc;
     JLLM_REQUIRE(ldx >= out->cols, "quantize_fp8: rows of %d values, %lld apart", out->cols, ldx);
     if (out->rows == 0) return JLLM_OK;
-    const int blocks = (out->cols + 127) / 128, size = dtype == JLLM_F32 ? 4 : 2;
+    const Chunks c(out->cols);
+    const int size = dtype == JLLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)x % 16) == 0 && ldx * size % 16 == 0;
-    const dim3 grid(grid_for((long long)out->rows * blocks, THREADS / 16));
+    const dim3 grid(grid_for((long long)out->rows * c.chunks, THREADS / 16));
     uint8_t* q = static_cast<uint8_t*>(const_cast<void*>(out->data));
     float* scale = const_cast<float*>(out->scale);
     if (dtype == JLLM_F32)
         jllm_launch(quantize_fp8_kernel<float>, grid, dim3(THREADS), 0, stream, LAUNCH_DEPENDENT, static_cast<const float*>(x), ldx, q, out->stride, scale,
-                    out->scale_ld, out->rows, out->cols, blocks, vec);
+                    out->scale_ld, out->rows, out->cols, c.blocks, c.chunks, c.per, vec);
     else
         jllm_launch(quantize_fp8_kernel<__nv_bfloat16>, grid, dim3(THREADS), 0, stream, LAUNCH_DEPENDENT, static_cast<const __nv_bfloat16*>(x), ldx, q, out->stride,
-                    scale, out->scale_ld, out->rows, out->cols, blocks, vec);
+                    scale, out->scale_ld, out->rows, out->cols, c.blocks, c.chunks, c.per, vec);
     return jllm_check_launch("quantize_fp8");
 }
 
@@ -221,15 +251,16 @@ JLLM_EXPORT int jllm_fp8_values(const BlockRows* rows, void* out, int dtype, lon
     if (rc != JLLM_OK) return rc;
     JLLM_REQUIRE(ldo >= rows->cols, "fp8_values: rows of %d values, %lld apart", rows->cols, ldo);
     if (rows->rows == 0) return JLLM_OK;
-    const int eights = (rows->cols + 7) / 8, size = dtype == JLLM_F32 ? 4 : 2;
+    const Chunks c(rows->cols);
+    const int size = dtype == JLLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)out % 16) == 0 && ldo * size % 16 == 0;
-    const dim3 grid(grid_for((long long)rows->rows * eights, THREADS));
+    const dim3 grid(grid_for((long long)rows->rows * c.chunks, THREADS / 16));
     const uint8_t* q = static_cast<const uint8_t*>(rows->data);
     if (dtype == JLLM_F32)
         jllm_launch(fp8_values_kernel<float>, grid, dim3(THREADS), 0, stream, LAUNCH_DEPENDENT, q, rows->stride, rows->scale, rows->scale_ld, static_cast<float*>(out), ldo,
-                    rows->rows, rows->cols, eights, vec);
+                    rows->rows, rows->cols, c.blocks, c.chunks, c.per, vec);
     else
         jllm_launch(fp8_values_kernel<__nv_bfloat16>, grid, dim3(THREADS), 0, stream, LAUNCH_DEPENDENT, q, rows->stride, rows->scale, rows->scale_ld,
-                    static_cast<__nv_bfloat16*>(out), ldo, rows->rows, rows->cols, eights, vec);
+                    static_cast<__nv_bfloat16*>(out), ldo, rows->rows, rows->cols, c.blocks, c.chunks, c.per, vec);
     return jllm_check_launch("fp8_values");
 }

@@ -18,8 +18,9 @@ struct BlockWeight {
 };
 // The pairs (row, choice) in the order of their groups: group g's are order[offsets[g]] .. order[offsets[g + 1] - 1]; place is the way back.
 struct RowGroupsView {
-    int *offsets, *order, *place;
+    int *offsets, *order, *place, *counts;      // counts: room for up to GROUP_BLOCKS blocks' pairs by group (of more than 2,048 pairs)
     int rows, top, groups;
 };
+constexpr int GROUP_BLOCKS = 128;
 // The kernels count rows, pairs and values in 32 bits and step past the end by up to a block's 8,192 values.
 constexpr int BLOCK_MOST = 0x7fffffff - 8191;

@@ -1775,7 +1775,7 @@ class _BlockWeight(ctypes.Structure):
 
 
 class _RowGroupsView(ctypes.Structure):
-    _fields_ = [("offsets", c_void_p), ("order", c_void_p), ("place", c_void_p), ("rows", c_int), ("top", c_int), ("groups", c_int)]
+    _fields_ = [("offsets", c_void_p), ("order", c_void_p), ("place", c_void_p), ("counts", c_void_p), ("rows", c_int), ("top", c_int), ("groups", c_int)]
 
 
 def _on_current_device(name, *tensors):
@@ -1971,19 +1971,19 @@ class RowGroups:
     """The (row, choice) pairs of a step in the order of the groups (experts) they ask: group g's pairs are order[offsets[g]] .. order[offsets[g + 1] - 1],
     each r * top + c of its row r and choice c, in ascending order; `order` is -1 behind the last pair. place[r, c] is where the pair (r, c) lies, -1 if it
     asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs."""
-    __slots__ = ("offsets", "order", "place", "rows", "top", "groups", "pairs", "_view", "view")
+    __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "pairs", "_view", "view")
 
-    def __init__(self, offsets, order, place, rows, top, groups):
-        self.offsets, self.order, self.place, self.rows, self.top, self.groups = offsets, order, place, rows, top, groups
+    def __init__(self, offsets, order, place, counts, rows, top, groups):
+        self.offsets, self.order, self.place, self.counts, self.rows, self.top, self.groups = offsets, order, place, counts, rows, top, groups
         self.pairs = rows * top
-        self._view = _RowGroupsView(offsets.data_ptr(), order.data_ptr(), place.data_ptr(), rows, top, groups)
+        self._view = _RowGroupsView(offsets.data_ptr(), order.data_ptr(), place.data_ptr(), counts.data_ptr(), rows, top, groups)
         self.view = ctypes.addressof(self._view)
 
     def first(self, rows: int) -> "RowGroups":
         """The same room for a step of fewer rows (to be filled anew)."""
         if not 0 <= rows <= self.rows:
             _refuse("RowGroups", f"0 to {self.rows} rows, got {rows}")
-        return RowGroups(self.offsets, self.order[:rows * self.top], self.place[:rows], rows, self.top, self.groups)
+        return RowGroups(self.offsets, self.order[:rows * self.top], self.place[:rows], self.counts, rows, self.top, self.groups)
 
 
 def row_groups(rows: int, top: int, groups: int, device) -> RowGroups:
@@ -1991,8 +1991,9 @@ def row_groups(rows: int, top: int, groups: int, device) -> RowGroups:
     if rows < 0 or top < 1 or rows * top > BLOCK_MOST or not 1 <= groups <= MOST_GROUPS:
         _refuse("row_groups", f"up to {BLOCK_MOST} pairs and 1 to {MOST_GROUPS} groups, got {rows} x {top} and {groups}")
     offsets = torch.zeros((groups + 1,), dtype=torch.int32, device=device)
+    counts = torch.zeros((min(128, -(-rows * top // 2048)), groups), dtype=torch.int32, device=device)          # (GROUP_BLOCKS)
     return RowGroups(offsets, torch.full((rows * top,), -1, dtype=torch.int32, device=device),
-                     torch.full((rows, top), -1, dtype=torch.int32, device=device), rows, top, groups)
+                     torch.full((rows, top), -1, dtype=torch.int32, device=device), counts, rows, top, groups)
 
 
 def group_rows(choice: torch.Tensor, groups: RowGroups) -> None:

@@ -275,7 +275,7 @@ def choices(rows, top, groups, seed=0, unused=0.2, few=None):
 
 
 @pytest.mark.parametrize("rows,top,groups", [(0, 2, 4), (1, 1, 1), (1, 8, 128), (3, 2, 1024), (31, 1, 5), (8, 8, 128), (128, 8, 7 + 1), (300, 4, 60), (1025, 3, 33), (4096, 8, 256),
-                                             (16384, 8, 256), (20011, 5, 1000)])
+                                             (16384, 8, 256), (20011, 5, 1000), (70001, 4, 300)])
 def test_group_rows(ops, rows, top, groups):
     choice = choices(rows, top, groups) if rows else torch.empty((0, top), dtype=torch.int32)
     if rows > 20:
