@@ -2,10 +2,15 @@
 // largest magnitude of the 128, rounded to float32, and q = v / scale rounded to e4m3, half to even (448 is e4m3's largest value, so nothing is
 // cut off). 128 values that hold an infinity or a NaN have the scale NaN and zeros, so that what is made of them is NaN and not a wrong number.
 //
-// The quotient is rounded ONCE. v (1 / scale) is within 2^-23 of it; both v ((1 / scale) (1 - 2^-22)) and v ((1 / scale) (1 + 2^-22)) are rounded to
-// e4m3, and where they agree that is the quotient's value, which lies between them. Where they do not (next to a tie between two e4m3 values: about one
-// value in 10^5 of float32 rows; of bfloat16 rows, whose 8 bits make exact ties common, one in some hundreds) the sign of v - tie * scale decides,
-// which one fused multiply-add gives (its product is exact, and its result has the sign of the exact difference).
+// The quotient v / scale is rounded ONCE, although float32 arithmetic finds it with an error, and a value next to a tie between two e4m3 values could fall to
+// the wrong side.
+// float32 rows: v ((1 / scale) (1 - 2^-20)) and v ((1 / scale) (1 + 2^-20)) are both rounded to e4m3, and where they agree that is the quotient's value, which
+// lies between them. Where they do not (one value in 10^4), the sign of v - tie * scale decides, which one fused multiply-add gives: its product is exact and
+// its result has the sign of the exact difference.
+// bfloat16 rows: their 8 bits make ties common (some lane of every second warp has one), so nothing branches. With v = a 2^i and m = b 2^j, a and b of 8 bits,
+// v 448 / m is a tie T or further than 2^-13 from it (7 a 2^x and T' b are whole numbers), and the quotient is that, shifted by the error that the scale's own
+// rounding left: to the same side for all of a block's values, which m - 448 scale tells. So the reciprocal is taken 2^-20 larger, or smaller; or, where the
+// scale is exact, the quotient is corrected by its residual, so that a tie is met exactly and falls to the even value.
 //
 // Memory bounds it. 16 lanes have a block of 128 values, 8 neighbouring values a lane, so a maximum is four exchanges and nothing meets beyond a
 // half warp; a thread has several blocks' values under way at a time.
@@ -61,9 +66,18 @@ template <> struct Eight<__nv_bfloat16> {
         }
     }
     __device__ __forceinline__ uint32_t most() const {
-        uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        auto two = [](uint32_t bits) {
+            __nv_bfloat162 b;
+            *reinterpret_cast<uint32_t*>(&b) = bits & 0x7fff7fffu;
+            return b;
+        };
+        __nv_bfloat162 b = __hmax2_nan(__hmax2_nan(two(w[0]), two(w[1])), __hmax2_nan(two(w[2]), two(w[3])));
+        uint32_t m = *reinterpret_cast<const uint32_t*>(&b);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 8; o > 0; o >>= 1) {
+            b = __hmax2_nan(two(m), two(__shfl_xor_sync(0xffffffffu, m, o)));
+            m = *reinterpret_cast<const uint32_t*>(&b);
+        }
         return max(m << 16, m & 0xffff0000u);
     }
     __device__ __forceinline__ float value(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
@@ -92,6 +106,38 @@ __device__ __forceinline__ uint32_t nearer_two(float v0, float v1, float scale, 
     from_e4m3x2(lo & 0x7f7fu, a0, a1);
     from_e4m3x2(hi & 0x7f7fu, b0, b1);
     return nearer(v0, scale, lo & 0xffu, hi & 0xffu, a0, b0) | nearer(v1, scale, lo >> 8, hi >> 8, a1, b1) << 8;
+}
+
+// Eight values over the scale in e4m3, two to a word; `inverse`: 1 / scale to 2^-22; `off`: the largest magnitude less 448 scales.
+__device__ __forceinline__ void rounded(const Eight<float>& v, float scale, float inverse, float, uint32_t (&two)[4]) {
+    const float below = inverse * (1.f - 9.5367431640625e-7f), above = inverse * (1.f + 9.5367431640625e-7f);      // 2^-20
+    uint32_t hi[4], differ = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        two[j] = e4m3x2(v.value(2 * j) * below, v.value(2 * j + 1) * below);
+        hi[j] = e4m3x2(v.value(2 * j) * above, v.value(2 * j + 1) * above);
+        differ |= two[j] ^ hi[j];
+    }
+    if (differ)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (two[j] != hi[j]) two[j] = nearer_two(v.value(2 * j), v.value(2 * j + 1), scale, two[j], hi[j]);
+}
+__device__ __forceinline__ void rounded(const Eight<__nv_bfloat16>& v, float scale, float inverse, float off, uint32_t (&two)[4]) {
+    const float first = off == 0.f ? inverse : inverse * (off > 0.f ? 1.f + 9.5367431640625e-7f : 1.f - 9.5367431640625e-7f), then = off == 0.f ? inverse : 0.f;
+    auto quotient = [&](float x) {
+        const float t = __fmul_rn(x, first);
+        return __fmaf_rn(__fmaf_rn(-t, scale, x), then, t);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two[j] = e4m3x2(quotient(v.value(2 * j)), quotient(v.value(2 * j + 1)));
+}
+
+// m / 448, correctly rounded: the quotient from the reciprocal and one correction by its residual (P. Markstein, IBM J. Res. Dev. 34, 1990); that it is so for this
+// divisor has been counted out over all significands.
+__device__ __forceinline__ float by_448(float m) {
+    const float y = 0.002232142857142857f, q = __fmul_rn(m, y);
+    return __fmaf_rn(__fmaf_rn(-kMost, q, m), y, q);
 }
 
 template <typename T>
@@ -124,23 +170,13 @@ __global__ void __launch_bounds__(THREADS) quantize_fp8_kernel(const T* __restri
             const uint32_t m = v[a].most();
             if (a >= here) continue;
             const bool bad = m >= 0x7f800000u;
-            const float s = __fdiv_rn(fmaxf(__uint_as_float(bad ? 0u : m), kTiny), kMost), inverse = __frcp_rn(s);
+            const float most = fmaxf(__uint_as_float(bad ? 0u : m), kTiny), s = by_448(most), inverse = __fdividef(1.f, s);
             if (lane16 == 0) dst_scale[a] = bad ? __uint_as_float(0x7fc00000u) : s;
             // (rows begin at multiples of 16 bytes and have room up to the next one: what is behind the last value is zero)
             if (room <= 128 * a) continue;
-            const float below = inverse * (1.f - 2.384185791015625e-7f), above = inverse * (1.f + 2.384185791015625e-7f);      // 2^-22
-            uint32_t lo[4], hi[4], differ = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lo[j] = e4m3x2(v[a].value(2 * j) * below, v[a].value(2 * j + 1) * below);
-                hi[j] = e4m3x2(v[a].value(2 * j) * above, v[a].value(2 * j + 1) * above);
-                differ |= lo[j] ^ hi[j];
-            }
-            if (differ)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (lo[j] != hi[j]) lo[j] = nearer_two(v[a].value(2 * j), v[a].value(2 * j + 1), s, lo[j], hi[j]);
-            *reinterpret_cast<uint2*>(dst + 128 * a) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+            uint32_t two[4];
+            rounded(v[a], s, inverse, __fmaf_rn(-kMost, s, most), two);
+            *reinterpret_cast<uint2*>(dst + 128 * a) = bad ? make_uint2(0u, 0u) : make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
         }
     }
 }
