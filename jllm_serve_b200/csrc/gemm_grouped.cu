@@ -796,59 +796,48 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
 // rows three: a block of 128 up rows may end inside the tile), so a k block costs one packed multiply-add for two values and nothing is shared
 // between threads. Sixteen warps do it: with eight (128 columns each) their way through a k block, one load of tensor memory behind the other, was
 // longer than the MMAs' and the copies'.
-constexpr int WIDE_PARK = 12;      // rows of 8 values, 12 apart: no two of eight lanes' 16-byte pieces share a bank
+// A row's 64 bytes of results leave together: a store whose 32 lanes each write 16 bytes of another row costs 32 lines, and what ends a unit stands in
+// nobody's shadow (4 us a unit of 128 x 256 that way).
+constexpr int WIDE_PARK = 32 * 64;      // bytes of a warp
 
-// 16 results of a pair (this lane's) -> out, columns from c0 on.
-template <typename Tout>
-__device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, float* park, const float (&v)[16], size_t p0, int rows, int c0, int last, bool vec, int lane) {
-    if (sizeof(Tout) == 2 && vec && c0 + 16 <= last) {
-        // (a lane's 32 bytes are a whole sector of the row)
-        if (lane < rows) {
-            Tout* dst = out + (p0 + lane) * f.ldo + c0;
-            __align__(16) Tout w[16];
-            if (f.accumulate == EPI_ADD) {
-                *reinterpret_cast<uint4*>(w) = reinterpret_cast<const uint4*>(dst)[0];
-                *reinterpret_cast<uint4*>(w + 8) = reinterpret_cast<const uint4*>(dst)[1];
+// N results of this lane's pair into its 64 bytes, from 16-byte piece `first` on: piece c of row r lies at place c ^ (r / 2).
+template <typename Tout, int N>
+__device__ __forceinline__ void park_row(uint8_t* park, const float (&v)[N], int first, int lane) {
+    constexpr int PER = 16 / sizeof(Tout);
 #pragma unroll
-                for (int q = 0; q < 16; ++q) w[q] = from_float<Tout>(__fadd_rn(v[q], to_float(w[q])));
-            } else {
+    for (int c = 0; c < N / PER; ++c) {
+        __align__(16) Tout w[PER];
 #pragma unroll
-                for (int q = 0; q < 16; ++q) w[q] = from_float<Tout>(v[q]);
-            }
-            reinterpret_cast<uint4*>(dst)[0] = *reinterpret_cast<const uint4*>(w);
-            reinterpret_cast<uint4*>(dst)[1] = *reinterpret_cast<const uint4*>(w + 8);
-        }
-        return;
+        for (int q = 0; q < PER; ++q) w[q] = from_float<Tout>(v[c * PER + q]);
+        *reinterpret_cast<uint4*>(park + lane * 64 + (((first + c) ^ (lane >> 1)) & 3) * 16) = *reinterpret_cast<const uint4*>(w);
     }
-    // eight columns at a time through the warp's shared memory, so that a row's 32 bytes leave together
+}
+// The warp's 32 rows of 64 bytes -> out, columns from c0 on.
+template <typename Tout>
+__device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, uint8_t* park, size_t p0, int rows, int c0, int last, bool vec, int lane) {
+    constexpr int PER = 16 / sizeof(Tout), COLS = 4 * PER;
+    __syncwarp();
+    if (vec && c0 + COLS <= last) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        __syncwarp();
-        *reinterpret_cast<float4*>(park + lane * WIDE_PARK) = make_float4(v[8 * h], v[8 * h + 1], v[8 * h + 2], v[8 * h + 3]);
-        *reinterpret_cast<float4*>(park + lane * WIDE_PARK + 4) = make_float4(v[8 * h + 4], v[8 * h + 5], v[8 * h + 6], v[8 * h + 7]);
-        __syncwarp();
-        const int c8 = c0 + 8 * h;
-        if (sizeof(Tout) == 4 && vec && c8 + 8 <= last) {
-#pragma unroll
-            for (int i = lane; i < 64; i += 32) {
-                const int j = i >> 1, c = (i & 1) * 4;
-                if (j >= rows) continue;
-                float* dst = reinterpret_cast<float*>(out) + (p0 + j) * f.ldo + c8 + c;
-                float4 x = *reinterpret_cast<const float4*>(park + j * WIDE_PARK + c);
-                if (f.accumulate == EPI_ADD) {
-                    const float4 old = *reinterpret_cast<const float4*>(dst);
-                    x = make_float4(__fadd_rn(x.x, old.x), __fadd_rn(x.y, old.y), __fadd_rn(x.z, old.z), __fadd_rn(x.w, old.w));
-                }
-                *reinterpret_cast<float4*>(dst) = x;
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2), c = lane & 3;
+            if (r >= rows) continue;
+            Tout* dst = out + (p0 + r) * f.ldo + c0 + c * PER;
+            uint4 x = *reinterpret_cast<const uint4*>(park + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
+            if (sizeof(Tout) == 4 && f.accumulate == EPI_ADD) {
+                const float4 old = *reinterpret_cast<const float4*>(dst);
+                x = make_uint4(__float_as_uint(__fadd_rn(__uint_as_float(x.x), old.x)), __float_as_uint(__fadd_rn(__uint_as_float(x.y), old.y)),
+                               __float_as_uint(__fadd_rn(__uint_as_float(x.z), old.z)), __float_as_uint(__fadd_rn(__uint_as_float(x.w), old.w)));
             }
-        } else {
-            const int c = lane & 7;
-            if (c8 + c < last)
-                for (int j = lane >> 3; j < rows; j += 4) {
-                    Tout* dst = out + (p0 + j) * f.ldo + c8 + c;
-                    const float x = park[j * WIDE_PARK + c];
-                    *dst = from_float<Tout>(f.accumulate == EPI_ADD ? __fadd_rn(x, to_float(*dst)) : x);
-                }
+            *reinterpret_cast<uint4*>(dst) = x;
+        }
+    } else {
+        for (int i = lane; i < 32 * COLS; i += 32) {
+            const int r = i / COLS, c = i % COLS;
+            if (r >= rows || c0 + c >= last) continue;
+            Tout* dst = out + (p0 + r) * f.ldo + c0 + c;
+            const Tout x = *reinterpret_cast<const Tout*>(park + r * 64 + (((c / PER) ^ (r >> 1)) & 3) * 16 + c % PER * sizeof(Tout));
+            *dst = sizeof(Tout) == 4 && f.accumulate == EPI_ADD ? from_float<Tout>(__fadd_rn(to_float(x), to_float(*dst))) : x;
         }
     }
 }
@@ -858,7 +847,7 @@ __global__ void __launch_bounds__(Wide<FP8>::THREADS, 1)
 gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Args g, Tout* __restrict__ out) {
     using S = Wide<FP8>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(16) float parks[S::EPILOGUE][32 * WIDE_PARK];
+    __shared__ __align__(16) uint8_t parks[S::EPILOGUE][WIDE_PARK];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_word;
     const Share share(g);               // (blocks by themselves)
@@ -892,7 +881,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::MANY));
         const int quad = warp & 3, set = (warp - S::FIRST) >> 2, half = set >> 1, token = quad * 32 + lane;
         const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(set * 64);
-        float* park = parks[warp - S::FIRST];
+        uint8_t* park = parks[warp - S::FIRST];
         const bool vec = ((uintptr_t)out & 15u) == 0 && (((size_t)g.f.ldo * sizeof(Tout)) & 15u) == 0;
         const int last = GLU ? g.f.N >> 1 : g.f.N;
         pdl_wait();          // the rows' scales, and what is added into, were written by the kernels before
@@ -903,34 +892,40 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             const int tile = unit.tile + half, rows = min(32, unit.here - quad * 32), c_set = tile * (GLU ? 64 : 128) + (set & 1) * (GLU ? 32 : 64);
             const bool mine = tile < g.tiles && rows > 0;
             const size_t p0 = (size_t)(unit.first + quad * 32);
-            // 32 columns of this lane's pair to results
-            auto finish = [&](const float (&v)[32], int c) {
-                float x[16];
+            // 16 columns of this lane's pair, the c-th of the warp's, to results
+            auto finish = [&](float (&v)[16], int c) {
+                constexpr int COLS = 64 / sizeof(Tout);
                 if constexpr (GLU) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float eight[8];
-                        glu_units<8, true>(g.f.glu, [&](int q) { return v[16 * h + q]; }, [&](int q) { return v[16 * h + 8 + q]; }, 1.f, eight);
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) x[8 * h + q] = eight[q];
-                    }
-                    if (c_set + 16 * c < last) leave_rows<Tout>(g.f, out, park, x, p0, rows, c_set + 16 * c, last, vec, lane);
+                    float eight[8];
+                    glu_units<8, true>(g.f.glu, [&](int q) { return v[q]; }, [&](int q) { return v[8 + q]; }, 1.f, eight);
+                    constexpr int TIMES = COLS / 8;          // eights of a row's 64 bytes
+                    if (c % TIMES == 0) __syncwarp();
+                    park_row<Tout>(park, eight, c % TIMES * (4 / TIMES), lane);
+                    const int c0 = c_set + c / TIMES * COLS;
+                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
                 } else {
+                    const int c16 = c_set + 16 * c;
+                    if (g.f.has_bias)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c0 = c_set + 32 * c + 16 * h;
-                        if (c0 >= last) break;
+                        for (int q = 0; q < 16; ++q) v[q] = c16 + q < last ? __fadd_rn(v[q], g.f.bias[c16 + q]) : 0.f;
+                    if (g.f.accumulate == EPI_RELU2)
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
-                            x[q] = v[16 * h + q];
-                            if (g.f.has_bias && c0 + q < last) x[q] = __fadd_rn(x[q], g.f.bias[c0 + q]);
-                            if (g.f.accumulate == EPI_RELU2) {
-                                const float z = x[q] < 0.f ? 0.f : x[q];              // (what is not a number stays so: a maximum would drop it)
-                                x[q] = __fmul_rn(z, z);
-                            }
+                            const float z = v[q] < 0.f ? 0.f : v[q];              // (what is not a number stays so: a maximum would drop it)
+                            v[q] = __fmul_rn(z, z);
                         }
-                        leave_rows<Tout>(g.f, out, park, x, p0, rows, c0, last, vec, lane);
+                    if (sizeof(Tout) == 2 && g.f.accumulate == EPI_ADD && lane < rows) {
+                        // (added here, so that the sum is rounded once)
+                        const Tout* old = out + (p0 + lane) * g.f.ldo + c16;
+#pragma unroll
+                        for (int q = 0; q < 16; ++q)
+                            if (c16 + q < last) v[q] = __fadd_rn(v[q], to_float(old[q]));
                     }
+                    constexpr int TIMES = COLS / 16;
+                    if (c % TIMES == 0) __syncwarp();
+                    park_row<Tout>(park, v, c % TIMES * (4 / TIMES), lane);
+                    const int c0 = c_set + c / TIMES * COLS;
+                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
                 }
             };
             if constexpr (FP8) {
@@ -979,10 +974,10 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 }
                 if (ok && mine)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float v[32];
+                    for (int c = 0; c < 4; ++c) {
+                        float v[16];
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) halves(sums[16 * c + q], v[2 * q], v[2 * q + 1]);
+                        for (int q = 0; q < 8; ++q) halves(sums[8 * c + q], v[2 * q], v[2 * q + 1]);
                         finish(v, c);
                     }
             } else {
@@ -990,19 +985,19 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint32_t from = taddr + (uint32_t)(buffer * S::COLUMNS);
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(from + 32 * c, r);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[16];
+                    tmem_ld(from + 16 * c, r);
                     tmem_ld_wait();
-                    if (c == 1) {           // the buffer is another unit's as soon as its last values are read
+                    if (c == 3) {           // the buffer is another unit's as soon as its last values are read
                         tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(ring.taken(buffer));
                     }
-                    float v[32];
+                    float v[16];
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(r[q]);
+                    for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(r[q]);
                     if (mine) finish(v, c);
                 }
                 if (++buffer == S::BUFFERS) { buffer = 0; parity ^= 1u; }
