@@ -28,6 +28,8 @@
 #include "fp8_view.h"
 #include "tcgen05_common.cuh"
 
+#include <cmath>
+
 namespace {
 
 using namespace tc;
@@ -127,6 +129,7 @@ struct Narrow {
                          TMEM = BUFFERS * COLUMNS < 32 ? 32 : BUFFERS * COLUMNS;
     // four warps have the tile's weight rows; with 32 rows and more two sets of them share the rows
     static constexpr int SETS = NT >= 32 ? 2 : 1, EPILOGUE = 4 * SETS, FIRST = 2, THREADS = 32 * (FIRST + EPILOGUE);
+    static constexpr bool CLUSTERS = FP8 && NT <= 32;          // (the parts of 64 rows leave no room for a ring beside another block)
     static constexpr int GATHER = 0, GATHER_WARPS = 1, GATHER_ROWS = NT;          // the producer fetches rows itself
     static constexpr uint32_t STAGE = TILES * TILE_BYTES + NT * 128;
 };
@@ -698,7 +701,7 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                 }
                 // the unit's pairs that this warp finishes, 16 at a time: its own, or of a cluster's block its share's
                 int t = t0, end = min(t0 + MINE, unit.here), step = 16;
-                if (blocks > 1) {
+                if (S::CLUSTERS && blocks > 1) {
                     // (one unit a cluster) every block sends what it has of a token to the block that finishes it, itself among them
                     const int tokens = (unit.here + 7) & ~7, part = g.share, lo = rank * part;
                     if (thread == 0) mbar_expect_tx(ring.parts(), (uint32_t)blocks * (uint32_t)max(0, min(part, tokens - lo)) * 512u);
@@ -728,7 +731,7 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                 if (ok)
 #pragma unroll 1
                     for (; t < end; t += step) {
-                        if (blocks > 1) {
+                        if (S::CLUSTERS && blocks > 1) {
                             const uint8_t* parts = aligned + parts_at + (size_t)(t - rank * g.share) * 512 + (size_t)row * 16;
 #pragma unroll 1
                             for (int q = 0; q < 4 && t + 4 * q < end; ++q) {
@@ -1140,7 +1143,7 @@ int launch_narrow(const Product& p, const Cut& cut) {
     using S = Narrow<FP8, NT>;
     auto kern = gemm_grouped_narrow_kernel<FP8, NT, GLU, Tout>;
     static const size_t own = own_smem((const void*)kern);
-    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, FP8}, p, cut);
+    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, S::CLUSTERS}, p, cut);
 }
 template <bool FP8, bool GLU, typename Tout>
 int launch_wide(const Product& p, const Cut& cut) {
@@ -1164,23 +1167,116 @@ int launch_product(const Product& p, const Cut& cut) {
     return p.args.f.glu ? launch_cut<FP8, true, __nv_bfloat16>(p, cut) : launch_cut<FP8, false, __nv_bfloat16>(p, cut);
 }
 
-Cut choose(bool fp8, int groups, int pairs, int tiles, int k_blocks) {
-    const int sms = jllm_device_sm_count(), asked = groups < pairs ? groups : pairs, mean = (pairs + asked - 1) / asked;
-    Cut cut{128, 1, 1, 1};
-    if (groups == 1) {
-        cut.nt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
-        const int units = tiles * ((mean + cut.nt - 1) / cut.nt);
-        if (fp8 && cut.nt <= 64 && units < sms) {
-            cut.blocks = sms / units;
-            if (cut.blocks > 8) cut.blocks = 8;
-            while (cut.blocks > 1 && k_blocks / cut.blocks < 2) --cut.blocks;
-        }
-        if (cut.nt == 128) cut.mt = 2;
-    } else {
-        cut.nt = mean <= 6 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : 128;
-        if (cut.nt == 128) cut.mt = 2;
+// Clusters of that many blocks that the device runs at a time, `per_sm` blocks an SM; asked once per device.
+int resident_clusters(int blocks, int per_sm) {
+    static int known[64][2][9] = {};          // (one more than the answer)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int& answer = known[dev][per_sm - 1][blocks];
+    if (answer) return answer - 1;
+    using S = Narrow<true, 16>;
+    auto kern = gemm_grouped_narrow_kernel<true, 16, false, float>;
+    const size_t own = own_smem((const void*)kern), smem = (per_sm == 1 ? 227 * 1024 : 113 * 1024) - own;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (own == 0 || jllm_allow_smem((const void*)kern, smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
     }
-    return cut;
+    // (the driver counts one block an SM for whatever allocates tensor memory; two run where shared memory has room)
+    if (per_sm == 2) {
+        const int alone = resident_clusters(blocks, 1);
+        if (n < 2 * alone) n = 2 * alone;
+    }
+    answer = n + 1;
+    return n;
+}
+
+// Counts that put the cuts in order; a count is no time, though it is fitted to microseconds. Fitted to products launched back to back on weights larger
+// than L2.
+// One weight, e4m3 (9,837 sizes of 1 to 2,048 rows against 64 to 24,576 weight rows of 128 to 12,288 values, up to 25 cuts each; on 3,000 that the fit has not
+// seen what is chosen is 1.7% slower than the best cut of each size in the geometric mean, 11% at the 95th percentile): a block's k blocks, alone on its SM or beside
+// another one, each longer the more SMs take in at once; what a unit costs beside them; sending.
+struct Narrowly {
+    int nt;
+    double start, alone, alone_all, beside, beside_all, unit, send, block, token;
+};
+constexpr Narrowly NARROW[3] = {{16, 2.46, 0.184, 0.099, 0.243, 0.341, 0.82, 0.51, 0.034, 0.062},
+                                {32, 2.09, 0.186, 0.142, 0.434, 0.128, 1.52, 0.85, 0.0, 0.043},
+                                {64, 1.86, 0.234, 0.128, 0.550, 0.0, 2.62, 0.0, 0.0, 0.0}};
+double narrow_count(const Narrowly& c, int blocks, int rows, int tiles, int k_blocks, int sms) {
+    const int one = resident_clusters(blocks, 1), two = resident_clusters(blocks, 2), spans = (rows + c.nt - 1) / c.nt;
+    if (blocks > k_blocks || one < 1 || two < 1) return 1e30;
+    const long long units = (long long)spans * tiles, all = units * blocks;
+    const double each = (k_blocks + blocks - 1) / blocks;
+    double run = units <= one ? each * (c.alone + c.alone_all * all / sms) + c.unit
+                              : (double)((units + two - 1) / two) * (each * (c.beside + c.beside_all * (all < 2 * sms ? all / (2.0 * sms) : 1.0)) + c.unit);
+    if (blocks > 1) run += c.send + c.block * blocks + c.token * ((rows + spans - 1) / spans) * (1.0 - 1.0 / blocks);
+    const double read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
+    return c.start + (run > read ? run : read);
+}
+double wide_count(int rows, int tiles, int k_blocks, int sms) {
+    const long long units = (long long)((tiles + 1) / 2) * ((rows + 127) / 128), rounds = (units + sms - 1) / sms;
+    const double busy = units < sms ? (double)units / sms : 1.0, run = rounds * (k_blocks * (0.5 + 0.118 * busy) + 3.38), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
+    return 1.27 + (run > read ? run : read);
+}
+// Groups (11,092 sizes: 1 to 2,048 rows of 1 to 8 choices among 4 to 128 groups, 128 to 4,096 weight rows of as many values; 3.5%; by the mean of a group's pairs
+// alone 7%): the host knows neither which groups are asked nor how often, so both are reckoned from even choices, half a span more than the pairs fill.
+struct Grouping {
+    double start, k_block, unit, row;
+};
+constexpr int SPANS[4] = {16, 32, 64, 128};
+constexpr Grouping GROUPING[2][2][4] = {          // [e4m3][by pair][span]
+    {{{4.27, 0.265, 0.0, 0.097}, {4.50, 0.274, 0.0, 0.087}, {3.64, 0.505, 1.61, 0.063}, {4.61, 0.432, 3.92, 0.045}},
+     {{3.89, 0.225, 0.0, 0.049}, {3.99, 0.225, 0.0, 0.039}, {4.15, 0.220, 0.0, 0.037}, {4.54, 0.301, 3.27, 0.028}}},
+    {{{4.79, 0.271, 0.0, 0.120}, {3.94, 0.332, 1.47, 0.068}, {2.87, 0.588, 2.87, 0.061}, {1.01, 0.538, 6.81, 0.041}},
+     {{4.37, 0.240, 0.0, 0.097}, {4.60, 0.249, 0.0, 0.073}, {5.37, 0.232, 0.0, 0.059}, {1.30, 0.426, 6.06, 0.028}}}};
+
+// The cut for a product. (Worked out once per size: the choice is kept.)
+Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int tiles, int k_blocks) {
+    static std::mutex mu;
+    static std::unordered_map<MapKey, Cut, MapKeyHash> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return {16, 1, 1, 2};
+    const MapKey key{nullptr, rows, (long long)tiles << 32 | (unsigned)k_blocks, groups ? (long long)groups->groups << 32 | (unsigned)groups->top : 0,
+                     dev << 2 | (int)fp8 << 1 | (int)by_pair};
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    const int sms = jllm_device_sm_count();
+    Cut best{16, 1, 1, 2};
+    double least = 1e30;
+    auto offer = [&](double count, const Cut& cut) {
+        if (count < least) least = count, best = cut;
+    };
+    if (!groups) {
+        for (const Narrowly& c : NARROW)
+            for (int blocks = 1; blocks <= (fp8 && c.nt <= 32 ? 8 : 1); ++blocks) offer(narrow_count(c, blocks, rows, tiles, k_blocks, sms), {c.nt, 1, blocks, 2});
+        offer(wide_count(rows, tiles, k_blocks, sms), {128, 2, 1, 1});
+    } else {
+        const double pairs = (double)groups->rows * groups->top, share = groups->top < groups->groups ? (double)groups->top / groups->groups : 1.0;
+        const double asked = groups->groups * (1.0 - pow(1.0 - share, groups->rows)), mean = pairs / (asked > 1.0 ? asked : 1.0);
+        for (int i = 0; i < 4; ++i) {
+            const Grouping& c = GROUPING[fp8][by_pair][i];
+            const int nt = SPANS[i], places = nt == 128 ? sms : 2 * sms;
+            const double spans = mean <= 0.5 * nt ? asked : pairs / nt + 0.5 * asked, units = spans * (nt == 128 ? (tiles + 1) / 2 : tiles);
+            const double rounds = units <= sms ? 1.0 : units < places ? 1.0 : units / places, read = asked * tiles * (double)TILE_BYTES * k_blocks / 6e6;
+            const double run = rounds * (k_blocks * c.k_block + c.unit + c.row * (mean < nt ? mean : nt));
+            offer(c.start + (run > read ? run : read), {nt, nt == 128 ? 2 : 1, 1, nt == 128 ? 1 : 2});
+        }
+    }
+    if (known.size() >= 4096) known.clear();
+    return known[key] = best;
 }
 
 // A test of the waits: what the next product of this thread is to miss, and how long its waits last.
@@ -1240,6 +1336,6 @@ JLLM_EXPORT int jllm_gemm_grouped(const BlockRows* rows, const BlockWeight* weig
                   weight->scale_ld, rows->scale_ld, weight->groups, groups ? groups->top : 1, M, (N + 127) / 128, weight->k_blocks, 0, 0, K * bytes, (int)(rows->stride / 16),
                   Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, N, swiglu_word}, 0, 1, 0, 16, starve.what, starve.limit_us, error_word};
     p.rows = rows, p.pairs = (int)pairs, p.out_dtype = out_dtype, p.out = out, p.stream = stream;
-    const Cut cut = cut_code ? cut_of(cut_code) : choose(fp8, groups ? weight->groups : 1, (int)pairs, p.args.tiles, weight->k_blocks);
+    const Cut cut = cut_code ? cut_of(cut_code) : choose(fp8, groups, by_pair != 0, M, p.args.tiles, weight->k_blocks);
     return fp8 ? launch_product<true>(p, cut) : launch_product<false>(p, cut);
 }

@@ -1778,19 +1778,24 @@ class _RowGroupsView(ctypes.Structure):
     _fields_ = [("offsets", c_void_p), ("order", c_void_p), ("place", c_void_p), ("counts", c_void_p), ("rows", c_int), ("top", c_int), ("groups", c_int)]
 
 
-def _on_current_device(name, *tensors):
-    """The launchers run on the current device's current stream: what they are given lies there."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    for t in tensors:
-        if not t.is_cuda or t.device.index != here:
-            _refuse(name, f"everything lies on the current CUDA device, got {t.device}")
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _on_current_device(name, *devices):
+    """The launchers run on the current device's current stream: what they are given lies there. `devices`: what `Tensor.get_device` says."""
+    first = devices[0]
+    for d in devices:
+        if d != first or d < 0:
+            _refuse(name, f"everything lies on one CUDA device, got {devices} (-1: none)")
+    if first != _current_device():
+        _refuse(name, f"everything lies on the current CUDA device, got device {first}")
 
 
 class Fp8Rows:
     """Rows of activations in 8-bit floating point: value j of row r stands for data[r, j] * scale[r, j // 128]. data float8_e4m3fn [rows, cols],
     its rows beginning at multiples of 16 bytes; scales float32 [rows, blocks filled up to a multiple of four], 16-byte aligned (`fp8_rows` makes
     such). `scale` are the blocks that the columns have. A slice of rows is `rows8[lo:hi]`."""
-    __slots__ = ("data", "scales", "scale", "rows", "cols", "shape", "blocks", "on_gpu", "_view", "view")
+    __slots__ = ("data", "scales", "scale", "rows", "cols", "shape", "blocks", "device", "_view", "view")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         if data.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32 or data.dim() != 2 or scales.dim() != 2 or scales.shape[0] != data.shape[0]:
@@ -1798,11 +1803,11 @@ class Fp8Rows:
         self.data, self.scales = data, scales
         self.rows, self.cols = self.shape = tuple(data.shape)
         self.blocks = -(-self.cols // BLOCK)
-        self.on_gpu = data.is_cuda and scales.is_cuda and data.device == scales.device
+        self.device = data.get_device() if data.device.type != "meta" else -1          # (-1: no GPU)
         stride = data.stride(0) if self.rows > 1 else -(-self.cols // 16) * 16              # (a single row's stride says nothing)
         ld = scales.shape[1]
         if (self.cols < 1 or (self.cols > 1 and data.stride(1) != 1) or stride < self.cols or stride % 16 or data.data_ptr() % 16 or max(self.shape) > BLOCK_MOST
-                or ld % 4 or ld < self.blocks or not scales.is_contiguous() or scales.data_ptr() % 16):
+                or ld % 4 or ld < self.blocks or not scales.is_contiguous() or scales.data_ptr() % 16 or data.device != scales.device):
             _refuse("Fp8Rows", f"neighbouring values that begin at multiples of 16 bytes and scales in whole fours, got {self.shape}, strides {data.stride()}, "
                                f"scales {tuple(scales.shape)}, {scales.stride()} at {data.data_ptr():#x}, {scales.data_ptr():#x}")
         self.scale = scales[:, :self.blocks]
@@ -1832,7 +1837,7 @@ def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
     name = "quantize_fp8"
     if x.dtype not in _DT:
         _refuse(name, f"float32 or bfloat16 rows, got {x.dtype}")
-    _on_current_device(name, x, out.data, out.scales)
+    _on_current_device(name, x.get_device(), out.device)
     _call("jllm_quantize_fp8", x.data_ptr(), _DT[x.dtype], _row_stride(name, "x", x, out.shape), out.view, _stream())
 
 
@@ -1841,7 +1846,7 @@ def fp8_values(rows8: Fp8Rows, out: torch.Tensor) -> torch.Tensor:
     name = "fp8_values"
     if out.dtype not in _DT:
         _refuse(name, f"float32 or bfloat16 values, got {out.dtype}")
-    _on_current_device(name, out, rows8.data, rows8.scales)
+    _on_current_device(name, out.get_device(), rows8.device)
     _call("jllm_fp8_values", rows8.view, out.data_ptr(), _DT[out.dtype], _row_stride(name, "out", out, rows8.shape), _stream())
     return out
 
@@ -1855,7 +1860,7 @@ class PackedBlocks:
     def __init__(self, data: torch.Tensor, scales: torch.Tensor | None, groups: int, rows: int, cols: int, glu: bool = False):
         self.data, self.scales, self.groups, self.rows, self.cols, self.glu = data, scales, groups, rows, cols, glu
         self.shape, self.tiles, self.k_blocks = (rows, cols), data.shape[1], data.shape[2]
-        self.fp8 = scales is not None
+        self.fp8, self.device = scales is not None, data.get_device()
         self._view = _BlockWeight(data.data_ptr(), _p(scales), groups, rows, cols, self.k_blocks, scales.shape[2] if self.fp8 else 0, int(glu))
         self.view = ctypes.addressof(self._view)
 
@@ -1883,7 +1888,7 @@ def _pack_bytes(name, w: torch.Tensor, glu: bool) -> torch.Tensor:
         padded[:, :N, :K] = torch.stack([_glu_order(one) for one in w]) if glu else w
         tiles = padded.view(G * T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)
         return tiles.gather(3, _swizzle_index(w.device).expand(G * T, KB, 128, 8, 16)).contiguous().view(G, T, KB, 128, 128)
-    _on_current_device(name, w)
+    _on_current_device(name, w.get_device())
     packed = torch.empty((G, T, KB, 128, 128), dtype=torch.int8, device=w.device)
     for g in range(G):
         _call("jllm_pack_int8", w[g].data_ptr(), K, N, K, int(glu), packed[g].data_ptr(), _stream())
@@ -1955,13 +1960,13 @@ def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor 
     word = _product_words(name, w, swiglu)
     if not w.fp8 or w.groups != 1 or a.cols != w.cols or out.dtype not in _DT:
         _refuse(name, f"e4m3 rows and one e4m3 weight of {w.cols} columns and a float32 or bfloat16 result, got {a.cols} columns, {w.groups} weights and {out.dtype}")
-    _on_current_device(name, a.data, a.scales, w.data, out)
+    _on_current_device(name, a.device, w.device, out.get_device())
     if bias is None:
         b, b_dtype = 0, F32
     else:
         if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_contiguous():
             _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
-        _on_current_device(name, bias)
+        _on_current_device(name, bias.get_device(), w.device)
         b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
     _call("jllm_gemm_grouped", a.view, w.view, 0, 0, b, b_dtype, out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows)), int(accumulate), word, cut, _stream())
@@ -1971,11 +1976,11 @@ class RowGroups:
     """The (row, choice) pairs of a step in the order of the groups (experts) they ask: group g's pairs are order[offsets[g]] .. order[offsets[g + 1] - 1],
     each r * top + c of its row r and choice c, in ascending order; `order` is -1 behind the last pair. place[r, c] is where the pair (r, c) lies, -1 if it
     asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs."""
-    __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "pairs", "_view", "view")
+    __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "pairs", "device", "_view", "view")
 
     def __init__(self, offsets, order, place, counts, rows, top, groups):
         self.offsets, self.order, self.place, self.counts, self.rows, self.top, self.groups = offsets, order, place, counts, rows, top, groups
-        self.pairs = rows * top
+        self.pairs, self.device = rows * top, offsets.get_device()
         self._view = _RowGroupsView(offsets.data_ptr(), order.data_ptr(), place.data_ptr(), counts.data_ptr(), rows, top, groups)
         self.view = ctypes.addressof(self._view)
 
@@ -2002,7 +2007,7 @@ def group_rows(choice: torch.Tensor, groups: RowGroups) -> None:
     name = "group_rows"
     if choice.dtype != torch.int32 or choice.shape != groups.place.shape:
         _refuse(name, f"int32 choices {tuple(groups.place.shape)}, got {choice.dtype} {tuple(choice.shape)}")
-    _on_current_device(name, choice, groups.offsets)
+    _on_current_device(name, choice.get_device(), groups.device)
     _call("jllm_group_rows", choice.data_ptr(), _row_stride(name, "choice", choice, (groups.rows, groups.top)), groups.view, _stream())
 
 
@@ -2019,10 +2024,10 @@ def gemm_grouped(a, w: PackedBlocks, groups: RowGroups, out: torch.Tensor, swigl
         _refuse(name, f"{rows} rows of {w.cols} {'e4m3' if w.fp8 else 'bfloat16'} values, {groups.groups} weights and a float32 or bfloat16 result, got "
                       f"{type(a).__name__} {tuple(a.shape)}, {w.groups} weights and {out.dtype}")
     if w.fp8:
-        _on_current_device(name, a.data, a.scales, w.data, groups.offsets, out)
+        _on_current_device(name, a.device, w.device, groups.device, out.get_device())
         view = a.view
     else:
-        _on_current_device(name, a, w.data, groups.offsets, out)
+        _on_current_device(name, a.get_device(), w.device, groups.device, out.get_device())
         stride = _row_stride(name, "a", a, (rows, w.cols))
         if a.dtype != torch.bfloat16 or a.data_ptr() % 16 or stride % 8:
             _refuse(name, f"bfloat16 rows that begin at multiples of 16 bytes, got {a.dtype}, stride {stride} at {a.data_ptr():#x}")
@@ -2038,7 +2043,7 @@ def combine_groups(answers: torch.Tensor, groups: RowGroups, share: torch.Tensor
     name = "combine_groups"
     if answers.dtype not in _DT or out.dtype not in _DT or share.dtype != torch.float32 or answers.dim() != 2:
         _refuse(name, f"float32 or bfloat16 answers and result and float32 shares, got {answers.dtype}, {out.dtype} and {share.dtype}")
-    _on_current_device(name, answers, groups.offsets, share, out)
+    _on_current_device(name, answers.get_device(), groups.device, share.get_device(), out.get_device())
     dim = answers.shape[1]
     _call("jllm_combine_groups", answers.data_ptr(), _DT[answers.dtype], _row_stride(name, "answers", answers, (groups.pairs, dim)), groups.view,
           share.data_ptr(), _row_stride(name, "share", share, (groups.rows, groups.top)), out.data_ptr(), _DT[out.dtype],
