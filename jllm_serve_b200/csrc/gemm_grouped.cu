@@ -306,27 +306,32 @@ __device__ __forceinline__ bool produce(const CUtensorMap* map_a, const Args& g,
             tma_load_2d(ring.rows(s_), map_a, kb * 128, unit.first, ring.full(s_));
             for (int t = g.box; t < unit.width; t += g.box) tma_load_2d(ring.rows(s_) + t * 128, map_a, kb * 128, unit.first + t, ring.full(s_));
         };
-        // (of one group the first weights are known in front of the wait, and nobody's output)
+        // The first weights are asked for before anything that has to be waited for: of one group in front of the wait for the kernel in front (they are nobody's
+        // output), of groups in front of where their rows are.
         int i = 0;
         if (!waited) {
-            if (!g.offsets) {
-                const int early = min(ring.stages, share.n_kb);
-                for (; i < early; ++i, w += TILE_BYTES)
-                    if (elect_one()) weights(i);
-                __syncwarp();
-                pdl_wait();
-                for (i = 0; i < early; ++i)
-                    if (elect_one()) rows(i, share.kb_lo + i);
-                __syncwarp();
-                issued = early;
-                s = early == ring.stages ? 0 : early, parity = early == ring.stages ? 0u : 1u;
-            }
+            const int early = min(ring.stages, share.n_kb);
+            for (; i < early; ++i, w += TILE_BYTES)
+                if (elect_one()) weights(i);
+            __syncwarp();
             pdl_wait();
             pdl_trigger();
             waited = true;
+            if (S::GATHER == 0 && g.order) fetch.begin(g, unit, 0);
+            for (i = 0; i < early; ++i) {
+                if (g.order) {
+                    if constexpr (S::GATHER == 0) {
+                        fetch.ask(g, ring, i, 0, share.kb_lo + i);
+                        fetch.asked(ring);
+                    }
+                } else if (elect_one()) rows(i, share.kb_lo + i);
+                __syncwarp();
+            }
+            issued = early;
+            s = early == ring.stages ? 0 : early, parity = early == ring.stages ? 0u : 1u;
+        } else if (S::GATHER == 0 && g.order) {
+            fetch.begin(g, unit, 0);
         }
-        if constexpr (S::GATHER == 0)
-            if (g.order) fetch.begin(g, unit, 0);
         for (; i < share.n_kb; ++i, w += TILE_BYTES) {
             if (!warp_wait(ring.empty(s), parity, abort_flag, 2 * limit)) { ok = false; break; }
             const int kb = share.kb_lo + i;
@@ -1230,17 +1235,17 @@ double wide_count(int rows, int tiles, int k_blocks, int sms) {
     const double busy = units < sms ? (double)units / sms : 1.0, run = rounds * (k_blocks * (0.5 + 0.118 * busy) + 3.38), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
     return 1.27 + (run > read ? run : read);
 }
-// Groups (11,092 sizes: 1 to 2,048 rows of 1 to 8 choices among 4 to 128 groups, 128 to 4,096 weight rows of as many values; 3.5%; by the mean of a group's pairs
-// alone 7%): the host knows neither which groups are asked nor how often, so both are reckoned from even choices, half a span more than the pairs fill.
+// Groups (11,092 sizes: 1 to 2,048 rows of 1 to 8 choices among 4 to 128 groups, 128 to 4,096 weight rows of as many values; 1 to 2% on those that the fit has not seen; by
+// the mean of a group's pairs alone 7%): the host knows neither which groups are asked nor how often, so both are reckoned from even choices, half a span more than the pairs fill.
 struct Grouping {
     double start, k_block, unit, row;
 };
 constexpr int SPANS[4] = {16, 32, 64, 128};
 constexpr Grouping GROUPING[2][2][4] = {          // [e4m3][by pair][span]
-    {{{4.27, 0.265, 0.0, 0.097}, {4.50, 0.274, 0.0, 0.087}, {3.64, 0.505, 1.61, 0.063}, {4.61, 0.432, 3.92, 0.045}},
-     {{3.89, 0.225, 0.0, 0.049}, {3.99, 0.225, 0.0, 0.039}, {4.15, 0.220, 0.0, 0.037}, {4.54, 0.301, 3.27, 0.028}}},
-    {{{4.79, 0.271, 0.0, 0.120}, {3.94, 0.332, 1.47, 0.068}, {2.87, 0.588, 2.87, 0.061}, {1.01, 0.538, 6.81, 0.041}},
-     {{4.37, 0.240, 0.0, 0.097}, {4.60, 0.249, 0.0, 0.073}, {5.37, 0.232, 0.0, 0.059}, {1.30, 0.426, 6.06, 0.028}}}};
+    {{{4.51, 0.263, 0.031, 0.109}, {5.14, 0.264, 0.069, 0.067}, {4.19, 0.645, 0.961, 0.080}, {8.00, 0.327, 4.21, 0.025}},
+     {{3.87, 0.219, 0.023, 0.059}, {3.93, 0.229, 0.051, 0.040}, {4.10, 0.220, 0.022, 0.037}, {7.17, 0.175, 0.02, 0.043}}},
+    {{{4.03, 0.323, 0.026, 0.154}, {3.98, 0.320, 1.88, 0.046}, {4.05, 0.836, 4.39, 0.065}, {3.04, 0.516, 7.90, 0.036}},
+     {{3.76, 0.305, 0.026, 0.132}, {4.58, 0.321, 0.040, 0.075}, {4.75, 0.313, 0.038, 0.072}, {2.24, 0.389, 6.84, 0.020}}}};
 
 // The cut for a product. (Worked out once per size: the choice is kept.)
 Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int tiles, int k_blocks) {
@@ -1270,9 +1275,9 @@ Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int ti
             const Grouping& c = GROUPING[fp8][by_pair][i];
             const int nt = SPANS[i], places = nt == 128 ? sms : 2 * sms;
             const double spans = mean <= 0.5 * nt ? asked : pairs / nt + 0.5 * asked, units = spans * (nt == 128 ? (tiles + 1) / 2 : tiles);
-            const double rounds = units <= sms ? 1.0 : units < places ? 1.0 : units / places, read = asked * tiles * (double)TILE_BYTES * k_blocks / 6e6;
+            const double rounds = units <= sms ? 1.0 : units < places ? 1.0 : units / places, read = asked * tiles * (double)TILE_BYTES * k_blocks / 6.2e6;
             const double run = rounds * (k_blocks * c.k_block + c.unit + c.row * (mean < nt ? mean : nt));
-            offer(c.start + (run > read ? run : read), {nt, nt == 128 ? 2 : 1, 1, nt == 128 ? 1 : 2});
+            offer(c.start + sqrt(sqrt(run * run * run * run + read * read * read * read)), {nt, nt == 128 ? 2 : 1, 1, nt == 128 ? 1 : 2});
         }
     }
     if (known.size() >= 4096) known.clear();
