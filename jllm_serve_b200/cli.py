@@ -24,7 +24,7 @@ DEFAULTS: Dict[str, Tuple[str, str]] = {
     "model.random-weights": ("", "seed: make random weights for --model-config instead of reading a folder"),
     "model.config": ("", "a config.json to use with model.random-weights"),
     "backend.dtype": ("bf16", "bf16 | fp32 (true 32-bit, no tensor cores)"),
-    "backend.weights": ("", "int8: the layers' weights and rows in 8-bit integers (bf16 models of attention and dense feed-forward layers)"),
+    "backend.weights": ("", "int8, fp8: the layers' weights and rows in 8-bit integers or floating point (bf16 models of attention and dense feed-forward layers)"),
     "backend.ctx": ("0", "context length; 0 = the model's max_position_embeddings"),
     "backend.batch": ("512", "rows of one prompt portion (the reference's backend.batch)"),
     "backend.kv-block": ("16", "positions per cache page"),
@@ -147,10 +147,10 @@ class Settings:
     def validate(self) -> "Settings":
         if self.get("backend.dtype") not in ("bf16", "fp32", "bfloat16", "float32"):
             raise SettingsError(f"backend.dtype must be bf16 or fp32, got '{self.get('backend.dtype')}'")
-        if self.get("backend.weights") not in ("", "int8"):
-            raise SettingsError(f"backend.weights must be int8 or empty, got '{self.get('backend.weights')}'")
-        if self.get("backend.weights") == "int8" and self.get("backend.dtype") not in ("bf16", "bfloat16"):
-            raise SettingsError("backend.weights int8 goes with backend.dtype bf16")
+        if self.get("backend.weights") not in ("", "int8", "fp8"):
+            raise SettingsError(f"backend.weights must be int8, fp8 or empty, got '{self.get('backend.weights')}'")
+        if self.get("backend.weights") and self.get("backend.dtype") not in ("bf16", "bfloat16"):
+            raise SettingsError(f"backend.weights {self.get('backend.weights')} goes with backend.dtype bf16")
         self.integer("backend.ctx", 0)
         self.integer("backend.batch", 1)
         self.integer("backend.kv-block", 1)
@@ -191,7 +191,7 @@ USAGE = """usage: jllm <command> [options]
   bench      measure prefill/decode throughput on a synthetic prompt
   config     print the effective configuration and where each value comes from
 options (override with --config <file> or flags):
-  --model <dir>   --random-weights <seed> --model-config <config.json>   --dtype bf16|fp32   --weights int8
+  --model <dir>   --random-weights <seed> --model-config <config.json>   --dtype bf16|fp32   --weights int8|fp8
   --ctx <n>  --batch <n>  --page-size <n>  --num-pages <n|auto>  --kv-share <0..1>  --max-batch-tokens <n>
   --max-running <n>
   --temp <t> --top-k <k> --top-p <p> --min-p <p> --seed <s> --max-tokens <n> --ignore-eos

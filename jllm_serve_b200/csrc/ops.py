@@ -1864,6 +1864,14 @@ class PackedBlocks:
         self._view = _BlockWeight(data.data_ptr(), _p(scales), groups, rows, cols, self.k_blocks, scales.shape[2] if self.fp8 else 0, int(glu))
         self.view = ctypes.addressof(self._view)
 
+    def take_rows(self, lo: int, hi: int) -> "PackedBlocks":
+        """Rows [lo, hi) of a weight that is not packed for gated units, lo a multiple of 128: a view of its tiles."""
+        if self.groups != 1 or self.glu or lo % 128 or not 0 <= lo < hi <= self.rows:
+            _refuse("PackedBlocks", f"rows of one plain weight from a multiple of 128 on, got [{lo}, {hi}) of {self.rows} ({self.groups} weights, glu {self.glu})")
+        tiles = slice(lo // 128, -(-hi // 128))
+        scales = self.scales[:, 16 * tiles.start: 16 * tiles.stop] if self.fp8 else None
+        return PackedBlocks(self.data[:, tiles], scales, 1, hi - lo, self.cols)
+
     def unpack(self) -> torch.Tensor:
         """The [groups, rows, cols] values again (e4m3 without their scales), rows in the order they were packed in (tests)."""
         G, T, KB = self.data.shape[:3]

@@ -63,7 +63,7 @@ class Engine:
         tokens going from one step into the next on the device; the host reads them one step later (what `step_once`
         returns lags by a step; `run_until_done` and `generate` do not care). `fill_portions`: a step whose first prompt
         portion left room in `max_batch_tokens` takes the portions of the next waiting prompts too (False: one portion
-        to a step, as the reference plans its passes). `weights` "int8": the layers' products in 8-bit integers (`ModelRunner`)."""
+        to a step, as the reference plans its passes). `weights` "int8", "fp8": the layers' products in 8-bit integers or floating point (`ModelRunner`)."""
         self.runner = ModelRunner(model_dir, config=config, seed=seed, dtype=dtype, device=device,
                                   page_size=page_size, num_pages=num_pages, max_tokens=max_tokens_cached,
                                   max_batch_tokens=max_batch_tokens, max_requests=max_running, ctx=ctx,

@@ -47,8 +47,8 @@ class DecoderModel:
         self.blocks = []
         for l, layer in enumerate(spec.layers):
             cls = part_class("block", layer.arrangement)
-            if runtime.weights == "int8" and not getattr(cls, "takes_int8", lambda _: False)(layer):
-                raise ConfigError("weights in 8-bit integers are built for layers of an RMS norm in front of attention over heads' keys and "
+            if runtime.weights and not getattr(cls, "takes_int8", lambda _: False)(layer):
+                raise ConfigError(f"weights in 8-bit {'integers' if runtime.weights == 'int8' else 'floating point'} are built for layers of an RMS norm in front of attention over heads' keys and "
                                   f"values and in front of a dense gated feed-forward; layer {l} is another")
             self.blocks.append(cls(layer, core.dim, tensors, cls_prefix(layer, names, l), runtime, self.position_encodings))
         self.final_norm = part_class("norm", spec.final_norm.kind)(spec.final_norm, core.dim, tensors,

@@ -49,15 +49,17 @@ class ModelRunner:
         loaded (never more than `max_requests` full contexts need). `weights` "int8": the layers' weights are rounded to 8-bit integers
         when they are loaded, one scale a row, and the rows that meet them at every step, one scale a token (bfloat16 models of
         attention and dense feed-forward layers; embedding, head, norms and cache stay as they are, and between a layer's products the
-        attention's result and the gated units are bfloat16 before their 8 bits, what is added to the residual float32)."""
+        attention's result and the gated units are bfloat16 before their 8 bits, what is added to the residual float32). "fp8": the same in 8-bit
+        floating point (e4m3), one scale for every 128 x 128 of a weight and for every 128 values of a row; the norms' results are bfloat16 too before
+        their 8 bits."""
         ops.require_device()
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
         self.dtype = _as_dtype(dtype)
-        if weights not in (None, "int8"):
-            raise ValueError(f"weights {weights!r} are not built (int8, or None: as the compute dtype)")
-        if weights == "int8" and self.dtype != torch.bfloat16:
-            raise ValueError("weights in 8-bit integers go with the compute dtype bfloat16")
+        if weights not in (None, "int8", "fp8"):
+            raise ValueError(f"weights {weights!r} are not built (int8, fp8, or None: as the compute dtype)")
+        if weights and self.dtype != torch.bfloat16:
+            raise ValueError("weights in 8 bits go with the compute dtype bfloat16")
         self.weights = weights
         if model_dir is not None:
             spec, raw = load_config(model_dir)
@@ -329,6 +331,6 @@ class ModelRunner:
 
     def describe(self) -> str:
         core = self.spec.core
-        return (f"{core.description} | dtype={str(self.dtype).replace('torch.', '')}{' weights=int8' if self.weights else ''} ctx={self.ctx} "
+        return (f"{core.description} | dtype={str(self.dtype).replace('torch.', '')}{f' weights={self.weights}' if self.weights else ''} ctx={self.ctx} "
                 f"page={self.page_size} pages={self.cache.num_pages} groups={len(self.cache.paged)} "
                 f"max_batch_tokens={self.max_rows}")

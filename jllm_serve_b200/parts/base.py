@@ -35,7 +35,7 @@ class Runtime:
     max_positions: int                     # the context: positions 0 .. max_positions - 1 can be cached
     max_rows: int                          # most rows (tokens) in one step
     page_size: int
-    weights: str = ""                      # "int8": the products of the parts that know it run in 8-bit integers (parts/linear.py)
+    weights: str = ""                      # "int8", "fp8": the products of the parts that know it run in 8-bit integers or floating point (parts/linear.py)
 
     def __post_init__(self):
         self._buffers: Dict[str, torch.Tensor] = {}
@@ -62,6 +62,17 @@ class Runtime:
         if held is None:
             whole = self._int8_rows.get((name, cols, None)) or ops.int8_rows(self.max_rows, cols, self.device)
             self._int8_rows[(name, cols, None)] = whole
+            held = self._int8_rows[key] = whole[:rows]
+        return held
+
+    def fp8_rows(self, name: str, cols: int, rows: int):
+        """The same of rows in 8-bit floating point."""
+        from ..csrc import ops
+        key = ("fp8", name, cols, rows)
+        held = self._int8_rows.get(key)
+        if held is None:
+            whole = self._int8_rows.get(("fp8", name, cols, None)) or ops.fp8_rows(self.max_rows, cols, self.device)
+            self._int8_rows[("fp8", name, cols, None)] = whole
             held = self._int8_rows[key] = whole[:rows]
         return held
 

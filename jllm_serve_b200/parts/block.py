@@ -63,7 +63,7 @@ class PreNormBlock(Block):
 
     @classmethod
     def takes_int8(cls, spec) -> bool:
-        """Whether a layer of this spec runs with its products in 8-bit integers."""
+        """Whether a layer of this spec runs with its products in 8 bits (integers or floating point)."""
         return (cls is PreNormBlock and spec.norm.kind == "rmsnorm" and spec.mixer.kind == "gqa_attention" and not spec.mixer.wide
                 and spec.feed_forward is not None and spec.feed_forward.kind == "dense_glu" and not spec.input_conv
                 and float(getattr(spec, "residual_scale", 1.0)) == 1.0)

@@ -8,7 +8,8 @@ PACKED once, when the part is built (`ops.pack_weight`: tiles of 128 rows x 64 k
 tensor cores read, so a tile is one contiguous bulk copy), and the row-major copy is let go.
 
 With `Runtime.weights` "int8" the layers' products are `Int8Linear`s instead: weight and rows in 8-bit integers, a scale a weight row
-and a scale a token (`ops.gemm_int8`). Half the bytes of a bfloat16 weight, on tensor cores of twice the rate.
+and a scale a token (`ops.gemm_int8`). Half the bytes of a bfloat16 weight, on tensor cores of twice the rate. With "fp8" they are `Fp8Linear`s:
+both in 8-bit floating point, with a scale for every 128 x 128 of a weight and every 128 values of a row (`ops.gemm_fp8`).
 """
 from __future__ import annotations
 
@@ -91,6 +92,36 @@ class Int8Linear:
         ops.gemm_int8(a, self.packed, out, self.bias, ops.EPILOGUE_RELU2 if relu2 else accumulate, swiglu)
 
 
+class Fp8Linear:
+    """`Linear` in 8-bit floating point. The rows come as a norm's or a part's bfloat16 result and are rounded here. `glu`: the weight's rows are all
+    gate rows, then all up rows, for `forward(swiglu=...)`."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, runtime, glu: bool = False):
+        assert weight.dim() == 2
+        self.bias, self.rt = bias, runtime
+        self.out_features, self.in_features = weight.shape
+        self.packed = ops.quantize_weight_fp8(weight, glu)
+
+    def rows(self, lo: int, hi: int) -> "Fp8Linear":
+        """The product with rows [lo, hi) of the weight only (a view of its tiles)."""
+        out = Fp8Linear.__new__(Fp8Linear)
+        out.bias, out.rt = (self.bias[lo:hi] if self.bias is not None else None), self.rt
+        out.out_features, out.in_features = hi - lo, self.in_features
+        out.packed = self.packed.take_rows(lo, hi)
+        return out
+
+    def forward(self, a: torch.Tensor, out: torch.Tensor, accumulate: bool = False, swiglu=False, relu2: bool = False) -> None:
+        """a [rows, in]: float32 or bfloat16 rows; otherwise as `Linear.forward`."""
+        if a.shape[0] == 0:
+            return
+        rows8 = self.rt.fp8_rows("product_input", self.in_features, a.shape[0])
+        ops.quantize_fp8(a, rows8)
+        ops.gemm_fp8(rows8, self.packed, out, self.bias, ops.EPILOGUE_RELU2 if relu2 else accumulate, swiglu)
+
+
+LOW_BIT = {"int8": Int8Linear, "fp8": Fp8Linear}          # what a layer's products are with `Runtime.weights`
+
+
 def layer_linear(weight: torch.Tensor, bias: torch.Tensor | None, runtime):
     """The product of a layer's part with a weight [out, in], as the runtime has them."""
-    return Int8Linear(weight, bias, runtime) if runtime.weights == "int8" else Linear(weight, bias)
+    return LOW_BIT[runtime.weights](weight, bias, runtime) if runtime.weights else Linear(weight, bias)

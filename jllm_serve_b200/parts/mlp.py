@@ -13,7 +13,7 @@ import torch
 from ..csrc import ops
 from ..weights.loader import TensorWant
 from .base import FeedForward, register_feed_forward
-from .linear import Int8Linear, Linear
+from .linear import LOW_BIT, Linear
 
 
 class DenseGlu(FeedForward):
@@ -28,14 +28,15 @@ class DenseGlu(FeedForward):
         self.glu = ops.glu_descriptor(self.activation, self.limit)
         self.overwrite = False                                      # True: the result replaces x instead of being added to it
         gate, up = tensors.pop(prefix + names[0]), tensors.pop(prefix + names[1])
-        if runtime.weights == "int8":
+        if runtime.weights:
             # The units are bfloat16 in front of their 8 bits, as the attention's result is: against a layer of 4,096 x 12,288 without any
             # rounding the result is off by 3.506% with that step and 3.503% without it (256 rows of normal values), and gate, up and
             # units of 2,048 rows take 190 us for 201.
             self.fused = spec.hidden % 8 == 0
-            self.gate_up = Int8Linear(torch.cat([gate, up], dim=0), None, runtime, glu=self.fused)
+            low_bit = LOW_BIT[runtime.weights]
+            self.gate_up = low_bit(torch.cat([gate, up], dim=0), None, runtime, glu=self.fused)
             del gate, up
-            self.down = Int8Linear(tensors.pop(prefix + names[2]), None, runtime)
+            self.down = low_bit(tensors.pop(prefix + names[2]), None, runtime)
             return
         # bfloat16: blocks of 8 gate rows followed by their 8 up rows, so that the product's epilogue holds a
         # gate value and its up value together and applies SwiGLU itself (no [rows, 2 hidden] round trip)

@@ -106,3 +106,22 @@ def test_calls_are_refused_in_front_of_a_launch():
         with pytest.raises(ops.KernelError):
             call()
     assert ops.launch_count == before
+
+
+def test_rows_of_a_packed_weight():
+    w, scale = e4m3(300, 200), torch.rand(3, 2)
+    packed = ops.pack_fp8(w, scale)
+    part = packed.take_rows(128, 290)
+    assert part.shape == (162, 200) and torch.equal(part.unpack()[0].view(torch.uint8), w[128:290].view(torch.uint8)) and torch.equal(part.scales[0, [0, 16], :2], scale[1:])
+    for lo, hi in ((30, 100), (128, 128), (0, 301), (-128, 10)):
+        with pytest.raises(ops.KernelError):
+            packed.take_rows(lo, hi)
+
+
+def test_settings_of_the_command_line(tmp_path):
+    from jllm_serve_b200.cli import Settings, SettingsError
+    load = lambda *args: Settings.load(list(args), env={}, cwd=tmp_path).validate()      # noqa: E731
+    assert load("--weights", "fp8").get("backend.weights") == "fp8"
+    for args in (("--weights", "fp4"), ("--weights", "fp8", "--dtype", "fp32")):
+        with pytest.raises(SettingsError):
+            load(*args)
