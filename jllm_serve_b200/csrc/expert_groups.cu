@@ -263,7 +263,8 @@ JLLM_EXPORT int jllm_group_rows(const int* choice, int ld, const RowGroupsView* 
     const int warps = pairs <= 8 * 32 ? 8 : pairs <= 16 * 32 ? 16 : MOST_WARPS;
     const int run = (int)(((pairs + (long long)blocks * warps - 1) / ((long long)blocks * warps) + 31) / 32 * 32);
     const size_t smem = ((size_t)(warps + 3) * g->groups + (run <= 32 * HELD ? (size_t)warps * run : 0)) * sizeof(int);
-    if (jllm_allow_smem((const void*)group_rows_kernel, smem) != cudaSuccess) return jllm_fail(JLLM_CUDA_ERROR, "group_rows: %zu bytes of shared memory refused", smem);
+    if (smem > 48 * 1024 && jllm_allow_smem((const void*)group_rows_kernel, smem) != cudaSuccess)
+        return jllm_fail(JLLM_CUDA_ERROR, "group_rows: %zu bytes of shared memory refused", smem);
     if (blocks > 1) {
         JLLM_REQUIRE(g->counts, "group_rows: no room for the blocks' counts");
         jllm_launch(count_rows_kernel, dim3(blocks), dim3(1024), 0, stream, LAUNCH_DEPENDENT, choice, ld, g->top, pairs, g->groups, warps * run, g->counts);

@@ -28,6 +28,7 @@
 #include "fp8_view.h"
 #include "tcgen05_common.cuh"
 
+#include <atomic>
 #include <cmath>
 
 namespace {
@@ -1068,6 +1069,7 @@ struct Kind {
     size_t stage, fixed, own;    // bytes of a stage, of barriers and alignment, and what the kernel holds by itself
     int tmem, threads;
     bool clusters;
+    std::atomic<bool>* allowed;  // [64]: by device, whether the kernel may have an SM's shared memory
 };
 
 template <typename Tout>
@@ -1107,8 +1109,14 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
     // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: of a cluster's blocks, which have 256
     // columns at most, no more than two are on an SM (113 KB), nor one beside blocks of another product that together want more than the rest.
     const size_t smem = stages * each + parts + fixed;
-    if (jllm_allow_smem((const void*)kern, smem) != cudaSuccess)
-        return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: %zu bytes of shared memory refused", smem);
+    // (what a kernel may have is asked of the driver once per device, and all of it)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: no device");
+    if (!kind.allowed[dev].load(std::memory_order_relaxed)) {
+        if (cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(227 * 1024 - own)) != cudaSuccess)
+            return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: %zu bytes of shared memory refused", 227 * 1024 - own);
+        kind.allowed[dev].store(true, std::memory_order_relaxed);
+    }
     const long long at_once = (long long)sms * cut.per_sm, grid = cut.blocks > 1 ? units * cut.blocks : units < at_once ? units : at_once;
     JLLM_REQUIRE(g.starve == STARVE_NOTHING || (grid <= 64 && (g.starve != STARVE_PARTS || cut.blocks > 1)),
                  "gemm_grouped: the starved product of the wait test has at most 64 blocks, and a cluster where parts are missed");
@@ -1148,14 +1156,16 @@ int launch_narrow(const Product& p, const Cut& cut) {
     using S = Narrow<FP8, NT>;
     auto kern = gemm_grouped_narrow_kernel<FP8, NT, GLU, Tout>;
     static const size_t own = own_smem((const void*)kern);
-    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, S::CLUSTERS}, p, cut);
+    static std::atomic<bool> allowed[64];
+    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, S::CLUSTERS, allowed}, p, cut);
 }
 template <bool FP8, bool GLU, typename Tout>
 int launch_wide(const Product& p, const Cut& cut) {
     using S = Wide<FP8>;
     auto kern = gemm_grouped_wide_kernel<FP8, GLU, Tout>;
     static const size_t own = own_smem((const void*)kern, S::LAUNCHED);          // (what the warps hand over has to be there)
-    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, false}, p, cut);
+    static std::atomic<bool> allowed[64];
+    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, false, allowed}, p, cut);
 }
 
 template <bool FP8, bool GLU, typename Tout>
@@ -1249,15 +1259,17 @@ constexpr Grouping GROUPING[2][2][4] = {          // [e4m3][by pair][span]
 
 // The cut for a product. (Worked out once per size: the choice is kept.)
 Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int tiles, int k_blocks) {
-    static std::mutex mu;
-    static std::unordered_map<MapKey, Cut, MapKeyHash> known;
+    struct Known {
+        MapKey key;
+        Cut cut;
+    };
+    static thread_local Known known[256];          // (a place for every size: another size there takes it)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return {16, 1, 1, 2};
-    const MapKey key{nullptr, rows, (long long)tiles << 32 | (unsigned)k_blocks, groups ? (long long)groups->groups << 32 | (unsigned)groups->top : 0,
+    const MapKey key{nullptr, rows + 1, (long long)tiles << 32 | (unsigned)k_blocks, groups ? (long long)groups->groups << 32 | (unsigned)groups->top : 0,
                      dev << 2 | (int)fp8 << 1 | (int)by_pair};
-    std::lock_guard<std::mutex> lock(mu);
-    const auto it = known.find(key);
-    if (it != known.end()) return it->second;
+    Known& place = known[MapKeyHash()(key) % 256];
+    if (place.key == key) return place.cut;
     const int sms = jllm_device_sm_count();
     Cut best{16, 1, 1, 2};
     double least = 1e30;
@@ -1280,8 +1292,8 @@ Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int ti
             offer(c.start + sqrt(sqrt(run * run * run * run + read * read * read * read)), {nt, nt == 128 ? 2 : 1, 1, nt == 128 ? 1 : 2});
         }
     }
-    if (known.size() >= 4096) known.clear();
-    return known[key] = best;
+    place = {key, best};
+    return best;
 }
 
 // A test of the waits: what the next product of this thread is to miss, and how long its waits last.

@@ -1781,14 +1781,9 @@ class _RowGroupsView(ctypes.Structure):
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on_current_device(name, *devices):
+def _elsewhere(name, *devices):
     """The launchers run on the current device's current stream: what they are given lies there. `devices`: what `Tensor.get_device` says."""
-    first = devices[0]
-    for d in devices:
-        if d != first or d < 0:
-            _refuse(name, f"everything lies on one CUDA device, got {devices} (-1: none)")
-    if first != _current_device():
-        _refuse(name, f"everything lies on the current CUDA device, got device {first}")
+    _refuse(name, f"everything lies on the current CUDA device, got devices {devices} (-1: none)")
 
 
 class Fp8Rows:
@@ -1837,7 +1832,8 @@ def quantize_fp8(x: torch.Tensor, out: Fp8Rows) -> None:
     name = "quantize_fp8"
     if x.dtype not in _DT:
         _refuse(name, f"float32 or bfloat16 rows, got {x.dtype}")
-    _on_current_device(name, x.get_device(), out.device)
+    if not 0 <= x.get_device() == out.device == _current_device():
+        _elsewhere(name, x.get_device(), out.device)
     _call("jllm_quantize_fp8", x.data_ptr(), _DT[x.dtype], _row_stride(name, "x", x, out.shape), out.view, _stream())
 
 
@@ -1846,7 +1842,8 @@ def fp8_values(rows8: Fp8Rows, out: torch.Tensor) -> torch.Tensor:
     name = "fp8_values"
     if out.dtype not in _DT:
         _refuse(name, f"float32 or bfloat16 values, got {out.dtype}")
-    _on_current_device(name, out.get_device(), rows8.device)
+    if not 0 <= out.get_device() == rows8.device == _current_device():
+        _elsewhere(name, out.get_device(), rows8.device)
     _call("jllm_fp8_values", rows8.view, out.data_ptr(), _DT[out.dtype], _row_stride(name, "out", out, rows8.shape), _stream())
     return out
 
@@ -1896,7 +1893,8 @@ def _pack_bytes(name, w: torch.Tensor, glu: bool) -> torch.Tensor:
         padded[:, :N, :K] = torch.stack([_glu_order(one) for one in w]) if glu else w
         tiles = padded.view(G * T, 128, KB, 8, 16).permute(0, 2, 1, 3, 4)
         return tiles.gather(3, _swizzle_index(w.device).expand(G * T, KB, 128, 8, 16)).contiguous().view(G, T, KB, 128, 128)
-    _on_current_device(name, w.get_device())
+    if w.get_device() != _current_device():
+        _elsewhere(name, w.get_device())
     packed = torch.empty((G, T, KB, 128, 128), dtype=torch.int8, device=w.device)
     for g in range(G):
         _call("jllm_pack_int8", w[g].data_ptr(), K, N, K, int(glu), packed[g].data_ptr(), _stream())
@@ -1965,16 +1963,18 @@ def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor 
     [rows, w.rows / 2]. The weight, its scales and the bias are read before what is in front on the stream has ended: not what a kernel right in front
     writes. `cut` (tests): tokens of a span x 1,000, 128-row tiles of a unit x 100, blocks an SM x 10, blocks of a cluster; 0: as the sizes have it."""
     name = "gemm_fp8"
-    word = _product_words(name, w, swiglu)
+    word = _product_words(name, w, swiglu) if swiglu or w.glu else 0
     if not w.fp8 or w.groups != 1 or a.cols != w.cols or out.dtype not in _DT:
         _refuse(name, f"e4m3 rows and one e4m3 weight of {w.cols} columns and a float32 or bfloat16 result, got {a.cols} columns, {w.groups} weights and {out.dtype}")
-    _on_current_device(name, a.device, w.device, out.get_device())
+    if not 0 <= a.device == w.device == out.get_device() == _current_device():
+        _elsewhere(name, a.device, w.device, out.get_device())
     if bias is None:
         b, b_dtype = 0, F32
     else:
         if bias.shape != (w.rows,) or bias.dtype not in _DT or not bias.is_contiguous():
             _refuse(name, f"a bias of {w.rows} float32 or bfloat16 values, got {bias.dtype} {tuple(bias.shape)}")
-        _on_current_device(name, bias.get_device(), w.device)
+        if bias.get_device() != w.device:
+            _elsewhere(name, bias.get_device(), w.device)
         b, b_dtype = bias.data_ptr(), _DT[bias.dtype]
     _call("jllm_gemm_grouped", a.view, w.view, 0, 0, b, b_dtype, out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (a.rows, w.rows // 2 if word else w.rows)), int(accumulate), word, cut, _stream())
@@ -1984,11 +1984,11 @@ class RowGroups:
     """The (row, choice) pairs of a step in the order of the groups (experts) they ask: group g's pairs are order[offsets[g]] .. order[offsets[g + 1] - 1],
     each r * top + c of its row r and choice c, in ascending order; `order` is -1 behind the last pair. place[r, c] is where the pair (r, c) lies, -1 if it
     asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs."""
-    __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "pairs", "device", "_view", "view")
+    __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "shape", "pairs", "device", "_view", "view")
 
     def __init__(self, offsets, order, place, counts, rows, top, groups):
         self.offsets, self.order, self.place, self.counts, self.rows, self.top, self.groups = offsets, order, place, counts, rows, top, groups
-        self.pairs, self.device = rows * top, offsets.get_device()
+        self.shape, self.pairs, self.device = (rows, top), rows * top, offsets.get_device()
         self._view = _RowGroupsView(offsets.data_ptr(), order.data_ptr(), place.data_ptr(), counts.data_ptr(), rows, top, groups)
         self.view = ctypes.addressof(self._view)
 
@@ -2013,10 +2013,11 @@ def group_rows(choice: torch.Tensor, groups: RowGroups) -> None:
     """Fills `groups` from choice int32 [rows, top], any row stride: the group that each row asks with each of its choices; anything outside [0, groups) asks
     nobody (the rows that fill a batch up, an entry without weights)."""
     name = "group_rows"
-    if choice.dtype != torch.int32 or choice.shape != groups.place.shape:
-        _refuse(name, f"int32 choices {tuple(groups.place.shape)}, got {choice.dtype} {tuple(choice.shape)}")
-    _on_current_device(name, choice.get_device(), groups.device)
-    _call("jllm_group_rows", choice.data_ptr(), _row_stride(name, "choice", choice, (groups.rows, groups.top)), groups.view, _stream())
+    if choice.dtype != torch.int32:
+        _refuse(name, f"int32 choices {groups.shape}, got {choice.dtype}")
+    if not 0 <= choice.get_device() == groups.device == _current_device():
+        _elsewhere(name, choice.get_device(), groups.device)
+    _call("jllm_group_rows", choice.data_ptr(), _row_stride(name, "choice", choice, groups.shape), groups.view, _stream())
 
 
 def gemm_grouped(a, w: PackedBlocks, groups: RowGroups, out: torch.Tensor, swiglu=False, by_pair: bool = False, cut: int = 0) -> None:
@@ -2026,21 +2027,22 @@ def gemm_grouped(a, w: PackedBlocks, groups: RowGroups, out: torch.Tensor, swigl
     act(gate) * up) float32 or bfloat16, any row stride; rows behind the last pair stay as they were. Only weights that are asked are read. `cut` (tests) as
     in `gemm_fp8`, without clusters."""
     name = "gemm_grouped"
-    word = _product_words(name, w, swiglu)
+    word = _product_words(name, w, swiglu) if swiglu or w.glu else 0
     rows = groups.pairs if by_pair else groups.rows
-    if w.groups != groups.groups or isinstance(a, Fp8Rows) != w.fp8 or tuple(a.shape) != (rows, w.cols) or out.dtype not in _DT:
+    if w.groups != groups.groups or isinstance(a, Fp8Rows) != w.fp8 or a.shape != (rows, w.cols) or out.dtype not in _DT:
         _refuse(name, f"{rows} rows of {w.cols} {'e4m3' if w.fp8 else 'bfloat16'} values, {groups.groups} weights and a float32 or bfloat16 result, got "
                       f"{type(a).__name__} {tuple(a.shape)}, {w.groups} weights and {out.dtype}")
     if w.fp8:
-        _on_current_device(name, a.device, w.device, groups.device, out.get_device())
-        view = a.view
+        device, view = a.device, a.view
     else:
-        _on_current_device(name, a.get_device(), w.device, groups.device, out.get_device())
+        device = a.get_device()
         stride = _row_stride(name, "a", a, (rows, w.cols))
         if a.dtype != torch.bfloat16 or a.data_ptr() % 16 or stride % 8:
             _refuse(name, f"bfloat16 rows that begin at multiples of 16 bytes, got {a.dtype}, stride {stride} at {a.data_ptr():#x}")
         held = _BlockRows(a.data_ptr(), 0, 2 * stride, rows, w.cols, 0)
         view = ctypes.addressof(held)
+    if not 0 <= device == w.device == groups.device == out.get_device() == _current_device():
+        _elsewhere(name, device, w.device, groups.device, out.get_device())
     _call("jllm_gemm_grouped", view, w.view, groups.view, int(by_pair), 0, F32, out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (groups.pairs, w.rows // 2 if word else w.rows)), 0, word, cut, _stream())
 
@@ -2051,10 +2053,11 @@ def combine_groups(answers: torch.Tensor, groups: RowGroups, share: torch.Tensor
     name = "combine_groups"
     if answers.dtype not in _DT or out.dtype not in _DT or share.dtype != torch.float32 or answers.dim() != 2:
         _refuse(name, f"float32 or bfloat16 answers and result and float32 shares, got {answers.dtype}, {out.dtype} and {share.dtype}")
-    _on_current_device(name, answers.get_device(), groups.device, share.get_device(), out.get_device())
+    if not 0 <= answers.get_device() == groups.device == share.get_device() == out.get_device() == _current_device():
+        _elsewhere(name, answers.get_device(), groups.device, share.get_device(), out.get_device())
     dim = answers.shape[1]
     _call("jllm_combine_groups", answers.data_ptr(), _DT[answers.dtype], _row_stride(name, "answers", answers, (groups.pairs, dim)), groups.view,
-          share.data_ptr(), _row_stride(name, "share", share, (groups.rows, groups.top)), out.data_ptr(), _DT[out.dtype],
+          share.data_ptr(), _row_stride(name, "share", share, groups.shape), out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (groups.rows, dim)), dim, int(bool(accumulate)), _stream())
 
 
