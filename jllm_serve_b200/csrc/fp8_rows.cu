@@ -21,7 +21,7 @@ namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;      // 2^-100
 constexpr float kMost = 448.f;
-constexpr int THREADS = 256, AT_A_TIME = 4;      // blocks of a half warp: neighbours in a row
+constexpr int THREADS = 128, AT_A_TIME = 4;      // blocks of a half warp: neighbours in a row
 
 // Eight neighbouring values of a lane, as they are stored.
 template <typename T> struct Eight;
@@ -241,16 +241,20 @@ __global__ void __launch_bounds__(THREADS) fp8_values_kernel(const uint8_t* __re
     }
 }
 
-// Blocks of threads for `items` threads' work: as many as the SMs hold, or fewer.
-int grid_for(long long items, int per_block) {
-    const long long all = (items + per_block - 1) / per_block, most = (long long)jllm_device_sm_count() * 8;
-    return (int)(all < most ? all : most > 0 ? most : 1);
+// Blocks of threads for `items` half warps' work.
+int grid_for(long long items) {
+    const long long all = (items + THREADS / 16 - 1) / (THREADS / 16);
+    return (int)(all < 0x7fffffff ? all : 0x7fffffff);
 }
 
-// A row's blocks in equal chunks of up to AT_A_TIME.
+// A row's blocks in equal chunks: of up to AT_A_TIME, or, where that leaves SMs without a half warp, single ones (8 x 4,096 2.1 -> 1.5 us).
 struct Chunks {
     int blocks, chunks, per;
-    explicit Chunks(int cols) : blocks((cols + 127) / 128), chunks((blocks + AT_A_TIME - 1) / AT_A_TIME), per((blocks + chunks - 1) / chunks) {}
+    Chunks(int rows, int cols) : blocks((cols + 127) / 128) {
+        const int most = (long long)rows * blocks <= 16LL * jllm_device_sm_count() ? 1 : AT_A_TIME;
+        chunks = (blocks + most - 1) / most;
+        per = (blocks + chunks - 1) / chunks;
+    }
 };
 
 int check(const char* name, const BlockRows* r) {
@@ -267,10 +271,10 @@ JLLM_EXPORT int jllm_quantize_fp8(const void* x, int dtype, long long ldx, const
     if (rc != JLLM_OK) return rc;
     JLLM_REQUIRE(ldx >= out->cols, "quantize_fp8: rows of %d values, %lld apart", out->cols, ldx);
     if (out->rows == 0) return JLLM_OK;
-    const Chunks c(out->cols);
+    const Chunks c(out->rows, out->cols);
     const int size = dtype == JLLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)x % 16) == 0 && ldx * size % 16 == 0;
-    const dim3 grid(grid_for((long long)out->rows * c.chunks, THREADS / 16));
+    const dim3 grid(grid_for((long long)out->rows * c.chunks));
     uint8_t* q = static_cast<uint8_t*>(const_cast<void*>(out->data));
     float* scale = const_cast<float*>(out->scale);
     if (dtype == JLLM_F32)
@@ -287,10 +291,10 @@ JLLM_EXPORT int jllm_fp8_values(const BlockRows* rows, void* out, int dtype, lon
     if (rc != JLLM_OK) return rc;
     JLLM_REQUIRE(ldo >= rows->cols, "fp8_values: rows of %d values, %lld apart", rows->cols, ldo);
     if (rows->rows == 0) return JLLM_OK;
-    const Chunks c(rows->cols);
+    const Chunks c(rows->rows, rows->cols);
     const int size = dtype == JLLM_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)out % 16) == 0 && ldo * size % 16 == 0;
-    const dim3 grid(grid_for((long long)rows->rows * c.chunks, THREADS / 16));
+    const dim3 grid(grid_for((long long)rows->rows * c.chunks));
     const uint8_t* q = static_cast<const uint8_t*>(rows->data);
     if (dtype == JLLM_F32)
         jllm_launch(fp8_values_kernel<float>, grid, dim3(THREADS), 0, stream, LAUNCH_DEPENDENT, q, rows->stride, rows->scale, rows->scale_ld, static_cast<float*>(out), ldo,
