@@ -1,6 +1,6 @@
 """Times the hand-written kernels alone on the layer shapes of a model, against their rooflines.
 
-    python -m jllm_serve_b200.kernel_bench [--rows 8] [--prompt 2048] [--context 4096] [--repeat 20] [--only NAME] [--eager] [--int8]
+    python -m jllm_serve_b200.kernel_bench [--rows 8] [--prompt 2048] [--context 4096] [--repeat 20] [--only NAME] [--eager] [--int8] [--fp8] [--experts]
 
 Every kernel runs on random tensors of the shapes one layer of the Qwen3-8B configuration gives it
 (hidden 4096, 32/8 heads of 128, intermediate 12288), timed with CUDA events over `--repeat` calls (replayed
@@ -8,7 +8,8 @@ as one CUDA graph unless `--eager`) that rotate through several copies of the we
 them from HBM. It prints, per kernel,
 microseconds per call and the achieved GB/s (weight or cache bytes, the decode kernels) or TFLOP/s (the
 prefill kernels). With `--repeat 1` it is the small workload that profilers are pointed at. `--int8`: the layer's linears in 8-bit
-integers instead (products, norms and quantised rows of both steps).
+integers instead (products, norms and quantised rows of both steps). `--fp8`: the same in 8-bit floating point. `--experts`: a layer of 128 routed
+experts (2048 x 768, eight a row) instead, bfloat16 and in 8-bit floating point: grouping, both products, the answers' sum.
 """
 from __future__ import annotations
 
@@ -44,6 +45,8 @@ def main() -> int:
                     help="the products of the prefill step also on every product kernel that takes their shape, not only "
                          "on the one the dispatch chooses")
     ap.add_argument("--int8", action="store_true", help="the layer's linears in 8-bit integers, and nothing else")
+    ap.add_argument("--fp8", action="store_true", help="the layer's linears in 8-bit floating point, and nothing else")
+    ap.add_argument("--experts", action="store_true", help="a layer of routed experts, and nothing else")
     args = ap.parse_args()
 
     from .csrc import ops
@@ -68,6 +71,11 @@ def main() -> int:
 
     if args.int8:
         int8_cases(ops, case, args, dev, (M, T), D, (H + 2 * Hkv) * hd, F)
+    if args.fp8:
+        fp8_cases(ops, case, args, dev, (M, T), D, (H + 2 * Hkv) * hd, F)
+    if args.experts:
+        expert_cases(ops, case, args, dev, (M, T))
+    if args.int8 or args.fp8 or args.experts:
         run_cases(cases, args)
         ops.check_kernel_errors()
         return 0
@@ -199,6 +207,60 @@ def int8_cases(ops, case, args, dev, steps, D, qkv, F) -> None:
         hs = [torch.randn(rows, F, device=dev).bfloat16() for _ in range(copies)]
         h8 = [ops.int8_rows(rows, F, dev) for _ in hs]
         case(f"{step} int8 quantise units", lambda i, hs=hs, h8=h8: ops.quantize_int8(hs[i], h8[i]), copies, rows * F * 3)
+
+
+def fp8_cases(ops, case, args, dev, steps, D, qkv, F) -> None:
+    """The linears of one layer in 8-bit floating point, at a decode step's rows and a prompt's, with the results that a layer gives them."""
+    def weights(n, k, glu=False):
+        copies = max(2, int(300e6 // (n * k)) + 1) if args.repeat > 1 else 1
+        return [ops.quantize_weight_fp8(torch.randn(n, k, device=dev) * k ** -0.5, glu) for _ in range(copies)]
+
+    named = {"qkv": weights(qkv, D), "o (+= residual)": weights(D, D), "gate_up + swiglu": weights(2 * F, D, True), "down (+= residual)": weights(D, F)}
+    for step, rows in zip(("decode", "prefill"), steps):
+        for what, ws in named.items():
+            n, k = ws[0].shape
+            a = ops.fp8_rows(rows, k, dev)
+            ops.quantize_fp8(torch.randn(rows, k, device=dev), a)
+            glu, add = ws[0].glu, what.endswith("residual)")
+            out = torch.zeros(rows, n // 2 if glu else n, device=dev, dtype=torch.float32 if add else torch.bfloat16)
+            size = dict(bytes_=n * k) if step == "decode" else dict(flops=2 * rows * n * k)
+            case(f"{step} fp8 gemm {what}", lambda i, a=a, ws=ws, out=out, glu=glu, add=add: ops.gemm_fp8(a, ws[i], out, accumulate=add, swiglu=glu),
+                 len(ws), **size)
+        for what, cols in (("normed rows", D), ("units", F)):
+            copies = max(2, int(300e6 // (rows * cols * 3)) + 1) if step == "prefill" and args.repeat > 1 else 1
+            xs = [torch.randn(rows, cols, device=dev).bfloat16() for _ in range(copies)]
+            x8 = [ops.fp8_rows(rows, cols, dev) for _ in xs]
+            case(f"{step} fp8 quantise {what}", lambda i, xs=xs, x8=x8: ops.quantize_fp8(xs[i], x8[i]), copies, rows * cols * 3)
+
+
+def expert_cases(ops, case, args, dev, steps) -> None:
+    """A layer of 128 experts of 768 units over 2,048 values, eight a row by even chance."""
+    E, top, D, F = 128, 8, 2048, 768
+    copies = 2 if args.repeat > 1 else 1
+    gu, dn = torch.randn(E, 2 * F, D, device=dev) * D ** -0.5, torch.randn(E, D, F, device=dev) * F ** -0.5
+    kinds = {"bf16": [(ops.pack_grouped(gu.bfloat16(), True), ops.pack_grouped(dn.bfloat16())) for _ in range(copies)],
+             "fp8": [(ops.quantize_weight_fp8(gu, True), ops.quantize_weight_fp8(dn)) for _ in range(copies)]}
+    del gu, dn
+    for step, rows in zip(("decode", "prefill"), steps):
+        choice = torch.rand(rows, E, device=dev).topk(top, dim=1).indices.int()
+        groups, share = ops.row_groups(rows, top, E, dev), torch.rand(rows, top, device=dev)
+        ops.group_rows(choice, groups)
+        asked = int((groups.offsets[1:] > groups.offsets[:-1]).sum())
+        case(f"{step} experts grouping", lambda i, c=choice, g=groups: ops.group_rows(c, g), 1, 12 * rows * top)
+        x, answers, out = torch.randn(rows, D, device=dev).bfloat16(), torch.randn(rows * top, D, device=dev), torch.empty(rows, D, device=dev)
+        for kind, ws in kinds.items():
+            size = 1 if kind == "fp8" else 2
+            units = torch.randn(rows * top, F, device=dev).to(torch.float32 if kind == "fp8" else torch.bfloat16)
+            a, u = x, units
+            if kind == "fp8":
+                a, u = ops.fp8_rows(rows, D, dev), ops.fp8_rows(rows * top, F, dev)
+                ops.quantize_fp8(x, a)
+                ops.quantize_fp8(units, u)
+            def work(n, k):      # noqa: E306
+                return dict(bytes_=asked * n * k * size) if step == "decode" else dict(flops=2 * rows * top * n * k)
+            case(f"{step} experts {kind} gate_up + swiglu", lambda i, a=a, ws=ws, g=groups, o=units: ops.gemm_grouped(a, ws[i][0], g, o, swiglu="silu"), copies, **work(2 * F, D))
+            case(f"{step} experts {kind} down", lambda i, u=u, ws=ws, g=groups, o=answers: ops.gemm_grouped(u, ws[i][1], g, o, by_pair=True), copies, **work(D, F))
+        case(f"{step} experts sum", lambda i, a=answers, g=groups, s=share, o=out: ops.combine_groups(a, g, s, o), 1, rows * top * D * 4)
 
 
 def run_cases(cases, args) -> None:
