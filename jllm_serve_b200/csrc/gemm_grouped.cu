@@ -851,7 +851,9 @@ __device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, uint8_t* 
     }
 }
 
-template <bool FP8, bool GLU, typename Tout>
+// CLUSTER: two or four blocks share a unit's k blocks (one unit a cluster). When all have theirs, the rings are idle: each block finishes a part of the unit's
+// columns, the others send theirs of it into its ring.
+template <bool FP8, bool GLU, bool CLUSTER, typename Tout>
 __global__ void __launch_bounds__(Wide<FP8>::THREADS, 1)
 gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Args g, Tout* __restrict__ out) {
     using S = Wide<FP8>;
@@ -859,14 +861,14 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     __shared__ __align__(16) uint8_t parks[S::EPILOGUE][WIDE_PARK];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_word;
-    const Share share(g);               // (blocks by themselves)
+    const Share share(g);
     Ring<S> ring;
     ring.base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     ring.stages = g.stages;
     ring.bars = ring.base + (uint32_t)g.stages * S::STAGE;
     int* before = reinterpret_cast<int*>(smem_raw + (ring.parts() + 8 - smem_u32(smem_raw)));
     int* at = before + g.groups + 1;
-    const int n_kb = g.k_blocks;
+    const int n_kb = share.n_kb;
     const unsigned long long limit = g.limit_us ? g.limit_us * 1000ull : WAIT_NS;
     volatile int* abort_flag = &abort_word;
     auto give_up = [&](int code) {
@@ -874,7 +876,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         __threadfence();               // (before anybody follows the flag and has a code of his own)
         *abort_flag = 1;
     };
-    const uint32_t tmem_base = begin<S>(g, ring, blockIdx.x, before, at, &tmem_base_slot, &abort_word);
+    const uint32_t tmem_base = begin<S>(g, ring, CLUSTER ? share.rank : (int)blockIdx.x, before, at, &tmem_base_slot, &abort_word);
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     Units<S> units(g, before, at);
@@ -885,6 +887,10 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (warp == 0) ok = produce<S>(&map_a, g, ring, units, share, abort_flag, limit, issued, [&] { give_up(41); });
         else if (warp == 1) ok = multiply<FP8, true, S>(g, ring, units, share, tmem_base, abort_flag, limit, issued, [&] { give_up(42); });
         else if (g.order) ok = fetch_rows<S>(g, ring, units, (warp - S::GATHER) * S::GATHER_ROWS, abort_flag, limit, [&] { give_up(41); });
+        if constexpr (CLUSTER) {
+            cluster_arrive();          // (the rings are idle when everybody is here)
+            cluster_wait();
+        }
     } else {
         // ---------------- epilogue: TMEM lanes 32 * (warp % 4) = the unit's pairs, columns 64 * set on ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::MANY));
@@ -942,8 +948,8 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sums[j] = 0;
                 const bool has = token < unit.here;
-                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? g.order[unit.first + token] / g.top : unit.first + token) : 0) * g.sa_ld;
-                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld;
+                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? g.order[unit.first + token] / g.top : unit.first + token) : 0) * g.sa_ld + share.kb_lo;
+                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld + share.kb_lo;
                 // of gate and up rows in eights: the gates' scale, and the up rows' in front of and behind the edge of their block of 128
                 const int edge = GLU ? ((128 - ((last + tile * 64) & 127)) >> 3) - (set & 1) * 4 : 0;
                 float sa = has ? sa_row[0] : 0.f, sw[GLU ? 3 : 1];
@@ -981,7 +987,49 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (lane == 0) mbar_arrive(ring.taken(buffer));
                     if (++buffer == S::BUFFERS) { buffer = 0; parity ^= 1u; }
                 }
-                if (ok && mine)
+                if constexpr (CLUSTER) {
+                    // the unit's 16 chunks of 16 columns in order, `per` to a block; a warp's four are one block's
+                    const int blocks = g.blocks, rank = share.rank, per = 16 / blocks, owner = set * 4 / per;
+                    if (warp == S::FIRST && lane == 0) {
+                        const int there = unit.tile + 1 < g.tiles ? per : min(per, max(0, 8 - rank * per));          // (a second tile may be missing)
+                        mbar_expect_tx(ring.parts(), (uint32_t)((blocks - 1) * there * unit.here) * 64u);
+                    }
+                    cluster_arrive();
+                    cluster_wait();
+                    // [block that sends][chunk][4 columns' place][pair]: 16 bytes
+                    if (ok && mine && owner != rank) {
+                        const uint32_t to = in_block(ring.base + (uint32_t)((rank - (rank > owner ? 1 : 0)) * per + set * 4 - owner * per) * 8192u + (uint32_t)token * 16u, owner);
+                        const uint32_t bar = in_block(ring.parts(), owner);
+                        if (lane < rows)
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) {
+                                float v[4];
+                                halves(sums[2 * q], v[0], v[1]);
+                                halves(sums[2 * q + 1], v[2], v[3]);
+                                asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                                             ::"r"(to + (uint32_t)q * 2048u), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+                                               "r"(__float_as_uint(v[3])), "r"(bar)
+                                             : "memory");
+                            }
+                    }
+                    if (ok && mine && owner == rank) ok = __all_sync(0xffffffffu, wait_cluster(ring.parts(), 0, abort_flag, 2 * limit));
+                    if (ok && mine && owner == rank) {
+                        const uint8_t* parts = smem_raw + (ring.base - smem_u32(smem_raw)) + (size_t)(set * 4 - owner * per) * 8192 + token * 16;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float v[16];
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) halves(sums[8 * c + q], v[2 * q], v[2 * q + 1]);
+                            for (int p = 0; p < blocks - 1; ++p)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const float4 x = *reinterpret_cast<const float4*>(parts + (size_t)p * per * 8192 + (4 * c + q) * 2048);
+                                    v[4 * q] += x.x, v[4 * q + 1] += x.y, v[4 * q + 2] += x.z, v[4 * q + 3] += x.w;
+                                }
+                            finish(v, c);
+                        }
+                    }
+                } else if (ok && mine) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         float v[16];
@@ -989,6 +1037,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                         for (int q = 0; q < 8; ++q) halves(sums[8 * c + q], v[2 * q], v[2 * q + 1]);
                         finish(v, c);
                     }
+                }
             } else {
                 ok = __all_sync(0xffffffffu, mbar_wait(ring.sums(buffer), parity, abort_flag, 2 * limit));
                 if (!ok) break;
@@ -1014,7 +1063,13 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         if (!ok && lane == 0) give_up(43);
     }
-    finish_block<S>(ring, ok, issued, tmem_base, limit);
+    [[maybe_unused]] const bool gave_up = finish_block<S>(ring, ok, issued, tmem_base, limit);
+    // No block of a cluster leaves before everything sent to it is there: its memory is the next block's at once.
+    if constexpr (CLUSTER) {
+        cluster_arrive();
+        cluster_wait();
+        if (gave_up) drain(ring.parts(), 0, now_ns(), limit);
+    }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
@@ -1068,7 +1123,8 @@ struct Kind {
     int rows, tiles;             // of a unit
     size_t stage, fixed, own;    // bytes of a stage, of barriers and alignment, and what the kernel holds by itself
     int tmem, threads;
-    bool clusters;
+    int clusters;                // blocks of one at most (0: none)
+    bool parts_in_ring;          // what a cluster's blocks send one another lies in their rings, which are idle then (else behind them)
     std::atomic<bool>* allowed;  // [64]: by device, whether the kernel may have an SM's shared memory
 };
 
@@ -1086,10 +1142,10 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
     const int span = (int)(((g.rows + spans - 1) / spans + 15) / 16 * 16), most_rows = g.rows < span ? g.rows : span;
     g.spans = (int)spans, g.span = span;
     g.share = cut.blocks > 1 ? ((most_rows + 7) / 8 + cut.blocks - 1) / cut.blocks * 8 : 0;
-    JLLM_REQUIRE(cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= g.k_blocks && (cut.blocks == 1 || (kind.clusters && !g.offsets)),
+    JLLM_REQUIRE(cut.blocks >= 1 && cut.blocks <= 8 && cut.blocks <= g.k_blocks && (cut.blocks == 1 || (cut.blocks <= kind.clusters && !g.offsets && (!kind.parts_in_ring || 16 % cut.blocks == 0))),
                  "gemm_grouped: no clusters of %d blocks for such a product", cut.blocks);
     // An SM has 228 KB, a block 227 at most; each block's last KB is the system's, `own` what the kernel holds by itself.
-    const size_t lists = g.offsets ? 8 * (size_t)(g.groups + 1) : 0, parts = cut.blocks > 1 ? (size_t)cut.blocks * g.share * 512 : 0, fixed = kind.fixed + lists, each = kind.stage + 16;
+    const size_t lists = g.offsets ? 8 * (size_t)(g.groups + 1) : 0, parts = cut.blocks > 1 && !kind.parts_in_ring ? (size_t)cut.blocks * g.share * 512 : 0, fixed = kind.fixed + lists, each = kind.stage + 16;
     const size_t own = kind.own;
     const size_t all = cut.per_sm == 1 ? 227 * 1024 : 113 * 1024;
     JLLM_REQUIRE((cut.per_sm == 1 || cut.per_sm == 2) && kind.tmem * cut.per_sm <= 512 && own + fixed + parts + (FETCHED + 1) * each <= all,
@@ -1157,15 +1213,16 @@ int launch_narrow(const Product& p, const Cut& cut) {
     auto kern = gemm_grouped_narrow_kernel<FP8, NT, GLU, Tout>;
     static const size_t own = own_smem((const void*)kern);
     static std::atomic<bool> allowed[64];
-    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, S::CLUSTERS, allowed}, p, cut);
+    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, S::CLUSTERS ? 8 : 0, false, allowed}, p, cut);
 }
-template <bool FP8, bool GLU, typename Tout>
+template <bool FP8, bool GLU, bool CLUSTER, typename Tout>
 int launch_wide(const Product& p, const Cut& cut) {
     using S = Wide<FP8>;
-    auto kern = gemm_grouped_wide_kernel<FP8, GLU, Tout>;
+    static_assert(3 * 4 * 8192 <= (FETCHED + 1) * S::STAGE, "three blocks' parts of a quarter of the columns, one block's of a half");
+    auto kern = gemm_grouped_wide_kernel<FP8, GLU, CLUSTER, Tout>;
     static const size_t own = own_smem((const void*)kern, S::LAUNCHED);          // (what the warps hand over has to be there)
     static std::atomic<bool> allowed[64];
-    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, false, allowed}, p, cut);
+    return launch<Tout>(kern, Kind{S::ROWS, S::TILES, S::STAGE, fixed_smem<S>(), own, S::TMEM, S::THREADS, CLUSTER ? 4 : 0, true, allowed}, p, cut);
 }
 
 template <bool FP8, bool GLU, typename Tout>
@@ -1173,7 +1230,11 @@ int launch_cut(const Product& p, const Cut& cut) {
     if (cut.nt == 16 && cut.mt == 1) return launch_narrow<FP8, 16, GLU, Tout>(p, cut);
     if (cut.nt == 32 && cut.mt == 1) return launch_narrow<FP8, 32, GLU, Tout>(p, cut);
     if (cut.nt == 64 && cut.mt == 1) return launch_narrow<FP8, 64, GLU, Tout>(p, cut);
-    if (cut.nt == 128 && cut.mt == 2) return launch_wide<FP8, GLU, Tout>(p, cut);
+    if (cut.nt == 128 && cut.mt == 2) {
+        if constexpr (FP8)
+            if (cut.blocks > 1) return launch_wide<FP8, GLU, true, Tout>(p, cut);
+        return launch_wide<FP8, GLU, false, Tout>(p, cut);
+    }
     return jllm_fail(JLLM_BAD_ARGUMENT, "gemm_grouped: no kernel for spans of %d pairs and %d tiles", cut.nt, cut.mt);
 }
 template <bool FP8>
@@ -1240,9 +1301,12 @@ double narrow_count(const Narrowly& c, int blocks, int rows, int tiles, int k_bl
     const double read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
     return c.start + (run > read ? run : read);
 }
-double wide_count(int rows, int tiles, int k_blocks, int sms) {
-    const long long units = (long long)((tiles + 1) / 2) * ((rows + 127) / 128), rounds = (units + sms - 1) / sms;
-    const double busy = units < sms ? (double)units / sms : 1.0, run = rounds * (k_blocks * (0.5 + 0.118 * busy) + 3.38), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
+double wide_count(int blocks, int rows, int tiles, int k_blocks, int sms) {
+    const int one = resident_clusters(blocks, 1);
+    if (blocks > k_blocks || one < 1) return 1e30;
+    const long long units = (long long)((tiles + 1) / 2) * ((rows + 127) / 128), rounds = (units + one - 1) / one;
+    const double busy = units < one ? (double)units * blocks / sms : 1.0, each = (k_blocks + blocks - 1) / blocks;
+    const double run = rounds * (each * (0.5 + 0.118 * busy) + 3.38 + (blocks > 1 ? 1.5 + 0.5 * blocks : 0.0)), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
     return 1.27 + (run > read ? run : read);
 }
 // Groups (11,092 sizes: 1 to 2,048 rows of 1 to 8 choices among 4 to 128 groups, 128 to 4,096 weight rows of as many values; 1 to 2% on those that the fit has not seen; by
@@ -1279,7 +1343,7 @@ Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int ti
     if (!groups) {
         for (const Narrowly& c : NARROW)
             for (int blocks = 1; blocks <= (fp8 && c.nt <= 32 ? 8 : 1); ++blocks) offer(narrow_count(c, blocks, rows, tiles, k_blocks, sms), {c.nt, 1, blocks, 2});
-        offer(wide_count(rows, tiles, k_blocks, sms), {128, 2, 1, 1});
+        for (int blocks = 1; blocks <= (fp8 ? 4 : 1); blocks *= 2) offer(wide_count(blocks, rows, tiles, k_blocks, sms), {128, 2, blocks, 1});
     } else {
         const double pairs = (double)groups->rows * groups->top, share = groups->top < groups->groups ? (double)groups->top / groups->groups : 1.0;
         const double asked = groups->groups * (1.0 - pow(1.0 - share, groups->rows)), mean = pairs / (asked > 1.0 ? asked : 1.0);

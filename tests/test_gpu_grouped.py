@@ -214,6 +214,15 @@ def test_product_of_clusters(ops, nt, blocks):
         run_product(ops, rows, 272, 1800, glu=True, dtype=torch.bfloat16, cut=nt * 1000 + 110 + blocks, seed=rows)
 
 
+@pytest.mark.parametrize("cut", [128212, 128214])
+@pytest.mark.parametrize("rows,n,k", [(1, 100, 520), (31, 300, 700), (128, 256, 1024), (129, 384, 2049), (300, 129, 640), (97, 1003, 1930)])
+def test_product_of_wide_clusters(ops, rows, n, k, cut):
+    run_product(ops, rows, n, k, cut=cut, bias=rnd(n, seed=4))
+    run_product(ops, rows, n, k, cut=cut, accumulate=True, dtype=torch.bfloat16)
+    run_product(ops, rows, 16 * (n // 16), k, glu=True, cut=cut)
+    run_product(ops, rows, 16 * (n // 16), k, glu=True, dtype=torch.bfloat16, cut=cut)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(3, 200, 260), (70, 333, 500)])
 def test_epilogues(ops, rows, n, k, dtype):

@@ -127,7 +127,7 @@ def test_the_same_bits_at_every_run(ops):
     a = ops.fp8_rows(24, 4096, DEV)
     ops.quantize_fp8(torch.randn(24, 4096, generator=g).to(DEV), a)
     w = ops.quantize_weight_fp8(torch.randn(512, 4096, generator=g).to(DEV))
-    for cut in (0, 32124, 16128, 16121, 64121, 128211):
+    for cut in (0, 32124, 16128, 16121, 64121, 128211, 128212, 128214):
         outs = []
         for _ in range(8):
             out = torch.empty(24, 512, device=DEV)

@@ -44,7 +44,8 @@ def product(ops, kind, rows, width, dim, groups=0):
 @pytest.mark.parametrize("what,cut,rows,dim,code", [
     ("copy", 32121, 20, 1024, 42), ("copy", 16111, 9, 1024, 42), ("copy", 32124, 20, 1024, 42), ("copy", 128211, 100, 1024, 42), ("copy", 64121, 60, 640, 42),
     ("release", 32111, 20, 1024, 41), ("release", 32121, 20, 1024, 42), ("release", 128211, 100, 1024, 42), ("release", 128211, 100, 256, 41),
-    ("parts", 32122, 20, 1024, 43), ("parts", 16128, 16, 1024, 43), ("parts", 16114, 3, 512, 43)])
+    ("parts", 32122, 20, 1024, 43), ("parts", 16128, 16, 1024, 43), ("parts", 16114, 3, 512, 43), ("parts", 128212, 100, 512, 43),
+    ("parts", 128214, 20, 640, 43), ("copy", 128212, 100, 512, 42)])
 def test_a_wait_that_runs_out_returns_and_is_reported(ops, what, cut, rows, dim, code):
     run, want = product(ops, "fp8", rows, 256, dim)
     ops.gemm_grouped_starve_next(what)
@@ -79,7 +80,7 @@ def test_groups_whose_wait_runs_out(ops, kind, what, cut):
 
 def test_a_short_limit_does_not_disturb_a_product_that_misses_nothing(ops):
     run, want = product(ops, "fp8", 40, 256, 1024)
-    for cut in (16121, 32124, 64111, 128211):
+    for cut in (16121, 32124, 64111, 128211, 128212, 128214):
         out = torch.empty(40, 256, device=DEV)
         ops.gemm_grouped_starve_next("nothing", 2000)
         run(out, cut)
@@ -115,7 +116,7 @@ def test_refusals(ops):
     ops.gemm_grouped_starve_next("parts")
     with pytest.raises(ops.KernelError):               # a block alone has nobody who could send
         run(torch.empty(20, 256, device=DEV), 32121)
-    for cut in (64122, 128212, 128111, 48121, 16129, 16131, 32101):      # no kernel, no cluster, no such number of blocks
+    for cut in (64122, 128213, 128218, 128222, 128111, 48121, 16129, 16131, 32101):      # no kernel, no cluster, no such number of blocks
         with pytest.raises(ops.KernelError):
             run(torch.empty(20, 256, device=DEV), cut)
     run(torch.empty(20, 256, device=DEV), 32121)
