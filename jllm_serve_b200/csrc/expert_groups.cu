@@ -6,10 +6,11 @@
 // number: no atomics, and the order is the pairs'), and each pair keeps its number among its warp's of that expert; (2) the warps' counts, and the
 // experts' in front, become each warp's first place for each expert; (3) every pair has its place, and the block's pairs leave in their experts' order.
 // Up to 2,048 pairs are one block and one launch. Of more, a launch in front counts every block's pairs by expert, and (2) adds up the blocks in front.
-// Latency bounds the small ones; of 131,072 pairs a cluster of eight blocks took 23 us for the votes and scattered words of 8 SMs.
+// Latency bounds the small ones: 64 pairs of 128 experts 2.2 us, 16,384 6.1, 131,072 of 256 9.6 (a cluster of eight blocks took 23 us for the votes and scattered words
+// of 8 SMs).
 //
 // combine_groups reads every answer once and writes every row once: memory bounds it. The sum runs over a row's choices in their order in float32,
-// whatever place the pairs have: equal bits in every batch.
+// whatever place the pairs have: equal bits in every batch. 2,048 rows of eight float32 answers of 2,048 values 23.6 us (5.8 TB/s), bfloat16 12.1; 16 rows 2.3 us.
 #include "common.cuh"
 #include "fp8_view.h"
 
@@ -178,6 +179,7 @@ __global__ void __launch_bounds__(MOST_WARPS * 32) group_rows_kernel(const int* 
 template <typename Ta, typename Tout, int PER>
 __global__ void __launch_bounds__(256) combine_groups_kernel(const Ta* __restrict__ answers, int lda, const int* __restrict__ place, const float* __restrict__ share, int ld_share, int top,
                                                              Tout* __restrict__ out, int ldo, int rows, int cols, int pieces, bool add) {
+    const unsigned pairs = (unsigned)rows * (unsigned)top;          // (a place of a larger step, not filled anew, is none)
     pdl_wait();
     pdl_trigger();
     const long long items = (long long)rows * pieces;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(256) combine_groups_kernel(const Ta* __restric
                 there[i] = false;
                 if (j + i >= top) continue;
                 const int p = place[(size_t)row * top + j + i];
-                there[i] = p >= 0;
+                there[i] = (unsigned)p < pairs;
                 if (!there[i]) continue;
                 w[i] = share[(size_t)row * ld_share + j + i];
                 const Ta* src = answers + (size_t)p * lda + c0;

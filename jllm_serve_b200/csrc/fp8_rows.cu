@@ -13,7 +13,8 @@
 // scale is exact, the quotient is corrected by its residual, so that a tie is met exactly and falls to the even value.
 //
 // Memory bounds it. 16 lanes have a block of 128 values, 8 neighbouring values a lane, so a maximum is four exchanges and nothing meets beyond a
-// half warp; a thread has several blocks' values under way at a time.
+// half warp; a thread has several blocks' values under way at a time. 2,048 x 12,288 bfloat16 17.6 us for 75 MB (4.3 TB/s; the same taken back to bfloat16 13.1
+// us, 5.8), float32 22.6 us for 126 MB (5.6); 8 x 4,096 1.65 us.
 #include "common.cuh"
 #include "fp8_view.h"
 
@@ -164,7 +165,6 @@ __global__ void __launch_bounds__(THREADS) quantize_fp8_kernel(const T* __restri
         }
         uint8_t* dst = q + (size_t)row * ldq + first * 128 + lane16 * 8;
         float* dst_scale = scale + (size_t)row * ld_scale + first;
-        const int room = ((cols + 15) & ~15) - first * 128 - lane16 * 8;
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a) {
             const uint32_t m = v[a].most();
@@ -172,11 +172,16 @@ __global__ void __launch_bounds__(THREADS) quantize_fp8_kernel(const T* __restri
             const bool bad = m >= 0x7f800000u;
             const float most = fmaxf(__uint_as_float(bad ? 0u : m), kTiny), s = by_448(most), inverse = __fdividef(1.f, s);
             if (lane16 == 0) dst_scale[a] = bad ? __uint_as_float(0x7fc00000u) : s;
-            // (rows begin at multiples of 16 bytes and have room up to the next one: what is behind the last value is zero)
-            if (room <= 128 * a) continue;
+            const int values = left - 128 * a;
+            if (values <= 0) continue;
             uint32_t two[4];
             rounded(v[a], s, inverse, __fmaf_rn(-kMost, s, most), two);
-            *reinterpret_cast<uint2*>(dst + 128 * a) = bad ? make_uint2(0u, 0u) : make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+            const uint2 eight = bad ? make_uint2(0u, 0u) : make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+            if (values >= 8) *reinterpret_cast<uint2*>(dst + 128 * a) = eight;
+            else
+#pragma unroll
+                for (int j = 0; j < 7; ++j)          // (what is behind a row's last value is not touched: who reads rows reads no further either)
+                    if (j < values) dst[128 * a + j] = (uint8_t)((j < 4 ? eight.x : eight.y) >> 8 * (j & 3));
         }
     }
 }

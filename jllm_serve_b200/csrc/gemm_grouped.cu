@@ -14,7 +14,7 @@
 // know them). One warp brings weights (bulk copies) and rows into a ring that runs on over the units, one issues the MMAs, the others take the sums
 // from tensor memory. So the copies of the next unit are under way while this one ends. Rows that lie together come by TMA boxes; rows that are
 // fetched from all over by 16-byte asynchronous copies of whole warps, four rows an instruction (gathers of four rows by TMA took 30 ns each and
-// an SM: 128 rows x 1,536 x 2,048 of each of 128 groups 281 us, against 154 of rows that lie together).
+// an SM: 16,384 pairs of 128 groups against 1,536 x 2,048, bfloat16, 281 us; now 175, and 151 of rows that lie together).
 //
 // In 8 bits the sums of ONE k block are made by the tensor cores (float32) and lie in one of several buffers in tensor memory; the epilogue warps
 // multiply them by both scales and add them into float32 registers. The scales of a block are float32 numbers of any value: the hardware's own
@@ -22,7 +22,15 @@
 //
 // Two kernels. NARROW, groups of few rows: the weight rows are the M side of the MMAs and up to 64 rows of a group, filled up to a multiple of 16, the
 // N side, so that of many small groups nothing is wasted on a side of 128. WIDE, groups of many: 128 rows are the M side and two tiles of the weight the
-// N side.
+// N side. Which one, and how it is cut, follows from counts that are fitted to measured sizes (`choose`).
+//
+// What bounds them. Few rows: memory. Eight rows of eight choices among 128 weights of 1,536 x 2,048 (bfloat16, 49 asked) 48 us for 308 MB (6.4 TB/s, 0.98 of the
+// measured copy), sixteen rows in 8 bits 46 us for 250 MB; one row in 8 bits against 24,576 x 4,096 18 us (5.6 TB/s), against 4,096 x 4,096 6.4 us (launch, scales, ring,
+// the cluster's parts: about 4 us beside the stream). Many rows: bfloat16 groups are near memory too (2,048 rows, 128 groups of 1,536 x 2,048: 175 us for 128 of
+// bytes). In 8 bits it is the way of a k block from the tensor cores to the epilogue's registers and back, over two buffers, which are all of tensor
+// memory: some 1,000 cycles a k block and SM, where its MMAs (128 x 256 x 128) take 512 and the 118 instructions of each of sixteen warps 470 of the schedulers'. 2,048 x
+// 24,576 x 4,096 take 221 us (1.86 PFLOP/s), 264 one behind the other for long (the power limit); with no sums in the epilogue, 170. Measured slower: the two tiles of a k block
+// handed over apart (1 to 2%), eight warps of twice the columns, k blocks unrolled by four.
 //
 // The waits on barriers in shared memory end by the clock and raise the products' error word (41: the producer, 42: the MMAs, 43: the epilogue).
 #include "fp8_view.h"
@@ -48,12 +56,12 @@ struct Args {
     const float *scale_w, *scale_a;       // [groups, tiles * 16, sw_ld] and [rows, sa_ld]: multiples of four values a row
     const int *offsets, *order;           // null: one group of `rows`; null: a pair's row is the pair
     int sw_ld, sa_ld;
-    int groups, top, rows, tiles, k_blocks;
+    int groups, top, rows, pairs, tiles, k_blocks;
     int spans, span;                      // of one group: spans of so many rows
     int row_bytes, row_step;              // of `a`: bytes that count, and 16-byte pieces from row to row
     Finish f;
     int stages, blocks, share;            // blocks of a cluster, tokens that each of them finishes
-    int box;                              // rows that one copy brings, of rows that lie together: a copy costs some 30 ns, whatever it brings
+    int box;                              // rows that one copy brings, of rows that lie together
     int starve, limit_us;                 // a test of the waits (below); 0, 0
     int* error_word;
 };
@@ -168,7 +176,7 @@ constexpr size_t fixed_smem() { return 1024 + 8 * (2 * S::BUFFERS + 1) + 64; }
 template <class S>
 __device__ __forceinline__ void list_units(const Args& g, int* before, int* at) {
     pdl_wait();          // (the offsets are the kernel in front's)
-    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = g.offsets[i];
+    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = min(g.offsets[i], g.pairs);          // (of a larger step, not filled anew: within bounds)
     __syncthreads();
     if (threadIdx.x >= 32) return;
     const int lane = threadIdx.x, each = (g.groups + 31) / 32, lo = min(lane * each, g.groups), hi = min(lo + each, g.groups), tiles = (g.tiles + S::TILES - 1) / S::TILES;
@@ -234,6 +242,9 @@ struct Share {
     }
 };
 
+// The row that pair p asks with (one that exists, whatever the order says).
+__device__ __forceinline__ uint32_t row_of(const Args& g, int p) { return min((uint32_t)(g.order[p] / g.top), (uint32_t)g.rows - 1u); }
+
 // Rows of a unit that lie anywhere, fetched by a warp: this lane's are [16-byte piece lane % 8] of rows r0 + 4 i + lane / 8.
 template <class S>
 struct Fetch {
@@ -246,7 +257,7 @@ struct Fetch {
 #pragma unroll
         for (int i = 0; i < S::GATHER_ROWS / 4; ++i) {
             const int r = 4 * i + (lane >> 3);
-            if (r < rows) piece[i] = (uint32_t)(g.order[unit.first + r0 + r] / g.top) * (uint32_t)g.row_step;
+            if (r < rows) piece[i] = row_of(g, unit.first + r0 + r) * (uint32_t)g.row_step;
         }
     }
     // k block kb into stage s (rows r0 on)
@@ -638,7 +649,7 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
                 const int edge = GLU ? (128 - (((g.f.N >> 1) + unit.tile * 64) & 127)) >> 3 : 0, eight = row >> 3;
                 const int kind = GLU && (eight & 1) ? ((eight >> 1) < edge ? 1 : 2) : 0;
                 const bool has = thread < unit.here;
-                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? g.order[unit.first + thread] / g.top : unit.first + thread) : 0) * g.sa_ld;
+                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? row_of(g, unit.first + thread) : (uint32_t)(unit.first + thread)) : 0u) * g.sa_ld;
                 float4 sa_next = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (has) sa_next = *reinterpret_cast<const float4*>(sa_row + (kb_lo & ~3));
                 if (thread < NT && (g.offsets || u != share.unit)) ask_weights(unit, kb_lo & ~3);
@@ -948,7 +959,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sums[j] = 0;
                 const bool has = token < unit.here;
-                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? g.order[unit.first + token] / g.top : unit.first + token) : 0) * g.sa_ld + share.kb_lo;
+                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? row_of(g, unit.first + token) : (uint32_t)(unit.first + token)) : 0u) * g.sa_ld + share.kb_lo;
                 const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld + share.kb_lo;
                 // of gate and up rows in eights: the gates' scale, and the up rows' in front of and behind the edge of their block of 128
                 const int edge = GLU ? ((128 - ((last + tile * 64) & 127)) >> 3) - (set & 1) * 4 : 0;
@@ -1076,30 +1087,17 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 
 // Rows of `bytes` bytes, `ld` bytes apart, read in boxes of box_rows x 128 bytes with the 128-byte swizzle.
 int rows_map_for(const void* ptr, long long rows, long long bytes, long long ld, int box_rows, CUtensorMap* out) {
-    static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-    static std::mutex mu;
-    const MapKey key{ptr, rows, bytes, ld, box_rows};
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = cache.find(key);
-    if (it != cache.end()) {
-        *out = it->second;
-        return JLLM_OK;
-    }
     EncodeTiledFn fn = encode_fn();
     if (!fn) return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: the driver does not offer cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld};
     const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
     const cuuint32_t elem[2] = {1, 1};
-    CUtensorMap map;
-    const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return jllm_fail(JLLM_CUDA_ERROR, "gemm_grouped: cuTensorMapEncodeTiled failed (%d) for [%lld, %lld] bytes, ld %lld", (int)r, rows, bytes, ld);
-    if (cache.size() > 4096) cache.clear();
-    cache.emplace(key, map);
-    *out = map;
     return JLLM_OK;
 }
 
@@ -1159,9 +1157,11 @@ int launch(void (*kern)(const CUtensorMap, const Args, Tout*), const Kind& kind,
     g.stages = stages;
     // (a span's rows in one copy; of groups some of the next group's come along, of wide ones at most 63)
     g.box = !g.offsets ? span : kind.rows < 64 ? kind.rows : 64;
-    CUtensorMap map;
-    const int rc = rows_map_for(p.rows->data, p.rows->rows, g.row_bytes, p.rows->stride, g.box, &map);
-    if (rc != JLLM_OK) return rc;
+    CUtensorMap map = {};
+    if (!g.order) {          // (fetched rows need none)
+        const int rc = rows_map_for(p.rows->data, p.rows->rows, g.row_bytes, p.rows->stride, g.box, &map);
+        if (rc != JLLM_OK) return rc;
+    }
     // Blocks that wait for one another must not wait for tensor memory that others hold who wait in turn: of a cluster's blocks, which have 256
     // columns at most, no more than two are on an SM (113 KB), nor one beside blocks of another product that together want more than the rest.
     const size_t smem = stages * each + parts + fixed;
@@ -1245,11 +1245,11 @@ int launch_product(const Product& p, const Cut& cut) {
 
 // Clusters of that many blocks that the device runs at a time, `per_sm` blocks an SM; asked once per device.
 int resident_clusters(int blocks, int per_sm) {
-    static int known[64][2][9] = {};          // (one more than the answer)
+    static std::atomic<int> known[64][2][9];          // (one more than the answer; who asks first at once with another finds the same)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int& answer = known[dev][per_sm - 1][blocks];
-    if (answer) return answer - 1;
+    std::atomic<int>& answer = known[dev][per_sm - 1][blocks];
+    if (const int a = answer.load(std::memory_order_relaxed)) return a - 1;
     using S = Narrow<true, 16>;
     auto kern = gemm_grouped_narrow_kernel<true, 16, false, float>;
     const size_t own = own_smem((const void*)kern), smem = (per_sm == 1 ? 227 * 1024 : 113 * 1024) - own;
@@ -1274,7 +1274,7 @@ int resident_clusters(int blocks, int per_sm) {
         const int alone = resident_clusters(blocks, 1);
         if (n < 2 * alone) n = 2 * alone;
     }
-    answer = n + 1;
+    answer.store(n + 1, std::memory_order_relaxed);
     return n;
 }
 
@@ -1414,7 +1414,7 @@ JLLM_EXPORT int jllm_gemm_grouped(const BlockRows* rows, const BlockWeight* weig
     const bool gather = groups && !by_pair;
     Product p;
     p.args = Args{static_cast<const uint8_t*>(weight->data), static_cast<const uint8_t*>(rows->data), weight->scale, rows->scale, groups ? groups->offsets : nullptr, gather ? groups->order : nullptr,
-                  weight->scale_ld, rows->scale_ld, weight->groups, groups ? groups->top : 1, M, (N + 127) / 128, weight->k_blocks, 0, 0, K * bytes, (int)(rows->stride / 16),
+                  weight->scale_ld, rows->scale_ld, weight->groups, groups ? groups->top : 1, M, (int)pairs, (N + 127) / 128, weight->k_blocks, 0, 0, K * bytes, (int)(rows->stride / 16),
                   Finish{VecRef{bias, bias_dtype}, (int)(bias != nullptr), ldo, accumulate, N, swiglu_word}, 0, 1, 0, 16, starve.what, starve.limit_us, error_word};
     p.rows = rows, p.pairs = (int)pairs, p.out_dtype = out_dtype, p.out = out, p.stream = stream;
     const Cut cut = cut_code ? cut_of(cut_code) : choose(fp8, groups, by_pair != 0, M, p.args.tiles, weight->k_blocks);

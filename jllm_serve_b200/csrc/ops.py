@@ -1817,7 +1817,7 @@ class Fp8Rows:
 
 
 def fp8_rows(rows: int, cols: int, device) -> Fp8Rows:
-    """Room for `rows` rows of `cols` values in 8 bits (what `quantize_fp8` writes). (The bytes that fill a row up to 16 are there, and nobody's.)"""
+    """Room for `rows` rows of `cols` values in 8 bits (what `quantize_fp8` writes)."""
     if rows < 0 or cols < 1 or max(rows, cols) > BLOCK_MOST:
         _refuse("fp8_rows", f"up to {BLOCK_MOST} rows of as many values, got {rows} x {cols}")
     data = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
@@ -1958,7 +1958,8 @@ def _product_words(name, w: PackedBlocks, swiglu) -> int:
 
 def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate=False, swiglu=False, cut: int = 0) -> None:
     """out (+)= a @ w^T (+ bias) in 8-bit floating point: the tensor cores sum the products of 128 k in float32, both blocks' scales multiply each such sum
-    and the sums over the blocks are float32. out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or bfloat16; `accumulate` as the other
+    and the sums over the blocks are float32 (so is the scales' product: where it passes 2^127, or falls under 2^-126, results are infinite or not numbers, or
+    lose digits). out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or bfloat16; `accumulate` as the other
     products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`; no bias, nothing added): out[r, j] = act(gate_j) * up_j,
     [rows, w.rows / 2]. The weight, its scales and the bias are read before what is in front on the stream has ended: not what a kernel right in front
     writes. `cut` (tests): tokens of a span x 1,000, 128-row tiles of a unit x 100, blocks an SM x 10, blocks of a cluster; 0: as the sizes have it."""
@@ -1993,7 +1994,7 @@ class RowGroups:
         self.view = ctypes.addressof(self._view)
 
     def first(self, rows: int) -> "RowGroups":
-        """The same room for a step of fewer rows (to be filled anew)."""
+        """The same room for a step of fewer rows, to be filled anew (what is made of it before that is nothing, though within its bounds)."""
         if not 0 <= rows <= self.rows:
             _refuse("RowGroups", f"0 to {self.rows} rows, got {rows}")
         return RowGroups(self.offsets, self.order[:rows * self.top], self.place[:rows], self.counts, rows, self.top, self.groups)
