@@ -30,7 +30,8 @@
 // bytes). In 8 bits it is the way of a k block from the tensor cores to the epilogue's registers and back, over two buffers, which are all of tensor
 // memory: some 1,000 cycles a k block and SM, where its MMAs (128 x 256 x 128) take 512 and the 118 instructions of each of sixteen warps 470 of the schedulers'. 2,048 x
 // 24,576 x 4,096 take 221 us (1.86 PFLOP/s), 264 one behind the other for long (the power limit); with no sums in the epilogue, 170. Measured slower: the two tiles of a k block
-// handed over apart (1 to 2%), eight warps of twice the columns, k blocks unrolled by four.
+// handed over apart (1 to 2%), eight warps of twice the columns, k blocks unrolled by four. Also slower: the last round's units shared out by weight rows (8-bit down of
+// 2,048 rows 118 us for 102).
 //
 // The waits on barriers in shared memory end by the clock and raise the products' error word (41: the producer, 42: the MMAs, 43: the epilogue).
 #include "fp8_view.h"
