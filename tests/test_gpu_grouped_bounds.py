@@ -118,3 +118,35 @@ def test_two_host_threads_at_once(ops):
         t.join()
     torch.cuda.synchronize()
     assert not wrong
+
+
+def test_first_calls_inside_a_capture(ops):
+    """Sizes that no call had before: what a first call asks of the driver may be asked while a stream is captured."""
+    rows, n, k = 37, 1111, 1313
+    x, w = rnd(rows, k).to(DEV), ops.quantize_weight_fp8(rnd(n, k).to(DEV))
+    packed = ops.pack_grouped(rnd(11, 152, 88).to(torch.bfloat16).to(DEV))
+    few = rnd(rows, 88).to(torch.bfloat16).to(DEV)
+    choice = (torch.arange(rows * 2, dtype=torch.int32).view(rows, 2) % 11).to(DEV)
+    rows8, room = ops.fp8_rows(rows, k, DEV), ops.row_groups(rows, 2, 11, DEV)
+    out, answers, summed = torch.zeros((rows, n), device=DEV), torch.zeros((2 * rows, 152), device=DEV), torch.zeros((rows, 152), device=DEV)
+    share = torch.full((rows, 2), 0.5, device=DEV)
+
+    def step():
+        ops.quantize_fp8(x, rows8)
+        ops.gemm_fp8(rows8, w, out)
+        ops.group_rows(choice, room)
+        ops.gemm_grouped(few, packed, room, answers)
+        ops.combine_groups(answers, room, share, summed)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph.replay()
+    torch.cuda.synchronize()
+    replayed = [t.clone() for t in (out, answers, summed)]
+    for t in (out, answers, summed):
+        t.zero_()
+    step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(replayed, (out, answers, summed)))
