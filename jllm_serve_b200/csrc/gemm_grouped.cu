@@ -960,24 +960,37 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sums[j] = 0;
                 const bool has = token < unit.here;
-                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? row_of(g, unit.first + token) : (uint32_t)(unit.first + token)) : 0u) * g.sa_ld + share.kb_lo;
-                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld + share.kb_lo;
+                const float* sa_row = g.scale_a + (size_t)(has ? (g.order ? row_of(g, unit.first + token) : (uint32_t)(unit.first + token)) : 0u) * g.sa_ld;
+                const float* sw_row = g.scale_w + (size_t)((size_t)unit.e * g.tiles + (tile < g.tiles ? tile : unit.tile)) * 16 * g.sw_ld;
                 // of gate and up rows in eights: the gates' scale, and the up rows' in front of and behind the edge of their block of 128
                 const int edge = GLU ? ((128 - ((last + tile * 64) & 127)) >> 3) - (set & 1) * 4 : 0;
-                float sa = has ? sa_row[0] : 0.f, sw[GLU ? 3 : 1];
-                sw[0] = sw_row[0];
-                if constexpr (GLU) sw[1] = sw_row[g.sw_ld], sw[2] = sw_row[15 * g.sw_ld];
-                for (int kb = 0; kb < n_kb; ++kb) {
-                    uint64_t scale[GLU ? 3 : 1];
-#pragma unroll
-                    for (int q = 0; q < (GLU ? 3 : 1); ++q) {
-                        const uint32_t both = __float_as_uint(__fmul_rn(sa, sw[q]));
-                        scale[q] = pair_of(both, both);
+                constexpr int CLASSES = GLU ? 3 : 1;
+                if (lane < CLASSES) sw_row += (lane == 0 ? 0 : lane == 1 ? 1 : 15) * g.sw_ld;
+                // The scales of four k blocks, four blocks ahead, in what is the results' place later (two halves: the pairs' [32][4], the weight's [3][4]). (A lane's own
+                // loads, one for every k block, took 32 lines each, half of what an SM's cache can do in that time.)
+                auto ask = [&](int four, int half_) {
+                    const uint32_t to = smem_u32(park) + (uint32_t)half_ * 1024u;
+                    cp_async_16(to + (uint32_t)lane * 16u, sa_row + four, has ? 16 : 0);
+                    if (lane < CLASSES) cp_async_16(to + 512u + (uint32_t)lane * 16u, sw_row + four, 16);
+                };
+                int lap = 0;
+                const int kb_end = share.kb_lo + n_kb;
+                __syncwarp();          // (the unit in front has left)
+                ask(share.kb_lo & ~3, 1);
+                for (int kb = share.kb_lo; kb < kb_end; ++kb) {
+                    if (kb == share.kb_lo || (kb & 3) == 0) {
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        __syncwarp();
+                        lap ^= 1;
+                        if ((kb & ~3) + 4 < kb_end) ask((kb & ~3) + 4, lap ^ 1);
                     }
-                    if (kb + 1 < n_kb) {          // (a block ahead)
-                        if (has) sa = sa_row[kb + 1];
-                        sw[0] = sw_row[kb + 1];
-                        if constexpr (GLU) sw[1] = sw_row[g.sw_ld + kb + 1], sw[2] = sw_row[15 * g.sw_ld + kb + 1];
+                    const float* at_ = reinterpret_cast<const float*>(park) + lap * 256 + (kb & 3);
+                    const float sa = at_[lane * 4];
+                    uint64_t scale[CLASSES];
+#pragma unroll
+                    for (int q = 0; q < CLASSES; ++q) {
+                        const uint32_t both = __float_as_uint(__fmul_rn(sa, at_[128 + 4 * q]));
+                        scale[q] = pair_of(both, both);
                     }
                     ok = __all_sync(0xffffffffu, mbar_wait(ring.sums(buffer), parity, abort_flag, 2 * limit));
                     if (!ok) break;
@@ -999,6 +1012,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (lane == 0) mbar_arrive(ring.taken(buffer));
                     if (++buffer == S::BUFFERS) { buffer = 0; parity ^= 1u; }
                 }
+                if (!ok) asm volatile("cp.async.wait_all;" ::: "memory");
                 if constexpr (CLUSTER) {
                     // the unit's 16 chunks of 16 columns in order, `per` to a block; a warp's four are one block's
                     const int blocks = g.blocks, rank = share.rank, per = 16 / blocks, owner = set * 4 / per;
