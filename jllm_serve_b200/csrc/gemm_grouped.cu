@@ -1295,16 +1295,16 @@ int resident_clusters(int blocks, int per_sm) {
 
 // Counts that put the cuts in order; a count is no time, though it is fitted to microseconds. Fitted to products launched back to back on weights larger
 // than L2.
-// One weight, e4m3 (9,837 sizes of 1 to 2,048 rows against 64 to 24,576 weight rows of 128 to 12,288 values, up to 25 cuts each; on 3,000 that the fit has not
-// seen what is chosen is 1.7% slower than the best cut of each size in the geometric mean, 11% at the 95th percentile): a block's k blocks, alone on its SM or beside
-// another one, each longer the more SMs take in at once; what a unit costs beside them; sending.
+// One weight, e4m3 (4,092 sizes of up to 24 rows, 12,000 of 24 to 2,048, against 128 to 24,576 weight rows of 128 to 12,288 values, up to 20 cuts each; on those that
+// the fit has not seen what is chosen is 1.6% slower than the best cut of each size in the geometric mean, 11% at the 95th percentile): a block's k blocks, alone on
+// its SM or beside another one, each longer the more SMs take in at once; what a unit costs beside them; sending.
 struct Narrowly {
     int nt;
     double start, alone, alone_all, beside, beside_all, unit, send, block, token;
 };
-constexpr Narrowly NARROW[3] = {{16, 2.46, 0.184, 0.099, 0.243, 0.341, 0.82, 0.51, 0.034, 0.062},
-                                {32, 2.09, 0.186, 0.142, 0.434, 0.128, 1.52, 0.85, 0.0, 0.043},
-                                {64, 1.86, 0.234, 0.128, 0.550, 0.0, 2.62, 0.0, 0.0, 0.0}};
+constexpr Narrowly NARROW[3] = {{16, 2.57, 0.185, 0.060, 0.167, 0.385, 1.34, 0.711, 0.0352, 0.0579},
+                                {32, 2.38, 0.186, 0.113, 0.392, 0.103, 1.65, 0.708, 0.0839, 0.0381},
+                                {64, 1.40, 0.329, 0.0721, 0.550, 0.0641, 2.61, 0.0, 0.0, 0.0}};
 double narrow_count(const Narrowly& c, int blocks, int rows, int tiles, int k_blocks, int sms) {
     const int one = resident_clusters(blocks, 1), two = resident_clusters(blocks, 2), spans = (rows + c.nt - 1) / c.nt;
     if (blocks > k_blocks || one < 1 || two < 1) return 1e30;
@@ -1321,8 +1321,8 @@ double wide_count(int blocks, int rows, int tiles, int k_blocks, int sms) {
     if (blocks > k_blocks || one < 1) return 1e30;
     const long long units = (long long)((tiles + 1) / 2) * ((rows + 127) / 128), rounds = (units + one - 1) / one;
     const double busy = units < one ? (double)units * blocks / sms : 1.0, each = (k_blocks + blocks - 1) / blocks;
-    const double run = rounds * (each * (0.5 + 0.118 * busy) + 3.38 + (blocks > 1 ? 1.5 + 0.5 * blocks : 0.0)), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
-    return 1.27 + (run > read ? run : read);
+    const double run = rounds * (each * (0.455 + 0.124 * busy) + 4.28 + (blocks > 1 ? 5.3 + 0.234 * blocks : 0.0)), read = (double)tiles * TILE_BYTES * k_blocks / 6e6;
+    return 1.12 + (run > read ? run : read);
 }
 // Groups (11,092 sizes: 1 to 2,048 rows of 1 to 8 choices among 4 to 128 groups, 128 to 4,096 weight rows of as many values; 1 to 2% on those that the fit has not seen; by
 // the mean of a group's pairs alone 7%): the host knows neither which groups are asked nor how often, so both are reckoned from even choices, half a span more than the pairs fill.
