@@ -28,8 +28,9 @@
 // measured copy), sixteen rows in 8 bits 46 us for 250 MB; one row in 8 bits against 24,576 x 4,096 18 us (5.6 TB/s), against 4,096 x 4,096 6.4 us (launch, scales, ring,
 // the cluster's parts: about 4 us beside the stream). Many rows: bfloat16 groups are near memory too (2,048 rows, 128 groups of 1,536 x 2,048: 175 us for 128 of
 // bytes). In 8 bits it is the way of a k block from the tensor cores to the epilogue's registers and back, over two buffers, which are all of tensor
-// memory: some 1,000 cycles a k block and SM, where its MMAs (128 x 256 x 128) take 512 and the 118 instructions of each of sixteen warps 470 of the schedulers'. 2,048 x
-// 24,576 x 4,096 take 221 us (1.86 PFLOP/s), 264 one behind the other for long (the power limit); with no sums in the epilogue, 170. Measured slower: the two tiles of a k block
+// memory: some 1,000 cycles a k block and SM where its MMAs (128 x 256 x 128) take 512. By cycle counts a warp of the sums spends 390 on its loads of tensor memory and
+// multiply-adds (256 are the float32 units' least), 140 on waiting, the rest on scales, barriers and, spread over a unit's k blocks, its results; the issuing warp waits 450 to 600
+// for a buffer and 90 for copies. 2,048 x 24,576 x 4,096 take 217 to 227 us (1.8 to 1.9 PFLOP/s), 264 one behind the other for long (the power limit). Measured slower: the two tiles of a k block
 // handed over apart (1 to 2%), eight warps of twice the columns, k blocks unrolled by four. Also slower: the last round's units shared out by weight rows (8-bit down of
 // 2,048 rows 118 us for 102).
 //
@@ -814,8 +815,8 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
 
 // ---- many rows to a group: the rows are the M side ----
 // A thread of the epilogue has one pair and 64 of the unit's 256 columns: the pair's scale is a register, a tile's scale is one number (of gate and up
-// rows three: a block of 128 up rows may end inside the tile), so a k block costs one packed multiply-add for two values and nothing is shared
-// between threads. Sixteen warps do it: with eight (128 columns each) their way through a k block, one load of tensor memory behind the other, was
+// rows three: a block of 128 up rows may end inside the tile), so a k block costs one packed multiply-add for two values.
+// Sixteen warps do it: with eight (128 columns each) their way through a k block, one load of tensor memory behind the other, was
 // longer than the MMAs' and the copies'.
 // A row's 64 bytes of results leave together: a store whose 32 lanes each write 16 bytes of another row costs 32 lines, and what ends a unit stands in
 // nobody's shadow (4 us a unit of 128 x 256 that way).
