@@ -1918,8 +1918,11 @@ def pack_fp8(data: torch.Tensor, scale: torch.Tensor, glu: bool = False) -> Pack
     if glu:
         half = N // 2
         first = torch.stack([first[:half // 8], first[:half // 8] + half], dim=1).reshape(-1)
-    scales = torch.zeros((G, T * 16, -(-KB // 4) * 4), dtype=torch.float32, device=data.device)
-    scales[:, :first.numel(), :KB] = scale[:, first // BLOCK]
+    filled = torch.zeros((G, T * 16, -(-KB // 4) * 4), dtype=torch.float32, device=data.device)
+    filled[:, :first.numel(), :KB] = scale[:, first // BLOCK]
+    # A product reads its weight's tiles and scales before it waits for the kernel in front of it. The last thing here is therefore a copy: a product right behind
+    # it begins when the copy has ended, and a copy begins when all kernels in front have.
+    scales = torch.empty_like(filled).copy_(filled)
     return PackedBlocks(packed, scales, G, N, K, glu)
 
 
@@ -1961,8 +1964,8 @@ def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor 
     and the sums over the blocks are float32 (so is the scales' product: where it passes 2^127, or falls under 2^-126, results are infinite or not numbers, or
     lose digits). out [rows, w.rows] float32 or bfloat16, any row stride; bias float32 or bfloat16; `accumulate` as the other
     products have it (True: added into out; EPILOGUE_RELU2). `swiglu` (of a weight packed with `glu`; no bias, nothing added): out[r, j] = act(gate_j) * up_j,
-    [rows, w.rows / 2]. The weight, its scales and the bias are read before what is in front on the stream has ended: not what a kernel right in front
-    writes. `cut` (tests): tokens of a span x 1,000, 128-row tiles of a unit x 100, blocks an SM x 10, blocks of a cluster; 0: as the sizes have it."""
+    [rows, w.rows / 2]. The weight and its scales are read before what is in front on the stream has ended: they may be packed right in front of the product
+    (`pack_fp8`, `quantize_weight_fp8`), but a kernel there must not write over them. `cut` (tests): tokens of a span x 1,000, 128-row tiles of a unit x 100, blocks an SM x 10, blocks of a cluster; 0: as the sizes have it."""
     name = "gemm_fp8"
     word = _product_words(name, w, swiglu) if swiglu or w.glu else 0
     if not w.fp8 or w.groups != 1 or a.cols != w.cols or out.dtype not in _DT:
