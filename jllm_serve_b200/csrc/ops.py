@@ -1139,6 +1139,8 @@ def pack_weight(w: torch.Tensor) -> PackedWeight:
         padded = w
     tiles = padded.view(T, 128, KB, 8, 8).permute(0, 2, 1, 3, 4)                   # [T, KB, 128 rows, 8 chunks, 8]
     data = tiles.gather(3, _swizzle_index(w.device).expand(T, KB, 128, 8, 8)).contiguous().view(T, KB, 128, 64)
+    # (a product reads its weight before it waits for the kernel in front of it: behind a copy, of whatever, it begins when the copy and so the gathering has ended)
+    torch.empty(1, device=w.device).copy_(torch.empty(1, device=w.device))
     return PackedWeight(data, N, K)
 
 

@@ -38,3 +38,11 @@ def test_an_8_bit_weight_ends_with_a_copy(shape, glu):
     with Watch() as watch:
         ops.quantize_weight_fp8(torch.ones(shape), glu)
     assert ends_with_a_copy(watch.seen)
+
+
+@pytest.mark.parametrize("shape", [(128, 64), (5, 8), (300, 200)])
+def test_a_bfloat16_weight_ends_with_a_copy(shape):
+    """(A plain matrix that a product is given is packed in front of it.)"""
+    with Watch() as watch:
+        ops.pack_weight(torch.ones(shape, dtype=torch.bfloat16))
+    assert ends_with_a_copy(watch.seen)
