@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(THREADS) quantize_fp8_kernel(const T* __restri
             if (values >= 8) *reinterpret_cast<uint2*>(dst + 128 * a) = eight;
             else
 #pragma unroll
-                for (int j = 0; j < 7; ++j)          // (what is behind a row's last value is not touched: who reads rows reads no further either)
+                for (int j = 0; j < 7; ++j)          // (what is behind a row's last value is neither written nor, where rows are read, read)
                     if (j < values) dst[128 * a + j] = (uint8_t)((j < 4 ? eight.x : eight.y) >> 8 * (j & 3));
         }
     }
@@ -223,22 +223,22 @@ __global__ void __launch_bounds__(THREADS) fp8_values_kernel(const uint8_t* __re
         const int here = min(per, blocks - first), left = cols - first * 128 - lane16 * 8;
         const uint8_t* src = q + (size_t)row * ldq + first * 128 + lane16 * 8;
         T* dst = out + (size_t)row * ldo + first * 128 + lane16 * 8;
-        uint2 w[AT_A_TIME];
+        Bytes8 w[AT_A_TIME];
         float s[AT_A_TIME];
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a)
             if (a < here && left > 128 * a) {
-                w[a] = *reinterpret_cast<const uint2*>(src + 128 * a);
+                w[a] = bytes_of(src + 128 * a, left - 128 * a);
                 s[a] = scale[(size_t)row * ld_scale + first + a];
             }
 #pragma unroll
         for (int a = 0; a < AT_A_TIME; ++a)
             if (a < here && left > 128 * a) {
                 float v[8];
-                from_e4m3x2(w[a].x & 0xffffu, v[0], v[1]);
-                from_e4m3x2(w[a].x >> 16, v[2], v[3]);
-                from_e4m3x2(w[a].y & 0xffffu, v[4], v[5]);
-                from_e4m3x2(w[a].y >> 16, v[6], v[7]);
+                from_e4m3x2(w[a].lo & 0xffffu, v[0], v[1]);
+                from_e4m3x2(w[a].lo >> 16, v[2], v[3]);
+                from_e4m3x2(w[a].hi & 0xffffu, v[4], v[5]);
+                from_e4m3x2(w[a].hi >> 16, v[6], v[7]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], s[a]);
                 store8(dst + 128 * a, v, left - 128 * a, vec);

@@ -24,3 +24,22 @@ struct RowGroupsView {
 constexpr int GROUP_BLOCKS = 128;
 // The kernels count rows, pairs and values in 32 bits and step past the end by up to a block's 8,192 values.
 constexpr int BLOCK_MOST = 0x7fffffff - 8191;
+
+#ifdef __CUDACC__
+#define JLLM_HERE __host__ __device__ __forceinline__
+#else
+#define JLLM_HERE inline
+#endif
+struct alignas(8) Bytes8 {
+    uint32_t lo, hi;
+};
+// Eight neighbouring bytes that begin at a multiple of 8, of which `left` exist: one load where all do, else none behind the last (the end of a row may be the
+// end of its memory).
+JLLM_HERE Bytes8 bytes_of(const uint8_t* p, int left) {
+    if (left >= 8) return *reinterpret_cast<const Bytes8*>(p);
+    Bytes8 b = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+        if (j < left) (j < 4 ? b.lo : b.hi) |= (uint32_t)p[j] << 8 * (j & 3);
+    return b;
+}
