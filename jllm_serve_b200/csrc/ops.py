@@ -1936,9 +1936,17 @@ def pack_grouped(weight: torch.Tensor, glu: bool = False) -> PackedBlocks:
     return PackedBlocks(_pack_bytes("pack_grouped", weight, glu), None, *weight.shape, glu)
 
 
+def _e4m3(x: torch.Tensor) -> torch.Tensor:
+    """float64 values of magnitudes up to 448 -> e4m3, rounded once, half to even (torch's own conversion goes through float32, where a value next to a tie
+    becomes the tie)."""
+    exponent = (x.abs().view(torch.int64) >> 52).clamp(min=1023 - 6)          # (as it is stored; smaller values have the steps of 2^-6)
+    step = ((exponent - 3) << 52).view(torch.float64)
+    return (torch.round(x / step) * step).float().to(torch.float8_e4m3fn)
+
+
 def quantize_weight_fp8(weight: torch.Tensor, glu: bool = False) -> PackedBlocks:
-    """A float32 or bfloat16 weight [rows, cols], or [groups, rows, cols], rounded to e4m3 with a scale for every 128 x 128 block (the largest magnitude over
-    448), and packed."""
+    """A float32 or bfloat16 weight [rows, cols], or [groups, rows, cols], in e4m3 with a scale for every 128 x 128 block, and packed: scale = max(m, 2^-100) / 448
+    with m a block's largest magnitude, rounded to float32, q = weight / scale rounded once to e4m3, half to even."""
     if weight.dtype not in _DT or weight.dim() not in (2, 3) or not weight.numel():
         _refuse("quantize_weight_fp8", f"a float32 or bfloat16 weight [rows, cols] or [groups, rows, cols], got {weight.dtype} {tuple(weight.shape)}")
     if weight.dim() == 2:
@@ -1946,11 +1954,17 @@ def quantize_weight_fp8(weight: torch.Tensor, glu: bool = False) -> PackedBlocks
     G, N, K = weight.shape
     data = torch.empty((G, N, K), dtype=torch.float8_e4m3fn, device=weight.device)
     scale = torch.empty((G, -(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=weight.device)
-    for g in range(G):                            # (a weight at a time: the blocks are float32 beside it)
-        padded = torch.nn.functional.pad(weight[g].float(), (0, -K % BLOCK, 0, -N % BLOCK))
-        blocks = padded.view(scale.shape[1], BLOCK, scale.shape[2], BLOCK)
-        scale[g] = blocks.abs().amax(dim=(1, 3)).clamp(min=2.0 ** -100) / 448.0
-        data[g] = (blocks / scale[g][:, None, :, None]).clamp(-448.0, 448.0).view(padded.shape)[:N, :K].to(torch.float8_e4m3fn)
+    step = max(1, (1 << 24) // (BLOCK * BLOCK * scale.shape[2])) * BLOCK          # rows at a time: some 2^24 values are float64 beside the weight
+    for g in range(G):
+        for lo in range(0, N, step):
+            part = weight[g, lo:lo + step].double()
+            rows = part.shape[0]
+            padded = torch.nn.functional.pad(part, (0, -K % BLOCK, 0, -rows % BLOCK))
+            blocks = padded.view(-1, BLOCK, scale.shape[2], BLOCK)
+            # (m / 448 is never a tie of float32's and 2^-28 of itself or further from one: float64's rounding of it does not matter)
+            part_scale = (blocks.abs().amax(dim=(1, 3)).clamp(min=2.0 ** -100) / 448.0).float()
+            scale[g, lo // BLOCK:lo // BLOCK + part_scale.shape[0]] = part_scale
+            data[g, lo:lo + step] = _e4m3(blocks / part_scale.double()[:, None, :, None]).view(padded.shape)[:rows, :K]
     return pack_fp8(data, scale, glu)
 
 
