@@ -2073,9 +2073,11 @@ def combine_groups(answers: torch.Tensor, groups: RowGroups, share: torch.Tensor
     name = "combine_groups"
     if answers.dtype not in _DT or out.dtype not in _DT or share.dtype != torch.float32 or answers.dim() != 2:
         _refuse(name, f"float32 or bfloat16 answers and result and float32 shares, got {answers.dtype}, {out.dtype} and {share.dtype}")
+    dim = answers.shape[1]
+    if dim > BLOCK_MOST:          # (a launcher's argument would drop what 32 bits do not hold)
+        _refuse(name, f"answers of up to {BLOCK_MOST} columns, got {dim}")
     if not 0 <= answers.get_device() == groups.device == share.get_device() == out.get_device() == _current_device():
         _elsewhere(name, answers.get_device(), groups.device, share.get_device(), out.get_device())
-    dim = answers.shape[1]
     _call("jllm_combine_groups", answers.data_ptr(), _DT[answers.dtype], _row_stride(name, "answers", answers, (groups.pairs, dim)), groups.view,
           share.data_ptr(), _row_stride(name, "share", share, groups.shape), out.data_ptr(), _DT[out.dtype],
           _row_stride(name, "out", out, (groups.rows, dim)), dim, int(bool(accumulate)), _stream())
