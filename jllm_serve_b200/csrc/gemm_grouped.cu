@@ -140,6 +140,7 @@ struct Narrow {
                          TMEM = BUFFERS * COLUMNS < 32 ? 32 : BUFFERS * COLUMNS;
     // four warps have the tile's weight rows; with 32 rows and more two sets of them share the rows
     static constexpr int SETS = NT >= 32 ? 2 : 1, EPILOGUE = 4 * SETS, FIRST = 2, THREADS = 32 * (FIRST + EPILOGUE);
+    static constexpr bool ONE = FP8;                           // products of one weight without groups: in 8 bits alone
     static constexpr bool CLUSTERS = FP8 && NT <= 32;          // (the parts of 64 rows leave no room for a ring beside another block)
     static constexpr int GATHER = 0, GATHER_WARPS = 1, GATHER_ROWS = NT;          // the producer fetches rows itself
     static constexpr uint32_t STAGE = TILES * TILE_BYTES + NT * 128;
@@ -149,6 +150,7 @@ struct Wide {
     static constexpr int ROWS = 128, TILES = 2, TOGETHER = 1, COLUMNS = 256, BUFFERS = 2, TMEM = BUFFERS * COLUMNS;
     // four warps have the rows; four sets of them share the 256 columns
     static constexpr int SETS = 4, EPILOGUE = 4 * SETS, FIRST = 4, THREADS = 32 * (FIRST + EPILOGUE);
+    static constexpr bool ONE = FP8;
     static constexpr int GATHER = 2, GATHER_WARPS = 2, GATHER_ROWS = 64;
     static constexpr uint32_t STAGE = TILES * TILE_BYTES + ROWS * 128;
     // The threads are launched with 96 registers; the copying and issuing warps give of theirs what the sums need.
@@ -208,11 +210,11 @@ struct Units {
     int e = 0;                            // the group of the unit that was asked for last (units are asked for in ascending order)
 
     __device__ __forceinline__ Units(const Args& g_, const int* before_, const int* at_) : g(g_), before(before_), at(at_) {
-        total = g.offsets ? before[g.groups] : (g.tiles + S::TILES - 1) / S::TILES * g.spans;
+        total = !S::ONE || g.offsets ? before[g.groups] : (g.tiles + S::TILES - 1) / S::TILES * g.spans;
     }
     // the whole warp calls it
     __device__ __forceinline__ Unit operator()(int u) {
-        if (!g.offsets) {
+        if (S::ONE && !g.offsets) {
             const int t = u / g.spans, first = (u - t * g.spans) * g.span;
             return {0, t * S::TILES, first, min(g.span, g.rows - first), g.span};
         }
@@ -464,7 +466,7 @@ __device__ __forceinline__ uint32_t begin(const Args& g, const Ring<S>& ring, in
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)), "r"((uint32_t)S::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (g.offsets) list_units<S>(g, before, at);
+    if (!S::ONE || g.offsets) list_units<S>(g, before, at);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -495,7 +497,7 @@ __device__ __forceinline__ bool finish_block(const Ring<S>& ring, bool ok, int i
 
 // What 16 pairs x 32 weight rows of a warp have come to, parked in shared memory as [16][32] floats -> out, pairs [lo, hi) of the 16 that begin at
 // row p0, 16 bytes a lane where `vec`.
-template <bool GLU, typename Tout>
+template <bool GLU, bool ADDS, typename Tout>
 __device__ __forceinline__ void leave(const Finish& f, Tout* out, const float* park, size_t p0, int lo, int hi, int n0, bool vec, int lane) {
     constexpr int PER = 16 / sizeof(Tout);
     if constexpr (GLU) {
@@ -541,7 +543,7 @@ __device__ __forceinline__ void leave(const Finish& f, Tout* out, const float* p
 #pragma unroll
             for (int q = 0; q < PER; q += 4) *reinterpret_cast<float4*>(v + q) = *reinterpret_cast<const float4*>(park + j * 32 + c + q);
             __align__(16) Tout w[PER];
-            if (f.accumulate == EPI_ADD) {
+            if (ADDS && f.accumulate == EPI_ADD) {
                 *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(dst);
 #pragma unroll
                 for (int q = 0; q < PER; ++q) v[q] = __fadd_rn(v[q], to_float(w[q]));
@@ -554,7 +556,7 @@ __device__ __forceinline__ void leave(const Finish& f, Tout* out, const float* p
         for (int j = lo; j < hi; ++j) {
             Tout* dst = out + (p0 + j) * f.ldo + n0 + lane;
             const float v = park[j * 32 + lane];
-            *dst = from_float<Tout>(f.accumulate == EPI_ADD ? __fadd_rn(v, to_float(*dst)) : v);
+            *dst = from_float<Tout>(ADDS && f.accumulate == EPI_ADD ? __fadd_rn(v, to_float(*dst)) : v);
         }
     }
 }
@@ -627,15 +629,16 @@ gemm_grouped_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __gr
         for (int u = share.unit; u < units.total && (FP8 || ok); u += share.step) {
             const Unit unit = units(u);
             const int n = unit.tile * 128 + row;
-            const float bias = g.f.has_bias && n < g.f.N ? g.f.bias[n] : 0.f;
+            const float bias = S::ONE && g.f.has_bias && n < g.f.N ? g.f.bias[n] : 0.f;
             const bool vec = lines && n - lane + 32 <= g.f.N;
             // the pairs [lo, hi) of the 16 from t on, parked
             auto finish = [&](int t, int lo, int hi) {
                 __syncwarp();
-                leave<GLU, Tout>(g.f, out, park, (size_t)(unit.first + t), lo, hi, n - lane, vec, lane);
+                leave<GLU, S::ONE, Tout>(g.f, out, park, (size_t)(unit.first + t), lo, hi, n - lane, vec, lane);
                 __syncwarp();
             };
             auto finished = [&](float v) {
+                if constexpr (!S::ONE) return v;
                 v = g.f.has_bias ? __fadd_rn(v, bias) : v;
                 if (g.f.accumulate == EPI_RELU2) {
                     const float z = v < 0.f ? 0.f : v;              // (what is not a number stays so: a maximum would drop it)
@@ -835,7 +838,7 @@ __device__ __forceinline__ void park_row(uint8_t* park, const float (&v)[N], int
     }
 }
 // The warp's 32 rows of 64 bytes -> out, columns from c0 on.
-template <typename Tout>
+template <bool ADDS, typename Tout>
 __device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, uint8_t* park, size_t p0, int rows, int c0, int last, bool vec, int lane) {
     constexpr int PER = 16 / sizeof(Tout), COLS = 4 * PER;
     __syncwarp();
@@ -846,7 +849,7 @@ __device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, uint8_t* 
             if (r >= rows) continue;
             Tout* dst = out + (p0 + r) * f.ldo + c0 + c * PER;
             uint4 x = *reinterpret_cast<const uint4*>(park + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
-            if (sizeof(Tout) == 4 && f.accumulate == EPI_ADD) {
+            if (ADDS && sizeof(Tout) == 4 && f.accumulate == EPI_ADD) {
                 const float4 old = *reinterpret_cast<const float4*>(dst);
                 x = make_uint4(__float_as_uint(__fadd_rn(__uint_as_float(x.x), old.x)), __float_as_uint(__fadd_rn(__uint_as_float(x.y), old.y)),
                                __float_as_uint(__fadd_rn(__uint_as_float(x.z), old.z)), __float_as_uint(__fadd_rn(__uint_as_float(x.w), old.w)));
@@ -859,7 +862,7 @@ __device__ __forceinline__ void leave_rows(const Finish& f, Tout* out, uint8_t* 
             if (r >= rows || c0 + c >= last) continue;
             Tout* dst = out + (p0 + r) * f.ldo + c0 + c;
             const Tout x = *reinterpret_cast<const Tout*>(park + r * 64 + (((c / PER) ^ (r >> 1)) & 3) * 16 + c % PER * sizeof(Tout));
-            *dst = sizeof(Tout) == 4 && f.accumulate == EPI_ADD ? from_float<Tout>(__fadd_rn(to_float(x), to_float(*dst))) : x;
+            *dst = ADDS && sizeof(Tout) == 4 && f.accumulate == EPI_ADD ? from_float<Tout>(__fadd_rn(to_float(x), to_float(*dst))) : x;
         }
     }
 }
@@ -930,19 +933,19 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (c % TIMES == 0) __syncwarp();
                     park_row<Tout>(park, eight, c % TIMES * (4 / TIMES), lane);
                     const int c0 = c_set + c / TIMES * COLS;
-                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
+                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<S::ONE && !GLU, Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
                 } else {
                     const int c16 = c_set + 16 * c;
-                    if (g.f.has_bias)
+                    if (S::ONE && g.f.has_bias)
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q] = c16 + q < last ? __fadd_rn(v[q], g.f.bias[c16 + q]) : 0.f;
-                    if (g.f.accumulate == EPI_RELU2)
+                    if (S::ONE && g.f.accumulate == EPI_RELU2)
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
                             const float z = v[q] < 0.f ? 0.f : v[q];              // (what is not a number stays so: a maximum would drop it)
                             v[q] = __fmul_rn(z, z);
                         }
-                    if (sizeof(Tout) == 2 && g.f.accumulate == EPI_ADD && lane < rows) {
+                    if (S::ONE && sizeof(Tout) == 2 && g.f.accumulate == EPI_ADD && lane < rows) {
                         // (added here, so that the sum is rounded once)
                         const Tout* old = out + (p0 + lane) * g.f.ldo + c16;
 #pragma unroll
@@ -953,7 +956,7 @@ gemm_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (c % TIMES == 0) __syncwarp();
                     park_row<Tout>(park, v, c % TIMES * (4 / TIMES), lane);
                     const int c0 = c_set + c / TIMES * COLS;
-                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
+                    if (c % TIMES == TIMES - 1 && c0 < last) leave_rows<S::ONE && !GLU, Tout>(g.f, out, park, p0, rows, c0, last, vec, lane);
                 }
             };
             if constexpr (FP8) {
@@ -1358,8 +1361,8 @@ Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int ti
     };
     if (!groups) {
         for (const Narrowly& c : NARROW)
-            for (int blocks = 1; blocks <= (fp8 && c.nt <= 32 ? 8 : 1); ++blocks) offer(narrow_count(c, blocks, rows, tiles, k_blocks, sms), {c.nt, 1, blocks, 2});
-        for (int blocks = 1; blocks <= (fp8 ? 4 : 1); blocks *= 2) offer(wide_count(blocks, rows, tiles, k_blocks, sms), {128, 2, blocks, 1});
+            for (int blocks = 1; blocks <= (c.nt <= 32 ? 8 : 1); ++blocks) offer(narrow_count(c, blocks, rows, tiles, k_blocks, sms), {c.nt, 1, blocks, 2});
+        for (int blocks = 1; blocks <= 4; blocks *= 2) offer(wide_count(blocks, rows, tiles, k_blocks, sms), {128, 2, blocks, 1});
     } else {
         const double pairs = (double)groups->rows * groups->top, share = groups->top < groups->groups ? (double)groups->top / groups->groups : 1.0;
         const double asked = groups->groups * (1.0 - pow(1.0 - share, groups->rows)), mean = pairs / (asked > 1.0 ? asked : 1.0);
@@ -1367,7 +1370,7 @@ Cut choose(bool fp8, const RowGroupsView* groups, bool by_pair, int rows, int ti
             const Grouping& c = GROUPING[fp8][by_pair][i];
             const int nt = SPANS[i], places = nt == 128 ? sms : 2 * sms;
             const double spans = mean <= 0.5 * nt ? asked : pairs / nt + 0.5 * asked, units = spans * (nt == 128 ? (tiles + 1) / 2 : tiles);
-            const double rounds = units <= sms ? 1.0 : units < places ? 1.0 : units / places, read = asked * tiles * (double)TILE_BYTES * k_blocks / 6.2e6;
+            const double rounds = units < places ? 1.0 : units / places, read = asked * tiles * (double)TILE_BYTES * k_blocks / 6.2e6;
             const double run = rounds * (k_blocks * c.k_block + c.unit + c.row * (mean < nt ? mean : nt));
             offer(c.start + sqrt(sqrt(run * run * run * run + read * read * read * read)), {nt, nt == 128 ? 2 : 1, 1, nt == 128 ? 1 : 2});
         }
@@ -1395,7 +1398,7 @@ JLLM_EXPORT int jllm_gemm_grouped_starve_next(int what, int limit_us) {
     return JLLM_OK;
 }
 
-// `rows`: what is multiplied (of e4m3, with the scales), [M, K]; `weight`: the packed weight(s) [N, K]; `groups`: null (one weight, out [M, N]) or
+// `rows`: what is multiplied (of e4m3, with the scales), [M, K]; `weight`: the packed weight(s) [N, K]; `groups`: null (one weight of e4m3, out [M, N]) or
 // the groups of pairs (out [pairs, N], of which the rows behind the last pair stay as they were), `by_pair` whether `rows` are the pairs'
 // already. With `swiglu_word` out has N / 2 columns. `cut` (tests): see Cut; 0 as the sizes have it.
 JLLM_EXPORT int jllm_gemm_grouped(const BlockRows* rows, const BlockWeight* weight, const RowGroupsView* groups, int by_pair, const void* bias,
@@ -1415,6 +1418,7 @@ JLLM_EXPORT int jllm_gemm_grouped(const BlockRows* rows, const BlockWeight* weig
     JLLM_REQUIRE(!fp8 || (rows->scale_ld % 4 == 0 && rows->scale_ld >= weight->k_blocks && weight->scale_ld % 4 == 0 && weight->scale_ld >= weight->k_blocks &&
                           ((uintptr_t)rows->scale % 16) == 0 && ((uintptr_t)weight->scale % 16) == 0),
                  "gemm_grouped: scales lie in rows of whole fours (%d and %d for %d blocks)", rows->scale_ld, weight->scale_ld, weight->k_blocks);
+    JLLM_REQUIRE(fp8 || groups, "gemm_grouped: a product of one weight is built for e4m3 rows and weights");
     JLLM_REQUIRE(groups ? groups->groups == weight->groups && groups->groups >= 1 && groups->groups <= MAX_GROUPS && (by_pair ? pairs : groups->rows) == M
                         : weight->groups == 1,
                  "gemm_grouped: %d weights (1 to %d), %d rows and the groups of another product", weight->groups, MAX_GROUPS, M);
