@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(MOST_WARPS * 32) group_rows_kernel(const int* 
                                                                      int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ place) {
     extern __shared__ int counts[];
     __shared__ unsigned long long sums[MOST_WARPS + 1];
+    static_assert(sizeof(sums) <= 1024, "beside 47 KB in a launch's 48");
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x, rank = blockIdx.x;
     int *mine = counts + warp * groups, *block_first = counts + warps * groups, *local_first = block_first + groups, *all_of = local_first + groups;
     uint32_t* sorted = reinterpret_cast<uint32_t*>(all_of + groups);
@@ -265,7 +266,8 @@ JLLM_EXPORT int jllm_group_rows(const int* choice, int ld, const RowGroupsView* 
     const int warps = pairs <= 8 * 32 ? 8 : pairs <= 16 * 32 ? 16 : MOST_WARPS;
     const int run = (int)(((pairs + (long long)blocks * warps - 1) / ((long long)blocks * warps) + 31) / 32 * 32);
     const size_t smem = ((size_t)(warps + 3) * g->groups + (run <= 32 * HELD ? (size_t)warps * run : 0)) * sizeof(int);
-    if (smem > 48 * 1024 && jllm_allow_smem((const void*)group_rows_kernel, smem) != cudaSuccess)
+    // (a launch has 48 KB without asking, of which the kernel holds some hundred bytes by itself)
+    if (smem > 47 * 1024 && jllm_allow_smem((const void*)group_rows_kernel, smem) != cudaSuccess)
         return jllm_fail(JLLM_CUDA_ERROR, "group_rows: %zu bytes of shared memory refused", smem);
     if (blocks > 1) {
         JLLM_REQUIRE(g->counts, "group_rows: no room for the blocks' counts");
