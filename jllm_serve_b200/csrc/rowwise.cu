@@ -1119,6 +1119,10 @@ JLLM_EXPORT int jllm_norm_chain(float* x, const float* a, const void* gain_a, co
     JLLM_REQUIRE(dim <= 48 * 256, "norm_chain: a row of %d values is above %d", dim, 48 * 256);
     if (rows == 0) return JLLM_OK;
     const size_t smem = (size_t)dim * sizeof(float);
+    // (a launch has 48 KB without asking, of which the kernels hold some hundred bytes by themselves)
+    if (smem > 47 * 1024 && (jllm_allow_smem((const void*)norm_chain_kernel<float>, smem) != cudaSuccess ||
+                             jllm_allow_smem((const void*)norm_chain_kernel<__nv_bfloat16>, smem) != cudaSuccess))
+        return jllm_fail(JLLM_CUDA_ERROR, "norm_chain: %zu bytes of shared memory refused", smem);
     const VecRef ga{gain_a, gain_dtype}, gb{gain_b, gain_dtype}, gp{gain_post, gain_dtype}, gn{gain_next, gain_dtype};
     if (dim % 4 == 0 && dim <= 8192 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)a % 16) == 0 && ((uintptr_t)b % 16) == 0 &&
         ((uintptr_t)next % 16) == 0) {
