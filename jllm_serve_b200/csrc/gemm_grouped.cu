@@ -176,16 +176,24 @@ struct Ring {
 template <class S>
 constexpr size_t fixed_smem() { return 1024 + 8 * (2 * S::BUFFERS + 1) + 64; }
 
-// Units in front of every group, by the whole block (a lane has 32 neighbouring groups at most); a __syncthreads has to follow.
+// Units in front of every group, by the whole block (a lane has 32 neighbouring groups at most); a __syncthreads has to follow. Offsets are a kernel's output, which
+// the host cannot check: a larger step's that were not filled anew are cut off at the pairs there are, and numbers that do not ascend from 0 on are no pairs, so
+// that whatever they are nothing outside the rows and the result is touched.
 template <class S>
 __device__ __forceinline__ void list_units(const Args& g, int* before, int* at) {
     pdl_wait();          // (the offsets are the kernel in front's)
-    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = min(g.offsets[i], g.pairs);          // (of a larger step, not filled anew: within bounds)
+    for (int i = threadIdx.x; i <= g.groups; i += blockDim.x) at[i] = min(g.offsets[i], g.pairs);
     __syncthreads();
     if (threadIdx.x >= 32) return;
-    const int lane = threadIdx.x, each = (g.groups + 31) / 32, lo = min(lane * each, g.groups), hi = min(lo + each, g.groups), tiles = (g.tiles + S::TILES - 1) / S::TILES;
-    int sum = 0;
-    for (int i = lo; i < hi; ++i) sum += (at[i + 1] - at[i] + S::ROWS - 1) / S::ROWS * tiles;
+    const int lane = threadIdx.x, each = (g.groups + 31) / 32, lo = min(lane * each, g.groups), hi = min(lo + each, g.groups);
+    int tiles = (g.tiles + S::TILES - 1) / S::TILES, sum = 0;
+    bool wrong = false;
+    for (int i = lo; i < hi; ++i) {
+        const int here = at[i], next = at[i + 1];
+        wrong |= here < 0 || next < here;
+        sum += wrong ? 0 : (next - here + S::ROWS - 1) / S::ROWS * tiles;
+    }
+    if (__any_sync(0xffffffffu, wrong)) sum = tiles = 0;
     int run = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -2003,7 +2003,8 @@ def gemm_fp8(a: Fp8Rows, w: PackedBlocks, out: torch.Tensor, bias: torch.Tensor 
 class RowGroups:
     """The (row, choice) pairs of a step in the order of the groups (experts) they ask: group g's pairs are order[offsets[g]] .. order[offsets[g + 1] - 1],
     each r * top + c of its row r and choice c, in ascending order; `order` is -1 behind the last pair. place[r, c] is where the pair (r, c) lies, -1 if it
-    asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs."""
+    asks nobody. Made by `row_groups`, filled by `group_rows`; until then there are no pairs, and none where the offsets do not ascend from 0 on (a product reads
+    and writes within its rows and its result whatever the numbers are)."""
     __slots__ = ("offsets", "order", "place", "counts", "rows", "top", "groups", "shape", "pairs", "device", "_view", "view")
 
     def __init__(self, offsets, order, place, counts, rows, top, groups):
