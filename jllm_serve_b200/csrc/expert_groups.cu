@@ -10,7 +10,7 @@
 // of 8 SMs).
 //
 // combine_groups reads every answer once and writes every row once: memory bounds it. The sum runs over a row's choices in their order in float32,
-// whatever place the pairs have: equal bits in every batch. 2,048 rows of eight float32 answers of 2,048 values 23.6 us (5.8 TB/s), bfloat16 12.1; 16 rows 2.3 us.
+// whatever place the pairs have: equal bits in every batch. 2,048 rows of eight float32 answers of 2,048 values 24.4 to 24.9 us (5.5 TB/s; 23.6 at best), bfloat16 12.1; 16 rows 2.3 us.
 #include "common.cuh"
 #include "fp8_view.h"
 

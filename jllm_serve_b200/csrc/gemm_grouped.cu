@@ -30,7 +30,7 @@
 // bytes). In 8 bits it is the way of a k block from the tensor cores to the epilogue's registers and back, over two buffers, which are all of tensor
 // memory: some 1,000 cycles a k block and SM where its MMAs (128 x 256 x 128) take 512. By cycle counts a warp of the sums spends 390 on its loads of tensor memory and
 // multiply-adds (256 are the float32 units' least), 140 on waiting, the rest on scales, barriers and, spread over a unit's k blocks, its results; the issuing warp waits 450 to 600
-// for a buffer and 90 for copies. 2,048 x 24,576 x 4,096 take 217 to 227 us (1.8 to 1.9 PFLOP/s), 264 one behind the other for long (the power limit). Measured slower: the two tiles of a k block
+// for a buffer and 90 for copies. 2,048 x 24,576 x 4,096 take 213 to 227 us (1.8 to 1.9 PFLOP/s), 264 one behind the other for long (the power limit). Measured slower: the two tiles of a k block
 // handed over apart (1 to 2%), eight warps of twice the columns, k blocks unrolled by four. Also slower: the last round's units shared out by weight rows (8-bit down of
 // 2,048 rows 118 us for 102).
 //
